@@ -313,6 +313,95 @@ int sy_matmul(sy_ctx* ctx, const float* a, const float* b, float* c, int m, int 
 int sy_attention(sy_ctx* ctx, const sy_tensor* qkv, int heads, int key_dim,
                  int head_dim, float scale, const sy_tensor* o, const sy_tensor* v);
 
+/* Rotary positions of query and key heads.  No counterpart in the reference,
+ * whose attention takes positions from the depthwise `pe` conv
+ * (src/SimdYolo/PtModel.cs:434-437); for attention on maps and sequences that
+ * sy_block_attention serves.  The first `dim` of a head's head_dim channels
+ * are turned in pairs by position * frequency, y = (a c - b s, b c + a s); the
+ * others are copied.  With 2 axes the first half of `dim` turns with the row,
+ * the second with the column.  In an axis' part of P channels pair i has the
+ * frequency base^(-2i/P) and is channels (2i, 2i+1) when interleaved, (i,
+ * i + P/2) otherwise.  Scaled for positions past the range that a model was
+ * trained on, by `factor`: SY_ROTARY_LINEAR divides frequencies by it,
+ * SY_ROTARY_BASE multiplies the base by factor^(P/(P-2)), SY_ROTARY_PARTS
+ * (YaRN: Peng et al., 2023) divides the frequencies of pairs that make up to
+ * `low` turns over `original` positions, keeps those of `high` turns and more,
+ * goes linearly between, and multiplies cosines and sines by
+ * 0.1 ln(factor) + 1.  Angles are formed in 64 bits. */
+#define SY_ROTARY_PLAIN 0
+#define SY_ROTARY_LINEAR 1
+#define SY_ROTARY_BASE 2
+#define SY_ROTARY_PARTS 3
+typedef struct sy_rotary_config {
+  int32_t head_dim, dim; /* channels of a head (a multiple of 4, up to 512) and how many of them rotate */
+  int32_t axes;          /* 1: token index; 2: row and column */
+  int32_t interleaved;
+  float base;
+  int32_t scaling; /* SY_ROTARY_*; the fields below are read by the scalings that name them */
+  float factor, low, high;
+  int32_t original;
+} sy_rotary_config;
+/* Heads of one tensor: head h's channels start at x_stride * h of the view
+ * (0: head_dim), so the q heads of a qkv tensor are read in place. */
+typedef struct sy_rotary_heads {
+  sy_tensor x, y;
+  int32_t heads, x_stride, y_stride;
+} sy_rotary_heads;
+/* The handle lives as long as the context. */
+int sy_rotary_create(sy_ctx* ctx, const sy_rotary_config* cfg, uint64_t* rotary);
+/* Rotates one or two sets of heads (queries and keys) of the same tokens.
+ * positions: device, [n][h*w][axes], or NULL for the token's index (2 axes:
+ * its row and column).  y may be x itself; other overlaps are refused.  Views
+ * are 16-byte aligned, strides and ldc multiples of 4. */
+int sy_rotary_run(sy_ctx* ctx, uint64_t rotary, const sy_rotary_heads* parts, int n_parts,
+                  const int32_t* positions);
+
+/* Attention over the key blocks that a cheap score selects for each query.
+ * No counterpart in the reference, whose attention (PtModel.cs:429-437) meets
+ * every key; for maps and sequences where that is too many.  Keys stand on the
+ * map of the views k and v, in windows of block_h x block_w pixels (those at the
+ * right and lower edge may be cut), numbered row by row; a sequence is a map
+ * one pixel high.  Per call sequence: sy_block_means, sy_block_select,
+ * sy_block_attention.
+ *
+ * Sequences (map and windows one pixel high) may have valid keys in front only,
+ * lengths[n] of them, and be causal: query i of image b stands at position
+ * starts[b] + i (starts NULL: i) and sees the keys up to its own.  Both are
+ * device arrays of int32 or NULL; lengths are taken between 0 and the row. */
+typedef struct sy_block_config {
+  int32_t heads, kv_heads;   /* heads % kv_heads == 0; heads / kv_heads neighbours share a key head */
+  int32_t key_dim, head_dim; /* channels of a query or key head, of a value head: multiples of 4 up to 128 */
+  int32_t q_stride, k_stride, v_stride; /* channels from a head to the next (0: dense) */
+  int32_t block_h, block_w;  /* up to 1024 keys */
+  int32_t selected;          /* blocks for each query, 1 to 64 */
+  int32_t causal;
+  float scale;
+} sy_block_config;
+/* Mean key of every block and key head into the view means [n, kv_heads *
+ * key_dim, ceil(h / block_h), ceil(w / block_w)], summed in 64 bits; 0 for a
+ * block without valid keys.  With tokens > 0 only the blocks that hold the
+ * positions starts[b] .. starts[b] + tokens - 1 are renewed (a cache that has
+ * grown by them); with 0 all are. */
+int sy_block_means(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* k, const int32_t* starts, int tokens,
+                   const int32_t* lengths, const sy_tensor* means);
+/* The blocks of each query (pixel of q) and key head into blocks (device,
+ * [n][h*w][kv_heads][selected]): those with the largest scores, the product of
+ * the block's mean and the sum of the query heads that share the key head, among
+ * the blocks with a visible key; ties go to the lower block, NaN stands behind
+ * every number.  A causal query's own block is always among them.  Ascending,
+ * then -1 where fewer are visible.  Choices are those of scores in 64 bits. */
+int sy_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q, const sy_tensor* means,
+                    const int32_t* starts, const int32_t* lengths, int32_t* blocks);
+/* o = softmax(scale q k^T) v over the visible keys of each query's blocks; o
+ * is a view of heads * head_dim channels on q's map.  blocks as
+ * sy_block_select writes it, or any: entries outside 0 .. blocks - 1 are
+ * skipped, one named twice counts twice.  A query without a key gets zeros.
+ * Keys that are not visible are not read into any result, whatever they hold.
+ * o must not overlap q, k or v. */
+int sy_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q, const sy_tensor* k,
+                       const sy_tensor* v, const int32_t* blocks, const int32_t* starts, const int32_t* lengths,
+                       const sy_tensor* o);
+
 /* Per-instance mask geometry returned by sy_mask_decode: the crop in source
  * pixels and the offset (in floats) of its width*height probabilities in the
  * output buffer. */

@@ -31,6 +31,15 @@ internal struct SyDecodeOptions { public float Confidence, Iou; public int MaxDe
 [StructLayout(LayoutKind.Sequential)]
 internal struct SyMaskInfo { public int Left, Top, Width, Height; public long Offset; }
 
+[StructLayout(LayoutKind.Sequential)]
+internal struct SyRotaryConfig { public int HeadDim, Dim, Axes, Interleaved; public float Base; public int Scaling; public float Factor, Low, High; public int Original; }
+
+[StructLayout(LayoutKind.Sequential)]
+internal struct SyRotaryHeads { public SyTensor X, Y; public int Heads, XStride, YStride; }
+
+[StructLayout(LayoutKind.Sequential)]
+internal struct SyBlockConfig { public int Heads, KvHeads, KeyDim, HeadDim, QStride, KStride, VStride, BlockH, BlockW, Selected, Causal; public float Scale; }
+
 internal static unsafe partial class HipNative
 {
     private const string Lib = "simdyolo_hip";
@@ -83,6 +92,19 @@ internal static unsafe partial class HipNative
     internal static partial int EndToEndTopKNoAlloc(nint ctx, nint head, int batch, int channels, int anchors, int nc, int maximum, int onnxRules, nint output);
     [LibraryImport(Lib, EntryPoint = "sy_attention")]
     internal static partial int Attention(nint ctx, in SyTensor qkv, int heads, int keyDim, int headDim, float scale, in SyTensor o, in SyTensor v);
+
+    // ------------------------------------------------------------ rotary positions, attention over key blocks
+    // positions, starts, lengths and blocks are device pointers to int (0 where the header allows NULL).
+    [LibraryImport(Lib, EntryPoint = "sy_rotary_create")]
+    internal static partial int RotaryCreate(nint ctx, in SyRotaryConfig cfg, out ulong rotary);
+    [LibraryImport(Lib, EntryPoint = "sy_rotary_run")]
+    internal static partial int RotaryRun(nint ctx, ulong rotary, SyRotaryHeads* parts, int count, nint positions);
+    [LibraryImport(Lib, EntryPoint = "sy_block_means")]
+    internal static partial int BlockMeans(nint ctx, in SyBlockConfig cfg, in SyTensor k, nint starts, int tokens, nint lengths, in SyTensor means);
+    [LibraryImport(Lib, EntryPoint = "sy_block_select")]
+    internal static partial int BlockSelect(nint ctx, in SyBlockConfig cfg, in SyTensor q, in SyTensor means, nint starts, nint lengths, nint blocks);
+    [LibraryImport(Lib, EntryPoint = "sy_block_attention")]
+    internal static partial int BlockAttention(nint ctx, in SyBlockConfig cfg, in SyTensor q, in SyTensor k, in SyTensor v, nint blocks, nint starts, nint lengths, in SyTensor o);
 
     // ------------------------------------------------------------ generic device ops
     // IDeviceBackend.Compute: one tensor.comp operation; inputs[3] / lengths[3] are the A, B, D bindings.

@@ -17,6 +17,7 @@ SY_OK, SY_EINVAL, SY_EUNSUPPORTED, SY_EDEVICE, SY_ENOMEM, SY_ESTATE = range(6)
 LAYOUT_NHWC, LAYOUT_NCHW = 0, 1
 CONV_AUTO, CONV_IGEMM, CONV_WINOGRAD, CONV_DIRECT, CONV_WINOGRAD3, CONV_DEPTHWISE, CONV_WINOGRAD2 = range(7)
 ARCH_YOLOV8, ARCH_YOLO11, ARCH_YOLO26 = 0, 1, 2
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_PARTS = range(4)
 
 # Every exported symbol declared in include/simdyolo_hip.h.
 EXPORTS = (
@@ -28,6 +29,7 @@ EXPORTS = (
     "sy_add", "sy_resize_nearest", "sy_maxpool", "sy_sppf_pool", "sy_copy", "sy_detect_decode", "sy_e2e_topk",
     "sy_e2e_topk_noalloc",
     "sy_mask_decode", "sy_attention", "sy_compute", "sy_matmul",
+    "sy_rotary_create", "sy_rotary_run", "sy_block_means", "sy_block_select", "sy_block_attention",
     "sy_graph_begin", "sy_graph_end", "sy_graph_launch", "sy_graph_destroy",
     "sy_timer_start", "sy_timer_stop", "sy_profile_enable", "sy_profile_read",
     "sy_model_layout", "sy_model_create", "sy_model_destroy", "sy_model_output_shape", "sy_model_predict_raw",
@@ -84,6 +86,25 @@ class MaskInfo(ctypes.Structure):
                 ("height", ctypes.c_int32), ("offset", ctypes.c_int64)]
 
 
+class RotaryConfig(ctypes.Structure):
+    _fields_ = [("head_dim", ctypes.c_int32), ("dim", ctypes.c_int32), ("axes", ctypes.c_int32),
+                ("interleaved", ctypes.c_int32), ("base", ctypes.c_float), ("scaling", ctypes.c_int32),
+                ("factor", ctypes.c_float), ("low", ctypes.c_float), ("high", ctypes.c_float),
+                ("original", ctypes.c_int32)]
+
+
+class RotaryHeads(ctypes.Structure):
+    """Heads of the view x, rotated into the view y; strides in channels (0: head_dim)."""
+    _fields_ = [("x", Tensor), ("y", Tensor), ("heads", ctypes.c_int32), ("x_stride", ctypes.c_int32),
+                ("y_stride", ctypes.c_int32)]
+
+
+class BlockConfig(ctypes.Structure):
+    _fields_ = [(f, ctypes.c_int32) for f in ("heads", "kv_heads", "key_dim", "head_dim", "q_stride", "k_stride",
+                                              "v_stride", "block_h", "block_w", "selected", "causal")] + \
+        [("scale", ctypes.c_float)]
+
+
 class DecodeOptions(ctypes.Structure):
     _fields_ = [("confidence", ctypes.c_float), ("iou", ctypes.c_float), ("max_detections", ctypes.c_int32),
                 ("max_candidates", ctypes.c_int32), ("class_count", ctypes.c_int32),
@@ -97,6 +118,7 @@ _f = ctypes.c_float
 _fp = ctypes.POINTER(ctypes.c_float)
 _tp = ctypes.POINTER(Tensor)
 _u64p = ctypes.POINTER(ctypes.c_uint64)
+_bp = ctypes.POINTER(BlockConfig)
 
 _SIGS = {
     "sy_create": (_i, [_i, ctypes.POINTER(_vp)]),
@@ -134,6 +156,11 @@ _SIGS = {
     "sy_mask_decode": (_i, [_vp, _tp, _vp, _i, _i, ctypes.POINTER(DetectionT), ctypes.POINTER(LetterboxT), _vp,
                             ctypes.c_size_t, ctypes.POINTER(MaskInfo)]),
     "sy_attention": (_i, [_vp, _tp, _i, _i, _i, _f, _tp, _tp]),
+    "sy_rotary_create": (_i, [_vp, ctypes.POINTER(RotaryConfig), _u64p]),
+    "sy_rotary_run": (_i, [_vp, ctypes.c_uint64, ctypes.POINTER(RotaryHeads), _i, _vp]),
+    "sy_block_means": (_i, [_vp, _bp, _tp, _vp, _i, _vp, _tp]),
+    "sy_block_select": (_i, [_vp, _bp, _tp, _tp, _vp, _vp, _vp]),
+    "sy_block_attention": (_i, [_vp, _bp, _tp, _tp, _tp, _vp, _vp, _vp, _tp]),
     "sy_compute": (_i, [_vp, _i, ctypes.POINTER(_vp), ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_uint32),
                         ctypes.c_int64, _vp, ctypes.c_size_t]),
     "sy_matmul": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, ctypes.POINTER(ctypes.c_int32),

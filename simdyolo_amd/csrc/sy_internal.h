@@ -60,6 +60,7 @@ std::shared_timed_mutex& capture_lock();
 // ------------------------------------------------------------- context
 
 struct ConvPlan;
+struct RotaryPlan;
 
 enum Algo { kAuto = 0, kIgemm = 1, kWinograd = 2, kDirect = 3, kWinograd3 = 4, kDepthwise = 5, kWinograd2 = 6 };
 
@@ -97,6 +98,7 @@ struct sy_ctx {
   // persistent allocations owned by the context (weights)
   std::vector<void*> owned;
   std::vector<std::unique_ptr<sy::ConvPlan>> convs;
+  std::vector<std::shared_ptr<const sy::RotaryPlan>> rotaries;
   // scratch (Winograd transforms, staging); grows outside capture only
   char* scratch = nullptr;
   size_t scratch_size = 0;
@@ -174,6 +176,21 @@ int ensure_host_stage(sy_ctx* ctx, size_t bytes);
 inline bool graph_stale(const sy_ctx* ctx, uint64_t graph) {
   return graph > 0 && graph <= ctx->graph_gen.size() && ctx->graph_gen[graph - 1] != ctx->scratch_gen;
 }
+
+// The context's device as the thread's current one, and back: for launches and
+// allocations of callers that work on another device.
+struct DeviceScope {
+  int before = -1;
+  explicit DeviceScope(const sy_ctx* ctx) {
+    int now = -1;
+    if (hipGetDevice(&now) == hipSuccess && now != ctx->device && hipSetDevice(ctx->device) == hipSuccess) before = now;
+  }
+  ~DeviceScope() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+};
 
 // Kernel-launch bracketing for per-kernel profiling.
 void prof_begin(sy_ctx* ctx, const char* name, double flops, double bytes);
@@ -287,6 +304,36 @@ int op_matmul(sy_ctx* ctx, const float* a, const float* b, float* c, int m, int 
 int op_attention(sy_ctx* ctx, const sy_tensor* qkv, int heads, int kd, int hd, float scale, const sy_tensor* o,
                  const sy_tensor* v);
 size_t attention_scratch_bytes(int B, int H, int W, int heads, int kd, int hd);
+
+// Rotary positions: the pairs' frequencies, prepared by sy_rotary_create.
+constexpr int kRotaryMaxDim = 512;  // channels of a head; the frequencies travel as kernel arguments
+struct RotaryPlan {
+  sy_rotary_config cfg;
+  int half;                         // pairs of one axis
+  float amplitude;                  // cosines and sines times this
+  double turns[kRotaryMaxDim / 2];  // frequency / 2 pi, pair by pair
+};
+int op_rotary_create(sy_ctx* ctx, const sy_rotary_config* cfg, uint64_t* rotary);
+int op_rotary_run(sy_ctx* ctx, uint64_t rotary, const sy_rotary_heads* parts, int n_parts, const int32_t* positions);
+
+// Attention over chosen key blocks: what the config and the views say, checked.
+struct BlockShape {
+  int n, tq, tk;         // images, queries and keys of each
+  int kh, kw, bh, bw;    // key map and its windows
+  int by, bx, blocks;    // windows down, across, in all
+  int heads, kv, group;  // query heads, key heads, query heads of one key head
+  int kd, hd, qs, ks, vs, selected, causal;
+  float scale;
+};
+int block_shape(const sy_block_config* cfg, BlockShape* s);
+int block_heads(const sy_tensor* t, int heads, int dim, int stride, const char* what);
+int op_block_means(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* k, const int32_t* starts, int tokens,
+                   const int32_t* lengths, const sy_tensor* means);
+int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q, const sy_tensor* means,
+                    const int32_t* starts, const int32_t* lengths, int32_t* blocks);
+int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q, const sy_tensor* k,
+                       const sy_tensor* v, const int32_t* blocks, const int32_t* starts, const int32_t* lengths,
+                       const sy_tensor* o);
 
 int64_t pool_out_size(int len, int k, int s, int before, int after, int ceil_mode);
 

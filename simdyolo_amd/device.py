@@ -161,6 +161,34 @@ class HipContext:
         check(self._lib.sy_attention(self.handle, ctypes.byref(qkv), heads, key_dim, head_dim, float(scale),
                                      ctypes.byref(o), ctypes.byref(v)))
 
+    def rotary_create(self, head_dim: int, dim: int, axes: int = 1, interleaved: bool = False, base: float = 10000.0,
+                      scaling: int = N.ROTARY_PLAIN, factor: float = 1.0, low: float = 1.0, high: float = 32.0,
+                      original: int = 0) -> int:
+        cfg = N.RotaryConfig(head_dim, dim, axes, int(interleaved), base, scaling, factor, low, high, original)
+        h = ctypes.c_uint64()
+        check(self._lib.sy_rotary_create(self.handle, ctypes.byref(cfg), ctypes.byref(h)))
+        return h.value
+
+    def rotary(self, rotary: int, parts, positions: int | None = None):
+        """Rotates one or two RotaryHeads; `positions` is a device pointer to int32 [n][h*w][axes]."""
+        arr = (N.RotaryHeads * len(parts))(*parts)
+        check(self._lib.sy_rotary_run(self.handle, rotary, arr, len(parts), positions))
+
+    def block_means(self, cfg: N.BlockConfig, k: Tensor, means: Tensor, starts: int | None = None, tokens: int = 0,
+                    lengths: int | None = None):
+        check(self._lib.sy_block_means(self.handle, ctypes.byref(cfg), ctypes.byref(k), starts, tokens, lengths,
+                                       ctypes.byref(means)))
+
+    def block_select(self, cfg: N.BlockConfig, q: Tensor, means: Tensor, blocks_ptr: int, starts: int | None = None,
+                     lengths: int | None = None):
+        check(self._lib.sy_block_select(self.handle, ctypes.byref(cfg), ctypes.byref(q), ctypes.byref(means), starts,
+                                        lengths, blocks_ptr))
+
+    def block_attention(self, cfg: N.BlockConfig, q: Tensor, k: Tensor, v: Tensor, blocks_ptr: int, o: Tensor,
+                        starts: int | None = None, lengths: int | None = None):
+        check(self._lib.sy_block_attention(self.handle, ctypes.byref(cfg), ctypes.byref(q), ctypes.byref(k),
+                                           ctypes.byref(v), blocks_ptr, starts, lengths, ctypes.byref(o)))
+
     def compute(self, op: int, inputs, params, work_items: int, out_ptr: int, out_len: int):
         """One tensor.comp op. `inputs` holds up to three (device_ptr, length_in_floats) pairs or None for
         the A, B and D bindings; `params` up to 32 uint32 slots (floats passed as their bit pattern)."""
