@@ -20,7 +20,6 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kKeys = 64;    // keys of a tile; longer blocks are so many tiles ("parts" of the block)
-constexpr int kRows = 128;   // rows of a tile: 32 for each of four waves
 constexpr int kMaxBlocks = 12288;  // of a sorted list: counters in LDS
 
 struct BlockArgs {
@@ -32,10 +31,11 @@ struct BlockArgs {
   int parts;         // tiles of a block along its keys
   // Segments: `span` queries of one image and key head each, `segs` of them to a plane.
   int span, segs, first;  // first: of the launch
-  int sorted;        // 0: tiles are the (query, slot) pairs themselves
-  int row_tiles;     // of a pair, where not sorted
+  int now;           // segments of the launch
   // Sorted lists of each segment.
-  int chunks, tile_cap;  // chunks of the counting sort; tiles at most
+  int rows;          // of a tile
+  unsigned trash;    // a row of results that nobody reads
+  int chunk, chunks, tile_cap;  // queries of a workgroup of the sort, such workgroups; tiles at most
   int *counts, *list, *tile_count;
   int4* tiles;
   // Results of the launch's segments, row by row.
@@ -43,7 +43,7 @@ struct BlockArgs {
   float* part;       // weighted values
 };
 
-constexpr int kChunk = 1024;  // queries that a workgroup of the sort counts
+constexpr int kSortThreads = 512;
 
 // Keys of image b that query i sees: those before this position.
 __device__ __forceinline__ int visible(const BlockArgs& a, int b, int i) {
@@ -66,29 +66,50 @@ __device__ __forceinline__ const int* list_of(const BlockArgs& a, int b, int i, 
 
 // --------------------------------------------------------------- sorted lists
 
-// Counts, per segment and chunk of queries, how often each block is named.
-__global__ __launch_bounds__(256) void block_count_kernel(const BlockArgs a) {
-  extern __shared__ int hist[];
+// The pairs of one chunk of a segment, four at a time in every thread: f(pair, block) for those whose block
+// is seen.
+template <class F>
+__device__ __forceinline__ void for_pairs(const BlockArgs& a, int seg, int chunk, F f) {
   const BlockShape& s = a.s;
-  const int seg = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-  const int plane = seg / a.segs, b = plane / s.kv, g = plane % s.kv;
+  const int plane = seg / a.segs, b = plane / s.kv, g = plane - b * s.kv;
   const int i0 = seg % a.segs * a.span, i1 = min(i0 + a.span, s.tq);
-  const int from = i0 + chunk * kChunk, to = min(from + kChunk, i1);
-  for (int j = threadIdx.x; j < s.blocks; j += 256) hist[j] = 0;
-  __syncthreads();
-  const int pairs = max(to - from, 0) * s.selected;
-  for (int t = threadIdx.x; t < pairs; t += 256) {
-    const int d = t / s.selected, i = from + d;
-    const int j = list_of(a, b, i, g)[t - d * s.selected];
-    if (block_seen(a, j, visible(a, b, i))) atomicAdd(&hist[j], 1);
+  const int from = i0 + chunk * a.chunk, to = min(from + a.chunk, i1);
+  const int pairs = max(to - from, 0) * s.selected, skip = (from - i0) * s.selected;
+  const int* lists = list_of(a, b, from, g);
+  const int length = a.lengths ? min(max(a.lengths[b], 0), s.tk) : s.tk;
+  const long long start = a.starts ? a.starts[b] : 0;
+  for (int t0 = threadIdx.x; t0 < pairs; t0 += 4 * kSortThreads) {
+    int j[4], d[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int t = min(t0 + u * kSortThreads, pairs - 1);
+      d[u] = t / s.selected;
+      j[u] = lists[(long long)d[u] * s.kv * s.selected + t - d[u] * s.selected];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int t = t0 + u * kSortThreads;
+      int end = length;
+      if (s.causal) end = (int)min((long long)end, max(start + from + d[u] + 1, 0LL));
+      if (t < pairs && block_seen(a, j[u], end)) f(skip + t, j[u]);
+    }
   }
-  __syncthreads();
-  int* out = a.counts + ((long long)seg * a.chunks + chunk) * s.blocks;
-  for (int j = threadIdx.x; j < s.blocks; j += 256) out[j] = hist[j];
 }
 
-// Exclusive sum over the workgroup's 1024 threads; *total: of all.
-__device__ __forceinline__ int2 scan1024(int2 v, int2* lds, int2* total) {
+// Counts, per segment and chunk of queries, how often each block is named.
+__global__ __launch_bounds__(kSortThreads) void block_count_kernel(const BlockArgs a) {
+  extern __shared__ int hist[];
+  const int seg = blockIdx.x / a.chunks, chunk = blockIdx.x - seg * a.chunks;
+  for (int j = threadIdx.x; j < a.s.blocks; j += kSortThreads) hist[j] = 0;
+  __syncthreads();
+  for_pairs(a, seg, chunk, [&](int, int j) { atomicAdd(&hist[j], 1); });
+  __syncthreads();
+  int* out = a.counts + ((long long)seg * a.chunks + chunk) * a.s.blocks;
+  for (int j = threadIdx.x; j < a.s.blocks; j += kSortThreads) out[j] = hist[j];
+}
+
+// Exclusive sum over the workgroup's threads; *total: of all.
+__device__ __forceinline__ int2 scan_threads(int2 v, int2* lds, int2* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int2 x = v;
 #pragma unroll
@@ -102,7 +123,8 @@ __device__ __forceinline__ int2 scan1024(int2 v, int2* lds, int2* total) {
   if (lane == 63) lds[wave] = x;
   __syncthreads();
   int2 before = make_int2(0, 0), all = make_int2(0, 0);
-  for (int w = 0; w < 16; ++w) {
+#pragma unroll
+  for (int w = 0; w < kSortThreads / 64; ++w) {
     const int2 t = lds[w];
     if (w < wave) before = make_int2(before.x + t.x, before.y + t.y);
     all = make_int2(all.x + t.x, all.y + t.y);
@@ -112,66 +134,59 @@ __device__ __forceinline__ int2 scan1024(int2 v, int2* lds, int2* total) {
   return make_int2(before.x + x.x - v.x, before.y + x.y - v.y);
 }
 
-// Per segment: where each chunk's pairs of each block start in the list, and the tiles.
-__global__ __launch_bounds__(1024) void block_scan_kernel(const BlockArgs a) {
-  __shared__ int2 lds[16];
-  __shared__ int4 work[1024];
+// Puts the pairs in the order of their blocks (within a block in no certain order: a row's result does not
+// depend on its neighbours in a tile).  Every chunk's workgroup sums the counts of its segment for itself; the
+// first one writes the tiles.  With one chunk (`alone`) it does the counting, too.
+__global__ __launch_bounds__(kSortThreads) void block_scatter_kernel(const BlockArgs a) {
+  extern __shared__ int hist[];
+  __shared__ int2 lds[kSortThreads / 64];
+  __shared__ int4 work[kSortThreads];
   const BlockShape& s = a.s;
-  const int seg = blockIdx.x;
-  int* counts = a.counts + (long long)seg * a.chunks * s.blocks;
+  const int seg = blockIdx.x / a.chunks, chunk = blockIdx.x - seg * a.chunks;
+  const int* counts = a.counts + (long long)seg * a.chunks * s.blocks;
   int4* tiles = a.tiles + (long long)seg * a.tile_cap;
   int2 base = make_int2(0, 0);
-  for (int j0 = 0; j0 < s.blocks; j0 += 1024) {
+  if (a.chunks == 1) {
+    for (int j = threadIdx.x; j < s.blocks; j += kSortThreads) hist[j] = 0;
+    __syncthreads();
+    for_pairs(a, seg, chunk, [&](int, int j) { atomicAdd(&hist[j], 1); });
+    __syncthreads();
+  }
+  for (int j0 = 0; j0 < s.blocks; j0 += kSortThreads) {
     const int j = j0 + threadIdx.x;
-    int n = 0;
-    if (j < s.blocks)
-      for (int c = 0; c < a.chunks; ++c) n += counts[(long long)c * s.blocks + j];
-    const int t = (int)(((long long)n * s.group + kRows - 1) / kRows);
-    int2 total;
-    const int2 at = scan1024(make_int2(n, t * a.parts), lds, &total);
+    int n = 0, before = 0;  // pairs of block j, those of earlier chunks
     if (j < s.blocks) {
-      int place = base.x + at.x;
-      for (int c = 0; c < a.chunks; ++c) {
-        int* p = counts + (long long)c * s.blocks + j;
-        const int m = *p;
-        *p = place;
-        place += m;
+      if (a.chunks == 1)
+        n = hist[j];
+      else
+#pragma unroll 8
+        for (int c = 0; c < a.chunks; ++c) {
+          const int m = counts[(long long)c * s.blocks + j];
+          n += m;
+          if (c < chunk) before += m;
+        }
+    }
+    const int t = (int)(((long long)n * s.group + a.rows - 1) / a.rows);
+    int2 total;
+    const int2 at = scan_threads(make_int2(n, t * a.parts), lds, &total);
+    if (j < s.blocks) hist[j] = base.x + at.x + before;
+    if (chunk == 0) {
+      work[threadIdx.x] = make_int4(base.x + at.x, n, base.y + at.y, t);
+      __syncthreads();
+      const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+      for (int u = wave; u < min(kSortThreads, s.blocks - j0); u += kSortThreads / 64) {
+        const int4 w = work[u];
+        for (int x = lane; x < w.w * a.parts; x += 64)
+          tiles[w.z + x] = make_int4(j0 + u, x % a.parts | (x / a.parts) << 8, w.x, w.y);
       }
+      __syncthreads();
     }
-    // The tiles of this thread's block, written by all threads of a wave in turn.
-    work[threadIdx.x] = make_int4(base.x + at.x, n, base.y + at.y, t);
-    __syncthreads();
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int u = wave; u < min(1024, s.blocks - j0); u += 16) {
-      const int4 w = work[u];
-      for (int x = lane; x < w.w * a.parts; x += 64)
-        tiles[w.z + x] = make_int4(j0 + u, x % a.parts | (x / a.parts) << 8, w.x, w.y);
-    }
-    __syncthreads();
     base = make_int2(base.x + total.x, base.y + total.y);
   }
-  if (threadIdx.x == 0) a.tile_count[seg] = base.y;
-}
-
-// Puts the pairs in the order of their blocks (within a block in no certain order: a row's result does not
-// depend on its neighbours in a tile).
-__global__ __launch_bounds__(256) void block_scatter_kernel(const BlockArgs a) {
-  extern __shared__ int hist[];
-  const BlockShape& s = a.s;
-  const int seg = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-  const int plane = seg / a.segs, b = plane / s.kv, g = plane % s.kv;
-  const int i0 = seg % a.segs * a.span, i1 = min(i0 + a.span, s.tq);
-  const int from = i0 + chunk * kChunk, to = min(from + kChunk, i1);
-  const int* place = a.counts + ((long long)seg * a.chunks + chunk) * s.blocks;
-  for (int j = threadIdx.x; j < s.blocks; j += 256) hist[j] = place[j];
+  if (chunk == 0 && threadIdx.x == 0) a.tile_count[seg] = base.y;
   __syncthreads();
   int* list = a.list + (long long)seg * a.span * s.selected;
-  const int pairs = max(to - from, 0) * s.selected;
-  for (int t = threadIdx.x; t < pairs; t += 256) {
-    const int d = t / s.selected, i = from + d;
-    const int j = list_of(a, b, i, g)[t - d * s.selected];
-    if (block_seen(a, j, visible(a, b, i))) list[atomicAdd(&hist[j], 1)] = (i - i0) * s.selected + t - d * s.selected;
-  }
+  for_pairs(a, seg, chunk, [&](int pair, int j) { list[atomicAdd(&hist[j], 1)] = pair; });
 }
 
 // ---------------------------------------------------------------------- tiles
@@ -206,12 +221,16 @@ __device__ __forceinline__ void mfma_parts(const bf16x8 (&a)[3], const bf16x8 (&
   rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[1], rest, 0, 0, 0);
 }
 
-// One tile: up to 64 keys of a block, up to 128 rows.
+// Work item of a workgroup: each of the 8 XCDs takes workgroups in turn, and with them one eighth of the items in a
+// row, so that tiles of one block and the queries of one head meet in one L2.
+__device__ __forceinline__ unsigned item_of(unsigned block, unsigned grid) { return (block & 7) * (grid >> 3) + (block >> 3); }
+
+// One tile: up to 64 keys of a block and a.rows rows of its list, 32 at a time for each of W waves.
 //
-// Keys, then values, stand in LDS as three bf16 parts (Henry, Tang and Heinecke, 2019: a float's 24 bits over
-// its whole exponent range, six of the nine part products taken), in the order in which the matrix
-// instruction's lanes take them, so that a fragment is one 16-byte read without bank conflicts.  The values' loads are
-// under way while the keys are multiplied, and take the keys' place afterwards.
+// Keys and values stand in LDS as three bf16 parts (Henry, Tang and Heinecke, 2019: a float's 24 bits over its whole
+// exponent range, six of the nine part products taken), in the order in which the matrix instruction's lanes
+// take them, so that a fragment is one 16-byte read without bank conflicts.  Once they stand there the waves run on
+// their own: no barrier, the next rows' queries under way while the weights meet the values.
 //
 // S^T = K Q^T: a lane holds one row's scores (keys 8 (r / 4) + 4 half + r % 4), so maximum and sum are in-lane
 // but for one exchange, and the weights are already the A operand of O = P V under the key order
@@ -220,205 +239,319 @@ __device__ __forceinline__ void mfma_parts(const bf16x8 (&a)[3], const bf16x8 (&
 //
 // The maximum m is the largest score times c = scale log2(e), rounded once; weights are 2^(s c - m) with one
 // rounding of the exponent, and m is kept as it is, so that slots join exactly.
-template <int KS, int DT>
-__global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(const BlockArgs a) {
-  constexpr int KF = 2 * KS * 3, VF = 4 * DT * 3;         // fragments of 64 lanes x 16 bytes
-  constexpr int KI = (kKeys * KS * 2 + 255) / 256;        // 8-channel pieces of keys per thread
-  constexpr int VI = (8 * 32 * DT + 255) / 256;           // 8-key pieces of values per thread
-  __shared__ u32x4 frag[(KF > VF ? KF : VF) * 64];
-  __shared__ int token[kKeys];
-  __shared__ int place[kRows];
+template <int KS, int DT, int W>
+__global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(const BlockArgs a) {
+  constexpr int T = 64 * W;
+  constexpr int KF = 2 * KS * 3, VF = 4 * DT * 3;  // fragments of 64 lanes x 16 bytes
+  constexpr int KI = kKeys * KS * 2 / T;           // 8-channel pieces of keys per thread
+  constexpr int VI = 8 * 32 * DT / T;              // 8-key pieces of values per thread
+  __shared__ u32x4 frag[(KF + VF) * 64];
+  __shared__ unsigned k_at[kKeys], v_at[kKeys];    // floats from the block's first key
+  __shared__ unsigned place[W][32];
   const BlockShape& s = a.s;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, r32 = lane & 31;
 
-  // The tile: block, part of it, rows.
-  int seg, j, part, row0, rows, from = 0, pair = 0;
-  if (a.sorted) {
-    seg = blockIdx.x / a.tile_cap;
-    const int t = blockIdx.x - seg * a.tile_cap;
-    seg += a.first;
-    if (t >= a.tile_count[seg]) return;
-    const int4 rec = a.tiles[(long long)seg * a.tile_cap + t];
-    j = rec.x;
-    part = rec.y & 255;
-    row0 = (rec.y >> 8) * kRows;
-    from = rec.z;
-    rows = rec.w * s.group;
-  } else {
-    int t = blockIdx.x;
-    part = t % a.parts;
-    t /= a.parts;
-    row0 = t % a.row_tiles * kRows;
-    t /= a.row_tiles;
-    pair = t % (a.span * s.selected);
-    seg = a.first + t / (a.span * s.selected);
-    rows = s.group;
-  }
-  const int plane = seg / a.segs, b = plane / s.kv, g = plane - b * s.kv;
-  const int i0 = seg % a.segs * a.span;
-  if (!a.sorted) {
-    const int i = i0 + pair / s.selected;
-    if (i >= s.tq) return;
-    j = list_of(a, b, i, g)[pair % s.selected];
-    if (!block_seen(a, j, visible(a, b, i))) return;
-  }
+  const unsigned item = item_of(blockIdx.x, gridDim.x);
+  int seg = item / a.tile_cap;
+  const int t = item - seg * a.tile_cap;
+  if (seg >= a.now) return;
+  seg += a.first;
+  if (t >= a.tile_count[seg]) return;
+  const int4 rec = a.tiles[(long long)seg * a.tile_cap + t];
+  const int j = rec.x, part = rec.y & 255, row0 = (rec.y >> 8) * a.rows;
+  const int rows = min(rec.w * s.group - row0, a.rows);
+  const int plane = seg / a.segs, b = plane / s.kv, g = plane - b * s.kv, i0 = (seg - plane * a.segs) * a.span;
+  const int* list = a.list + (long long)seg * a.span * s.selected + rec.z;
   const int y0 = j / s.bx * s.bh, x0 = j % s.bx * s.bw;
   const int cols = min(s.bw, s.kw - x0), size = min(s.bh, s.kh - y0) * cols;
   const int origin = y0 * s.kw + x0;
   // Keys of this part that exist: in the window and, in a sequence, before its end.
-  int keys = size;
-  if (a.lengths) keys = min(keys, min(max(a.lengths[b], 0), s.tk) - origin);
+  const int length = a.lengths ? min(max(a.lengths[b], 0), s.tk) : s.tk;
+  const long long start = a.starts ? a.starts[b] : 0;
+  int keys = a.lengths ? min(size, length - origin) : size;
   keys = min(max(keys - part * kKeys, 0), kKeys);
-  if (tid < kKeys) {
-    const int t = tid < keys ? part * kKeys + tid : 0;
-    token[tid] = origin + t / cols * s.kw + t % cols;
-  }
 
-  // The lane's row.
-  const int row = row0 + wave * 32 + r32;
-  const bool mine = row < rows, busy = row0 + wave * 32 < rows;
-  int i = 0, h = 0, limit = 0, at = -1;
-  {
-    const int rr = min(row, rows - 1), e = rr / s.group;
-    h = rr - e * s.group;
-    const int id = a.sorted ? a.list[(long long)seg * a.span * s.selected + from + e] : pair;
-    const int d = id / s.selected;
-    i = i0 + d;
-    at = (((seg - a.first) * a.span + d) * s.selected + id - d * s.selected) * a.parts + part;
-    limit = keys;
-    if (s.causal) limit = min(limit, visible(a, b, i) - origin - part * kKeys);
-    if (half == 0) place[wave * 32 + r32] = mine ? at * s.group + h : -1;
-  }
-  __syncthreads();
-
-  // Loads: queries, keys, values.
-  const float* kb = a.k + (long long)b * s.tk * a.ldk + (long long)g * s.ks;
-  const float* vb = a.v + (long long)b * s.tk * a.ldv + (long long)g * s.vs;
-  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  f32x4 kr[KI][2];
-  float vr[VI][8];
-#pragma unroll
-  for (int n = 0; n < KI; ++n) {
-    const int x = tid + 256 * n, key = x / (2 * KS), c = 8 * (x - key * 2 * KS);
-    const float* p = kb + token[key & (kKeys - 1)] * a.ldk + c;
-    kr[n][0] = c < s.kd ? *(const f32x4*)p : zero;
-    kr[n][1] = c + 4 < s.kd ? *(const f32x4*)(p + 4) : zero;
-  }
+  // The lane's row in the wave's turn r: its query, the keys it sees, where its results go.
+  const float* qb = a.q + ((long long)b * s.tq + i0) * a.ldq + (long long)g * s.group * s.qs + 8 * half;
+  auto pair_of = [&](int r) { return list[min(row0 + min(r + r32, rows - 1), rec.w * s.group - 1) / s.group]; };
   f32x4 qr[KS][2];
-  {
-    const float* p = a.q + ((long long)b * s.tq + i) * a.ldq + ((long long)g * s.group + h) * s.qs + 8 * half;
+  int limit;
+  unsigned to;  // row of the results
+  auto load_q = [&](int r, int pair) __attribute__((always_inline)) {
+    const int x = row0 + min(r + r32, rows - 1), h = x % s.group, d = pair / s.selected;
+    limit = keys;
+    if (s.causal) {
+      const long long end = min((long long)length, max(start + i0 + d + 1, 0LL));
+      limit = min(keys, (int)end - origin - part * kKeys);
+    }
+    const unsigned slot = (unsigned)((seg - a.first) * a.span * s.selected + pair) * a.parts + part;
+    to = r + r32 < rows ? slot * s.group + h : a.trash;
+    const float* p = qb + (long long)d * a.ldq + h * s.qs;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) qr[ks][u] = 16 * ks + 8 * half + 4 * u < s.kd ? *(const f32x4*)(p + 16 * ks + 4 * u) : zero;
+      for (int u = 0; u < 2; ++u) {
+        const int c = 16 * ks + 4 * u;
+        qr[ks][u] = c + 8 * half < s.kd ? *(const f32x4*)(p + c) : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+  };
+  int r = wave * 32;
+  int pair = pair_of(r);
+  if (tid < kKeys) {
+    const int u = tid < keys ? part * kKeys + tid : 0, y = u / cols;
+    k_at[tid] = (y * s.kw + u - y * cols) * (unsigned)a.ldk;
+    v_at[tid] = (y * s.kw + u - y * cols) * (unsigned)a.ldv;
   }
-#pragma unroll
-  for (int n = 0; n < VI; ++n) {
-    const int x = tid + 256 * n, c = x % (32 * DT), piece = x / (32 * DT);  // piece: 2 st + half
-    const int first = 16 * (piece >> 1) + 4 * (piece & 1);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int key = first + 8 * (e >> 2) + (e & 3);
-      const float v = vb[token[key] * a.ldv + min(c, s.hd - 1)];
-      vr[n][e] = key < keys ? v : 0.f;
-    }
-  }
+  __syncthreads();
 
-  // Keys into LDS: piece c of key t is lanes t % 32 + 32 (c % 2) of step c / 2.
+  {
+    const float* kb = a.k + ((long long)b * s.tk + origin) * a.ldk + (long long)g * s.ks;
+    const float* vb = a.v + ((long long)b * s.tk + origin) * a.ldv + (long long)g * s.vs;
+    float kr[KI][8], vr[VI][8];
 #pragma unroll
-  for (int n = 0; n < KI; ++n) {
-    const int x = tid + 256 * n, key = x / (2 * KS), c = x - key * 2 * KS;
-    if (KI * 256 == kKeys * KS * 2 || key < kKeys) {
+    for (int n = 0; n < KI; ++n) {
+      const int x = tid + T * n, key = x / (2 * KS), c = 8 * (x - key * 2 * KS);
+      const float* p = kb + (k_at[key] + c);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const f32x4 f = c + 4 * u < s.kd ? *(const f32x4*)(p + 4 * u) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kr[n][4 * u + e] = f[e];
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < VI; ++n) {
+      const int x = tid + T * n, c = min(x % (32 * DT), s.hd - 1), piece = x / (32 * DT);  // piece: 2 step + half
+      const int first = 16 * (piece >> 1) + 4 * (piece & 1);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) vr[n][e] = vb[v_at[first + 8 * (e >> 2) + (e & 3)] + c];
+    }
+    load_q(r, pair);
+    // Piece c of key t: lanes t % 32 + 32 (c % 2) of step c / 2, turned by c so that a thread group's writes meet
+    // different banks.
+#pragma unroll
+    for (int n = 0; n < KI; ++n) {
+      const int x = tid + T * n, key = x / (2 * KS), c = x - key * 2 * KS;
       bf16x8 p[3];
-      const float f[8] = {kr[n][0][0], kr[n][0][1], kr[n][0][2], kr[n][0][3], kr[n][1][0], kr[n][1][1], kr[n][1][2], kr[n][1][3]};
-      parts8(f, p);
+      parts8(kr[n], p);
 #pragma unroll
       for (int m = 0; m < 3; ++m)
-        frag[(((key >> 5) * KS + (c >> 1)) * 3 + m) * 64 + (c & 1) * 32 + (key & 31)] = __builtin_bit_cast(u32x4, p[m]);
+        frag[(((key >> 5) * KS + (c >> 1)) * 3 + m) * 64 + (c & 1) * 32 + ((key + c) & 31)] = __builtin_bit_cast(u32x4, p[m]);
+    }
+    // Keys that do not exist weigh nothing, whatever stands there.
+    if (keys < kKeys)
+#pragma unroll
+      for (int n = 0; n < VI; ++n) {
+        const int piece = (tid + T * n) / (32 * DT), first = 16 * (piece >> 1) + 4 * (piece & 1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (first + 8 * (e >> 2) + (e & 3) >= keys) vr[n][e] = 0.f;
+      }
+#pragma unroll
+    for (int n = 0; n < VI; ++n) {
+      const int x = tid + T * n, c = x % (32 * DT), piece = x / (32 * DT);
+      bf16x8 p[3];
+      parts8(vr[n], p);
+#pragma unroll
+      for (int m = 0; m < 3; ++m)
+        frag[KF * 64 + (((piece >> 1) * DT + (c >> 5)) * 3 + m) * 64 + (piece & 1) * 32 + (c & 31)] =
+            __builtin_bit_cast(u32x4, p[m]);
     }
   }
   __syncthreads();
 
-  float w[32];
-  float mx = -INFINITY, sum = 0.f;
-  if (busy) {
+  const float c = s.scale * 1.4426950408889634f;
+  for (; r < rows; r += 32 * W) {
+    const int next = pair_of(r + 32 * W < rows ? r + 32 * W : r);
     f32x16 sc[2], rest[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[t][r] = rest[t][r] = 0.f;
+      for (int x = 0; x < 16; ++x) sc[t][x] = rest[t][x] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       bf16x8 q[3];
-      const float f[8] = {qr[ks][0][0], qr[ks][0][1], qr[ks][0][2], qr[ks][0][3], qr[ks][1][0], qr[ks][1][1], qr[ks][1][2], qr[ks][1][3]};
+      const float f[8] = {qr[ks][0][0], qr[ks][0][1], qr[ks][0][2], qr[ks][0][3],
+                          qr[ks][1][0], qr[ks][1][1], qr[ks][1][2], qr[ks][1][3]};
       parts8(f, q);
+      const int at = half * 32 + ((r32 + 2 * ks + half) & 31);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         bf16x8 k[3];
 #pragma unroll
-        for (int m = 0; m < 3; ++m) k[m] = __builtin_bit_cast(bf16x8, frag[((t * KS + ks) * 3 + m) * 64 + lane]);
+        for (int m = 0; m < 3; ++m) k[m] = __builtin_bit_cast(bf16x8, frag[((t * KS + ks) * 3 + m) * 64 + at]);
         mfma_parts(k, q, sc[t], rest[t]);
       }
     }
-    const float c = s.scale * 1.4426950408889634f;
+    const int seen = limit;
+    const unsigned mine = to;
+    const bool on = r + r32 < rows;
+    if (half == 0) place[wave][r32] = mine * (unsigned)s.hd;
+    if (r + 32 * W < rows) load_q(r + 32 * W, next);
+    float w[32];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float x = sc[t][r] + rest[t][r];
-        w[16 * t + r] = 32 * t + 8 * (r >> 2) + 4 * half + (r & 3) < limit ? x : -INFINITY;
-        mx = fmaxf(mx, w[16 * t + r]);
-      }
+      for (int x = 0; x < 16; ++x) w[16 * t + x] = sc[t][x] + rest[t][x];
+    if (__any(seen < kKeys))
+#pragma unroll
+      for (int x = 0; x < 32; ++x)
+        if (8 * (x >> 2) + 4 * half + (x & 3) >= seen) w[x] = -INFINITY;
+    float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < 32; ++x) mx = fmaxf(mx, w[x]);
     mx = fmaxf(mx, __shfl_xor(mx, 32)) * c;
     const float base = mx == -INFINITY ? 0.f : mx;  // no key, or none that weighs
 #pragma unroll
-    for (int r = 0; r < 32; ++r) {
-      w[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[r], c, -base));
-      sum += w[r];
+    for (int x = 0; x < 32; ++x) {
+      w[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[x], c, -base));
+      sum += w[x];
     }
     sum += __shfl_xor(sum, 32);
-  }
-  __syncthreads();
-
-#pragma unroll
-  for (int n = 0; n < VI; ++n) {
-    const int x = tid + 256 * n, c = x % (32 * DT), piece = x / (32 * DT);
-    bf16x8 p[3];
-    parts8(vr[n], p);
-#pragma unroll
-    for (int m = 0; m < 3; ++m)
-      frag[(((piece >> 1) * DT + (c >> 5)) * 3 + m) * 64 + (piece & 1) * 32 + (c & 31)] = __builtin_bit_cast(u32x4, p[m]);
-  }
-  __syncthreads();
-  if (!busy) return;
-
-  bf16x8 wp[4][3];
-#pragma unroll
-  for (int st = 0; st < 4; ++st) {
-    const float f[8] = {w[8 * st], w[8 * st + 1], w[8 * st + 2], w[8 * st + 3], w[8 * st + 4], w[8 * st + 5], w[8 * st + 6], w[8 * st + 7]};
-    parts8(f, wp[st]);
-  }
-  if (half == 0 && mine) a.stat[place[wave * 32 + r32]] = make_float2(mx, sum);
-#pragma unroll
-  for (int d = 0; d < DT; ++d) {
-    if (32 * d >= s.hd) break;
-    f32x16 acc, rest;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[r] = rest[r] = 0.f;
+    if (half == 0 && on) a.stat[mine] = make_float2(mx, sum);
+    bf16x8 wp[4][3];
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
-      bf16x8 v[3];
-#pragma unroll
-      for (int m = 0; m < 3; ++m) v[m] = __builtin_bit_cast(bf16x8, frag[((st * DT + d) * 3 + m) * 64 + lane]);
-      mfma_parts(wp[st], v, acc, rest);
+      const float f[8] = {w[8 * st],     w[8 * st + 1], w[8 * st + 2], w[8 * st + 3],
+                          w[8 * st + 4], w[8 * st + 5], w[8 * st + 6], w[8 * st + 7]};
+      parts8(f, wp[st]);
     }
-    const int c = 32 * d + r32;
+    __builtin_amdgcn_wave_barrier();
+    unsigned row_at[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int to = place[wave * 32 + 8 * (r >> 2) + 4 * half + (r & 3)];
-      if (to >= 0 && c < s.hd) a.part[(long long)to * s.hd + c] = acc[r] + rest[r];
+    for (int x = 0; x < 16; ++x) row_at[x] = place[wave][8 * (x >> 2) + 4 * half + (x & 3)] + r32;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      if (32 * d >= s.hd) break;
+      f32x16 acc, rs;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) acc[x] = rs[x] = 0.f;
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        bf16x8 v[3];
+#pragma unroll
+        for (int m = 0; m < 3; ++m) v[m] = __builtin_bit_cast(bf16x8, frag[KF * 64 + ((st * DT + d) * 3 + m) * 64 + lane]);
+        mfma_parts(wp[st], v, acc, rs);
+      }
+      if (32 * d + r32 < s.hd)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) a.part[row_at[x] + 32 * d] = acc[x] + rs[x];
     }
+  }
+}
+
+// ------------------------------------------------------------------ few queries
+
+constexpr int kFewRows = 4;
+
+// One (query, slot) pair and part of its block per workgroup, in plain float32: the keys are read once, for the few
+// heads that share them, and the time is their way from memory.  Four lanes score a key (16 keys to a wave), then
+// a lane takes two channels over the same 16 keys; the four waves' results meet in LDS.
+template <int KS>
+__global__ __launch_bounds__(256) void block_few_kernel(const BlockArgs a) {
+  __shared__ float weight[kFewRows][kKeys], q[kFewRows][128], out[4][kFewRows][128];
+  const BlockShape& s = a.s;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int x = blockIdx.x;
+  const int part = x % a.parts;
+  x /= a.parts;
+  const int pair = x % (a.span * s.selected), ls = x / (a.span * s.selected);
+  const int seg = a.first + ls, plane = seg / a.segs, b = plane / s.kv, g = plane - b * s.kv;
+  const int i = seg % a.segs * a.span + pair / s.selected;
+  if (i >= s.tq) return;
+  const int end = visible(a, b, i), j = list_of(a, b, i, g)[pair % s.selected];
+  if (!block_seen(a, j, end)) return;
+  const int y0 = j / s.bx * s.bh, x0 = j % s.bx * s.bw;
+  const int cols = min(s.bw, s.kw - x0), size = min(s.bh, s.kh - y0) * cols;
+  const int origin = y0 * s.kw + x0;
+  const int keys = min(max(min(size, s.kh > 1 ? size : end - origin) - part * kKeys, 0), kKeys);
+  const long long slot = ((long long)(ls * a.span * s.selected) + pair) * a.parts + part;
+  auto token = [&](int t) {
+    const int u = t < keys ? part * kKeys + t : 0, y = u / cols;
+    return (long long)b * s.tk + origin + y * s.kw + u - y * cols;
+  };
+  // A quarter key's channels 16 n + 4 (lane % 4) .. + 3; two channels of the wave's 16 keys.
+  const int key = wave * 16 + (lane >> 2), quarter = 4 * (lane & 3);
+  f32x4 k[KS];
+  f32x2v v[16];
+  {
+    const float* p = a.k + token(key) * a.ldk + (long long)g * s.ks + quarter;
+#pragma unroll
+    for (int n = 0; n < KS; ++n) k[n] = 16 * n + quarter < s.kd ? *(const f32x4*)(p + 16 * n) : f32x4{0.f, 0.f, 0.f, 0.f};
+    const float* vb = a.v + (long long)g * s.vs + min(2 * lane, s.hd - 2);
+#pragma unroll
+    for (int t = 0; t < 16; ++t) v[t] = *(const f32x2v*)(vb + token(wave * 16 + t) * a.ldv);
+  }
+  const float c = s.scale * 1.4426950408889634f;
+  for (int h0 = 0; h0 < s.group; h0 += kFewRows) {
+    const int heads = min(kFewRows, s.group - h0);
+    __syncthreads();
+    for (int u = tid; u < kFewRows * 128; u += 256) {
+      const int h = u >> 7, ch = u & 127;
+      q[h][ch] = h < heads && ch < s.kd
+                     ? a.q[((long long)b * s.tq + i) * a.ldq + (long long)(g * s.group + h0 + h) * s.qs + ch]
+                     : 0.f;
+    }
+    __syncthreads();
+    float sc[kFewRows];
+#pragma unroll
+    for (int h = 0; h < kFewRows; ++h) sc[h] = 0.f;
+#pragma unroll
+    for (int n = 0; n < KS; ++n)
+#pragma unroll
+      for (int h = 0; h < kFewRows; ++h) {
+        const f32x4 f = *(const f32x4*)&q[h][16 * n + quarter];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[h] = __builtin_fmaf(k[n][e], f[e], sc[h]);
+      }
+#pragma unroll
+    for (int h = 0; h < kFewRows; ++h) {
+      sc[h] += __shfl_xor(sc[h], 1);
+      sc[h] += __shfl_xor(sc[h], 2);
+    }
+    if ((lane & 3) == 0)
+#pragma unroll
+      for (int h = 0; h < kFewRows; ++h) weight[h][key] = key < keys ? sc[h] : -INFINITY;
+    __syncthreads();
+    float mx[kFewRows], sum[kFewRows], w[kFewRows];
+#pragma unroll
+    for (int h = 0; h < kFewRows; ++h) {
+      const float x = weight[h][lane];
+      float m = x;
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+      mx[h] = m * c;
+      w[h] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, mx[h] == -INFINITY ? 0.f : -mx[h]));
+      sum[h] = w[h];
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) sum[h] += __shfl_xor(sum[h], off);
+    }
+    f32x2v acc[kFewRows];
+#pragma unroll
+    for (int h = 0; h < kFewRows; ++h) acc[h] = f32x2v{0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+      if (wave * 16 + t >= keys) break;
+#pragma unroll
+      for (int h = 0; h < kFewRows; ++h) {
+        const float p = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w[h]), wave * 16 + t));
+        acc[h][0] = __builtin_fmaf(p, v[t][0], acc[h][0]);
+        acc[h][1] = __builtin_fmaf(p, v[t][1], acc[h][1]);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < kFewRows; ++h) *(f32x2v*)&out[wave][h][2 * lane] = acc[h];
+    __syncthreads();
+    for (int u = tid; u < heads * s.hd; u += 256) {
+      const int h = u / s.hd, ch = u - h * s.hd;
+      a.part[(slot * s.group + h0 + h) * s.hd + ch] = (out[0][h][ch] + out[1][h][ch]) + (out[2][h][ch] + out[3][h][ch]);
+    }
+    if (tid == 0)
+#pragma unroll
+      for (int h = 0; h < kFewRows; ++h)
+        if (h < heads) a.stat[slot * s.group + h0 + h] = make_float2(mx[h], sum[h]);
   }
 }
 
@@ -426,7 +559,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(
 
 // One row in plain float32 by one wave, weights normalised before they meet the values so that no finite average
 // overflows.  A lane scores one key of 64 and holds channels lane and lane + 64.
-__device__ __attribute__((noinline)) void block_row(const BlockArgs& a, int b, int i, int h, int lane, float (&y)[2]) {
+__device__ __forceinline__ void block_row(const BlockArgs& a, int b, int i, int h, int lane, float (&y)[2]) {
   const BlockShape& s = a.s;
   const int g = h / s.group, end = visible(a, b, i);
   const float* q = a.q + ((long long)b * s.tq + i) * a.ldq + (long long)h * s.qs;
@@ -478,52 +611,73 @@ __device__ __attribute__((noinline)) void block_row(const BlockArgs& a, int b, i
   y[1] = acc[1];
 }
 
-// Joins the slots of each row: lanes of 4 channels, L of them to a row.  A row that comes out infinite or NaN
-// (operands that are, sums that overflow, parts of hidden keys that are not finite) is computed again in plain
-// float32.
+// Joins the slots of each row: L lanes of 4 channels to a row.  The lanes first take a slot each (which block it
+// names, its statistics), then all of them go through the slots' values, whose loads depend on nothing.  A row
+// that comes out infinite or NaN (operands that are, sums that overflow, hidden keys of a tile that are not
+// finite) is computed again in plain float32.
 template <int L>
 __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long long rows) {
   const BlockShape& s = a.s;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, sub = lane & (L - 1), c = 4 * sub;
   const long long row = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;  // (segment, query, head of the group)
-  const int c = 4 * (threadIdx.x % L);
-  const int h = (int)(row % s.group), d = (int)(row / s.group % a.span), ls = (int)(row / s.group / a.span);
+  const int h = (int)(row % s.group);
+  const long long query = row / s.group;
+  const int d = (int)(query % a.span), ls = (int)(query / a.span);
   const int seg = a.first + ls, plane = seg / a.segs, b = plane / s.kv, g = plane - b * s.kv;
   const int i = seg % a.segs * a.span + d;
   const bool live = row < rows && i < s.tq;
-  bool again = false, any = false;
+  const int* list = list_of(a, live ? b : 0, live ? i : 0, live ? g : 0);
+  const int end = live ? visible(a, b, i) : 0, slots = s.selected * a.parts;
+  const long long first = live ? (query * slots) * s.group + h : 0;
+  const float* part = a.part + first * s.hd + min(c, s.hd - 4);
+  float top = -INFINITY, sum = 0.f;
+  bool any = false;
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
-  if (live) {
-    const int* list = list_of(a, b, i, g);
-    const int end = visible(a, b, i);
-    const long long slot0 = ((long long)ls * a.span + d) * s.selected;
-    float mx = -INFINITY, sum = 0.f;
-    for (int n = 0; n < s.selected; ++n) {
-      if (!block_seen(a, list[n], end)) continue;
-      any = true;
-      for (int p = 0; p < a.parts; ++p) mx = fmaxf(mx, a.stat[((slot0 + n) * a.parts + p) * s.group + h].x);
-    }
-    for (int n = 0; n < s.selected; ++n) {
-      if (!block_seen(a, list[n], end)) continue;
-      for (int p = 0; p < a.parts; ++p) {
-        const long long r = ((slot0 + n) * a.parts + p) * s.group + h;
-        const float2 st = a.stat[r];
-        const float f = st.x == -INFINITY && !(st.y != st.y) ? 0.f : __builtin_amdgcn_exp2f(st.x - mx);
-        sum = __builtin_fmaf(st.y, f, sum);
-        if (c < s.hd) {
-          const f32x4 v = *(const f32x4*)(a.part + r * s.hd + c);
+  for (int n0 = 0; n0 < slots; n0 += L) {
+    const int n = n0 + sub;
+    const bool on = n < slots && block_seen(a, list[min(n, slots - 1) / a.parts], end);
+    any |= on;
+    float2 st = make_float2(-INFINITY, 0.f);
+    if (on) st = a.stat[first + (long long)n * s.group];
+    float mx = st.x;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(v[e], f, y[e]);
-        }
+    for (int off = 1; off < L; off <<= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
+    mx = fmaxf(mx, top);
+    // Negative: there is nothing to read.  A slot without weight is read all the same: a NaN in it is the row's.
+    const float f = !on ? -1.f : st.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.x - mx);
+    const float old = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - mx);
+    top = mx;
+    sum = __builtin_fmaf(sum, old, st.y * f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] *= old;
+    const int count = min(L, slots - n0);
+    for (int u0 = 0; u0 < count; u0 += 8) {
+      f32x4 v[8];
+      float w[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        w[u] = __shfl(f, (lane & ~(L - 1)) + min(u0 + u, L - 1));
+        v[u] = *(const f32x4*)(part + (long long)min(n0 + u0 + u, slots - 1) * s.group * s.hd);
       }
-    }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      y[e] = any ? y[e] / sum : 0.f;
-      again |= c < s.hd && !(__builtin_fabsf(y[e]) <= FLT_MAX);
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (u0 + u < count) y[e] = w[u] < 0.f ? y[e] : __builtin_fmaf(v[u][e], w[u], y[e]);
     }
-    if (c < s.hd) *(f32x4*)(a.o + ((long long)b * s.tq + i) * a.ldo + (long long)(g * s.group + h) * s.hd + c) = y;
   }
+#pragma unroll
+  for (int off = 1; off < L; off <<= 1) {
+    sum += __shfl_xor(sum, off);
+    any = any | (bool)__shfl_xor((int)any, off);
+  }
+  bool again = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    y[e] = any ? y[e] / sum : 0.f;
+    again |= live && c < s.hd && !(__builtin_fabsf(y[e]) <= FLT_MAX);
+  }
+  if (live && c < s.hd) *(f32x4*)(a.o + ((long long)b * s.tq + i) * a.ldo + (long long)(g * s.group + h) * s.hd + c) = y;
   for (unsigned long long todo = __ballot(again); todo;) {
     const int from = __builtin_ctzll(todo) & ~(L - 1);
     const int rb = __shfl(b, from), ri = __shfl(i, from), rh = __shfl(g * s.group + h, from);
@@ -533,12 +687,18 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       if (lane + 64 * e < s.hd) o[lane + 64 * e] = z[e];
-    todo &= ~((L == 64 ? ~0ull : (1ull << L) - 1) << from);
+    todo &= ~(((1ull << L) - 1) << from);
   }
 }
 
 // Bytes of results that one launch leaves and the next one joins.
-constexpr double kPartials = 96e6;
+#ifndef SORT_FROM
+#define SORT_FROM 64
+#endif
+#ifndef KP
+#define KP 768e6
+#endif
+constexpr double kPartials = KP;
 
 int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q, const sy_tensor* k,
                        const sy_tensor* v, const int32_t* blocks, const int32_t* starts, const int32_t* lengths,
@@ -589,14 +749,22 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   a.segs = (s.tq + a.span - 1) / a.span;
   const long long segments = (long long)planes * a.segs;
   const int together = (int)std::min<double>((double)segments, std::max(1.0, std::floor(kPartials / (per_query * a.span))));
-  a.row_tiles = (s.group + kRows - 1) / kRows;
-  a.sorted = s.blocks <= kMaxBlocks && (long long)s.tq * s.selected > 64;
-  a.chunks = (a.span + kChunk - 1) / kChunk;
-  a.tile_cap = (int)std::min<long long>(
-      a.parts * (std::min<long long>(s.blocks, (long long)a.span * s.selected) + (long long)a.span * s.selected * s.group / kRows + 1),
-      0x7fffffff);
-  const long long result_rows = (long long)together * a.span * s.selected * a.parts * s.group;
-  SY_CHECK(result_rows < (1LL << 31), SY_EUNSUPPORTED, "block attention over %d heads to a key head", s.group);
+  const bool sorted = s.blocks <= kMaxBlocks && (long long)s.tq * s.selected > SORT_FROM;
+  // Rows of a tile: many, so that the keys are laid out seldom, but four rounds of tiles on the whole chip.
+  a.rows = 1024;
+  while (a.rows > 256 && (double)together * a.span * s.selected * a.parts * s.group < 4096.0 * a.rows) a.rows /= 2;
+  // 2048 pairs to a workgroup of the sort, but at most 32 of them to a segment (each reads all their counts).
+  a.chunk = std::max(std::max(1, 2048 / s.selected), (a.span + 31) / 32);
+  a.chunks = (a.span + a.chunk - 1) / a.chunk;
+  const long long pairs = (long long)a.span * s.selected;
+  const long long tile_cap = a.parts * (std::min<long long>(s.blocks, pairs) + pairs * s.group / a.rows + 1);
+  const long long result_rows = together * pairs * a.parts * s.group;
+  SY_CHECK((result_rows + 1) * s.hd < (1LL << 30) && tile_cap * together < (1LL << 24), SY_EUNSUPPORTED,
+           "block attention over %d heads to a key head", s.group);
+  SY_CHECK((double)s.bh * s.kw * std::max(k->ldc, v->ldc) < 4294967296.0, SY_EUNSUPPORTED,
+           "block windows that span 2^32 floats and more");
+  a.tile_cap = (int)tile_cap;
+  a.trash = (unsigned)result_rows;
   // Scratch: results, then lists.
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -604,11 +772,11 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
     at += (bytes + 255) & ~size_t(255);
     return from;
   };
-  const size_t part_at = take(sizeof(float) * result_rows * s.hd), stat_at = take(sizeof(float2) * result_rows);
-  const size_t count_at = a.sorted ? take(sizeof(int) * segments * a.chunks * s.blocks) : 0;
-  const size_t list_at = a.sorted ? take(sizeof(int) * segments * a.span * s.selected) : 0;
-  const size_t tile_at = a.sorted ? take(sizeof(int4) * segments * a.tile_cap) : 0;
-  const size_t number_at = a.sorted ? take(sizeof(int) * segments) : 0;
+  const size_t part_at = take(sizeof(float) * (result_rows + 1) * s.hd), stat_at = take(sizeof(float2) * result_rows);
+  const size_t count_at = sorted ? take(sizeof(int) * segments * a.chunks * s.blocks) : 0;
+  const size_t list_at = sorted ? take(sizeof(int) * segments * pairs) : 0;
+  const size_t tile_at = sorted ? take(sizeof(int4) * segments * tile_cap) : 0;
+  const size_t number_at = sorted ? take(sizeof(int) * segments) : 0;
   DeviceScope device(ctx);
   SY_TRY(ensure_scratch(ctx, at));
   a.part = (float*)(ctx->scratch + part_at);
@@ -618,32 +786,40 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   a.tiles = (int4*)(ctx->scratch + tile_at);
   a.tile_count = (int*)(ctx->scratch + number_at);
   const double keys = std::min((double)s.selected * s.bh * s.bw, (double)s.tk);
-  if (a.sorted) {
+  if (sorted) {
     ProfScope prof(ctx, "block_sort", 0, 8.0 * s.n * (double)s.tq * s.kv * s.selected);
     const size_t lds = sizeof(int) * s.blocks;
-    const dim3 grid((unsigned)(segments * a.chunks));
-    hipLaunchKernelGGL(block_count_kernel, grid, dim3(256), lds, ctx->stream, a);
-    hipLaunchKernelGGL(block_scan_kernel, dim3((unsigned)segments), dim3(1024), 0, ctx->stream, a);
-    hipLaunchKernelGGL(block_scatter_kernel, grid, dim3(256), lds, ctx->stream, a);
+    const dim3 grid((unsigned)(segments * a.chunks)), threads(kSortThreads);
+    if (a.chunks > 1) hipLaunchKernelGGL(block_count_kernel, grid, threads, lds, ctx->stream, a);
+    hipLaunchKernelGGL(block_scatter_kernel, grid, threads, lds, ctx->stream, a);
     SY_TRY(check_launch("block_sort"));
   }
   for (long long first = 0; first < segments; first += together) {
     const int now = (int)std::min<long long>(together, segments - first);
     const double share = (double)now / segments;
     a.first = (int)first;
+    a.now = now;
     {
       ProfScope prof(ctx, "block_attention", share * 2.0 * s.n * s.tq * s.heads * keys * (s.kd + s.hd),
                      share * 4.0 * s.n * ((double)s.tq * s.heads * (s.kd + s.hd) + (double)s.tk * s.kv * (s.kd + s.hd)));
-      const long long grid = (long long)now * (a.sorted ? a.tile_cap : (long long)a.span * s.selected * a.row_tiles * a.parts);
-      SY_CHECK(grid * 256 < (1LL << 32), SY_EUNSUPPORTED, "block attention grid too large");
-      auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, ctx->stream, a); };
-      auto pick = [&](auto two, auto four) { s.hd <= 64 ? launch(two) : launch(four); };
-      if (s.kd <= 32)
-        pick(block_tile_kernel<2, 2>, block_tile_kernel<2, 4>);
-      else if (s.kd <= 64)
-        pick(block_tile_kernel<4, 2>, block_tile_kernel<4, 4>);
-      else
-        pick(block_tile_kernel<8, 2>, block_tile_kernel<8, 4>);
+      if (sorted) {
+        const unsigned grid = (unsigned)((now * tile_cap + 7) / 8 * 8);
+        auto launch = [&](auto kernel, int waves) {
+          hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * waves), 0, ctx->stream, a);
+        };
+        if (s.kd <= 32)
+          s.hd <= 64 ? launch(block_tile_kernel<2, 2, 4>, 4) : launch(block_tile_kernel<2, 4, 4>, 4);
+        else if (s.kd <= 64)
+          s.hd <= 64 ? launch(block_tile_kernel<4, 2, 4>, 4) : launch(block_tile_kernel<4, 4, 4>, 4);
+        else
+          s.hd <= 64 ? launch(block_tile_kernel<8, 2, 4>, 4) : launch(block_tile_kernel<8, 4, 8>, 8);
+      } else {
+        const dim3 grid((unsigned)(now * pairs * a.parts));
+        if (s.kd <= 64)
+          hipLaunchKernelGGL(block_few_kernel<4>, grid, dim3(256), 0, ctx->stream, a);
+        else
+          hipLaunchKernelGGL(block_few_kernel<8>, grid, dim3(256), 0, ctx->stream, a);
+      }
       SY_TRY(check_launch("block_attention"));
     }
     {
