@@ -3,14 +3,16 @@
 //
 // The choice is made on scores in 64 bits: a product of floats is exact there and 128 of them sum within
 // 2^-46, so it does not hang on the order of a sum as it would in 32 bits.
-#include <cfloat>
+#include <climits>
 #include <cmath>
 
+#include "split.h"
 #include "sy_internal.h"
 
 namespace sy {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // The config alone; the views' part is filled in by the callers.
 int block_shape(const sy_block_config* c, BlockShape* s) {
@@ -169,6 +171,12 @@ int op_block_means(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* k, 
 }
 
 // ----------------------------------------------------------------- selection
+//
+// Many queries: scores in float32 from the matrix cores with a bound e on their error, twice over.  The first pass
+// keeps the largest ones of each query, so that the `selected`-th, t, is known; blocks further than 2 e above t are
+// chosen and those further below are not, whatever the rounding.  The second pass writes the blocks from t - 2 e up.
+// Where more than `selected` lie there, a few queries in a thousand, the query is ranked in 64 bits.
+// Few queries: scores in 64 bits, then a ranking.
 
 struct SelectArgs {
   const float *q, *m;
@@ -176,6 +184,12 @@ struct SelectArgs {
   int* out;
   long long ldq, ldm, rows;
   int tq, blocks, bw, kv, group, kd, qs, selected, causal;
+  // many queries: the means' parts, their largest norm for each of `chunks` of them
+  u32x4* parts;
+  float* norm;
+  int tiles, chunks;
+  // few queries: scores
+  long long* keys;
 };
 
 // 64-bit scores in an order of integers: NaN below every number, zeros alike.
@@ -184,90 +198,459 @@ __device__ __forceinline__ long long score_key(double s) {
   const long long b = __builtin_bit_cast(long long, s + 0.0);
   return b < 0 ? LLONG_MIN + 2 + ~b : b;
 }
-
-constexpr int kSelectChunk = 1024;
 constexpr long long kHidden = LLONG_MIN;
 
-// One wave per query and key head.
-__global__ __launch_bounds__(64) void select_kernel(const SelectArgs a) {
-  __shared__ double qsum[128];
-  __shared__ long long key[kSelectChunk + 64];
-  __shared__ int id[64], best_id[64];
-  __shared__ long long best_key[64];
-  const int lane = threadIdx.x;
-  const long long row = blockIdx.x;
-  const int g = (int)(row % a.kv), i = (int)(row / a.kv % a.tq);
-  const long long b = row / a.kv / a.tq;
-  const float* q = a.q + (b * a.tq + i) * a.ldq + (long long)g * a.group * a.qs;
-  for (int c = lane; c < a.kd; c += 64) {
-    double s = 0;
-    for (int h = 0; h < a.group; ++h) s += q[(long long)h * a.qs + c];
-    qsum[c] = s;
-  }
-  long long seen = a.blocks, forced = -1;  // blocks seen; one that is always taken
+// Blocks that query i of image b sees, and the one that is always taken (-1: none).
+__device__ __forceinline__ int seen_blocks(const SelectArgs& a, int b, int i, int* forced) {
+  long long seen = a.blocks;
+  *forced = -1;
   if (a.lengths) seen = min(seen, ((long long)max(a.lengths[b], 0) + a.bw - 1) / a.bw);
   if (a.causal) {
     const long long at = (long long)(a.starts ? a.starts[b] : 0) + i;
-    seen = at < 0 ? 0 : min(seen, at / a.bw + 1);
-    if (at >= 0 && at / a.bw < seen) forced = at / a.bw;
+    if (at < 0) return 0;
+    const long long own = at / a.bw;
+    if (own < seen) *forced = (int)own;
+    seen = min(seen, own + 1);
   }
+  return (int)seen;
+}
+
+// The largest of a wave's values, in every lane.
+__device__ __forceinline__ int wave_max_i32(int m) {
+  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x111, 0xf, 0xf, false));  // shifts within rows of 16
+  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x112, 0xf, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x114, 0xf, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x118, 0xf, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x142, 0xa, 0xf, false));  // row 0 / 2 into 1 / 3, 1 into 2 and 3
+  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(m, 63);
+}
+
+// Ranking by one wave: of the keys key(j), j < count, the `selected` largest, ties by the lower j.  Lane n ends with the
+// n-th; the number of them is returned.  Every lane keeps four new keys and one of the best so far in order;
+// the largest head of all is taken `selected` times.
+template <class F>
+__device__ __forceinline__ int rank_wave(int count, int selected, int lane, F key, long long* best_key, int* best_id) {
   int kept = 0;
+  long long bk = kHidden;
+  int bi = 0x7fffffff;
+  for (int j0 = 0; j0 < count; j0 += 256) {
+    long long k[5];
+    int id[5];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = j0 + 64 * u + lane;
+      k[u] = j < count ? key(j) : kHidden;
+      id[u] = j;
+    }
+    if (kept == selected) {
+      const long long least = __shfl(bk, selected - 1);
+      if (!__any(max(max(k[0], k[1]), max(k[2], k[3])) > least)) continue;
+    }
+    k[4] = lane < kept ? bk : kHidden;
+    id[4] = lane < kept ? bi : 0x7fffffff;
+#pragma unroll
+    for (int pass = 0; pass < 4; ++pass)
+#pragma unroll
+      for (int u = 4; u > pass; --u) {
+        const bool up = k[u] > k[u - 1] || (k[u] == k[u - 1] && id[u] < id[u - 1]);
+        const long long tk = up ? k[u] : k[u - 1];
+        const int ti = up ? id[u] : id[u - 1];
+        k[u] = up ? k[u - 1] : k[u];
+        id[u] = up ? id[u - 1] : id[u];
+        k[u - 1] = tk;
+        id[u - 1] = ti;
+      }
+    int n = 0;
+    for (; n < selected; ++n) {
+      const int hi = (int)(k[0] >> 32), top_hi = wave_max_i32(hi);
+      const unsigned lo = (unsigned)k[0];
+      // The low half's order as a signed one; lanes with a smaller high half out of it.
+      const int low = hi == top_hi ? (int)(lo ^ 0x80000000u) : INT_MIN, top_lo = wave_max_i32(low);
+      const long long top = (long long)top_hi << 32 | ((unsigned)top_lo ^ 0x80000000u);
+      if (top == kHidden) break;
+      const unsigned long long heads = __ballot(k[0] == top);
+      int winner = __builtin_ctzll(heads);
+      if (heads & (heads - 1)) {
+        const int first = -wave_max_i32(k[0] == top ? -id[0] : INT_MIN);
+        winner = __builtin_ctzll(__ballot(k[0] == top && id[0] == first));
+      }
+      const int won = __builtin_amdgcn_readlane(id[0], winner);
+      if (lane == n) {
+        bk = top;
+        bi = won;
+      }
+      if (lane == winner) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          k[u] = k[u + 1];
+          id[u] = id[u + 1];
+        }
+        k[4] = kHidden;
+        id[4] = 0x7fffffff;
+      }
+    }
+    kept = n;
+  }
+  *best_key = bk;
+  *best_id = lane < kept ? bi : 0x7fffffff;
+  return kept;
+}
+
+// Writes a wave's ranking in ascending order of blocks, then -1.
+__device__ __forceinline__ void write_row(int* out, int selected, int kept, int lane, int id) {
+  int place = 0;
+  for (int n = 0; n < kept; ++n) place += __builtin_amdgcn_readlane(id, n) < id;
+  if (lane < selected) out[lane < kept ? place : lane] = lane < kept ? id : -1;
+}
+
+// The sum of the query heads that share a key head, in 64 bits: channel c.
+__device__ __forceinline__ double query_sum(const SelectArgs& a, const float* q, int c) {
+  double s = 0;
+  for (int h = 0; h < a.group; ++h) s += q[(long long)h * a.qs + c];
+  return s;
+}
+
+// One query in 64 bits by one wave: a lane scores a block of 64.
+__device__ __forceinline__ void select_exact(const SelectArgs& a, int b, int i, int g, int lane, double* qsum) {
+  const float* q = a.q + ((long long)b * a.tq + i) * a.ldq + (long long)g * a.group * a.qs;
+  for (int c = lane; c < a.kd; c += 64) qsum[c] = query_sum(a, q, c);
+  __builtin_amdgcn_wave_barrier();
+  int forced;
+  const int seen = seen_blocks(a, b, i, &forced);
+  long long bk;
+  int bi;
+  const int kept = rank_wave(seen, a.selected, lane, [&](int j) {
+    if (j == forced) return (long long)LLONG_MAX;
+    const float* m = a.m + ((long long)b * a.blocks + j) * a.ldm + g * a.kd;
+    double s = 0;
+    for (int c = 0; c < a.kd; c += 4) {
+      const f32x4 v = *(const f32x4*)(m + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = __builtin_fma(qsum[c + e], (double)v[e], s);
+    }
+    return score_key(s);
+  }, &bk, &bi);
+  write_row(a.out + (((long long)b * a.tq + i) * a.kv + g) * a.selected, a.selected, kept, lane, bi);
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Eight floats as two bf16 parts, v = p[0] + p[1] up to 2^-18 of v.
+__device__ __forceinline__ void halves8(const float (&x)[8], bf16x8 (&p)[2]) {
+  u32x4 w[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f32x2v v = {x[2 * i], x[2 * i + 1]};
+    const unsigned hi = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+    v[0] -= __builtin_bit_cast(float, hi << 16);
+    v[1] -= __builtin_bit_cast(float, hi & 0xffff0000u);
+    w[0][i] = hi;
+    w[1][i] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+  }
+  p[0] = __builtin_bit_cast(bf16x8, w[0]);
+  p[1] = __builtin_bit_cast(bf16x8, w[1]);
+}
+
+constexpr int kPartTiles = 8;  // 32-block tiles of a workgroup below
+
+// The means of one key head as the A operands of the matrix instructions (32 blocks x 16 channels, two parts
+// each), and the largest norm among them.
+template <int KS>
+__global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
+  __shared__ float top[4];
+  const int plane = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, b = plane / a.kv, g = plane % a.kv;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  float most = 0.f;
+  for (int t = wave; t < kPartTiles; t += 4) {
+    const int tile = chunk * kPartTiles + t, j = tile * 32 + (lane & 31);
+    if (tile >= a.tiles) break;
+    const float* m = a.m + ((long long)b * a.blocks + min(j, a.blocks - 1)) * a.ldm + g * a.kd;
+    float norm = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      float f[8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int c = 16 * ks + 8 * half + 4 * u;
+        const f32x4 v = c < a.kd && j < a.blocks ? *(const f32x4*)(m + c) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f[4 * u + e] = v[e];
+          norm = __builtin_fmaf(v[e], v[e], norm);
+        }
+      }
+      bf16x8 p[2];
+      halves8(f, p);
+      u32x4* to = a.parts + (((long long)plane * a.tiles + tile) * KS + ks) * 2 * 64 + lane;
+      to[0] = __builtin_bit_cast(u32x4, p[0]);
+      to[64] = __builtin_bit_cast(u32x4, p[1]);
+    }
+    norm += __shfl_xor(norm, 32);
+    most = norm <= most ? most : norm;  // a NaN stays
+    if (norm != norm) most = norm;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    const float o = __shfl_xor(most, off);
+    most = o <= most || most != most ? most : o;
+  }
+  if (lane == 0) top[wave] = most;
   __syncthreads();
-  for (long long j0 = 0; j0 < seen; j0 += kSelectChunk) {
-    const int count = (int)min((long long)kSelectChunk, seen - j0);
-    for (int t = lane; t < count; t += 64) {
-      const float* m = a.m + (b * a.blocks + j0 + t) * a.ldm + g * a.kd;
-      double s = 0;
-      for (int c = 0; c < a.kd; ++c) s = __builtin_fma(qsum[c], (double)m[c], s);
-      key[kept + t] = j0 + t == forced ? LLONG_MAX : score_key(s);
-    }
-    if (lane < kept) {
-      key[lane] = best_key[lane];
-      id[lane] = best_id[lane];
-    }
-    __syncthreads();
-    // Candidates in ascending order of blocks: the first largest is the one wanted.
-    const int all = kept + count, want = min(a.selected, all);
-    for (int n = 0; n < want; ++n) {
-      long long top = kHidden;
-      int at = 0x7fffffff;
-      for (int t = lane; t < all; t += 64)
-        if (key[t] > top) {
-          top = key[t];
-          at = t;
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 4; ++w) most = top[w] <= most || most != most ? most : top[w];
+    a.norm[blockIdx.x] = most;
+  }
+}
+
+// 32 QT queries of one key head per wave, four waves to a workgroup that share nothing.
+//
+// S^T = M Q^T: a lane holds a query's scores of the blocks 8 (r / 4) + 4 half + r % 4 of a tile.  The SMAX + 1 largest
+// so far stay sorted in registers: a new score moves through them by one median of three each.  (Fewer wanted:
+// the list starts with infinities.)  The two halves' lists meet at the end.
+//
+// Error of a score: a part is off by 2^-9 of what it stands for, so operands by 2^-18 and the product left out by as much,
+// 3 x 2^-18 of sum |q||m|; a sum of at most 24 matrix instructions' results and 16 products within each, below
+// 2^-18; q itself rounded from 64 bits.  sum |q||m| <= |q||m| in norms (off by 2^-15 of themselves, from sums in
+// float32): e = 2^-15.5 |q| max|m|, taken as 2^-15.  Norms outside 2^-40 .. 2^40 could lose parts to
+// underflow: those queries are ranked in 64 bits.
+template <int KS, int SMAX, int QT>
+__global__ __launch_bounds__(256) void select_tile_kernel(const SelectArgs a) {
+  __shared__ double qsum[4][128];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, r32 = lane & 31;
+  const int groups = (a.tq + 128 * QT - 1) / (128 * QT);
+  const int plane = blockIdx.x / groups, b = plane / a.kv, g = plane - b * a.kv;
+  const int i0 = (blockIdx.x - plane * groups) * 128 * QT + wave * 32 * QT;
+  if (i0 >= a.tq) return;
+
+  float kn = 0.f;
+  for (int c = 0; c < a.chunks; ++c) {
+    const float o = a.norm[plane * a.chunks + c];
+    kn = o <= kn || kn != kn ? kn : o;
+  }
+  bf16x8 q[QT][KS][2];
+  float slack[QT];  // 2 e
+  int seen[QT], forced[QT], most = 0;
+  unsigned exact = 0;  // bit t: this lane's query t is ranked in 64 bits
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int i = min(i0 + 32 * t + r32, a.tq - 1);
+    const float* p = a.q + ((long long)b * a.tq + i) * a.ldq + (long long)g * a.group * a.qs + 8 * half;
+    float qn = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      float f[8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int c = 16 * ks + 4 * u;
+        if (c + 8 * half < a.kd) {
+          if (a.group == 1) {
+            const f32x4 v = *(const f32x4*)(p + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[4 * u + e] = v[e];
+          } else {
+            double s[4] = {0, 0, 0, 0};
+            for (int h = 0; h < a.group; ++h) {
+              const f32x4 v = *(const f32x4*)(p + (long long)h * a.qs + c);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[e] += v[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[4 * u + e] = (float)s[e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[4 * u + e] = 0.f;
         }
 #pragma unroll
-      for (int off = 32; off > 0; off >>= 1) {
-        const long long ok = __shfl_xor(top, off);
-        const int oa = __shfl_xor(at, off);
-        if (ok > top || (ok == top && oa < at)) {
-          top = ok;
-          at = oa;
+        for (int e = 0; e < 4; ++e) qn = __builtin_fmaf(f[4 * u + e], f[4 * u + e], qn);
+      }
+      halves8(f, q[t][ks]);
+    }
+    qn += __shfl_xor(qn, 32);
+    const bool fine = qn >= 0x1p-80f && qn <= 0x1p80f && kn >= 0x1p-80f && kn <= 0x1p80f;
+    if (!fine) exact |= 1u << t;
+    slack[t] = 0x1p-14f * (__builtin_sqrtf(qn) * __builtin_sqrtf(kn));
+    seen[t] = seen_blocks(a, b, i, &forced[t]);
+    most = max(most, seen[t]);
+  }
+  const int last = __builtin_amdgcn_readfirstlane((wave_max_i32(most) + 31) / 32);
+  const u32x4* parts = a.parts + (long long)plane * a.tiles * KS * 2 * 64 + lane;
+
+  // Scores of tile n, with what is not seen at -inf and what is forced at +inf.
+  auto scores = [&](int n, f32x16 (&sc)[QT]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[t][r] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const bf16x8 m0 = __builtin_bit_cast(bf16x8, parts[((long long)n * KS + ks) * 128]);
+      const bf16x8 m1 = __builtin_bit_cast(bf16x8, parts[((long long)n * KS + ks) * 128 + 64]);
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m1, q[t][ks][0], sc[t], 0, 0, 0);
+        sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m0, q[t][ks][1], sc[t], 0, 0, 0);
+        sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m0, q[t][ks][0], sc[t], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const int room = seen[t] - 32 * n - 4 * half, own = forced[t] - 32 * n - 4 * half;
+      if (__any(room < 32 || (own >= 0 && own < 32)))
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int at = 8 * (r >> 2) + (r & 3);
+          sc[t][r] = at >= room ? -INFINITY : at == own ? INFINITY : sc[t][r];
+        }
+    }
+  };
+
+  float list[QT][SMAX + 1];
+#pragma unroll
+  for (int t = 0; t < QT; ++t)
+#pragma unroll
+    for (int n = 0; n <= SMAX; ++n) list[t][n] = n < SMAX - a.selected && half == 0 ? INFINITY : -INFINITY;
+  for (int n = 0; n < last; ++n) {
+    f32x16 sc[QT];
+    scores(n, sc);
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      float top = sc[t][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, sc[t][r]);
+      if (!__any(top > list[t][SMAX])) continue;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = sc[t][r];
+#pragma unroll
+        for (int u = SMAX; u > 0; --u) list[t][u] = __builtin_amdgcn_fmed3f(list[t][u - 1], list[t][u], x);
+        list[t][0] = fmaxf(list[t][0], x);
+      }
+    }
+  }
+
+  float from[QT];  // scores from here up are written
+  unsigned count[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    float nth = INFINITY, after = INFINITY;
+    float other[SMAX + 1];
+#pragma unroll
+    for (int n = 0; n <= SMAX; ++n) other[n] = __shfl_xor(list[t][n], 32);
+#pragma unroll
+    for (int n = 0; n < SMAX; ++n) nth = fminf(nth, fmaxf(list[t][n], other[SMAX - 1 - n]));
+#pragma unroll
+    for (int n = 0; n <= SMAX; ++n) after = fminf(after, fmaxf(list[t][n], other[SMAX - n]));
+    from[t] = nth - slack[t];
+    if (seen[t] > a.selected && !(after < from[t])) exact |= 1u << t;
+    count[t] = 0;
+  }
+
+  for (int n = 0; n < last; ++n) {
+    f32x16 sc[QT];
+    scores(n, sc);
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      unsigned m = 0;
+#pragma unroll
+      for (int r = 15; r >= 0; --r) m = m << 1 | (sc[t][r] >= from[t] ? 1u : 0u);
+      if (!__any(m != 0)) continue;
+      m = (m | m << 8) & 0x00ff00ffu;
+      m = (m | m << 4) & 0x0f0f0f0fu;
+      const unsigned o = (unsigned)__shfl_xor((int)m, 32);
+      m = half ? o | m << 4 : m | o << 4;
+      const int room = seen[t] - 32 * n;
+      if (room < 32) m &= room > 0 ? (1u << room) - 1 : 0u;
+      const int i = i0 + 32 * t + r32;
+      int* out = a.out + (((long long)b * a.tq + i) * a.kv + g) * a.selected;
+      while (__any(m != 0)) {
+        if (m) {
+          const int bit = __builtin_ctz(m);
+          m &= m - 1;
+          if (half == 0 && i < a.tq && !(exact >> t & 1) && (int)count[t] < a.selected) out[count[t]] = 32 * n + bit;
+          ++count[t];
         }
       }
-      __syncthreads();
-      if (lane == 0) {
-        best_key[n] = top;
-        best_id[n] = at < kept ? id[at] : (int)(j0 + at - kept);
-        key[at] = kHidden;
-      }
-      __syncthreads();
     }
-    kept = want;
-    // Ascending again.
-    const int mine = lane < kept ? best_id[lane] : 0x7fffffff;
-    const long long mykey = lane < kept ? best_key[lane] : 0;
-    int place = 0;
-    for (int t = 0; t < kept; ++t) place += best_id[t] < mine;
-    __syncthreads();
-    if (lane < kept) {
-      best_id[place] = mine;
-      best_key[place] = mykey;
-    }
-    __syncthreads();
   }
-  if (lane < a.selected) a.out[row * a.selected + lane] = lane < kept ? best_id[lane] : -1;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int i = i0 + 32 * t + r32;
+    int* out = a.out + (((long long)b * a.tq + i) * a.kv + g) * a.selected;
+    if (half == 0 && i < a.tq && !(exact >> t & 1))
+      for (int n = count[t]; n < a.selected; ++n) out[n] = -1;
+    for (unsigned long long todo = __ballot(half == 0 && i < a.tq && (exact >> t & 1)); todo; todo &= todo - 1)
+      select_exact(a, b, i0 + 32 * t + __builtin_ctzll(todo), g, lane, qsum[wave]);
+  }
 }
+
+// Scores of 64 blocks in 64 bits, four lanes to a block, for each of few queries.
+template <int KS>
+__global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
+  __shared__ double qsum[128];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = 4 * (lane & 3);
+  const int chunks = (a.blocks + 63) / 64, plane = blockIdx.x / chunks, b = plane / a.kv, g = plane - b * a.kv;
+  const int j = (blockIdx.x - plane * chunks) * 64 + wave * 16 + (lane >> 2);
+  f32x4 k[KS];
+  const float* m = a.m + ((long long)b * a.blocks + min(j, a.blocks - 1)) * a.ldm + g * a.kd + quarter;
+#pragma unroll
+  for (int n = 0; n < KS; ++n) k[n] = 16 * n + quarter < a.kd ? *(const f32x4*)(m + 16 * n) : f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < a.tq; ++i) {
+    const float* q = a.q + ((long long)b * a.tq + i) * a.ldq + (long long)g * a.group * a.qs;
+    __syncthreads();
+    if (threadIdx.x < 128) qsum[threadIdx.x] = threadIdx.x < a.kd ? query_sum(a, q, threadIdx.x) : 0.0;
+    __syncthreads();
+    int forced;
+    const int seen = seen_blocks(a, b, i, &forced);
+    double s = 0;
+#pragma unroll
+    for (int n = 0; n < KS; ++n)
+      if (16 * n + quarter < a.kd)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = __builtin_fma(qsum[16 * n + quarter + e], (double)k[n][e], s);
+    s += __shfl_xor(s, 1);
+    s += __shfl_xor(s, 2);
+    if ((lane & 3) == 0 && j < a.blocks)
+      a.keys[((long long)plane * a.tq + i) * a.blocks + j] = j >= seen ? kHidden : j == forced ? LLONG_MAX : score_key(s);
+  }
+}
+
+// One query per workgroup: each wave ranks a quarter of its blocks, then every candidate counts those before it.
+__global__ __launch_bounds__(256) void rank_kernel(const SelectArgs a) {
+  __shared__ long long key[256];
+  __shared__ int id[256], chosen[64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long long* keys = a.keys + (long long)blockIdx.x * a.blocks;
+  const int part = (a.blocks + 3) / 4, from = min(wave * part, a.blocks), count = min(part, a.blocks - from);
+  long long bk;
+  int bi;
+  const int kept = rank_wave(count, a.selected, lane, [&](int j) { return keys[from + j]; }, &bk, &bi);
+  key[threadIdx.x] = lane < kept ? bk : kHidden;
+  id[threadIdx.x] = lane < kept ? from + bi : 0x7fffffff;
+  if (threadIdx.x < 64) chosen[threadIdx.x] = 0x7fffffff;
+  __syncthreads();
+  if (lane < kept) {
+    int before = 0;
+    for (int w = 0; w < 4; ++w)
+      for (int n = 0; n < a.selected; ++n) {
+        const long long k = key[64 * w + n];
+        before += k > key[threadIdx.x] || (k == key[threadIdx.x] && id[64 * w + n] < id[threadIdx.x]);
+      }
+    if (before < a.selected) chosen[before] = id[threadIdx.x];
+  }
+  __syncthreads();
+  if (wave == 0) {
+    const int mine = chosen[lane];
+    int place = 0;
+    for (int n = 0; n < a.selected; ++n) place += chosen[n] < mine;
+    const int row = blockIdx.x % a.tq, plane = blockIdx.x / a.tq;  // keys are [plane][query]
+    int* out = a.out + (((long long)(plane / a.kv) * a.tq + row) * a.kv + plane % a.kv) * a.selected;
+    if (lane < a.selected) out[mine != 0x7fffffff ? place : lane] = mine != 0x7fffffff ? mine : -1;
+  }
+}
+
+constexpr int kManyQueries = 16;  // from here on the matrix cores
 
 int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q, const sy_tensor* m,
                     const int32_t* starts, const int32_t* lengths, int32_t* blocks) {
@@ -298,11 +681,81 @@ int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q,
   a.selected = s.selected;
   a.causal = s.causal;
   a.rows = (long long)q->n * a.tq * s.kv;
-  SY_CHECK(a.rows * 64 < (1LL << 32), SY_EUNSUPPORTED, "block select grid too large");
   DeviceScope device(ctx);
-  ProfScope prof(ctx, "block_select", 2.0 * a.rows * a.blocks * s.kd,
-                 4.0 * q->n * ((double)a.tq * (s.heads * s.kd + s.kv * s.selected) + (double)a.blocks * s.kv * s.kd));
-  hipLaunchKernelGGL(select_kernel, dim3((unsigned)a.rows), dim3(64), 0, ctx->stream, a);
+  const int planes = q->n * s.kv, steps = s.kd <= 32 ? 2 : s.kd <= 64 ? 4 : 8;
+  const double flops = 2.0 * a.rows * a.blocks * s.kd;
+  const double bytes =
+      4.0 * q->n * ((double)a.tq * (s.heads * s.kd + s.kv * s.selected) + (double)a.blocks * s.kv * s.kd);
+  if (a.tq < kManyQueries) {
+    const long long grid = (long long)planes * ((a.blocks + 63) / 64);
+    SY_CHECK(grid * 256 < (1LL << 32) && a.rows * 256 < (1LL << 32), SY_EUNSUPPORTED, "block select grid too large");
+    SY_TRY(ensure_scratch(ctx, sizeof(long long) * a.rows * a.blocks));
+    a.keys = (long long*)ctx->scratch;
+    {
+      ProfScope prof(ctx, "block_score", flops, bytes);
+      const dim3 g((unsigned)grid);
+      if (steps <= 4)
+        hipLaunchKernelGGL(score_kernel<4>, g, dim3(256), 0, ctx->stream, a);
+      else
+        hipLaunchKernelGGL(score_kernel<8>, g, dim3(256), 0, ctx->stream, a);
+      SY_TRY(check_launch("block_score"));
+    }
+    ProfScope prof(ctx, "block_rank", 0, 8.0 * a.rows * a.blocks);
+    hipLaunchKernelGGL(rank_kernel, dim3((unsigned)a.rows), dim3(256), 0, ctx->stream, a);
+    return check_launch("block_rank");
+  }
+  a.tiles = (a.blocks + 31) / 32;
+  a.chunks = (a.tiles + kPartTiles - 1) / kPartTiles;
+  const size_t parts = sizeof(u32x4) * 128 * (size_t)planes * a.tiles * steps;
+  const int tiles = s.selected <= 16 && s.kd <= 64 ? 2 : 1;  // of 32 queries to a wave
+  const long long groups = (a.tq + 128 * tiles - 1) / (128 * tiles);
+  SY_CHECK((long long)planes * groups * 256 < (1LL << 32) && (long long)planes * a.chunks * 256 < (1LL << 32),
+           SY_EUNSUPPORTED, "block select grid too large");
+  SY_TRY(ensure_scratch(ctx, parts + sizeof(float) * planes * a.chunks));
+  a.parts = (u32x4*)ctx->scratch;
+  a.norm = (float*)(ctx->scratch + parts);
+  {
+    ProfScope prof(ctx, "block_parts", 0, 8.0 * planes * (double)a.blocks * s.kd);
+    const dim3 g((unsigned)(planes * a.chunks));
+    if (steps == 2)
+      hipLaunchKernelGGL(means_parts_kernel<2>, g, dim3(256), 0, ctx->stream, a);
+    else if (steps == 4)
+      hipLaunchKernelGGL(means_parts_kernel<4>, g, dim3(256), 0, ctx->stream, a);
+    else
+      hipLaunchKernelGGL(means_parts_kernel<8>, g, dim3(256), 0, ctx->stream, a);
+    SY_TRY(check_launch("block_parts"));
+  }
+  ProfScope prof(ctx, "block_select", flops, bytes);
+  const dim3 g((unsigned)(planes * groups));
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, dim3(256), 0, ctx->stream, a); };
+  if (steps == 2) {
+    if (s.selected <= 8)
+      launch(select_tile_kernel<2, 8, 2>);
+    else if (s.selected <= 16)
+      launch(select_tile_kernel<2, 16, 2>);
+    else if (s.selected <= 32)
+      launch(select_tile_kernel<2, 32, 1>);
+    else
+      launch(select_tile_kernel<2, 64, 1>);
+  } else if (steps == 4) {
+    if (s.selected <= 8)
+      launch(select_tile_kernel<4, 8, 2>);
+    else if (s.selected <= 16)
+      launch(select_tile_kernel<4, 16, 2>);
+    else if (s.selected <= 32)
+      launch(select_tile_kernel<4, 32, 1>);
+    else
+      launch(select_tile_kernel<4, 64, 1>);
+  } else {
+    if (s.selected <= 8)
+      launch(select_tile_kernel<8, 8, 1>);
+    else if (s.selected <= 16)
+      launch(select_tile_kernel<8, 16, 1>);
+    else if (s.selected <= 32)
+      launch(select_tile_kernel<8, 32, 1>);
+    else
+      launch(select_tile_kernel<8, 64, 1>);
+  }
   return check_launch("block_select");
 }
 
