@@ -65,14 +65,14 @@ struct MeansArgs {
   float* m;
   const int *starts, *lengths;
   long long ldk, ldm;
-  int tk, kh, kw, bh, bw, bx, blocks, ks, kd, units, lanes, tokens, slots;
+  int tk, kh, kw, bh, bw, bx, blocks, ks, kd, units, lanes, pieces, tokens, slots;
 };
 
-// One workgroup per block (with `tokens`: per block that may hold some) and image.  A lane sums four
-// channels over every (256 / lanes)-th key; the partial sums meet in LDS in one order.
+// One workgroup per image, block (with `tokens`: that may hold some) and 128 channels.  A lane sums four channels over
+// every (256 / lanes)-th key, eight keys under way at a time; the partial sums meet in LDS in one order.
 __global__ __launch_bounds__(256) void means_kernel(const MeansArgs a) {
   __shared__ double part[256][4];
-  const int b = blockIdx.x / a.slots, slot = blockIdx.x % a.slots;
+  const int piece = blockIdx.x % a.pieces, bs = blockIdx.x / a.pieces, b = bs / a.slots, slot = bs % a.slots;
   const int length = a.lengths ? min(max(a.lengths[b], 0), a.tk) : a.tk;
   int j = slot;
   if (a.tokens) {
@@ -87,31 +87,38 @@ __global__ __launch_bounds__(256) void means_kernel(const MeansArgs a) {
   const int keys = rows == 1 ? max(min(cols, length - (y0 * a.kw + x0)), 0) : rows * cols;
   const int lane = threadIdx.x % a.lanes, group = threadIdx.x / a.lanes, groups = 256 / a.lanes;
   const double inv = keys ? 1.0 / keys : 0.0;
-  for (int u0 = 0; u0 < a.units; u0 += a.lanes) {
-    const int u = u0 + lane, head = 4 * u / a.kd;
-    double s[4] = {0, 0, 0, 0};
-    if (u < a.units) {
-      const float* kb = a.k + (long long)b * a.tk * a.ldk + head * a.ks + (4 * u - head * a.kd);
-      for (int t = group; t < keys; t += groups) {
-        const long long row = (long long)(y0 + t / cols) * a.kw + x0 + t % cols;
-        const f32x4 v = *(const f32x4*)(kb + row * a.ldk);
+  const int u = piece * a.lanes + lane, head = 4 * u / a.kd;
+  double s[4] = {0, 0, 0, 0};
+  if (u < a.units) {
+    const float* kb = a.k + ((long long)b * a.tk + (long long)y0 * a.kw + x0) * a.ldk + head * a.ks + (4 * u - head * a.kd);
+    int y = 0, x = group;
+    for (int t = group; t < keys; t += 8 * groups) {
+      f32x4 v[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += v[e];
+      for (int n = 0; n < 8; ++n) {
+        for (; x >= cols; x -= cols) ++y;
+        const bool on = t + n * groups < keys;
+        v[n] = *(const f32x4*)(kb + (on ? ((long long)y * a.kw + x) * a.ldk : 0));
+        if (!on) v[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        x += groups;
       }
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v[n][e];
     }
+  }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part[threadIdx.x][e] = s[e];
-    __syncthreads();
-    if (group == 0 && u < a.units) {
-      for (int g = 1; g < groups; ++g)
+  for (int e = 0; e < 4; ++e) part[threadIdx.x][e] = s[e];
+  __syncthreads();
+  if (group == 0 && u < a.units) {
+    for (int g = 1; g < groups; ++g)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += part[g * a.lanes + lane][e];
-      f32x4 o;
+      for (int e = 0; e < 4; ++e) s[e] += part[g * a.lanes + lane][e];
+    f32x4 o;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = (float)(s[e] * inv);
-      *(f32x4*)(a.m + ((long long)b * a.blocks + j) * a.ldm + 4 * u) = o;
-    }
-    __syncthreads();
+    for (int e = 0; e < 4; ++e) o[e] = (float)(s[e] * inv);
+    *(f32x4*)(a.m + ((long long)b * a.blocks + j) * a.ldm + 4 * u) = o;
   }
 }
 
@@ -157,10 +164,11 @@ int op_block_means(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* k, 
   a.kd = s.kd;
   a.units = s.kv * s.kd / 4;
   a.lanes = 1;
-  while (a.lanes < a.units && a.lanes < 256) a.lanes *= 2;
+  while (a.lanes < a.units && a.lanes < 32) a.lanes *= 2;
+  a.pieces = (a.units + a.lanes - 1) / a.lanes;
   a.tokens = tokens;
   a.slots = tokens ? (int)std::min<long long>(a.blocks, (tokens - 1LL) / s.bw + 2) : a.blocks;
-  const long long grid = (long long)k->n * a.slots;
+  const long long grid = (long long)k->n * a.slots * a.pieces;
   SY_CHECK(grid * 256 < (1LL << 32), SY_EUNSUPPORTED, "block means grid too large");
   DeviceScope device(ctx);
   const double read = tokens ? (double)a.slots * s.bw : (double)a.tk;
@@ -173,9 +181,9 @@ int op_block_means(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* k, 
 // ----------------------------------------------------------------- selection
 //
 // Many queries: scores in float32 from the matrix cores with a bound e on their error, twice over.  The first pass
-// keeps the largest ones of each query, so that the `selected`-th, t, is known; blocks further than 2 e above t are
-// chosen and those further below are not, whatever the rounding.  The second pass writes the blocks from t - 2 e up.
-// Where more than `selected` lie there, a few queries in a thousand, the query is ranked in 64 bits.
+// keeps the largest ones of each query, so that the `selected`-th, t, is known; no block further than 2 e below t is
+// chosen, whatever the rounding.  The second pass writes the blocks from t - 2 e up.  Where more than `selected`
+// lie there, some queries in a hundred, those blocks are scored again in 64 bits and ranked.
 // Few queries: scores in 64 bits, then a ranking.
 
 struct SelectArgs {
@@ -263,21 +271,23 @@ __device__ __forceinline__ int rank_wave(int count, int selected, int lane, F ke
       }
     int n = 0;
     for (; n < selected; ++n) {
-      const int hi = (int)(k[0] >> 32), top_hi = wave_max_i32(hi);
-      const unsigned lo = (unsigned)k[0];
-      // The low half's order as a signed one; lanes with a smaller high half out of it.
-      const int low = hi == top_hi ? (int)(lo ^ 0x80000000u) : INT_MIN, top_lo = wave_max_i32(low);
-      const long long top = (long long)top_hi << 32 | ((unsigned)top_lo ^ 0x80000000u);
-      if (top == kHidden) break;
-      const unsigned long long heads = __ballot(k[0] == top);
-      int winner = __builtin_ctzll(heads);
+      // The high halves first; where they agree, the low ones (in the order of signed numbers), then the lower block.
+      const int hi = (int)(k[0] >> 32), top = wave_max_i32(hi);
+      unsigned long long heads = __ballot(hi == top);
       if (heads & (heads - 1)) {
-        const int first = -wave_max_i32(k[0] == top ? -id[0] : INT_MIN);
-        winner = __builtin_ctzll(__ballot(k[0] == top && id[0] == first));
+        const int low = hi == top ? (int)((unsigned)k[0] ^ 0x80000000u) : INT_MIN, top_low = wave_max_i32(low);
+        heads &= __ballot(low == top_low);
+        if (heads & (heads - 1)) {
+          const int mine = heads >> lane & 1 ? -id[0] : INT_MIN, first = wave_max_i32(mine);
+          heads = __ballot(mine == first);
+        }
       }
+      const int winner = __builtin_ctzll(heads);
+      const long long best = (long long)top << 32 | (unsigned)__builtin_amdgcn_readlane((int)k[0], winner);
+      if (best == kHidden) break;
       const int won = __builtin_amdgcn_readlane(id[0], winner);
       if (lane == n) {
-        bk = top;
+        bk = best;
         bi = won;
       }
       if (lane == winner) {
@@ -311,27 +321,55 @@ __device__ __forceinline__ double query_sum(const SelectArgs& a, const float* q,
   return s;
 }
 
-// One query in 64 bits by one wave: a lane scores a block of 64.
-__device__ __forceinline__ void select_exact(const SelectArgs& a, int b, int i, int g, int lane, double* qsum) {
+// The sum of query i's heads of group g, in 64 bits, for all lanes of a wave.
+__device__ __forceinline__ void query_sums(const SelectArgs& a, int b, int i, int g, int lane, double* qsum) {
   const float* q = a.q + ((long long)b * a.tq + i) * a.ldq + (long long)g * a.group * a.qs;
   for (int c = lane; c < a.kd; c += 64) qsum[c] = query_sum(a, q, c);
   __builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ long long exact_key(const SelectArgs& a, int b, int g, int j, const double* qsum) {
+  const float* m = a.m + ((long long)b * a.blocks + j) * a.ldm + g * a.kd;
+  double s = 0;
+#pragma unroll 4
+  for (int c = 0; c < a.kd; c += 4) {
+    const f32x4 v = *(const f32x4*)(m + c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s = __builtin_fma(qsum[c + e], (double)v[e], s);
+  }
+  return score_key(s);
+}
+
+// One query in 64 bits by one wave: a lane scores a block of 64.
+__device__ __forceinline__ void select_exact(const SelectArgs& a, int b, int i, int g, int lane, double* qsum) {
+  query_sums(a, b, i, g, lane, qsum);
   int forced;
   const int seen = seen_blocks(a, b, i, &forced);
   long long bk;
   int bi;
-  const int kept = rank_wave(seen, a.selected, lane, [&](int j) {
-    if (j == forced) return (long long)LLONG_MAX;
-    const float* m = a.m + ((long long)b * a.blocks + j) * a.ldm + g * a.kd;
-    double s = 0;
-    for (int c = 0; c < a.kd; c += 4) {
-      const f32x4 v = *(const f32x4*)(m + c);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s = __builtin_fma(qsum[c + e], (double)v[e], s);
-    }
-    return score_key(s);
-  }, &bk, &bi);
+  const int kept = rank_wave(seen, a.selected, lane,
+                             [&](int j) { return j == forced ? (long long)LLONG_MAX : exact_key(a, b, g, j, qsum); }, &bk, &bi);
   write_row(a.out + (((long long)b * a.tq + i) * a.kv + g) * a.selected, a.selected, kept, lane, bi);
+  __builtin_amdgcn_wave_barrier();
+}
+
+// The same among `count` candidates (up to 64, more than wanted) in ascending order: each counts those before it.
+__device__ __forceinline__ void select_among(const SelectArgs& a, int b, int i, int g, int lane, double* qsum,
+                                             const int* pool, int count) {
+  query_sums(a, b, i, g, lane, qsum);
+  int forced;
+  (void)seen_blocks(a, b, i, &forced);
+  const int j = pool[min(lane, count - 1)];
+  const long long key = j == forced ? LLONG_MAX : exact_key(a, b, g, j, qsum);
+  int before = 0;
+  for (int n = 0; n < count; ++n) {
+    const long long k = (long long)__builtin_amdgcn_readlane((int)(key >> 32), n) << 32 |
+                        (unsigned)__builtin_amdgcn_readlane((int)key, n);
+    before += k > key || (k == key && n < lane);
+  }
+  const unsigned long long chosen = __ballot(lane < count && before < a.selected);
+  if (chosen >> lane & 1)
+    a.out[(((long long)b * a.tq + i) * a.kv + g) * a.selected + __builtin_popcountll(chosen & ((1ull << lane) - 1))] = j;
   __builtin_amdgcn_wave_barrier();
 }
 
@@ -402,25 +440,27 @@ __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
   }
 }
 
-// 32 QT queries of one key head per wave, four waves to a workgroup that share nothing.
+// 32 queries of one key head per wave, four waves to a workgroup that share nothing.
 //
 // S^T = M Q^T: a lane holds a query's scores of the blocks 8 (r / 4) + 4 half + r % 4 of a tile.  The SMAX + 1 largest
 // so far stay sorted in registers: a new score moves through them by one median of three each.  (Fewer wanted:
 // the list starts with infinities.)  The two halves' lists meet at the end.
 //
-// Error of a score: a part is off by 2^-9 of what it stands for, so operands by 2^-18 and the product left out by as much,
-// 3 x 2^-18 of sum |q||m|; a sum of at most 24 matrix instructions' results and 16 products within each, below
-// 2^-18; q itself rounded from 64 bits.  sum |q||m| <= |q||m| in norms (off by 2^-15 of themselves, from sums in
-// float32): e = 2^-15.5 |q| max|m|, taken as 2^-15.  Norms outside 2^-40 .. 2^40 could lose parts to
-// underflow: those queries are ranked in 64 bits.
-template <int KS, int SMAX, int QT>
+// Error of a score: a part is off by 2^-8 of what it stands for, so two of them by 2^-16, twice (operands), and the
+// product of the second parts is left out, 2^-16 again: 3 x 2^-16 of sum |q||m|.  Sums of at most 24 matrix
+// instructions with 16 products each, and q rounded from 64 bits, stay below 2^-18.  sum |q||m| <= |q||m| in norms,
+// which sums in float32 and two roots change by less than 2^-16 of themselves: e = 3.5 x 2^-16 |q| max|m|.  Norms
+// outside 2^-40 .. 2^40 could lose parts to underflow: all blocks of those queries are scored in 64 bits.
+constexpr int kPools = 8;  // doubtful queries of a wave whose candidates are kept
+template <int KS, int SMAX>
 __global__ __launch_bounds__(256) void select_tile_kernel(const SelectArgs a) {
   __shared__ double qsum[4][128];
+  __shared__ int pool[4][kPools][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, r32 = lane & 31;
-  const int groups = (a.tq + 128 * QT - 1) / (128 * QT);
+  const int groups = (a.tq + 127) / 128;
   const int plane = blockIdx.x / groups, b = plane / a.kv, g = plane - b * a.kv;
-  const int i0 = (blockIdx.x - plane * groups) * 128 * QT + wave * 32 * QT;
+  const int i0 = (blockIdx.x - plane * groups) * 128 + wave * 32;
   if (i0 >= a.tq) return;
 
   float kn = 0.f;
@@ -428,14 +468,15 @@ __global__ __launch_bounds__(256) void select_tile_kernel(const SelectArgs a) {
     const float o = a.norm[plane * a.chunks + c];
     kn = o <= kn || kn != kn ? kn : o;
   }
-  bf16x8 q[QT][KS][2];
-  float slack[QT];  // 2 e
-  int seen[QT], forced[QT], most = 0;
-  unsigned exact = 0;  // bit t: this lane's query t is ranked in 64 bits
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int i = min(i0 + 32 * t + r32, a.tq - 1);
-    const float* p = a.q + ((long long)b * a.tq + i) * a.ldq + (long long)g * a.group * a.qs + 8 * half;
+  bf16x8 q[KS][2];
+  float slack;  // 2 e
+  bool exact;   // all blocks of this lane's query are scored in 64 bits
+  int forced;
+  const int i = i0 + r32;
+  const int seen = seen_blocks(a, b, min(i, a.tq - 1), &forced);
+  const int last = __builtin_amdgcn_readfirstlane((wave_max_i32(seen) + 31) / 32);
+  {
+    const float* p = a.q + ((long long)b * a.tq + min(i, a.tq - 1)) * a.ldq + (long long)g * a.group * a.qs + 8 * half;
     float qn = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -465,124 +506,123 @@ __global__ __launch_bounds__(256) void select_tile_kernel(const SelectArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) qn = __builtin_fmaf(f[4 * u + e], f[4 * u + e], qn);
       }
-      halves8(f, q[t][ks]);
+      halves8(f, q[ks]);
     }
     qn += __shfl_xor(qn, 32);
     const bool fine = qn >= 0x1p-80f && qn <= 0x1p80f && kn >= 0x1p-80f && kn <= 0x1p80f;
-    if (!fine) exact |= 1u << t;
-    slack[t] = 0x1p-14f * (__builtin_sqrtf(qn) * __builtin_sqrtf(kn));
-    seen[t] = seen_blocks(a, b, i, &forced[t]);
-    most = max(most, seen[t]);
+    exact = !fine;
+    slack = 7.f / 65536 * (__builtin_sqrtf(qn) * __builtin_sqrtf(kn));
   }
-  const int last = __builtin_amdgcn_readfirstlane((wave_max_i32(most) + 31) / 32);
   const u32x4* parts = a.parts + (long long)plane * a.tiles * KS * 2 * 64 + lane;
 
-  // Scores of tile n, with what is not seen at -inf and what is forced at +inf.
-  auto scores = [&](int n, f32x16 (&sc)[QT]) __attribute__((always_inline)) {
+  // Scores of tile n, whose parts are under way, with what is not seen at -inf and what is forced at +inf.
+  u32x4 m[KS][2];
+  auto load = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < QT; ++t)
+    for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[t][r] = 0.f;
+      for (int p = 0; p < 2; ++p) m[ks][p] = parts[((long long)n * KS + ks) * 128 + 64 * p];
+  };
+  auto scores = [&](int n) __attribute__((always_inline)) {
+    f32x16 sc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sc[r] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const bf16x8 m0 = __builtin_bit_cast(bf16x8, parts[((long long)n * KS + ks) * 128]);
-      const bf16x8 m1 = __builtin_bit_cast(bf16x8, parts[((long long)n * KS + ks) * 128 + 64]);
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m1, q[t][ks][0], sc[t], 0, 0, 0);
-        sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m0, q[t][ks][1], sc[t], 0, 0, 0);
-        sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m0, q[t][ks][0], sc[t], 0, 0, 0);
-      }
+      const bf16x8 m0 = __builtin_bit_cast(bf16x8, m[ks][0]), m1 = __builtin_bit_cast(bf16x8, m[ks][1]);
+      sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m1, q[ks][0], sc, 0, 0, 0);
+      sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m0, q[ks][1], sc, 0, 0, 0);
+      sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m0, q[ks][0], sc, 0, 0, 0);
     }
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      const int room = seen[t] - 32 * n - 4 * half, own = forced[t] - 32 * n - 4 * half;
-      if (__any(room < 32 || (own >= 0 && own < 32)))
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int at = 8 * (r >> 2) + (r & 3);
-          sc[t][r] = at >= room ? -INFINITY : at == own ? INFINITY : sc[t][r];
-        }
-    }
-  };
-
-  float list[QT][SMAX + 1];
-#pragma unroll
-  for (int t = 0; t < QT; ++t)
-#pragma unroll
-    for (int n = 0; n <= SMAX; ++n) list[t][n] = n < SMAX - a.selected && half == 0 ? INFINITY : -INFINITY;
-  for (int n = 0; n < last; ++n) {
-    f32x16 sc[QT];
-    scores(n, sc);
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      float top = sc[t][0];
-#pragma unroll
-      for (int r = 1; r < 16; ++r) top = fmaxf(top, sc[t][r]);
-      if (!__any(top > list[t][SMAX])) continue;
+    load(min(n + 1, last - 1));
+    const int room = seen - 32 * n - 4 * half, own = forced - 32 * n - 4 * half;
+    if (__any(room < 32 || (own >= 0 && own < 32)))
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float x = sc[t][r];
-#pragma unroll
-        for (int u = SMAX; u > 0; --u) list[t][u] = __builtin_amdgcn_fmed3f(list[t][u - 1], list[t][u], x);
-        list[t][0] = fmaxf(list[t][0], x);
+        const int at = 8 * (r >> 2) + (r & 3);
+        sc[r] = at >= room ? -INFINITY : at == own ? INFINITY : sc[r];
       }
-    }
-  }
+    return sc;
+  };
 
-  float from[QT];  // scores from here up are written
-  unsigned count[QT];
+  float list[SMAX + 1];
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    float nth = INFINITY, after = INFINITY;
-    float other[SMAX + 1];
-#pragma unroll
-    for (int n = 0; n <= SMAX; ++n) other[n] = __shfl_xor(list[t][n], 32);
-#pragma unroll
-    for (int n = 0; n < SMAX; ++n) nth = fminf(nth, fmaxf(list[t][n], other[SMAX - 1 - n]));
-#pragma unroll
-    for (int n = 0; n <= SMAX; ++n) after = fminf(after, fmaxf(list[t][n], other[SMAX - n]));
-    from[t] = nth - slack[t];
-    if (seen[t] > a.selected && !(after < from[t])) exact |= 1u << t;
-    count[t] = 0;
-  }
-
+  for (int n = 0; n <= SMAX; ++n) list[n] = n < SMAX - a.selected && half == 0 ? INFINITY : -INFINITY;
+  if (last > 0) load(0);
   for (int n = 0; n < last; ++n) {
-    f32x16 sc[QT];
-    scores(n, sc);
+    const f32x16 sc = scores(n);
+    float top = sc[0];
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      unsigned m = 0;
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, sc[r]);
+    if (!__any(top > list[SMAX])) continue;
 #pragma unroll
-      for (int r = 15; r >= 0; --r) m = m << 1 | (sc[t][r] >= from[t] ? 1u : 0u);
-      if (!__any(m != 0)) continue;
-      m = (m | m << 8) & 0x00ff00ffu;
-      m = (m | m << 4) & 0x0f0f0f0fu;
-      const unsigned o = (unsigned)__shfl_xor((int)m, 32);
-      m = half ? o | m << 4 : m | o << 4;
-      const int room = seen[t] - 32 * n;
-      if (room < 32) m &= room > 0 ? (1u << room) - 1 : 0u;
-      const int i = i0 + 32 * t + r32;
-      int* out = a.out + (((long long)b * a.tq + i) * a.kv + g) * a.selected;
-      while (__any(m != 0)) {
-        if (m) {
-          const int bit = __builtin_ctz(m);
-          m &= m - 1;
-          if (half == 0 && i < a.tq && !(exact >> t & 1) && (int)count[t] < a.selected) out[count[t]] = 32 * n + bit;
-          ++count[t];
+    for (int r = 0; r < 16; ++r) {
+#pragma unroll
+      for (int u = SMAX; u > 0; --u) list[u] = __builtin_amdgcn_fmed3f(list[u - 1], list[u], sc[r]);
+      list[0] = fmaxf(list[0], sc[r]);
+    }
+  }
+
+  // The n-th largest of two sorted lists is the least of the maxima of one's u-th and the other's (n - 1 - u)-th.
+  float nth = INFINITY, after = INFINITY, other[SMAX + 1];
+#pragma unroll
+  for (int n = 0; n <= SMAX; ++n) other[n] = __shfl_xor(list[n], 32);
+#pragma unroll
+  for (int n = 0; n < SMAX; ++n) nth = fminf(nth, fmaxf(list[n], other[SMAX - 1 - n]));
+#pragma unroll
+  for (int n = 0; n <= SMAX; ++n) after = fminf(after, fmaxf(list[n], other[SMAX - n]));
+  const float from = nth - slack;  // scores from here up are written
+  const bool doubt = !exact && i < a.tq && seen > a.selected && !(after < from);
+  const unsigned doubts = (unsigned)__ballot(doubt);  // of the lower half; the upper one agrees
+  int slot = doubt ? __builtin_popcount(doubts & ((1u << r32) - 1)) : -1;  // of a doubtful query's candidates
+  if (slot >= kPools) {
+    slot = -1;
+    exact = true;
+  }
+
+  int* out = a.out + (((long long)b * a.tq + i) * a.kv + g) * a.selected;
+  const bool mine = half == 0 && i < a.tq;
+  int count = 0;
+  if (last > 0) load(0);
+  for (int n = 0; n < last; ++n) {
+    const f32x16 sc = scores(n);
+    unsigned w = 0;
+#pragma unroll
+    for (int r = 15; r >= 0; --r) w = w + w + (sc[r] >= from);
+    if (!__any(w != 0)) continue;
+    // Four blocks of this half, four of the other, and so on.
+    w = (w | w << 8) & 0x00ff00ffu;
+    w = (w | w << 4) & 0x0f0f0f0fu;
+    const unsigned o = (unsigned)__shfl_xor((int)w, 32);
+    w = half ? o | w << 4 : w | o << 4;
+    const int room = seen - 32 * n;
+    if (room < 32) w &= room > 0 ? (1u << room) - 1 : 0u;
+    while (__any(w != 0)) {
+      if (w) {
+        const int j = 32 * n + __builtin_ctz(w);
+        w &= w - 1;
+        if (mine && !exact) {
+          if (slot >= 0) {
+            if (count < 64) pool[wave][slot][count] = j;
+          } else if (count < a.selected) {
+            out[count] = j;
+          }
         }
+        ++count;
       }
     }
   }
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int i = i0 + 32 * t + r32;
-    int* out = a.out + (((long long)b * a.tq + i) * a.kv + g) * a.selected;
-    if (half == 0 && i < a.tq && !(exact >> t & 1))
-      for (int n = count[t]; n < a.selected; ++n) out[n] = -1;
-    for (unsigned long long todo = __ballot(half == 0 && i < a.tq && (exact >> t & 1)); todo; todo &= todo - 1)
-      select_exact(a, b, i0 + 32 * t + __builtin_ctzll(todo), g, lane, qsum[wave]);
+  __builtin_amdgcn_wave_barrier();
+  if (slot >= 0 && count > 64) exact = true;
+  if (mine && !exact && slot < 0)
+    for (int n = count; n < a.selected; ++n) out[n] = -1;
+  for (unsigned long long todo = __ballot(mine && !exact && slot >= 0); todo; todo &= todo - 1) {
+    const int x = __builtin_ctzll(todo);
+    select_among(a, b, i0 + x, g, lane, qsum[wave], pool[wave][__builtin_amdgcn_readlane(slot, x)],
+                 __builtin_amdgcn_readlane(count, x));
   }
+  for (unsigned long long todo = __ballot(mine && exact); todo; todo &= todo - 1)
+    select_exact(a, b, i0 + __builtin_ctzll(todo), g, lane, qsum[wave]);
 }
 
 // Scores of 64 blocks in 64 bits, four lanes to a block, for each of few queries.
@@ -631,12 +671,13 @@ __global__ __launch_bounds__(256) void rank_kernel(const SelectArgs a) {
   if (threadIdx.x < 64) chosen[threadIdx.x] = 0x7fffffff;
   __syncthreads();
   if (lane < kept) {
-    int before = 0;
-    for (int w = 0; w < 4; ++w)
-      for (int n = 0; n < a.selected; ++n) {
-        const long long k = key[64 * w + n];
-        before += k > key[threadIdx.x] || (k == key[threadIdx.x] && id[64 * w + n] < id[threadIdx.x]);
-      }
+    int before = lane;  // of its own wave
+    for (int w = 1; w < 4; ++w) {
+      const int other = 64 * ((wave + w) & 3);
+#pragma unroll 8
+      for (int n = 0; n < a.selected; ++n)
+        before += key[other + n] > bk || (key[other + n] == bk && id[other + n] < from + bi);
+    }
     if (before < a.selected) chosen[before] = id[threadIdx.x];
   }
   __syncthreads();
@@ -707,8 +748,7 @@ int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q,
   a.tiles = (a.blocks + 31) / 32;
   a.chunks = (a.tiles + kPartTiles - 1) / kPartTiles;
   const size_t parts = sizeof(u32x4) * 128 * (size_t)planes * a.tiles * steps;
-  const int tiles = s.selected <= 16 && s.kd <= 64 ? 2 : 1;  // of 32 queries to a wave
-  const long long groups = (a.tq + 128 * tiles - 1) / (128 * tiles);
+  const long long groups = (a.tq + 127) / 128;
   SY_CHECK((long long)planes * groups * 256 < (1LL << 32) && (long long)planes * a.chunks * 256 < (1LL << 32),
            SY_EUNSUPPORTED, "block select grid too large");
   SY_TRY(ensure_scratch(ctx, parts + sizeof(float) * planes * a.chunks));
@@ -730,31 +770,31 @@ int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q,
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, dim3(256), 0, ctx->stream, a); };
   if (steps == 2) {
     if (s.selected <= 8)
-      launch(select_tile_kernel<2, 8, 2>);
+      launch(select_tile_kernel<2, 8>);
     else if (s.selected <= 16)
-      launch(select_tile_kernel<2, 16, 2>);
+      launch(select_tile_kernel<2, 16>);
     else if (s.selected <= 32)
-      launch(select_tile_kernel<2, 32, 1>);
+      launch(select_tile_kernel<2, 32>);
     else
-      launch(select_tile_kernel<2, 64, 1>);
+      launch(select_tile_kernel<2, 64>);
   } else if (steps == 4) {
     if (s.selected <= 8)
-      launch(select_tile_kernel<4, 8, 2>);
+      launch(select_tile_kernel<4, 8>);
     else if (s.selected <= 16)
-      launch(select_tile_kernel<4, 16, 2>);
+      launch(select_tile_kernel<4, 16>);
     else if (s.selected <= 32)
-      launch(select_tile_kernel<4, 32, 1>);
+      launch(select_tile_kernel<4, 32>);
     else
-      launch(select_tile_kernel<4, 64, 1>);
+      launch(select_tile_kernel<4, 64>);
   } else {
     if (s.selected <= 8)
-      launch(select_tile_kernel<8, 8, 1>);
+      launch(select_tile_kernel<8, 8>);
     else if (s.selected <= 16)
-      launch(select_tile_kernel<8, 16, 1>);
+      launch(select_tile_kernel<8, 16>);
     else if (s.selected <= 32)
-      launch(select_tile_kernel<8, 32, 1>);
+      launch(select_tile_kernel<8, 32>);
     else
-      launch(select_tile_kernel<8, 64, 1>);
+      launch(select_tile_kernel<8, 64>);
   }
   return check_launch("block_select");
 }
