@@ -20,6 +20,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kKeys = 64;    // keys of a tile; longer blocks are so many tiles ("parts" of the block)
+constexpr int kTileRows = 1024;
 constexpr int kMaxBlocks = 12288;  // of a sorted list: counters in LDS
 
 struct BlockArgs {
@@ -239,7 +240,7 @@ __device__ __forceinline__ unsigned item_of(unsigned block, unsigned grid) { ret
 //
 // The maximum m is the largest score times c = scale log2(e), rounded once; weights are 2^(s c - m) with one
 // rounding of the exponent, and m is kept as it is, so that slots join exactly.
-template <int KS, int DT, int W>
+template <int KS, int DT, int W, bool WHOLE>
 __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(const BlockArgs a) {
   constexpr int T = 64 * W;
   constexpr int KF = 2 * KS * 3, VF = 4 * DT * 3;  // fragments of 64 lanes x 16 bytes
@@ -248,6 +249,7 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
   __shared__ u32x4 frag[(KF + VF) * 64];
   __shared__ unsigned k_at[kKeys], v_at[kKeys];    // floats from the block's first key
   __shared__ unsigned place[W][32];
+  __shared__ int pair_at[kTileRows];
   const BlockShape& s = a.s;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, r32 = lane & 31;
@@ -272,14 +274,16 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
   int keys = a.lengths ? min(size, length - origin) : size;
   keys = min(max(keys - part * kKeys, 0), kKeys);
 
-  // The lane's row in the wave's turn r: its query, the keys it sees, where its results go.
-  const float* qb = a.q + ((long long)b * s.tq + i0) * a.ldq + (long long)g * s.group * s.qs + 8 * half;
-  auto pair_of = [&](int r) { return list[min(row0 + min(r + r32, rows - 1), rec.w * s.group - 1) / s.group]; };
+  // The lane's row in the wave's turn r: its query, the keys it sees, where its results go.  Channels past key_dim read
+  // the last ones again, which the keys' zeros cancel.
+  const float* qb = a.q + ((long long)b * s.tq + i0) * a.ldq + (long long)g * s.group * s.qs;
+  const int e0 = row0 / s.group, h0 = row0 - e0 * s.group;
   f32x4 qr[KS][2];
   int limit;
   unsigned to;  // row of the results
-  auto load_q = [&](int r, int pair) __attribute__((always_inline)) {
-    const int x = row0 + min(r + r32, rows - 1), h = x % s.group, d = pair / s.selected;
+  auto load_q = [&](int r) __attribute__((always_inline)) {
+    const int x = h0 + min(r + r32, rows - 1), e = x / s.group, h = x - e * s.group;
+    const int pair = pair_at[e], d = pair / s.selected;
     limit = keys;
     if (s.causal) {
       const long long end = min((long long)length, max(start + i0 + d + 1, 0LL));
@@ -291,13 +295,9 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int c = 16 * ks + 4 * u;
-        qr[ks][u] = c + 8 * half < s.kd ? *(const f32x4*)(p + c) : f32x4{0.f, 0.f, 0.f, 0.f};
-      }
+      for (int u = 0; u < 2; ++u) qr[ks][u] = *(const f32x4*)(p + min(16 * ks + 8 * half + 4 * u, s.kd - 4));
   };
-  int r = wave * 32;
-  int pair = pair_of(r);
+  for (int x = tid; x < (h0 + rows + s.group - 1) / s.group; x += T) pair_at[x] = list[e0 + x];
   if (tid < kKeys) {
     const int u = tid < keys ? part * kKeys + tid : 0, y = u / cols;
     k_at[tid] = (y * s.kw + u - y * cols) * (unsigned)a.ldk;
@@ -305,6 +305,7 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
   }
   __syncthreads();
 
+  int r = wave * 32;
   {
     const float* kb = a.k + ((long long)b * s.tk + origin) * a.ldk + (long long)g * s.ks;
     const float* vb = a.v + ((long long)b * s.tk + origin) * a.ldv + (long long)g * s.vs;
@@ -327,7 +328,7 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
 #pragma unroll
       for (int e = 0; e < 8; ++e) vr[n][e] = vb[v_at[first + 8 * (e >> 2) + (e & 3)] + c];
     }
-    load_q(r, pair);
+    load_q(r);
     // Piece c of key t: lanes t % 32 + 32 (c % 2) of step c / 2, turned by c so that a thread group's writes meet
     // different banks.
 #pragma unroll
@@ -361,9 +362,10 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
   }
   __syncthreads();
 
+  // The queries are here before the loop: in it they are waited for with the stores behind them still under way.
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   const float c = s.scale * 1.4426950408889634f;
   for (; r < rows; r += 32 * W) {
-    const int next = pair_of(r + 32 * W < rows ? r + 32 * W : r);
     f32x16 sc[2], rest[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -386,9 +388,8 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
     }
     const int seen = limit;
     const unsigned mine = to;
-    const bool on = r + r32 < rows;
-    if (half == 0) place[wave][r32] = mine * (unsigned)s.hd;
-    if (r + 32 * W < rows) load_q(r + 32 * W, next);
+    place[wave][r32] = mine * (unsigned)(4 * s.hd);
+    load_q(min(r + 32 * W, rows - 1));  // the last turn: something, to keep the count of loads
     float w[32];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -409,7 +410,7 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
       sum += w[x];
     }
     sum += __shfl_xor(sum, 32);
-    if (half == 0 && on) a.stat[mine] = make_float2(mx, sum);
+    a.stat[half ? a.trash : mine] = make_float2(mx, sum);
     bf16x8 wp[4][3];
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
@@ -418,26 +419,36 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
       parts8(f, wp[st]);
     }
     __builtin_amdgcn_wave_barrier();
-    unsigned row_at[16];
+    unsigned row_at[16];  // bytes
 #pragma unroll
-    for (int x = 0; x < 16; ++x) row_at[x] = place[wave][8 * (x >> 2) + 4 * half + (x & 3)] + r32;
+    for (int x = 0; x < 16; ++x) row_at[x] = place[wave][8 * (x >> 2) + 4 * half + (x & 3)] + 4 * r32;
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      if (32 * d >= s.hd) break;
-      f32x16 acc, rs;
+      if (!WHOLE && 32 * d >= s.hd) break;
+      // The five small products of every step first, then the leading ones on top.
+      f32x16 acc;
 #pragma unroll
-      for (int x = 0; x < 16; ++x) acc[x] = rs[x] = 0.f;
+      for (int x = 0; x < 16; ++x) acc[x] = 0.f;
+      bf16x8 lead[4];
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
         bf16x8 v[3];
 #pragma unroll
         for (int m = 0; m < 3; ++m) v[m] = __builtin_bit_cast(bf16x8, frag[KF * 64 + ((st * DT + d) * 3 + m) * 64 + lane]);
-        mfma_parts(wp[st], v, acc, rs);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wp[st][2], v[0], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wp[st][1], v[1], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wp[st][0], v[2], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wp[st][1], v[0], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wp[st][0], v[1], acc, 0, 0, 0);
+        lead[st] = v[0];
       }
-      if (32 * d + r32 < s.hd)
 #pragma unroll
-        for (int x = 0; x < 16; ++x) a.part[row_at[x] + 32 * d] = acc[x] + rs[x];
+      for (int st = 0; st < 4; ++st) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wp[st][0], lead[st], acc, 0, 0, 0);
+      char* base = (char*)(a.part + 32 * d);
+      if (WHOLE || 32 * d + r32 < s.hd)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) *(float*)(base + row_at[x]) = acc[x];
     }
   }
 }
@@ -751,7 +762,7 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   const int together = (int)std::min<double>((double)segments, std::max(1.0, std::floor(kPartials / (per_query * a.span))));
   const bool sorted = s.blocks <= kMaxBlocks && (long long)s.tq * s.selected > SORT_FROM;
   // Rows of a tile: many, so that the keys are laid out seldom, but four rounds of tiles on the whole chip.
-  a.rows = 1024;
+  a.rows = kTileRows;
   while (a.rows > 256 && (double)together * a.span * s.selected * a.parts * s.group < 4096.0 * a.rows) a.rows /= 2;
   // 2048 pairs to a workgroup of the sort, but at most 32 of them to a segment (each reads all their counts).
   a.chunk = std::max(std::max(1, 2048 / s.selected), (a.span + 31) / 32);
@@ -759,7 +770,7 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   const long long pairs = (long long)a.span * s.selected;
   const long long tile_cap = a.parts * (std::min<long long>(s.blocks, pairs) + pairs * s.group / a.rows + 1);
   const long long result_rows = together * pairs * a.parts * s.group;
-  SY_CHECK((result_rows + 1) * s.hd < (1LL << 30) && tile_cap * together < (1LL << 24), SY_EUNSUPPORTED,
+  SY_CHECK((result_rows + 1) * s.hd < (1LL << 30) - 128 && tile_cap * together < (1LL << 24), SY_EUNSUPPORTED,
            "block attention over %d heads to a key head", s.group);
   SY_CHECK((double)s.bh * s.kw * std::max(k->ldc, v->ldc) < 4294967296.0, SY_EUNSUPPORTED,
            "block windows that span 2^32 floats and more");
@@ -772,7 +783,8 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
     at += (bytes + 255) & ~size_t(255);
     return from;
   };
-  const size_t part_at = take(sizeof(float) * (result_rows + 1) * s.hd), stat_at = take(sizeof(float2) * result_rows);
+  const size_t part_at = take(sizeof(float) * ((result_rows + 1) * s.hd + 128)),
+               stat_at = take(sizeof(float2) * (result_rows + 1));
   const size_t count_at = sorted ? take(sizeof(int) * segments * a.chunks * s.blocks) : 0;
   const size_t list_at = sorted ? take(sizeof(int) * segments * pairs) : 0;
   const size_t tile_at = sorted ? take(sizeof(int4) * segments * tile_cap) : 0;
@@ -807,12 +819,21 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
         auto launch = [&](auto kernel, int waves) {
           hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * waves), 0, ctx->stream, a);
         };
+        auto pick = [&](auto whole2, auto part2, auto whole4, auto part4, int waves4) {
+          if (s.hd <= 64)
+            s.hd == 64 ? launch(whole2, 4) : launch(part2, 4);
+          else
+            s.hd == 128 ? launch(whole4, waves4) : launch(part4, waves4);
+        };
         if (s.kd <= 32)
-          s.hd <= 64 ? launch(block_tile_kernel<2, 2, 4>, 4) : launch(block_tile_kernel<2, 4, 4>, 4);
+          pick(block_tile_kernel<2, 2, 4, true>, block_tile_kernel<2, 2, 4, false>, block_tile_kernel<2, 4, 4, true>,
+               block_tile_kernel<2, 4, 4, false>, 4);
         else if (s.kd <= 64)
-          s.hd <= 64 ? launch(block_tile_kernel<4, 2, 4>, 4) : launch(block_tile_kernel<4, 4, 4>, 4);
+          pick(block_tile_kernel<4, 2, 4, true>, block_tile_kernel<4, 2, 4, false>, block_tile_kernel<4, 4, 4, true>,
+               block_tile_kernel<4, 4, 4, false>, 4);
         else
-          s.hd <= 64 ? launch(block_tile_kernel<8, 2, 4>, 4) : launch(block_tile_kernel<8, 4, 8>, 8);
+          pick(block_tile_kernel<8, 2, 4, true>, block_tile_kernel<8, 2, 4, false>, block_tile_kernel<8, 4, 8, true>,
+               block_tile_kernel<8, 4, 8, false>, 8);
       } else {
         const dim3 grid((unsigned)(now * pairs * a.parts));
         if (s.kd <= 64)
