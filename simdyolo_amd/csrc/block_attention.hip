@@ -38,6 +38,7 @@ struct BlockArgs {
   unsigned trash;    // a row of results that nobody reads
   int chunk, chunks, tile_cap;  // queries of a workgroup of the sort, such workgroups; tiles at most
   int *counts, *list, *tile_count;
+  int* pos;          // place of each pair in its list
   int4* tiles;
   // Results of the launch's segments, row by row.
   float2* stat;      // maximum (in powers of two) and sum
@@ -187,7 +188,12 @@ __global__ __launch_bounds__(kSortThreads) void block_scatter_kernel(const Block
   if (chunk == 0 && threadIdx.x == 0) a.tile_count[seg] = base.y;
   __syncthreads();
   int* list = a.list + (long long)seg * a.span * s.selected;
-  for_pairs(a, seg, chunk, [&](int pair, int j) { list[atomicAdd(&hist[j], 1)] = pair; });
+  int* pos = a.pos + (long long)seg * a.span * s.selected;
+  for_pairs(a, seg, chunk, [&](int pair, int j) {
+    const int at = atomicAdd(&hist[j], 1);
+    list[at] = pair;
+    pos[pair] = at;
+  });
 }
 
 // ---------------------------------------------------------------------- tiles
@@ -289,7 +295,7 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
       const long long end = min((long long)length, max(start + i0 + d + 1, 0LL));
       limit = min(keys, (int)end - origin - part * kKeys);
     }
-    const unsigned slot = (unsigned)((seg - a.first) * a.span * s.selected + pair) * a.parts + part;
+    const unsigned slot = (unsigned)((seg - a.first) * a.span * s.selected + rec.z + e0 + e) * a.parts + part;
     to = r + r32 < rows ? slot * s.group + h : a.trash;
     const float* p = qb + (long long)d * a.ldq + h * s.qs;
 #pragma unroll
@@ -639,8 +645,8 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
   const bool live = row < rows && i < s.tq;
   const int* list = list_of(a, live ? b : 0, live ? i : 0, live ? g : 0);
   const int end = live ? visible(a, b, i) : 0, slots = s.selected * a.parts;
-  const long long first = live ? (query * slots) * s.group + h : 0;
-  const float* part = a.part + first * s.hd + min(c, s.hd - 4);
+  const long long home = live ? (long long)ls * a.span * s.selected : 0, first = live ? (long long)d * s.selected : 0;
+  const float* part = a.part + min(c, s.hd - 4);
   float top = -INFINITY, sum = 0.f;
   bool any = false;
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
@@ -649,7 +655,13 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
     const bool on = n < slots && block_seen(a, list[min(n, slots - 1) / a.parts], end);
     any |= on;
     float2 st = make_float2(-INFINITY, 0.f);
-    if (on) st = a.stat[first + (long long)n * s.group];
+    int at = 0;
+    if (on) {
+      const int p = n / a.parts;
+      const long long pair = a.pos ? a.pos[(long long)a.first * a.span * s.selected + home + first + p] : first + p;
+      at = (int)(((home + pair) * a.parts + (n - p * a.parts)) * s.group + h);
+      st = a.stat[at];
+    }
     float mx = st.x;
 #pragma unroll
     for (int off = 1; off < L; off <<= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
@@ -668,7 +680,7 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         w[u] = __shfl(f, (lane & ~(L - 1)) + min(u0 + u, L - 1));
-        v[u] = *(const f32x4*)(part + (long long)min(n0 + u0 + u, slots - 1) * s.group * s.hd);
+        v[u] = *(const f32x4*)(part + (long long)__shfl(at, (lane & ~(L - 1)) + min(u0 + u, L - 1)) * s.hd);
       }
 #pragma unroll
       for (int u = 0; u < 8; ++u)
@@ -787,6 +799,7 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
                stat_at = take(sizeof(float2) * (result_rows + 1));
   const size_t count_at = sorted ? take(sizeof(int) * segments * a.chunks * s.blocks) : 0;
   const size_t list_at = sorted ? take(sizeof(int) * segments * pairs) : 0;
+  const size_t pos_at = sorted ? take(sizeof(int) * segments * pairs) : 0;
   const size_t tile_at = sorted ? take(sizeof(int4) * segments * tile_cap) : 0;
   const size_t number_at = sorted ? take(sizeof(int) * segments) : 0;
   DeviceScope device(ctx);
@@ -795,6 +808,7 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   a.stat = (float2*)(ctx->scratch + stat_at);
   a.counts = (int*)(ctx->scratch + count_at);
   a.list = (int*)(ctx->scratch + list_at);
+  a.pos = sorted ? (int*)(ctx->scratch + pos_at) : nullptr;
   a.tiles = (int4*)(ctx->scratch + tile_at);
   a.tile_count = (int*)(ctx->scratch + number_at);
   const double keys = std::min((double)s.selected * s.bh * s.bw, (double)s.tk);
