@@ -9,6 +9,7 @@
 // they stand.
 #include <algorithm>
 #include <cfloat>
+#include <climits>
 #include <cmath>
 
 #include "split.h"
@@ -16,12 +17,18 @@
 
 namespace sy {
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kKeys = 64;    // keys of a tile; longer blocks are so many tiles ("parts" of the block)
-constexpr int kTileRows = 1024;
+constexpr int kTileRows = 1024;  // rows of a tile at most
 constexpr int kMaxBlocks = 12288;  // of a sorted list: counters in LDS
+
+// What a tile leaves for a row beside its weighted values: the maximum (as a power of two), the sum of weights, and the
+// power of two that the values want.
+struct Stat {
+  float top, sum;
+  int scale;
+};
 
 struct BlockArgs {
   const float *q, *k, *v;
@@ -41,7 +48,7 @@ struct BlockArgs {
   int* pos;          // place of each pair in its list
   int4* tiles;
   // Results of the launch's segments, row by row.
-  float2* stat;      // maximum (in powers of two) and sum
+  Stat* stat;
   float* part;       // weighted values
 };
 
@@ -137,8 +144,8 @@ __device__ __forceinline__ int2 scan_threads(int2 v, int2* lds, int2* total) {
 }
 
 // Puts the pairs in the order of their blocks (within a block in no certain order: a row's result does not
-// depend on its neighbours in a tile).  Every chunk's workgroup sums the counts of its segment for itself; the
-// first one writes the tiles.  With one chunk (`alone`) it does the counting, too.
+// depend on its neighbours in a tile).  Every chunk's workgroup sums the counts of its segment for itself and
+// writes the tiles of some blocks.  With one chunk it does the counting, too.
 __global__ __launch_bounds__(kSortThreads) void block_scatter_kernel(const BlockArgs a) {
   extern __shared__ int hist[];
   __shared__ int2 lds[kSortThreads / 64];
@@ -172,17 +179,15 @@ __global__ __launch_bounds__(kSortThreads) void block_scatter_kernel(const Block
     int2 total;
     const int2 at = scan_threads(make_int2(n, t * a.parts), lds, &total);
     if (j < s.blocks) hist[j] = base.x + at.x + before;
-    if (chunk == 0) {
-      work[threadIdx.x] = make_int4(base.x + at.x, n, base.y + at.y, t);
-      __syncthreads();
-      const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-      for (int u = wave; u < min(kSortThreads, s.blocks - j0); u += kSortThreads / 64) {
-        const int4 w = work[u];
-        for (int x = lane; x < w.w * a.parts; x += 64)
-          tiles[w.z + x] = make_int4(j0 + u, x % a.parts | (x / a.parts) << 8, w.x, w.y);
-      }
-      __syncthreads();
+    work[threadIdx.x] = make_int4(base.x + at.x, n, base.y + at.y, t);
+    __syncthreads();
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int u = wave * a.chunks + chunk; u < min(kSortThreads, s.blocks - j0); u += kSortThreads / 64 * a.chunks) {
+      const int4 w = work[u];
+      for (int x = lane; x < w.w * a.parts; x += 64)
+        tiles[w.z + x] = make_int4(j0 + u, x % a.parts | (x / a.parts) << 8, w.x, w.y);
     }
+    __syncthreads();
     base = make_int2(base.x + total.x, base.y + total.y);
   }
   if (chunk == 0 && threadIdx.x == 0) a.tile_count[seg] = base.y;
@@ -198,46 +203,59 @@ __global__ __launch_bounds__(kSortThreads) void block_scatter_kernel(const Block
 
 // ---------------------------------------------------------------------- tiles
 
-// Eight floats as three bf16 parts each, v = p[0] + p[1] + p[2] exactly.
-__device__ __forceinline__ void parts8(const float (&x)[8], bf16x8 (&p)[3]) {
-  u32x4 w[3];
+// Exponent field of the power of two that takes a largest magnitude m into [2^14, 2^15): a row in that range splits
+// into f16 pairs h + l within 2^-22 of each element, or 2^-39 of m where that is more.  Rows below 2^-113 keep
+// the largest scale there is, and with it every bit of a float.
+__device__ __forceinline__ int pair_field(float m) { return min(268 - (int)(__builtin_bit_cast(unsigned, m) >> 23), 254); }
+
+__device__ __forceinline__ void pairs8(const float (&x)[8], float s, f16x8& h, f16x8& l) {
+  u32x4 hw, lw;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    f32x2v v = {x[2 * i], x[2 * i + 1]};
-#pragma unroll
-    for (int s = 0; s < 3; ++s) {
-      const unsigned b = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
-      w[s][i] = b;
-      if (s < 2) {
-        v[0] -= __builtin_bit_cast(float, b << 16);
-        v[1] -= __builtin_bit_cast(float, b & 0xffff0000u);
-      }
-    }
+    const float a = x[2 * i], b = x[2 * i + 1];
+    const f16x2 hi = __builtin_convertvector((f32x2v{a * s, b * s}), f16x2);
+    const f32x2v r = {__builtin_fmaf(a, s, -(float)hi[0]), __builtin_fmaf(b, s, -(float)hi[1])};
+    hw[i] = __builtin_bit_cast(unsigned, hi);
+    lw[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(r, f16x2));
   }
-#pragma unroll
-  for (int s = 0; s < 3; ++s) p[s] = __builtin_bit_cast(bf16x8, w[s]);
+  h = __builtin_bit_cast(f16x8, hw);
+  l = __builtin_bit_cast(f16x8, lw);
 }
 
-// main + rest += a b: the leading parts' product in main, the five next ones in rest.
-__device__ __forceinline__ void mfma_parts(const bf16x8 (&a)[3], const bf16x8 (&b)[3], f32x16& main, f32x16& rest) {
-  rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[2], b[0], rest, 0, 0, 0);
-  main = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], main, 0, 0, 0);
-  rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[1], rest, 0, 0, 0);
-  rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[2], rest, 0, 0, 0);
-  rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[0], rest, 0, 0, 0);
-  rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[1], rest, 0, 0, 0);
+// Largest magnitude of eight; a NaN counts as the larger.
+__device__ __forceinline__ float max8(const float (&x)[8]) {
+  unsigned m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max(m, __builtin_bit_cast(unsigned, x[e]) & 0x7fffffffu);
+  return __builtin_bit_cast(float, m);
+}
+
+// Largest (non-negative, as bits) of W neighbouring lanes, in each of them.
+template <int W>
+__device__ __forceinline__ float max_lanes(float f) {
+  int m = __builtin_bit_cast(int, f);
+  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0xb1, 0xf, 0xf, false));               // lane ^ 1
+  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x4e, 0xf, 0xf, false));               // lane ^ 2
+  if (W > 4) m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x141, 0xf, 0xf, false));  // 7 - lane
+  if (W > 8) m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x140, 0xf, 0xf, false));  // 15 - lane
+  return __builtin_bit_cast(float, m);
 }
 
 // Work item of a workgroup: each of the 8 XCDs takes workgroups in turn, and with them one eighth of the items in a
 // row, so that tiles of one block and the queries of one head meet in one L2.
 __device__ __forceinline__ unsigned item_of(unsigned block, unsigned grid) { return (block & 7) * (grid >> 3) + (block >> 3); }
 
-// One tile: up to 64 keys of a block and a.rows rows of its list, 32 at a time for each of W waves.
+// One tile: up to 64 keys of a block and a.rows rows of its list, 32 at a time for each of four waves.
 //
-// Keys and values stand in LDS as three bf16 parts (Henry, Tang and Heinecke, 2019: a float's 24 bits over its whole
-// exponent range, six of the nine part products taken), in the order in which the matrix instruction's lanes
-// take them, so that a fragment is one 16-byte read without bank conflicts.  Once they stand there the waves run on
-// their own: no barrier, the next rows' queries under way while the weights meet the values.
+// Products of float32 on the f16 matrix cores: an operand is a pair h + l of f16 values under a power of two of its own
+// row (a query, a key, the values of a key, the weights of a query), and h h + h l + l h is taken: 3 x 2^-22 of
+// each product at most, whatever the other rows hold.  The powers of queries and keys come back onto the scores;
+// those of the values meet the weights before these are split, so that a key's weight counts as much as what it
+// brings; the last one, of the weights' row, is left to the join.
+//
+// Keys and values stand in LDS as pairs, in the order in which the matrix instruction's lanes take them, so that a
+// fragment is one 16-byte read without bank conflicts.  Once they stand there the waves run on their own: no
+// barrier, the next rows' queries under way while the weights meet the values.
 //
 // S^T = K Q^T: a lane holds one row's scores (keys 8 (r / 4) + 4 half + r % 4), so maximum and sum are in-lane
 // but for one exchange, and the weights are already the A operand of O = P V under the key order
@@ -246,15 +264,15 @@ __device__ __forceinline__ unsigned item_of(unsigned block, unsigned grid) { ret
 //
 // The maximum m is the largest score times c = scale log2(e), rounded once; weights are 2^(s c - m) with one
 // rounding of the exponent, and m is kept as it is, so that slots join exactly.
-template <int KS, int DT, int W, bool WHOLE>
-__global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(const BlockArgs a) {
-  constexpr int T = 64 * W;
-  constexpr int KF = 2 * KS * 3, VF = 4 * DT * 3;  // fragments of 64 lanes x 16 bytes
-  constexpr int KI = kKeys * KS * 2 / T;           // 8-channel pieces of keys per thread
-  constexpr int VI = 8 * 32 * DT / T;              // 8-key pieces of values per thread
+template <int KS, int DT, bool WHOLE>
+__global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(const BlockArgs a) {
+  constexpr int KF = 2 * KS * 2, VF = 4 * DT * 2;  // fragments of 64 lanes x 16 bytes
+  constexpr int KI = kKeys * KS * 2 / 256;         // 8-channel pieces of keys per thread
+  constexpr int VI = 8 * 32 * DT / 256;            // 8-key pieces of values per thread
   __shared__ u32x4 frag[(KF + VF) * 64];
   __shared__ unsigned k_at[kKeys], v_at[kKeys];    // floats from the block's first key
-  __shared__ unsigned place[W][32];
+  __shared__ __align__(16) int k_power[kKeys], v_power[kKeys], v_below[kKeys];  // of two; v_below: from the largest
+  __shared__ unsigned place[4][32];
   __shared__ int pair_at[kTileRows];
   const BlockShape& s = a.s;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -303,7 +321,7 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
 #pragma unroll
       for (int u = 0; u < 2; ++u) qr[ks][u] = *(const f32x4*)(p + min(16 * ks + 8 * half + 4 * u, s.kd - 4));
   };
-  for (int x = tid; x < (h0 + rows + s.group - 1) / s.group; x += T) pair_at[x] = list[e0 + x];
+  for (int x = tid; x < (h0 + rows + s.group - 1) / s.group; x += 256) pair_at[x] = list[e0 + x];
   if (tid < kKeys) {
     const int u = tid < keys ? part * kKeys + tid : 0, y = u / cols;
     k_at[tid] = (y * s.kw + u - y * cols) * (unsigned)a.ldk;
@@ -315,21 +333,29 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
   {
     const float* kb = a.k + ((long long)b * s.tk + origin) * a.ldk + (long long)g * s.ks;
     const float* vb = a.v + ((long long)b * s.tk + origin) * a.ldv + (long long)g * s.vs;
-    float kr[KI][8], vr[VI][8];
-#pragma unroll
-    for (int n = 0; n < KI; ++n) {
-      const int x = tid + T * n, key = x / (2 * KS), c = 8 * (x - key * 2 * KS);
-      const float* p = kb + (k_at[key] + c);
+    float kr[KI][8], vm[VI][8], vr[VI][8];
+    auto load8 = [&](const float* p, int c, int dim, float (&to8)[8]) __attribute__((always_inline)) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const f32x4 f = c + 4 * u < s.kd ? *(const f32x4*)(p + 4 * u) : f32x4{0.f, 0.f, 0.f, 0.f};
+        const f32x4 f = *(const f32x4*)(p + min(c + 4 * u, dim - 4));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) kr[n][4 * u + e] = f[e];
+        for (int e = 0; e < 4; ++e) to8[4 * u + e] = c + 4 * u < dim ? f[e] : 0.f;
       }
+    };
+#pragma unroll
+    for (int n = 0; n < KI; ++n) {
+      const int x = tid + 256 * n, key = x / (2 * KS);
+      load8(kb + k_at[key], 8 * (x - key * 2 * KS), s.kd, kr[n]);
+    }
+    // The values twice: a key's channels across neighbouring lanes, for their largest, and eight keys of a channel.
+#pragma unroll
+    for (int n = 0; n < VI; ++n) {
+      const int x = tid + 256 * n, key = x / (4 * DT);
+      load8(vb + v_at[key], 8 * (x - key * 4 * DT), s.hd, vm[n]);
     }
 #pragma unroll
     for (int n = 0; n < VI; ++n) {
-      const int x = tid + T * n, c = min(x % (32 * DT), s.hd - 1), piece = x / (32 * DT);  // piece: 2 step + half
+      const int x = tid + 256 * n, c = min(x % (32 * DT), s.hd - 1), piece = x / (32 * DT);  // piece: 2 step + half
       const int first = 16 * (piece >> 1) + 4 * (piece & 1);
 #pragma unroll
       for (int e = 0; e < 8; ++e) vr[n][e] = vb[v_at[first + 8 * (e >> 2) + (e & 3)] + c];
@@ -339,69 +365,91 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
     // different banks.
 #pragma unroll
     for (int n = 0; n < KI; ++n) {
-      const int x = tid + T * n, key = x / (2 * KS), c = x - key * 2 * KS;
-      bf16x8 p[3];
-      parts8(kr[n], p);
+      const int x = tid + 256 * n, key = x / (2 * KS), c = x - key * 2 * KS;
+      const int field = pair_field(max_lanes<2 * KS>(max8(kr[n])));
+      if (c == 0) k_power[key] = 127 - field;
+      f16x8 p[2];
+      pairs8(kr[n], exp_float(field), p[0], p[1]);
 #pragma unroll
-      for (int m = 0; m < 3; ++m)
-        frag[(((key >> 5) * KS + (c >> 1)) * 3 + m) * 64 + (c & 1) * 32 + ((key + c) & 31)] = __builtin_bit_cast(u32x4, p[m]);
+      for (int m = 0; m < 2; ++m)
+        frag[(((key >> 5) * KS + (c >> 1)) * 2 + m) * 64 + (c & 1) * 32 + ((key + c) & 31)] = __builtin_bit_cast(u32x4, p[m]);
     }
     // Keys that do not exist weigh nothing, whatever stands there.
-    if (keys < kKeys)
-#pragma unroll
-      for (int n = 0; n < VI; ++n) {
-        const int piece = (tid + T * n) / (32 * DT), first = 16 * (piece >> 1) + 4 * (piece & 1);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (first + 8 * (e >> 2) + (e & 3) >= keys) vr[n][e] = 0.f;
-      }
 #pragma unroll
     for (int n = 0; n < VI; ++n) {
-      const int x = tid + T * n, c = x % (32 * DT), piece = x / (32 * DT);
-      bf16x8 p[3];
-      parts8(vr[n], p);
+      const int x = tid + 256 * n, key = x / (4 * DT);
+      const int field = key < keys ? pair_field(max_lanes<4 * DT>(max8(vm[n]))) : 254;
+      if (x - key * 4 * DT == 0) v_power[key] = 127 - field;
+    }
+    __syncthreads();
+    if (tid < kKeys) v_below[tid] = v_power[tid] - wave_max_i32(v_power[tid]);
 #pragma unroll
-      for (int m = 0; m < 3; ++m)
-        frag[KF * 64 + (((piece >> 1) * DT + (c >> 5)) * 3 + m) * 64 + (piece & 1) * 32 + (c & 31)] =
+    for (int n = 0; n < VI; ++n) {
+      const int x = tid + 256 * n, c = x % (32 * DT), piece = x / (32 * DT);
+      const int first = 16 * (piece >> 1) + 4 * (piece & 1);
+      // Eight keys with a power each: scaled first, then split.
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int key = first + 8 * (e >> 2) + (e & 3);
+        f[e] = key < keys ? vr[n][e] * exp_float(127 - v_power[key]) : 0.f;
+      }
+      f16x8 p[2];
+      pairs8(f, 1.f, p[0], p[1]);
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+        frag[KF * 64 + (((piece >> 1) * DT + (c >> 5)) * 2 + m) * 64 + (piece & 1) * 32 + (c & 31)] =
             __builtin_bit_cast(u32x4, p[m]);
     }
   }
   __syncthreads();
+  const int v_most = v_power[0] - v_below[0];
 
   // The queries are here before the loop: in it they are waited for with the stores behind them still under way.
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   const float c = s.scale * 1.4426950408889634f;
-  for (; r < rows; r += 32 * W) {
+  for (; r < rows; r += 128) {
     f32x16 sc[2], rest[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int x = 0; x < 16; ++x) sc[t][x] = rest[t][x] = 0.f;
+    float qm = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qm = fmaxf(qm, fmaxf(max4(qr[ks][0]), max4(qr[ks][1])));
+    const int q_field = pair_field(fmaxf(qm, __shfl_xor(qm, 32)));
+    const float q_scale = exp_float(q_field);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      bf16x8 q[3];
+      f16x8 q[2];
       const float f[8] = {qr[ks][0][0], qr[ks][0][1], qr[ks][0][2], qr[ks][0][3],
                           qr[ks][1][0], qr[ks][1][1], qr[ks][1][2], qr[ks][1][3]};
-      parts8(f, q);
+      pairs8(f, q_scale, q[0], q[1]);
       const int at = half * 32 + ((r32 + 2 * ks + half) & 31);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        bf16x8 k[3];
-#pragma unroll
-        for (int m = 0; m < 3; ++m) k[m] = __builtin_bit_cast(bf16x8, frag[((t * KS + ks) * 3 + m) * 64 + at]);
-        mfma_parts(k, q, sc[t], rest[t]);
+        const f16x8 k0 = __builtin_bit_cast(f16x8, frag[((t * KS + ks) * 2) * 64 + at]);
+        const f16x8 k1 = __builtin_bit_cast(f16x8, frag[((t * KS + ks) * 2 + 1) * 64 + at]);
+        rest[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, q[0], rest[t], 0, 0, 0);
+        sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, q[0], sc[t], 0, 0, 0);
+        rest[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, q[1], rest[t], 0, 0, 0);
       }
     }
-    const int seen = limit;
+    const int seen = limit, q_power = 127 - q_field;
     const unsigned mine = to;
     place[wave][r32] = mine * (unsigned)(4 * s.hd);
-    load_q(min(r + 32 * W, rows - 1));  // the last turn: something, to keep the count of loads
+    load_q(min(r + 128, rows - 1));  // the last turn: something, to keep the count of loads
+    // Key 4 n + e of those that a lane holds is 8 n + 4 half + e.
     float w[32];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int n = 0; n < 8; ++n) {
+      const i32x4 power = *(const i32x4*)&k_power[8 * n + 4 * half];
 #pragma unroll
-      for (int x = 0; x < 16; ++x) w[16 * t + x] = sc[t][x] + rest[t][x];
-    if (__any(seen < kKeys))
+      for (int e = 0; e < 4; ++e)
+        w[4 * n + e] = __builtin_ldexpf(sc[n >> 2][4 * (n & 3) + e] + rest[n >> 2][4 * (n & 3) + e], power[e] + q_power);
+    }
+    const bool partly = __any(seen < kKeys);
+    if (partly)
 #pragma unroll
       for (int x = 0; x < 32; ++x)
         if (8 * (x >> 2) + 4 * half + (x & 3) >= seen) w[x] = -INFINITY;
@@ -416,13 +464,44 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
       sum += w[x];
     }
     sum += __shfl_xor(sum, 32);
-    a.stat[half ? a.trash : mine] = make_float2(mx, sum);
-    bf16x8 wp[4][3];
+    // Weights times the values' powers, from the largest of those that the row sees.
+    int most = v_most;
+    if (partly) {
+      most = -127;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const i32x4 power = *(const i32x4*)&v_power[8 * n + 4 * half];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (8 * n + 4 * half + e < seen) most = max(most, power[e]);
+      }
+      most = max(most, __shfl_xor(most, 32));
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const i32x4 power = *(const i32x4*)&v_power[8 * n + 4 * half];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[4 * n + e] = __builtin_ldexpf(w[4 * n + e], min(power[e] - most, 0));
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const i32x4 power = *(const i32x4*)&v_below[8 * n + 4 * half];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[4 * n + e] = __builtin_ldexpf(w[4 * n + e], power[e]);
+      }
+    }
+    float tm = 0.f;
+#pragma unroll
+    for (int x = 0; x < 32; ++x) tm = fmaxf(tm, w[x]);
+    const int w_field = pair_field(fmaxf(tm, __shfl_xor(tm, 32)));
+    const float w_scale = exp_float(w_field);
+    a.stat[half ? a.trash : mine] = Stat{mx, sum, most + 127 - w_field};
+    f16x8 wp[4][2];
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
       const float f[8] = {w[8 * st],     w[8 * st + 1], w[8 * st + 2], w[8 * st + 3],
                           w[8 * st + 4], w[8 * st + 5], w[8 * st + 6], w[8 * st + 7]};
-      parts8(f, wp[st]);
+      pairs8(f, w_scale, wp[st][0], wp[st][1]);
     }
     __builtin_amdgcn_wave_barrier();
     unsigned row_at[16];  // bytes
@@ -432,25 +511,20 @@ __global__ __launch_bounds__(64 * W, KS * DT >= 16 ? 2 : 3) void block_tile_kern
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       if (!WHOLE && 32 * d >= s.hd) break;
-      // The five small products of every step first, then the leading ones on top.
+      // The small products of every step first, then the leading ones on top.
       f32x16 acc;
 #pragma unroll
       for (int x = 0; x < 16; ++x) acc[x] = 0.f;
-      bf16x8 lead[4];
+      f16x8 lead[4];
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
-        bf16x8 v[3];
-#pragma unroll
-        for (int m = 0; m < 3; ++m) v[m] = __builtin_bit_cast(bf16x8, frag[KF * 64 + ((st * DT + d) * 3 + m) * 64 + lane]);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wp[st][2], v[0], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wp[st][1], v[1], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wp[st][0], v[2], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wp[st][1], v[0], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wp[st][0], v[1], acc, 0, 0, 0);
-        lead[st] = v[0];
+        lead[st] = __builtin_bit_cast(f16x8, frag[KF * 64 + ((st * DT + d) * 2) * 64 + lane]);
+        const f16x8 v1 = __builtin_bit_cast(f16x8, frag[KF * 64 + ((st * DT + d) * 2 + 1) * 64 + lane]);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(wp[st][1], lead[st], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(wp[st][0], v1, acc, 0, 0, 0);
       }
 #pragma unroll
-      for (int st = 0; st < 4; ++st) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wp[st][0], lead[st], acc, 0, 0, 0);
+      for (int st = 0; st < 4; ++st) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(wp[st][0], lead[st], acc, 0, 0, 0);
       char* base = (char*)(a.part + 32 * d);
       if (WHOLE || 32 * d + r32 < s.hd)
 #pragma unroll
@@ -568,7 +642,7 @@ __global__ __launch_bounds__(256) void block_few_kernel(const BlockArgs a) {
     if (tid == 0)
 #pragma unroll
       for (int h = 0; h < kFewRows; ++h)
-        if (h < heads) a.stat[slot * s.group + h0 + h] = make_float2(mx[h], sum[h]);
+        if (h < heads) a.stat[slot * s.group + h0 + h] = Stat{mx[h], sum[h], 0};
   }
 }
 
@@ -648,13 +722,14 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
   const long long home = live ? (long long)ls * a.span * s.selected : 0, first = live ? (long long)d * s.selected : 0;
   const float* part = a.part + min(c, s.hd - 4);
   float top = -INFINITY, sum = 0.f;
+  int power = INT_MIN;  // of y
   bool any = false;
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
   for (int n0 = 0; n0 < slots; n0 += L) {
     const int n = n0 + sub;
     const bool on = n < slots && block_seen(a, list[min(n, slots - 1) / a.parts], end);
     any |= on;
-    float2 st = make_float2(-INFINITY, 0.f);
+    Stat st = {-INFINITY, 0.f, INT_MIN};
     int at = 0;
     if (on) {
       const int p = n / a.parts;
@@ -662,24 +737,31 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
       at = (int)(((home + pair) * a.parts + (n - p * a.parts)) * s.group + h);
       st = a.stat[at];
     }
-    float mx = st.x;
+    float mx = st.top;
+    int most = st.scale;
 #pragma unroll
-    for (int off = 1; off < L; off <<= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
+    for (int off = 1; off < L; off <<= 1) {
+      mx = fmaxf(mx, __shfl_xor(mx, off));
+      most = max(most, __shfl_xor(most, off));
+    }
     mx = fmaxf(mx, top);
+    most = max(most, power);
     // Negative: there is nothing to read.  A slot without weight is read all the same: a NaN in it is the row's.
-    const float f = !on ? -1.f : st.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.x - mx);
+    const float f = !on ? -1.f : st.top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.top - mx);
     const float old = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - mx);
     top = mx;
-    sum = __builtin_fmaf(sum, old, st.y * f);
+    sum = __builtin_fmaf(sum, old, st.sum * f);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] *= old;
+    for (int e = 0; e < 4; ++e) y[e] = power == INT_MIN ? 0.f : __builtin_ldexpf(y[e] * old, power - most);
+    power = most;
+    const float fv = on ? __builtin_ldexpf(f, st.scale - most) : -1.f;
     const int count = min(L, slots - n0);
     for (int u0 = 0; u0 < count; u0 += 8) {
       f32x4 v[8];
       float w[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        w[u] = __shfl(f, (lane & ~(L - 1)) + min(u0 + u, L - 1));
+        w[u] = __shfl(fv, (lane & ~(L - 1)) + min(u0 + u, L - 1));
         v[u] = *(const f32x4*)(part + (long long)__shfl(at, (lane & ~(L - 1)) + min(u0 + u, L - 1)) * s.hd);
       }
 #pragma unroll
@@ -697,7 +779,7 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
   bool again = false;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    y[e] = any ? y[e] / sum : 0.f;
+    y[e] = any ? __builtin_ldexpf(y[e] / sum, power) : 0.f;
     again |= live && c < s.hd && !(__builtin_fabsf(y[e]) <= FLT_MAX);
   }
   if (live && c < s.hd) *(f32x4*)(a.o + ((long long)b * s.tq + i) * a.ldo + (long long)(g * s.group + h) * s.hd + c) = y;
@@ -796,7 +878,7 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
     return from;
   };
   const size_t part_at = take(sizeof(float) * ((result_rows + 1) * s.hd + 128)),
-               stat_at = take(sizeof(float2) * (result_rows + 1));
+               stat_at = take(sizeof(Stat) * (result_rows + 1));
   const size_t count_at = sorted ? take(sizeof(int) * segments * a.chunks * s.blocks) : 0;
   const size_t list_at = sorted ? take(sizeof(int) * segments * pairs) : 0;
   const size_t pos_at = sorted ? take(sizeof(int) * segments * pairs) : 0;
@@ -805,7 +887,7 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   DeviceScope device(ctx);
   SY_TRY(ensure_scratch(ctx, at));
   a.part = (float*)(ctx->scratch + part_at);
-  a.stat = (float2*)(ctx->scratch + stat_at);
+  a.stat = (Stat*)(ctx->scratch + stat_at);
   a.counts = (int*)(ctx->scratch + count_at);
   a.list = (int*)(ctx->scratch + list_at);
   a.pos = sorted ? (int*)(ctx->scratch + pos_at) : nullptr;
@@ -830,24 +912,22 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
                      share * 4.0 * s.n * ((double)s.tq * s.heads * (s.kd + s.hd) + (double)s.tk * s.kv * (s.kd + s.hd)));
       if (sorted) {
         const unsigned grid = (unsigned)((now * tile_cap + 7) / 8 * 8);
-        auto launch = [&](auto kernel, int waves) {
-          hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * waves), 0, ctx->stream, a);
-        };
-        auto pick = [&](auto whole2, auto part2, auto whole4, auto part4, int waves4) {
+        auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, ctx->stream, a); };
+        auto pick = [&](auto whole2, auto part2, auto whole4, auto part4) {
           if (s.hd <= 64)
-            s.hd == 64 ? launch(whole2, 4) : launch(part2, 4);
+            launch(s.hd == 64 ? whole2 : part2);
           else
-            s.hd == 128 ? launch(whole4, waves4) : launch(part4, waves4);
+            launch(s.hd == 128 ? whole4 : part4);
         };
         if (s.kd <= 32)
-          pick(block_tile_kernel<2, 2, 4, true>, block_tile_kernel<2, 2, 4, false>, block_tile_kernel<2, 4, 4, true>,
-               block_tile_kernel<2, 4, 4, false>, 4);
+          pick(block_tile_kernel<2, 2, true>, block_tile_kernel<2, 2, false>, block_tile_kernel<2, 4, true>,
+               block_tile_kernel<2, 4, false>);
         else if (s.kd <= 64)
-          pick(block_tile_kernel<4, 2, 4, true>, block_tile_kernel<4, 2, 4, false>, block_tile_kernel<4, 4, 4, true>,
-               block_tile_kernel<4, 4, 4, false>, 4);
+          pick(block_tile_kernel<4, 2, true>, block_tile_kernel<4, 2, false>, block_tile_kernel<4, 4, true>,
+               block_tile_kernel<4, 4, false>);
         else
-          pick(block_tile_kernel<8, 2, 4, true>, block_tile_kernel<8, 2, 4, false>, block_tile_kernel<8, 4, 8, true>,
-               block_tile_kernel<8, 4, 8, false>, 8);
+          pick(block_tile_kernel<8, 2, true>, block_tile_kernel<8, 2, false>, block_tile_kernel<8, 4, true>,
+               block_tile_kernel<8, 4, false>);
       } else {
         const dim3 grid((unsigned)(now * pairs * a.parts));
         if (s.kd <= 64)

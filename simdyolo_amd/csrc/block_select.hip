@@ -223,17 +223,6 @@ __device__ __forceinline__ int seen_blocks(const SelectArgs& a, int b, int i, in
   return (int)seen;
 }
 
-// The largest of a wave's values, in every lane.
-__device__ __forceinline__ int wave_max_i32(int m) {
-  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x111, 0xf, 0xf, false));  // shifts within rows of 16
-  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x112, 0xf, 0xf, false));
-  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x114, 0xf, 0xf, false));
-  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x118, 0xf, 0xf, false));
-  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x142, 0xa, 0xf, false));  // row 0 / 2 into 1 / 3, 1 into 2 and 3
-  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x143, 0xc, 0xf, false));
-  return __builtin_amdgcn_readlane(m, 63);
-}
-
 // Ranking by one wave: of the keys key(j), j < count, the `selected` largest, ties by the lower j.  Lane n ends with the
 // n-th; the number of them is returned.  Every lane keeps four new keys and one of the best so far in order;
 // the largest head of all is taken `selected` times.

@@ -137,4 +137,15 @@ __device__ __forceinline__ void unscale(const float (&ws)[TN], int se, f32x16 (&
         acc[i][j][r] = __builtin_fmaf(crs[i][j][r], 1.f / 2048, acc[i][j][r]) * xs * ws[j];
 }
 
+// The largest of a wave's values, in every lane.
+__device__ __forceinline__ int wave_max_i32(int m) {
+  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x111, 0xf, 0xf, false));  // shifts within rows of 16
+  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x112, 0xf, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x114, 0xf, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x118, 0xf, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x142, 0xa, 0xf, false));  // row 0 / 2 into 1 / 3, 1 into 2 and 3
+  m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(m, 63);
+}
+
 }  // namespace sy
