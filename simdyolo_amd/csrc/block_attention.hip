@@ -20,7 +20,7 @@ namespace sy {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kKeys = 64;    // keys of a tile; longer blocks are so many tiles ("parts" of the block)
-constexpr int kTileRows = 1024;  // rows of a tile at most
+constexpr int kTileRows = 512;  // rows of a tile at most
 constexpr int kMaxBlocks = 12288;  // of a sorted list: counters in LDS
 
 // What a tile leaves for a row beside its weighted values: the maximum (as a power of two), the sum of weights, and the
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(
   constexpr int KI = kKeys * KS * 2 / 256;         // 8-channel pieces of keys per thread
   constexpr int VI = 8 * 32 * DT / 256;            // 8-key pieces of values per thread
   __shared__ u32x4 frag[(KF + VF) * 64];
-  __shared__ unsigned k_at[kKeys], v_at[kKeys];    // floats from the block's first key
+  __shared__ unsigned v_at[kKeys];                 // floats from the block's first key
   __shared__ __align__(16) int k_power[kKeys], v_power[kKeys], v_below[kKeys];  // of two; v_below: from the largest
   __shared__ unsigned place[4][32];
   __shared__ int pair_at[kTileRows];
@@ -283,10 +283,13 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(
   const int t = item - seg * a.tile_cap;
   if (seg >= a.now) return;
   seg += a.first;
+  const int4 rec = a.tiles[(long long)seg * a.tile_cap + t];  // under way with the count
   if (t >= a.tile_count[seg]) return;
-  const int4 rec = a.tiles[(long long)seg * a.tile_cap + t];
-  const int j = rec.x, part = rec.y & 255, row0 = (rec.y >> 8) * a.rows;
-  const int rows = min(rec.w * s.group - row0, a.rows);
+  // Its share of the block's rows: as many as the other tiles', in 32s.
+  const int all = rec.w * s.group, tiles = (all + a.rows - 1) / a.rows, share = ((all + tiles - 1) / tiles + 31) & ~31;
+  const int j = rec.x, part = rec.y & 255, row0 = (rec.y >> 8) * share;
+  const int rows = min(all - row0, share);
+  if (rows <= 0) return;
   const int plane = seg / a.segs, b = plane / s.kv, g = plane - b * s.kv, i0 = (seg - plane * a.segs) * a.span;
   const int* list = a.list + (long long)seg * a.span * s.selected + rec.z;
   const int y0 = j / s.bx * s.bh, x0 = j % s.bx * s.bw;
@@ -321,13 +324,17 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(
 #pragma unroll
       for (int u = 0; u < 2; ++u) qr[ks][u] = *(const f32x4*)(p + min(16 * ks + 8 * half + 4 * u, s.kd - 4));
   };
-  for (int x = tid; x < (h0 + rows + s.group - 1) / s.group; x += 256) pair_at[x] = list[e0 + x];
-  if (tid < kKeys) {
-    const int u = tid < keys ? part * kKeys + tid : 0, y = u / cols;
-    k_at[tid] = (y * s.kw + u - y * cols) * (unsigned)a.ldk;
-    v_at[tid] = (y * s.kw + u - y * cols) * (unsigned)a.ldv;
-  }
-  __syncthreads();
+  // The key's place in floats from the block's first one; a quotient of numbers below 2^11, exact in float32.
+  const float per_row = 1.f / cols;
+  auto key_at = [&](int key, long long ld) __attribute__((always_inline)) {
+    const int u = key < keys ? part * kKeys + key : 0, y = (int)((u + 0.5f) * per_row);
+    return (unsigned)(y * s.kw + u - y * cols) * (unsigned)ld;
+  };
+  static_assert(kTileRows <= 512, "two pairs to a thread");
+  const int entries = (h0 + rows + s.group - 1) / s.group;
+  int first_pair[2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) first_pair[n] = list[e0 + min(tid + 256 * n, entries - 1)];
 
   int r = wave * 32;
   {
@@ -345,14 +352,20 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(
 #pragma unroll
     for (int n = 0; n < KI; ++n) {
       const int x = tid + 256 * n, key = x / (2 * KS);
-      load8(kb + k_at[key], 8 * (x - key * 2 * KS), s.kd, kr[n]);
+      load8(kb + key_at(key, a.ldk), 8 * (x - key * 2 * KS), s.kd, kr[n]);
     }
     // The values twice: a key's channels across neighbouring lanes, for their largest, and eight keys of a channel.
 #pragma unroll
     for (int n = 0; n < VI; ++n) {
       const int x = tid + 256 * n, key = x / (4 * DT);
-      load8(vb + v_at[key], 8 * (x - key * 4 * DT), s.hd, vm[n]);
+      load8(vb + key_at(key, a.ldv), 8 * (x - key * 4 * DT), s.hd, vm[n]);
     }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+      if (tid + 256 * n < kTileRows) pair_at[tid + 256 * n] = first_pair[n];
+    if (tid < kKeys) v_at[tid] = key_at(tid, a.ldv);
+    __syncthreads();
+    load_q(r);
 #pragma unroll
     for (int n = 0; n < VI; ++n) {
       const int x = tid + 256 * n, c = min(x % (32 * DT), s.hd - 1), piece = x / (32 * DT);  // piece: 2 step + half
@@ -360,7 +373,6 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(
 #pragma unroll
       for (int e = 0; e < 8; ++e) vr[n][e] = vb[v_at[first + 8 * (e >> 2) + (e & 3)] + c];
     }
-    load_q(r);
     // Piece c of key t: lanes t % 32 + 32 (c % 2) of step c / 2, turned by c so that a thread group's writes meet
     // different banks.
 #pragma unroll
@@ -448,7 +460,12 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(
       for (int e = 0; e < 4; ++e)
         w[4 * n + e] = __builtin_ldexpf(sc[n >> 2][4 * (n & 3) + e] + rest[n >> 2][4 * (n & 3) + e], power[e] + q_power);
     }
-    const bool partly = __any(seen < kKeys);
+    // Keys that do not exist, and in a causal tile those that some rows do not see.
+    const bool partly = __any(seen < keys);
+    if (keys < kKeys && !partly)
+#pragma unroll
+      for (int x = 0; x < 32; ++x)
+        if (8 * (x >> 2) + 4 * half + (x & 3) >= keys) w[x] = -INFINITY;
     if (partly)
 #pragma unroll
       for (int x = 0; x < 32; ++x)
@@ -796,14 +813,10 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
   }
 }
 
-// Bytes of results that one launch leaves and the next one joins.
-#ifndef SORT_FROM
-#define SORT_FROM 64
-#endif
-#ifndef KP
-#define KP 768e6
-#endif
-constexpr double kPartials = KP;
+// Bytes of results that one launch leaves and the next one joins.  Fewer would stay in the 256 MiB cache in front of
+// memory, but cost more in half-filled launches: 8,192 causal tokens of 16 heads (1.0 GB) 950 us in pieces of 256 MB, 695 of
+// 400 MB, 687 in one.
+constexpr double kPartials = 1200e6;
 
 int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q, const sy_tensor* k,
                        const sy_tensor* v, const int32_t* blocks, const int32_t* starts, const int32_t* lengths,
@@ -854,10 +867,16 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   a.segs = (s.tq + a.span - 1) / a.span;
   const long long segments = (long long)planes * a.segs;
   const int together = (int)std::min<double>((double)segments, std::max(1.0, std::floor(kPartials / (per_query * a.span))));
-  const bool sorted = s.blocks <= kMaxBlocks && (long long)s.tq * s.selected > SORT_FROM;
-  // Rows of a tile: many, so that the keys are laid out seldom, but four rounds of tiles on the whole chip.
+  // Pair by pair where sorting would not save many tiles: a tile of either kind takes about 10 ns (of 128 channels a
+  // sorted one 30), the sort and its longer tiles 10 us.  64 queries of 4 heads, 16 of 512 blocks each: 48 us pair by
+  // pair, 81 sorted; 256 queries 153 and 89; one 20x20 map (2 heads, 4 of 25 blocks) 32 and 21.
+  const double singles = (double)planes * s.tq * s.selected * a.parts;
+  const double shared = (double)planes * a.parts * std::min((double)s.blocks, (double)s.tq * s.selected);
+  const bool sorted = s.blocks <= kMaxBlocks && singles > 1.5 * shared + 1024;
+  // Rows of a tile at most: many, so that the keys are laid out seldom, but a round of tiles on the whole chip (three
+  // workgroups to a CU).
   a.rows = kTileRows;
-  while (a.rows > 256 && (double)together * a.span * s.selected * a.parts * s.group < 4096.0 * a.rows) a.rows /= 2;
+  while (a.rows > 128 && (double)together * a.span * s.selected * a.parts * s.group < 768.0 * a.rows) a.rows /= 2;
   // 2048 pairs to a workgroup of the sort, but at most 32 of them to a segment (each reads all their counts).
   a.chunk = std::max(std::max(1, 2048 / s.selected), (a.span + 31) / 32);
   a.chunks = (a.span + a.chunk - 1) / a.chunk;
