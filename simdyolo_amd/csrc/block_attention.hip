@@ -19,6 +19,7 @@ namespace sy {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
+constexpr int kFlat = 8;
 constexpr int kKeys = 64;    // keys of a tile; longer blocks are so many tiles ("parts" of the block)
 constexpr int kTileRows = 512;  // rows of a tile at most
 constexpr int kMaxBlocks = 12288;  // of a sorted list: counters in LDS
@@ -251,7 +252,9 @@ __device__ __forceinline__ unsigned item_of(unsigned block, unsigned grid) { ret
 // row (a query, a key, the values of a key, the weights of a query), and h h + h l + l h is taken: 3 x 2^-22 of
 // each product at most, whatever the other rows hold.  The powers of queries and keys come back onto the scores;
 // those of the values meet the weights before these are split, so that a key's weight counts as much as what it
-// brings; the last one, of the weights' row, is left to the join.
+// brings; the last one, of the weights' row, is left to the join.  Where the largest elements of all keys (of all
+// values) of a tile are within 2^kFlat of each other they share one power, which keeps 2^(kFlat - 39) of a
+// row's largest element and needs no power per score (per weight).
 //
 // Keys and values stand in LDS as pairs, in the order in which the matrix instruction's lanes take them, so that a
 // fragment is one 16-byte read without bank conflicts.  Once they stand there the waves run on their own: no
@@ -265,13 +268,14 @@ __device__ __forceinline__ unsigned item_of(unsigned block, unsigned grid) { ret
 // The maximum m is the largest score times c = scale log2(e), rounded once; weights are 2^(s c - m) with one
 // rounding of the exponent, and m is kept as it is, so that slots join exactly.
 template <int KS, int DT, bool WHOLE>
-__global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(const BlockArgs a) {
+__global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void block_tile_kernel(const BlockArgs a) {
   constexpr int KF = 2 * KS * 2, VF = 4 * DT * 2;  // fragments of 64 lanes x 16 bytes
   constexpr int KI = kKeys * KS * 2 / 256;         // 8-channel pieces of keys per thread
   constexpr int VI = 8 * 32 * DT / 256;            // 8-key pieces of values per thread
   __shared__ u32x4 frag[(KF + VF) * 64];
   __shared__ unsigned v_at[kKeys];                 // floats from the block's first key
-  __shared__ __align__(16) int k_power[kKeys], v_power[kKeys], v_below[kKeys];  // of two; v_below: from the largest
+  __shared__ float k_top[kKeys], v_top[kKeys];     // largest magnitude of a key, of its values
+  __shared__ __align__(16) int k_power[kKeys], v_power[kKeys];
   __shared__ unsigned place[4][32];
   __shared__ int pair_at[kTileRows];
   const BlockShape& s = a.s;
@@ -336,7 +340,8 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(
 #pragma unroll
   for (int n = 0; n < 2; ++n) first_pair[n] = list[e0 + min(tid + 256 * n, entries - 1)];
 
-  int r = wave * 32;
+  int r = wave * 32, k_one, v_most;
+  bool k_flat, v_flat;
   {
     const float* kb = a.k + ((long long)b * s.tk + origin) * a.ldk + (long long)g * s.ks;
     const float* vb = a.v + ((long long)b * s.tk + origin) * a.ldv + (long long)g * s.vs;
@@ -373,41 +378,58 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(
 #pragma unroll
       for (int e = 0; e < 8; ++e) vr[n][e] = vb[v_at[first + 8 * (e >> 2) + (e & 3)] + c];
     }
+    // Keys that do not exist weigh nothing, whatever stands there.
+#pragma unroll
+    for (int n = 0; n < KI; ++n) {
+      const int x = tid + 256 * n, key = x / (2 * KS);
+      const float top = max_lanes<2 * KS>(max8(kr[n]));
+      if (x - key * 2 * KS == 0) k_top[key] = key < keys ? top : 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < VI; ++n) {
+      const int x = tid + 256 * n, key = x / (4 * DT);
+      const float top = max_lanes<4 * DT>(max8(vm[n]));
+      if (x - key * 4 * DT == 0) v_top[key] = key < keys ? top : 0.f;
+    }
+    __syncthreads();
+    // One power for the whole tile where its rows are of one size.
+    const float kt = k_top[lane], vt = v_top[lane];
+    const int kp = 127 - pair_field(kt), vp = 127 - pair_field(vt), k_most = wave_max_i32(kp);
+    v_most = wave_max_i32(vp);
+    k_flat = !__any(kt != 0.f && kp < k_most - kFlat);
+    v_flat = !__any(vt != 0.f && vp < v_most - kFlat);
+    k_one = k_most;
+    if (wave == 0) {
+      k_power[lane] = kp;
+      v_power[lane] = vp;
+    }
     // Piece c of key t: lanes t % 32 + 32 (c % 2) of step c / 2, turned by c so that a thread group's writes meet
     // different banks.
 #pragma unroll
     for (int n = 0; n < KI; ++n) {
       const int x = tid + 256 * n, key = x / (2 * KS), c = x - key * 2 * KS;
-      const int field = pair_field(max_lanes<2 * KS>(max8(kr[n])));
-      if (c == 0) k_power[key] = 127 - field;
       f16x8 p[2];
-      pairs8(kr[n], exp_float(field), p[0], p[1]);
+      pairs8(kr[n], exp_float(k_flat ? 127 - k_most : pair_field(k_top[key])), p[0], p[1]);
 #pragma unroll
       for (int m = 0; m < 2; ++m)
         frag[(((key >> 5) * KS + (c >> 1)) * 2 + m) * 64 + (c & 1) * 32 + ((key + c) & 31)] = __builtin_bit_cast(u32x4, p[m]);
     }
-    // Keys that do not exist weigh nothing, whatever stands there.
-#pragma unroll
-    for (int n = 0; n < VI; ++n) {
-      const int x = tid + 256 * n, key = x / (4 * DT);
-      const int field = key < keys ? pair_field(max_lanes<4 * DT>(max8(vm[n]))) : 254;
-      if (x - key * 4 * DT == 0) v_power[key] = 127 - field;
-    }
-    __syncthreads();
-    if (tid < kKeys) v_below[tid] = v_power[tid] - wave_max_i32(v_power[tid]);
 #pragma unroll
     for (int n = 0; n < VI; ++n) {
       const int x = tid + 256 * n, c = x % (32 * DT), piece = x / (32 * DT);
       const int first = 16 * (piece >> 1) + 4 * (piece & 1);
-      // Eight keys with a power each: scaled first, then split.
-      float f[8];
+      float scale = exp_float(127 - v_most);
+      if (!v_flat) {  // a power for each of the eight: scaled before the split
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int key = first + 8 * (e >> 2) + (e & 3);
-        f[e] = key < keys ? vr[n][e] * exp_float(127 - v_power[key]) : 0.f;
+        for (int e = 0; e < 8; ++e) vr[n][e] *= exp_float(pair_field(v_top[first + 8 * (e >> 2) + (e & 3)]));
+        scale = 1.f;
       }
+      if (keys < kKeys)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (first + 8 * (e >> 2) + (e & 3) >= keys) vr[n][e] = 0.f;
       f16x8 p[2];
-      pairs8(f, 1.f, p[0], p[1]);
+      pairs8(vr[n], scale, p[0], p[1]);
 #pragma unroll
       for (int m = 0; m < 2; ++m)
         frag[KF * 64 + (((piece >> 1) * DT + (c >> 5)) * 2 + m) * 64 + (piece & 1) * 32 + (c & 31)] =
@@ -415,11 +437,17 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(
     }
   }
   __syncthreads();
-  const int v_most = v_power[0] - v_below[0];
+
+  auto k_at = [&](int t, int ks, int m) __attribute__((always_inline)) {
+    return __builtin_bit_cast(f16x8, frag[((t * KS + ks) * 2 + m) * 64 + half * 32 + ((r32 + 2 * ks + half) & 31)]);
+  };
+  auto v_at_lane = [&](int st, int d, int m) __attribute__((always_inline)) {
+    return __builtin_bit_cast(f16x8, frag[KF * 64 + ((st * DT + d) * 2 + m) * 64 + lane]);
+  };
 
   // The queries are here before the loop: in it they are waited for with the stores behind them still under way.
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-  const float c = s.scale * 1.4426950408889634f;
+  const float cs = s.scale * 1.4426950408889634f;
   for (; r < rows; r += 128) {
     f32x16 sc[2], rest[2];
 #pragma unroll
@@ -437,11 +465,9 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(
       const float f[8] = {qr[ks][0][0], qr[ks][0][1], qr[ks][0][2], qr[ks][0][3],
                           qr[ks][1][0], qr[ks][1][1], qr[ks][1][2], qr[ks][1][3]};
       pairs8(f, q_scale, q[0], q[1]);
-      const int at = half * 32 + ((r32 + 2 * ks + half) & 31);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const f16x8 k0 = __builtin_bit_cast(f16x8, frag[((t * KS + ks) * 2) * 64 + at]);
-        const f16x8 k1 = __builtin_bit_cast(f16x8, frag[((t * KS + ks) * 2 + 1) * 64 + at]);
+        const f16x8 k0 = k_at(t, ks, 0), k1 = k_at(t, ks, 1);
         rest[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, q[0], rest[t], 0, 0, 0);
         sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, q[0], sc[t], 0, 0, 0);
         rest[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, q[1], rest[t], 0, 0, 0);
@@ -452,13 +478,18 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(
     place[wave][r32] = mine * (unsigned)(4 * s.hd);
     load_q(min(r + 128, rows - 1));  // the last turn: something, to keep the count of loads
     // Key 4 n + e of those that a lane holds is 8 n + 4 half + e.
-    float w[32];
+    float w[32], c = cs;
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const i32x4 power = *(const i32x4*)&k_power[8 * n + 4 * half];
+    for (int x = 0; x < 32; ++x) w[x] = sc[x >> 4][x & 15] + rest[x >> 4][x & 15];
+    if (k_flat) {
+      c = __builtin_ldexpf(cs, k_one + q_power);
+    } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[4 * n + e] = __builtin_ldexpf(sc[n >> 2][4 * (n & 3) + e] + rest[n >> 2][4 * (n & 3) + e], power[e] + q_power);
+      for (int n = 0; n < 8; ++n) {
+        const i32x4 power = *(const i32x4*)&k_power[8 * n + 4 * half];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[4 * n + e] = __builtin_ldexpf(w[4 * n + e], power[e] + q_power);
+      }
     }
     // Keys that do not exist, and in a causal tile those that some rows do not see.
     const bool partly = __any(seen < keys);
@@ -481,36 +512,33 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(
       sum += w[x];
     }
     sum += __shfl_xor(sum, 32);
-    // Weights times the values' powers, from the largest of those that the row sees.
-    int most = v_most;
-    if (partly) {
-      most = -127;
+    // Where values differ in size: weights times their powers, from the largest of those that the row sees, and under a
+    // power of the row.  (One power for all: weights are at most 1.)
+    int most = v_most, w_field = 127 + 14;
+    if (!v_flat) {
+      if (partly) {
+        most = -127;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const i32x4 power = *(const i32x4*)&v_power[8 * n + 4 * half];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (8 * n + 4 * half + e < seen) most = max(most, power[e]);
+        }
+        most = max(most, __shfl_xor(most, 32));
+      }
+      float tm = 0.f;
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
         const i32x4 power = *(const i32x4*)&v_power[8 * n + 4 * half];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (8 * n + 4 * half + e < seen) most = max(most, power[e]);
+        for (int e = 0; e < 4; ++e) {
+          w[4 * n + e] = __builtin_ldexpf(w[4 * n + e], min(power[e] - most, 0));
+          tm = fmaxf(tm, w[4 * n + e]);
+        }
       }
-      most = max(most, __shfl_xor(most, 32));
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const i32x4 power = *(const i32x4*)&v_power[8 * n + 4 * half];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[4 * n + e] = __builtin_ldexpf(w[4 * n + e], min(power[e] - most, 0));
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const i32x4 power = *(const i32x4*)&v_below[8 * n + 4 * half];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[4 * n + e] = __builtin_ldexpf(w[4 * n + e], power[e]);
-      }
+      w_field = pair_field(fmaxf(tm, __shfl_xor(tm, 32)));
     }
-    float tm = 0.f;
-#pragma unroll
-    for (int x = 0; x < 32; ++x) tm = fmaxf(tm, w[x]);
-    const int w_field = pair_field(fmaxf(tm, __shfl_xor(tm, 32)));
     const float w_scale = exp_float(w_field);
     a.stat[half ? a.trash : mine] = Stat{mx, sum, most + 127 - w_field};
     f16x8 wp[4][2];
@@ -535,8 +563,8 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : 3) void block_tile_kernel(
       f16x8 lead[4];
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
-        lead[st] = __builtin_bit_cast(f16x8, frag[KF * 64 + ((st * DT + d) * 2) * 64 + lane]);
-        const f16x8 v1 = __builtin_bit_cast(f16x8, frag[KF * 64 + ((st * DT + d) * 2 + 1) * 64 + lane]);
+        lead[st] = v_at_lane(st, d, 0);
+        const f16x8 v1 = v_at_lane(st, d, 1);
         acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(wp[st][1], lead[st], acc, 0, 0, 0);
         acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(wp[st][0], v1, acc, 0, 0, 0);
       }
