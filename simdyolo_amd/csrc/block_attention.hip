@@ -889,12 +889,14 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   const int planes = s.n * s.kv;
   SY_CHECK((long long)s.n * s.kv < (1 << 24) && (long long)s.tq * s.selected < (1LL << 31), SY_EUNSUPPORTED,
            "block attention over %d x %d queries", s.n, s.tq);
-  // Segments: as many queries as keep the results of one in kPartials bytes.
-  const double per_query = 4.0 * s.selected * a.parts * s.group * (s.hd + 2);
-  a.span = (int)std::min<double>(s.tq, std::max(1.0, std::floor(kPartials / per_query)));
+  // Segments: as many queries as keep the results of one in kPartials bytes
+  // (and, pair by pair, its workgroups in 2^23), and as many segments to a launch.
+  const double per_query = std::max((sizeof(float) * s.hd + sizeof(Stat)) * (double)s.selected * a.parts * s.group / kPartials,
+                                    (double)s.selected * a.parts / (1 << 23));  // share of a launch
+  a.span = (int)std::min<double>(s.tq, std::max(1.0, std::floor(1.0 / per_query)));
   a.segs = (s.tq + a.span - 1) / a.span;
   const long long segments = (long long)planes * a.segs;
-  const int together = (int)std::min<double>((double)segments, std::max(1.0, std::floor(kPartials / (per_query * a.span))));
+  const int together = (int)std::min<double>((double)segments, std::max(1.0, std::floor(1.0 / (per_query * a.span))));
   // Pair by pair where sorting would not save many tiles: a tile of either kind takes about 10 ns (of 128 channels a
   // sorted one 30), the sort and its longer tiles 10 us.  64 queries of 4 heads, 16 of 512 blocks each: 48 us pair by
   // pair, 81 sorted; 256 queries 153 and 89; one 20x20 map (2 heads, 4 of 25 blocks) 32 and 21.

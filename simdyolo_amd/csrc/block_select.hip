@@ -196,8 +196,9 @@ struct SelectArgs {
   u32x4* parts;
   float* norm;
   int tiles, chunks;
-  // few queries: scores
+  // few queries: scores, and how many of them a workgroup takes
   long long* keys;
+  int queries;
 };
 
 // 64-bit scores in an order of integers: NaN below every number, zeros alike.
@@ -614,34 +615,41 @@ __global__ __launch_bounds__(256) void select_tile_kernel(const SelectArgs a) {
     select_exact(a, b, i0 + __builtin_ctzll(todo), g, lane, qsum[wave]);
 }
 
-// Scores of 64 blocks in 64 bits, four lanes to a block, for each of few queries.
+constexpr int kScoreQueries = 8;
+
+// Scores of 64 blocks and up to eight queries in 64 bits, four lanes to a block.
 template <int KS>
 __global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
-  __shared__ double qsum[128];
+  __shared__ double qsum[kScoreQueries][128];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = 4 * (lane & 3);
-  const int chunks = (a.blocks + 63) / 64, plane = blockIdx.x / chunks, b = plane / a.kv, g = plane - b * a.kv;
-  const int j = (blockIdx.x - plane * chunks) * 64 + wave * 16 + (lane >> 2);
+  const int chunks = (a.blocks + 63) / 64, chunk = blockIdx.x % chunks, rest = blockIdx.x / chunks;
+  const int batches = (a.tq + a.queries - 1) / a.queries, plane = rest / batches, b = plane / a.kv, g = plane - b * a.kv;
+  const int i0 = (rest - plane * batches) * a.queries, count = min(a.queries, a.tq - i0);
+  const int j = chunk * 64 + wave * 16 + (lane >> 2);
   f32x4 k[KS];
   const float* m = a.m + ((long long)b * a.blocks + min(j, a.blocks - 1)) * a.ldm + g * a.kd + quarter;
 #pragma unroll
   for (int n = 0; n < KS; ++n) k[n] = 16 * n + quarter < a.kd ? *(const f32x4*)(m + 16 * n) : f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < a.tq; ++i) {
-    const float* q = a.q + ((long long)b * a.tq + i) * a.ldq + (long long)g * a.group * a.qs;
-    __syncthreads();
-    if (threadIdx.x < 128) qsum[threadIdx.x] = threadIdx.x < a.kd ? query_sum(a, q, threadIdx.x) : 0.0;
-    __syncthreads();
+  for (int x = threadIdx.x; x < count * 128; x += 256) {
+    const int i = x >> 7, c = x & 127;
+    const float* q = a.q + ((long long)b * a.tq + i0 + i) * a.ldq + (long long)g * a.group * a.qs;
+    qsum[i][c] = c < a.kd ? query_sum(a, q, c) : 0.0;
+  }
+  __syncthreads();
+  for (int i = 0; i < count; ++i) {
     int forced;
-    const int seen = seen_blocks(a, b, i, &forced);
+    const int seen = seen_blocks(a, b, i0 + i, &forced);
     double s = 0;
 #pragma unroll
     for (int n = 0; n < KS; ++n)
       if (16 * n + quarter < a.kd)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s = __builtin_fma(qsum[16 * n + quarter + e], (double)k[n][e], s);
+        for (int e = 0; e < 4; ++e) s = __builtin_fma(qsum[i][16 * n + quarter + e], (double)k[n][e], s);
     s += __shfl_xor(s, 1);
     s += __shfl_xor(s, 2);
     if ((lane & 3) == 0 && j < a.blocks)
-      a.keys[((long long)plane * a.tq + i) * a.blocks + j] = j >= seen ? kHidden : j == forced ? LLONG_MAX : score_key(s);
+      a.keys[((long long)plane * a.tq + i0 + i) * a.blocks + j] =
+          j >= seen ? kHidden : j == forced ? LLONG_MAX : score_key(s);
   }
 }
 
@@ -680,7 +688,11 @@ __global__ __launch_bounds__(256) void rank_kernel(const SelectArgs a) {
   }
 }
 
-constexpr int kManyQueries = 16;  // from here on the matrix cores
+// The matrix cores from here on, and where there are few blocks (both take 10 us then).  Below, a wave's walk through all
+// blocks, twice, takes longer than all scores in 64 bits: 512 blocks of 128 channels, 16 of them, 4 key heads and 1 / 32 / 128
+// queries 50 / 57 / 67 us against 14 / 16 / 22; 4,096 blocks, 8 key heads, 128 queries 366 against 152; but 128 blocks of 64
+// channels, 32 key heads, 128 queries 28 against 33.
+constexpr int kManyRows = 2048, kFewBlocks = 64;
 
 int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q, const sy_tensor* m,
                     const int32_t* starts, const int32_t* lengths, int32_t* blocks) {
@@ -716,8 +728,10 @@ int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q,
   const double flops = 2.0 * a.rows * a.blocks * s.kd;
   const double bytes =
       4.0 * q->n * ((double)a.tq * (s.heads * s.kd + s.kv * s.selected) + (double)a.blocks * s.kv * s.kd);
-  if (a.tq < kManyQueries) {
-    const long long grid = (long long)planes * ((a.blocks + 63) / 64);
+  if (a.rows < kManyRows && a.blocks > kFewBlocks) {
+    const long long chunks = (long long)planes * ((a.blocks + 63) / 64);
+    a.queries = (int)std::min<long long>(kScoreQueries, std::max(1LL, chunks * a.tq / 2048));  // eight workgroups to a CU
+    const long long grid = chunks * ((a.tq + a.queries - 1) / a.queries);
     SY_CHECK(grid * 256 < (1LL << 32) && a.rows * 256 < (1LL << 32), SY_EUNSUPPORTED, "block select grid too large");
     SY_TRY(ensure_scratch(ctx, sizeof(long long) * a.rows * a.blocks));
     a.keys = (long long*)ctx->scratch;

@@ -9,6 +9,9 @@ from simdyolo_amd import Tensor
 from simdyolo_amd import _native as N
 
 
+UNIT = 2.0 ** -24  # half a step of float32, relative
+
+
 def rng(seed):
     return np.random.Generator(np.random.PCG64(seed))
 
@@ -97,10 +100,11 @@ def select(cfg, q, m, starts=None, lengths=None):
 def attend(cfg, q, k, v, blocks, h, w, scale, starts=None, lengths=None):
     """(output, bound) in float64.
 
-    A score is a sum of kd float32 products, each off by at most 2^-23, its partial sums by 2^-24 each, and is
-    multiplied by the scale: within (kd + 8) 2^-24 of sum |q||k| scale, which the exponential takes over twice
-    (score and maximum).  The exponential itself, its argument's rounding (relative to the argument, below 128)
-    and the joins of partial sums add 2^-17 at most, and sums over the keys 2^-24 for each key."""
+    A score is a sum of kd products, each off by at most 3 x 2^-22 = 12 x 2^-24 (pairs of f16 values; in plain float32
+    by 2^-24), its partial sums by 2^-24 each, and is multiplied by the scale: within (kd + 24) 2^-24 of sum |q||k|
+    scale, which the exponential takes over twice (score and maximum).  The exponential itself, its argument's
+    rounding (relative to the argument, below 128), the pairs of weights and values (3 x 2^-22 of each product) and the
+    joins of partial sums add 2^-17 at most, and sums over the keys 2^-24 for each key."""
     n, tq, heads, kd = q.shape
     kv, hd, t = cfg["kv_heads"], v.shape[-1], h * w
     out, bound = np.zeros((n, tq, heads, hd)), np.zeros((n, tq, heads, hd))
@@ -117,14 +121,15 @@ def attend(cfg, q, k, v, blocks, h, w, scale, starts=None, lengths=None):
                 if not at.size:
                     continue
                 kg, vg = k[b, at, g].astype(np.float64), v[b, at, g].astype(np.float64)
-                for x in range(g * (heads // kv), (g + 1) * (heads // kv)):
-                    with np.errstate(invalid="ignore", over="ignore"):
-                        s = kg @ q[b, i, x].astype(np.float64) * scale
-                        off = (kd + 8) * 2.0 ** -24 * (np.abs(kg) @ np.abs(q[b, i, x].astype(np.float64))).max() * scale
-                        p = np.exp(s - s.max())
-                        p /= p.sum()
-                        out[b, i, x] = p @ vg
-                        bound[b, i, x] = (p @ np.abs(vg)) * (2 * off + 2.0 ** -17 + at.size * 2.0 ** -24)
+                mine = slice(g * (heads // kv), (g + 1) * (heads // kv))
+                qg = q[b, i, mine].astype(np.float64)
+                with np.errstate(invalid="ignore", over="ignore"):
+                    s = qg @ kg.T * scale
+                    off = UNIT * (kd + 24) * (np.abs(qg) @ np.abs(kg).T).max(-1, keepdims=True) * scale
+                    p = np.exp(s - s.max(-1, keepdims=True))
+                    p /= p.sum(-1, keepdims=True)
+                    out[b, i, mine] = p @ vg
+                    bound[b, i, mine] = (p @ np.abs(vg)) * (2 * off + 2.0 ** -17 + at.size * UNIT)
     return out, bound
 
 

@@ -28,7 +28,8 @@ def choice(n, tq, cfg, h, w, seed, skew=1.0):
     return out
 
 
-def run(hip, cfg, q, k, v, blocks, h, w, qh=1, starts=None, lengths=None, scale=None, pads=True):
+def run(hip, cfg, q, k, v, blocks, h, w, qh=1, starts=None, lengths=None, scale=None, pads=True, sort=None):
+    """sort: whether the lists have to be sorted for tiles (many queries), or not to be."""
     n, tq, heads, kd = q.shape
     hd = v.shape[-1]
     gap, before = (4, 8) if pads else (0, 0)
@@ -38,7 +39,15 @@ def run(hip, cfg, q, k, v, blocks, h, w, qh=1, starts=None, lengths=None, scale=
         vv, sv, _ = d.view(v, h, w, gap=gap, before=gap)
         vo, _, read = d.view(np.full((n, tq, heads, hd), np.nan, np.float32), qh, tq // qh, pad=gap, before=before)
         cf = R.config(cfg, kd, hd, (sq, sk, sv), scale)
-        hip.block_attention(cf, vq, vk, vv, d.put(blocks.astype(np.int32)), vo, d.ints(starts), d.ints(lengths))
+        hip.profile_enable(True)
+        try:
+            hip.block_attention(cf, vq, vk, vv, d.put(blocks.astype(np.int32)), vo, d.ints(starts), d.ints(lengths))
+            hip.flush()
+            names = set(hip.profile_read())
+        finally:
+            hip.profile_enable(False)
+        assert names - {"block_sort"} == {"block_attention", "block_join"}
+        assert sort is None or ("block_sort" in names) == sort
         return read()
 
 
@@ -48,31 +57,37 @@ def check(got, exp, bound):
     assert (np.abs(got - exp)[fine] <= bound[fine]).all(), (np.abs(got - exp)[fine] / np.maximum(bound[fine], 1e-30)).max()
 
 
-# n, query map, key map, config, key dim, head dim
+# n, query map, key map, config, key dim, head dim, whether the pairs of query and block are sorted
 CASES = [
-    (1, (1, 1), (1, 1), R.shape(1, 1, 1, 1, 1), 4, 4),
-    (2, (20, 20), (20, 20), R.shape(2, 2, 4, 4, 4), 32, 64),
-    (1, (15, 25), (15, 25), R.shape(4, 4, 7, 7, 6), 32, 64),      # windows cut on both sides
-    (1, (6, 9), (30, 22), R.shape(2, 1, 5, 3, 9), 36, 20),        # queries of another map
-    (1, (1, 70), (1, 500), R.shape(3, 1, 1, 33, 7), 64, 128),     # blocks one key past a tile
-    (2, (1, 5), (1, 300), R.shape(8, 2, 1, 64, 3), 128, 128),
-    (1, (1, 2), (1, 40), R.shape(7, 1, 1, 31, 2), 80, 80),
-    (1, (1, 3), (2, 1500), R.shape(2, 2, 2, 512, 3), 16, 8),      # the largest block
-    (1, (1, 1), (1, 4096), R.shape(16, 2, 1, 16, 64), 64, 64),    # one query, the longest list
-    (1, (1, 90), (1, 90), R.shape(40, 2, 1, 8, 5), 32, 32),       # more heads to a key head than a tile's rows
-    (1, (1, 33), (1, 65), R.shape(5, 5, 1, 1, 64), 128, 4),       # blocks of one key
-    (1, (12, 40), (12, 40), R.shape(2, 2, 8, 8, 10), 128, 128),   # every block of the map
+    (1, (1, 1), (1, 1), R.shape(1, 1, 1, 1, 1), 4, 4, False),
+    (1, (6, 9), (30, 22), R.shape(2, 1, 5, 3, 9), 36, 20, False),      # queries of another map
+    (1, (1, 70), (1, 500), R.shape(3, 1, 1, 33, 7), 64, 128, False),   # blocks one key past a tile
+    (2, (1, 5), (1, 300), R.shape(8, 2, 1, 64, 3), 128, 128, False),
+    (1, (1, 2), (1, 40), R.shape(7, 1, 1, 31, 2), 80, 80, False),
+    (1, (1, 3), (2, 1500), R.shape(2, 2, 2, 512, 3), 16, 8, False),    # the largest block
+    (1, (1, 1), (1, 4096), R.shape(16, 2, 1, 16, 64), 64, 64, False),  # one query, the longest list
+    (1, (1, 33), (1, 65), R.shape(5, 5, 1, 1, 64), 128, 4, True),      # blocks of one key
+    (2, (20, 20), (20, 20), R.shape(2, 2, 4, 4, 4), 32, 64, True),
+    (1, (15, 25), (15, 25), R.shape(4, 4, 7, 7, 6), 32, 64, True),     # windows cut on both sides
+    (1, (12, 40), (12, 40), R.shape(2, 2, 8, 8, 10), 128, 128, True),  # every block of the map
+    (1, (1, 900), (1, 500), R.shape(3, 1, 1, 33, 7), 64, 128, True),   # tiles that start within a query's heads
+    (2, (1, 700), (1, 300), R.shape(8, 2, 1, 64, 3), 36, 20, True),
+    (1, (1, 300), (2, 1500), R.shape(2, 2, 2, 512, 3), 16, 8, True),
+    (1, (1, 560), (1, 30), R.shape(300, 1, 1, 4, 2), 8, 12, True),     # more heads to a key head than a tile's rows
+    (1, (1, 600), (1, 90), R.shape(20, 2, 1, 8, 5), 128, 64, True),
+    (1, (30, 30), (30, 30), R.shape(1, 1, 30, 30, 1), 32, 32, True),   # one block for all
+    (1, (1, 800), (1, 200), R.shape(2, 2, 1, 50, 2), 100, 100, True),
 ]
 
 
 @pytest.mark.parametrize("pads", [False, True], ids=["dense", "strided"])
 @pytest.mark.parametrize("case", CASES, ids=str)
 def test_shapes(hip, case, pads):
-    n, (qh, qw), (h, w), cfg, kd, hd = case
+    n, (qh, qw), (h, w), cfg, kd, hd, sort = case
     q, k, v = tensors(n, qh * qw, h * w, cfg, kd, hd, h + 13 * w)
     blocks = choice(n, qh * qw, cfg, h, w, 3)
     exp, bound = R.attend(cfg, q, k, v, blocks, h, w, kd ** -0.5)
-    check(run(hip, cfg, q, k, v, blocks, h, w, qh, pads=pads), exp, bound)
+    check(run(hip, cfg, q, k, v, blocks, h, w, qh, pads=pads, sort=sort), exp, bound)
 
 
 @pytest.mark.parametrize("skew", [0.0, 6.0])
@@ -84,7 +99,7 @@ def test_long_and_short_lists(hip, skew):
     if skew == 0.0:
         blocks[:] = [0, 7, 35]
     exp, bound = R.attend(cfg, q, k, v, blocks, h, w, kd ** -0.5)
-    check(run(hip, cfg, q, k, v, blocks, h, w, h), exp, bound)
+    check(run(hip, cfg, q, k, v, blocks, h, w, h, sort=True), exp, bound)
 
 
 @pytest.mark.parametrize("tq", [1, 3, 150])
@@ -96,7 +111,7 @@ def test_causal(hip, tq, starts, lengths):
     blocks = choice(4, tq, cfg, 1, w, 6, 0.5)
     blocks[:, :, :, 3] = (np.maximum(np.asarray(starts or [0] * 4), 0)[:, None, None] + np.arange(tq)[:, None]) // 16
     exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5, starts, lengths)
-    got = run(hip, cfg, q, k, v, blocks, 1, w, 1, starts, lengths)
+    got = run(hip, cfg, q, k, v, blocks, 1, w, 1, starts, lengths, sort=tq == 150)
     check(got, exp, bound)
     assert lengths is None or not got[0].any()
 
@@ -111,13 +126,13 @@ def test_lists(hip, tq):
     blocks[1, :, 0] = [10, -7, 2 ** 31 - 1, -2 ** 31, 11, 3]
     blocks[1, :, 1] = [4, 4, -1, 9, 4, 9]
     exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5)
-    got = run(hip, cfg, q, k, v, blocks, 1, w)
+    got = run(hip, cfg, q, k, v, blocks, 1, w, sort=tq == 80)
     check(got, exp, bound)
     assert not got[0, :, 0].any() and got[1, :, 0].any()
 
 
-@pytest.mark.parametrize("tq", [1, 80])
-@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf, np.finfo(np.float32).max], ids=str)
+@pytest.mark.parametrize("tq", [1, 300])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf, np.finfo(np.float32).max, 2.0 ** 60], ids=str)
 def test_hidden_keys_are_not_read(hip, tq, value):
     """Whatever stands behind a sequence, behind a causal query, in blocks not chosen."""
     cfg, kd, hd, w = R.shape(4, 2, 1, 16, 3, causal=1), 32, 32, 90
@@ -129,11 +144,11 @@ def test_hidden_keys_are_not_read(hip, tq, value):
     k[:, 16:32], v[:, 16:32] = value, value
     for b in range(2):
         k[b, lengths[b]:], v[b, lengths[b]:] = value, value
-    got = run(hip, cfg, q, k, v, blocks, 1, w, 1, starts, lengths)
+    got = run(hip, cfg, q, k, v, blocks, 1, w, 1, starts, lengths, sort=tq == 300)
     check(got, exp, bound)
 
 
-@pytest.mark.parametrize("tq", [1, 64])
+@pytest.mark.parametrize("tq", [1, 700])
 @pytest.mark.parametrize("part", ["q", "k", "v"])
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf], ids=str)
 def test_non_finite(hip, tq, part, value):
@@ -145,14 +160,14 @@ def test_non_finite(hip, tq, part, value):
     blocks[0, 0, 0] = [1, 3]
     with np.errstate(invalid="ignore", over="ignore"):
         exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5)
-    got = run(hip, cfg, q, k, v, blocks, 1, w)
+    got = run(hip, cfg, q, k, v, blocks, 1, w, sort=tq == 700)
     np.testing.assert_array_equal(np.isfinite(got), np.isfinite(exp))
     np.testing.assert_array_equal(np.isnan(got), np.isnan(exp))
     fine = np.isfinite(exp) & np.isfinite(bound)
-    assert (np.abs(got - exp)[fine] <= bound[fine]).all()
+    assert (np.abs(got[fine] - exp[fine]) <= bound[fine]).all()
 
 
-@pytest.mark.parametrize("tq", [1, 64])
+@pytest.mark.parametrize("tq", [1, 400])
 def test_scores_that_are_all_minus_infinite(hip, tq):
     """The formula's 0 / 0; where one score is finite, the others weigh nothing."""
     cfg, kd, hd, w = R.shape(2, 2, 1, 20, 3), 8, 8, 100
@@ -164,25 +179,43 @@ def test_scores_that_are_all_minus_infinite(hip, tq):
     blocks[..., 2] = 4
     exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5)
     assert np.isnan(exp[:, :, 0]).all() and np.isfinite(exp[:, :, 1]).all()
-    got = run(hip, cfg, q, k, v, blocks, 1, w)
+    got = run(hip, cfg, q, k, v, blocks, 1, w, sort=tq == 400)
     np.testing.assert_array_equal(np.isnan(got), np.isnan(exp))
     check(got[:, :, 1:], exp[:, :, 1:], np.abs(exp[:, :, 1:]) * 2.0 ** -16)
 
 
-@pytest.mark.parametrize("tq", [1, 100])
+@pytest.mark.parametrize("tq", [1, 300])
 @pytest.mark.parametrize("scales", [(1e-6, 1e6, 1e-20), (30.0, 1.0, 1e4), (0.0, 1.0, 1.0), (1e-30, 1e-30, 1e-30),
-                                    (1.0, 1.0, 1e30)], ids=str)
+                                    (1.0, 1.0, 1e30), (1e-30, 1e30, 1.0), (1.0, 1.0, 1e-37), (1e35, 1e-36, 1e-44)], ids=str)
 def test_operand_scales(hip, tq, scales):
-    """Operands of far apart magnitudes; values that grow by 2^14 from block to block."""
+    """Operands of far apart magnitudes, subnormal ones; values that grow by 2^14 from block to block."""
     cfg, kd, hd, w = R.shape(2, 2, 1, 16, 4), 32, 64, 96
     q, k, v = (a * np.float32(s) for a, s in zip(tensors(1, tq, w, cfg, kd, hd, 5), scales))
     v[:, 48:] *= np.float32(16384)
     blocks = choice(1, tq, cfg, 1, w, 8, 0.0)
     exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5)
-    check(run(hip, cfg, q, k, v, blocks, 1, w), exp, bound + 2.0 ** -126)
+    check(run(hip, cfg, q, k, v, blocks, 1, w, sort=tq == 300), exp, bound + 2.0 ** -126)
 
 
-@pytest.mark.parametrize("tq", [1, 100])
+@pytest.mark.parametrize("tq", [1, 300])
+@pytest.mark.parametrize("part", ["k", "v"])
+@pytest.mark.parametrize("step", [0.7, 3.0, 40.0])
+def test_keys_of_many_sizes(hip, tq, part, step):
+    """Keys, or values, that grow by e^step from one to the next within a block: beside, past and far past the range
+    within which they share a power of two."""
+    cfg, kd, hd, w = R.shape(2, 2, 1, 32, 3, causal=1), 32, 64, 96
+    q, k, v = tensors(1, tq, w, cfg, kd, hd, 5)
+    grow = np.exp(np.minimum(step * (np.arange(w) % 32), 80.0) - 40.0).astype(np.float32)[:, None, None]
+    if part == "k":
+        k, q = k * grow, q * np.float32(1e-17)
+    else:
+        v = v * grow
+    blocks = choice(1, tq, cfg, 1, w, 8, 0.0)
+    exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5)
+    check(run(hip, cfg, q, k, v, blocks, 1, w, sort=tq == 300), exp, bound)
+
+
+@pytest.mark.parametrize("tq", [1, 700])
 def test_heavy_key_in_a_light_block(hip, tq):
     """A key with values of 2^20 and no weight beside ordinary ones: their precision is their own."""
     cfg, kd, hd, w = R.shape(1, 1, 1, 32, 2), 32, 64, 96
@@ -194,21 +227,21 @@ def test_heavy_key_in_a_light_block(hip, tq):
     blocks[..., 1] = np.maximum(blocks[..., 1], 1)
     blocks[..., 0] = 0
     exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5)
-    check(run(hip, cfg, q, k, v, blocks, 1, w), exp, bound)
+    check(run(hip, cfg, q, k, v, blocks, 1, w, sort=tq == 700), exp, bound)
 
 
 @pytest.mark.parametrize("step", [0.5, 3.0, 60.0, -60.0])
 def test_creeping_maximum(hip, step):
     """Scores that rise or fall from one tile of keys to the next."""
     cfg, kd, hd, w = R.shape(1, 1, 1, 200, 3), 32, 64, 600
-    for tq in (1, 70):
+    for tq in (1, 150):
         q, k, v = tensors(1, tq, w, cfg, kd, hd, 8)
         q[:] = 1.0
         k *= np.float32(0.25)
         k[..., 0] += (np.float32(step) * (np.arange(w) // 32)).astype(np.float32)[:, None]
         blocks = choice(1, tq, cfg, 1, w, 8, 0.0)
         exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, 1.0)
-        check(run(hip, cfg, q, k, v, blocks, 1, w, scale=1.0), exp, bound)
+        check(run(hip, cfg, q, k, v, blocks, 1, w, scale=1.0, sort=tq == 150), exp, bound)
 
 
 def test_neighbours_do_not_change_a_row(hip):
@@ -216,7 +249,7 @@ def test_neighbours_do_not_change_a_row(hip):
     cfg, kd, hd, h, w = R.shape(4, 2, 4, 4, 3), 32, 64, 16, 24
     q, k, v = tensors(1, h * w, h * w, cfg, kd, hd, 4)
     blocks = choice(1, h * w, cfg, h, w, 5)
-    whole = run(hip, cfg, q, k, v, blocks, h, w, h)
+    whole = run(hip, cfg, q, k, v, blocks, h, w, h, sort=True)
     np.testing.assert_array_equal(whole, run(hip, cfg, q, k, v, blocks, h, w, h))
     turn = R.rng(3).permutation(h * w)
     moved = run(hip, cfg, np.ascontiguousarray(q[:, turn]), k, v, np.ascontiguousarray(blocks[:, turn]), h, w, h)

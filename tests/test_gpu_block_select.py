@@ -37,16 +37,33 @@ def close(got, exp, k):
     assert (np.abs(got - exp) <= np.abs(exp) * 2.0 ** -24 + np.abs(k).max() * 2.0 ** -45).all()
 
 
-def run_select(hip, cfg, q, m, h, w, starts=None, lengths=None, qh=None, gap=0):
-    """Selection on the means m [n, blocks, kv, kd]."""
+# Few queries are ranked as they are, many (2,048 and more pairs of query and key head, or 64 blocks and less) through
+# the matrix cores; of many, some are compared.
+FEW, MANY = 21, 2100
+
+
+def some(q, *more):
+    keep = np.unique(R.rng(1).permutation(q.shape[1])[:90])
+    return [np.ascontiguousarray(a[:, keep]) for a in (q, *more)]
+
+
+def run_select(hip, cfg, q, m, h, w, starts=None, lengths=None, qh=None, gap=0, many=None):
+    """Selection on the means m [n, blocks, kv, kd]; many: whether through the matrix cores."""
     n, tq, _, kd = q.shape
     with R.Device(hip) as d:
         vq, sq, _ = d.view(q, qh or 1, tq // (qh or 1), pad=8, gap=gap, before=4)
         vm, _ = means_view(d, cfg, n, h, w, kd, m)
         out = np.full((n, tq, cfg["kv_heads"], cfg["selected"]), 77, np.int32)
         p = d.put(out)
-        hip.block_select(R.config(cfg, kd, 4, (sq, 0, 0)), vq, vm, p, d.ints(starts), d.ints(lengths))
-        hip.flush()
+        hip.profile_enable(True)
+        try:
+            hip.block_select(R.config(cfg, kd, 4, (sq, 0, 0)), vq, vm, p, d.ints(starts), d.ints(lengths))
+            hip.flush()
+            names = set(hip.profile_read())
+        finally:
+            hip.profile_enable(False)
+        assert names in ({"block_score", "block_rank"}, {"block_parts", "block_select"})
+        assert many is None or ("block_parts" in names) == many
         return hip.d2h(p, out.shape, np.int32)
 
 
@@ -60,7 +77,7 @@ def test_maps(hip, case):
         hip.block_means(R.config(cfg, kd, 4, (0, sk, 0)), vk, vm)
         m = read()
     close(m, R.means(cfg, k, h, w), k)
-    keep = R.rng(1).permutation(h * w)[:200]  # a query's choice does not hang on the others
+    keep = R.rng(1).permutation(h * w)[:100]  # a query's choice does not hang on the others
     got = run_select(hip, cfg, q, m, h, w, qh=h, gap=4)
     exp = R.select(cfg, np.ascontiguousarray(q[:, keep]), m)
     np.testing.assert_array_equal(got[:, keep], exp)
@@ -128,52 +145,97 @@ def test_renewed_means(hip, starts, tokens):
                 np.testing.assert_array_equal(got[b, j], old[b, j])
 
 
+@pytest.mark.parametrize("tq", [FEW, MANY])
 @pytest.mark.parametrize("blocks", [3, 70, 1500])
-def test_ties_and_non_finite_means(hip, blocks):
+@pytest.mark.parametrize("selected", [1, 8, 13, 30, 64])
+def test_ties_and_non_finite_means(hip, tq, blocks, selected):
     """Equal means: the lower block.  NaN scores come last, infinities at the ends."""
-    cfg, kd = R.shape(2, 2, 1, 1, 8), 12
-    q, _ = tensors(2, 1, 9, cfg, kd, 5)
+    cfg, kd = R.shape(2, 2, 1, 1, selected), 12
+    q, _ = tensors(2, 1, tq, cfg, kd, 5)
     m = np.round(R.rng(6).standard_normal((2, blocks, 2, kd)) * 2).astype(np.float32)
     m[:, 1::3] = m[:, :1]
+
+    def compare():
+        got = run_select(hip, cfg, q, m, 1, blocks, many=tq == MANY or blocks <= 64)
+        few, got = some(q, got)
+        np.testing.assert_array_equal(got, R.select(cfg, few, m))
+    compare()
     m[0, blocks // 2, :, 3] = np.nan
     m[1, blocks // 3, 0, 2] = np.inf
     m[1, blocks // 4, 1, 2] = -np.inf
-    got = run_select(hip, cfg, q, m, 1, blocks)
-    np.testing.assert_array_equal(got, R.select(cfg, q, m))
+    compare()
     m[:] = np.nan
-    np.testing.assert_array_equal(run_select(hip, cfg, q, m, 1, blocks), R.select(cfg, q, m))
+    compare()
 
 
-def test_near_ties(hip):
-    """Scores that differ by less than float32 could tell: blocks that differ in the last bit of one channel."""
-    cfg, kd, blocks = R.shape(4, 1, 1, 1, 6), 64, 200
-    q, _ = tensors(1, 1, 33, cfg, kd, 8)
-    m = np.repeat(R.rng(3).standard_normal((1, 1, 1, kd)), blocks, 1).astype(np.float32)
+@pytest.mark.parametrize("tq", [FEW, MANY])
+@pytest.mark.parametrize("kd,selected", [(64, 6), (32, 16), (128, 40)])
+def test_near_ties(hip, tq, kd, selected):
+    """Scores that differ by less than float32 could tell: blocks that differ in the last bit of one channel, all of
+    them (a query's candidates do not fit anywhere) or a few near the border."""
+    cfg, blocks = R.shape(4, 1, 1, 1, selected), 200
+    q, _ = tensors(1, 1, tq, cfg, kd, 8)
+    near = np.repeat(R.rng(3).standard_normal((1, 1, 1, kd)), blocks, 1).astype(np.float32)
     at = R.rng(4).integers(0, kd, blocks)
     for j in range(blocks):
-        m[0, j, 0, at[j]] = np.nextafter(m[0, j, 0, at[j]], np.float32(np.inf if j % 2 else -np.inf))
-    got = run_select(hip, cfg, q, m, 1, blocks)
-    np.testing.assert_array_equal(got, R.select(cfg, q, m))
+        near[0, j, 0, at[j]] = np.nextafter(near[0, j, 0, at[j]], np.float32(np.inf if j % 2 else -np.inf))
+    apart = R.rng(9).standard_normal((1, blocks, 1, kd)).astype(np.float32)
+    for m in (near, np.where((np.arange(blocks) % 9 < 3)[:, None, None], near, apart)):
+        got = run_select(hip, cfg, q, m, 1, blocks, many=tq == MANY)
+        few, got = some(q, got)
+        np.testing.assert_array_equal(got, R.select(cfg, few, m))
 
 
-@pytest.mark.parametrize("scales", [(1e-30, 1e-12), (1e25, 1e20), (1e-42, 1.0)], ids=str)
-def test_far_scaled(hip, scales):
-    """Products below float32's range, above it, and of subnormal queries."""
+@pytest.mark.parametrize("tq", [FEW, MANY])
+def test_pairs_of_blocks_that_are_alike(hip, tq):
+    """Every block has a neighbour 2^-20 away: many queries of one wave are in doubt between two."""
+    cfg, kd, blocks = R.shape(2, 2, 1, 1, 7), 48, 300
+    q, _ = tensors(1, 1, tq, cfg, kd, 8)
+    m = R.rng(3).standard_normal((1, blocks, 2, kd)).astype(np.float32)
+    m[:, 1::2] = m[:, ::2] * np.float32(1 + 2.0 ** -20)
+    got = run_select(hip, cfg, q, m, 1, blocks, many=tq == MANY)
+    few, got = some(q, got)
+    np.testing.assert_array_equal(got, R.select(cfg, few, m))
+
+
+@pytest.mark.parametrize("tq", [FEW, MANY])
+@pytest.mark.parametrize("scales", [(1e-30, 1e-12), (1e25, 1e20), (1e-42, 1.0), (0.0, 1.0), (1.0, 0.0), (1e12, 1e-12)], ids=str)
+def test_far_scaled(hip, tq, scales):
+    """Products below float32's range, above it, of subnormal queries, of zeros."""
     cfg, kd, blocks = R.shape(2, 2, 1, 1, 5), 32, 90
-    q, _ = tensors(2, 1, 21, cfg, kd, 8)
+    q, _ = tensors(2, 1, tq, cfg, kd, 8)
     m = R.rng(3).standard_normal((2, blocks, 2, kd)).astype(np.float32)
     q, m = (q * np.float32(scales[0])).astype(np.float32), (m * np.float32(scales[1])).astype(np.float32)
-    np.testing.assert_array_equal(run_select(hip, cfg, q, m, 1, blocks), R.select(cfg, q, m))
+    got = run_select(hip, cfg, q, m, 1, blocks, many=tq == MANY)
+    few, got = some(q, got)
+    np.testing.assert_array_equal(got, R.select(cfg, few, m))
 
 
-def test_uneven_channels(hip):
+@pytest.mark.parametrize("tq", [FEW, MANY])
+def test_uneven_channels(hip, tq):
     """One channel far above the others, and cancelled: what decides lies 2^-30 below the largest product."""
     cfg, kd, blocks = R.shape(1, 1, 1, 1, 4), 16, 150
-    q, _ = tensors(1, 1, 40, cfg, kd, 1)
+    q, _ = tensors(1, 1, tq, cfg, kd, 1)
     m = R.rng(2).standard_normal((1, blocks, 1, kd)).astype(np.float32)
     q[..., 1] = -q[..., 0]
     m[..., 0] = m[..., 1] = np.float32(2.0 ** 30)
-    np.testing.assert_array_equal(run_select(hip, cfg, q, m, 1, blocks), R.select(cfg, q, m))
+    got = run_select(hip, cfg, q, m, 1, blocks, many=tq == MANY)
+    few, got = some(q, got)
+    np.testing.assert_array_equal(got, R.select(cfg, few, m))
+
+
+@pytest.mark.parametrize("kd,selected", [(32, 8), (64, 20), (128, 64)])
+def test_long_causal_rows(hip, kd, selected):
+    """More blocks than a wave's tile, a few of them seen by the first queries and all by the last."""
+    cfg = R.shape(6, 2, 1, 4, selected, causal=1)
+    tq, w, starts, lengths = 1500, 1600, (0, 100), (1490, 1600)
+    q, k = tensors(2, w, tq, cfg, kd, 3)
+    m = R.means(cfg, k, 1, w, lengths).astype(np.float32)
+    got = run_select(hip, cfg, q, m, 1, w, starts, lengths, many=True)
+    keep = np.unique(np.concatenate([np.arange(0, 120, 7), np.arange(1380, 1500, 9), R.rng(2).integers(0, tq, 40)]))
+    for i in keep:
+        exp = R.select(cfg, q[:, i:i + 1], m, [s + i for s in starts], lengths)
+        np.testing.assert_array_equal(got[:, i:i + 1], exp)
 
 
 def test_one_image_too_many(hip):
