@@ -307,6 +307,7 @@ __device__ __forceinline__ void write_row(int* out, int selected, int kept, int 
 // The sum of the query heads that share a key head, in 64 bits: channel c.
 __device__ __forceinline__ double query_sum(const SelectArgs& a, const float* q, int c) {
   double s = 0;
+#pragma unroll 4
   for (int h = 0; h < a.group; ++h) s += q[(long long)h * a.qs + c];
   return s;
 }
@@ -343,23 +344,42 @@ __device__ __forceinline__ void select_exact(const SelectArgs& a, int b, int i, 
   __builtin_amdgcn_wave_barrier();
 }
 
-// The same among `count` candidates (up to 64, more than wanted) in ascending order: each counts those before it.
+// The same among `count` candidates (up to 64, more than wanted) in ascending order: four lanes score one, then each
+// counts those before it.
 __device__ __forceinline__ void select_among(const SelectArgs& a, int b, int i, int g, int lane, double* qsum,
-                                             const int* pool, int count) {
+                                             long long* keys, const int* pool, int count) {
   query_sums(a, b, i, g, lane, qsum);
   int forced;
   (void)seen_blocks(a, b, i, &forced);
-  const int j = pool[min(lane, count - 1)];
-  const long long key = j == forced ? LLONG_MAX : exact_key(a, b, g, j, qsum);
+  const int quarter = 4 * (lane & 3);
+  for (int n0 = 0; n0 < count; n0 += 16) {
+    const int n = n0 + (lane >> 2), j = pool[min(n, count - 1)];
+    const float* m = a.m + ((long long)b * a.blocks + j) * a.ldm + g * a.kd;
+    f32x4 v[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[x] = *(const f32x4*)(m + min(16 * x + quarter, a.kd - 4));
+    double s = 0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+      if (16 * x + quarter < a.kd)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = __builtin_fma(qsum[16 * x + quarter + e], (double)v[x][e], s);
+    s += __shfl_xor(s, 1);
+    s += __shfl_xor(s, 2);
+    if ((lane & 3) == 0 && n < count) keys[n] = j == forced ? LLONG_MAX : score_key(s);
+  }
+  __builtin_amdgcn_wave_barrier();
+  const int mine = min(lane, count - 1);
+  const long long key = keys[mine];
   int before = 0;
+#pragma unroll 8
   for (int n = 0; n < count; ++n) {
-    const long long k = (long long)__builtin_amdgcn_readlane((int)(key >> 32), n) << 32 |
-                        (unsigned)__builtin_amdgcn_readlane((int)key, n);
+    const long long k = keys[n];
     before += k > key || (k == key && n < lane);
   }
   const unsigned long long chosen = __ballot(lane < count && before < a.selected);
   if (chosen >> lane & 1)
-    a.out[(((long long)b * a.tq + i) * a.kv + g) * a.selected + __builtin_popcountll(chosen & ((1ull << lane) - 1))] = j;
+    a.out[(((long long)b * a.tq + i) * a.kv + g) * a.selected + __builtin_popcountll(chosen & ((1ull << lane) - 1))] = pool[mine];
   __builtin_amdgcn_wave_barrier();
 }
 
@@ -446,6 +466,7 @@ template <int KS, int SMAX>
 __global__ __launch_bounds__(256) void select_tile_kernel(const SelectArgs a) {
   __shared__ double qsum[4][128];
   __shared__ int pool[4][kPools][64];
+  __shared__ long long keys[4][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, r32 = lane & 31;
   const int groups = (a.tq + 127) / 128;
@@ -466,37 +487,38 @@ __global__ __launch_bounds__(256) void select_tile_kernel(const SelectArgs a) {
   const int seen = seen_blocks(a, b, min(i, a.tq - 1), &forced);
   const int last = __builtin_amdgcn_readfirstlane((wave_max_i32(seen) + 31) / 32);
   {
-    const float* p = a.q + ((long long)b * a.tq + min(i, a.tq - 1)) * a.ldq + (long long)g * a.group * a.qs + 8 * half;
+    // A head's channels are under way together, up to 32 to a lane.
+    constexpr int KB = KS < 4 ? KS : 4;
+    const float* p = a.q + ((long long)b * a.tq + min(i, a.tq - 1)) * a.ldq + (long long)g * a.group * a.qs;
     float qn = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      float f[8];
+    for (int k0 = 0; k0 < KS; k0 += KB) {
+      double s[KB][8];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int c = 16 * ks + 4 * u;
-        if (c + 8 * half < a.kd) {
-          if (a.group == 1) {
-            const f32x4 v = *(const f32x4*)(p + c);
+      for (int ks = 0; ks < KB; ++ks)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f[4 * u + e] = v[e];
-          } else {
-            double s[4] = {0, 0, 0, 0};
-            for (int h = 0; h < a.group; ++h) {
-              const f32x4 v = *(const f32x4*)(p + (long long)h * a.qs + c);
+        for (int e = 0; e < 8; ++e) s[ks][e] = 0.0;
+      for (int h = 0; h < a.group; ++h) {
+        f32x4 v[KB][2];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[e] += v[e];
-            }
+        for (int ks = 0; ks < KB; ++ks)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f[4 * u + e] = (float)s[e];
-          }
-        } else {
+          for (int u = 0; u < 2; ++u) v[ks][u] = *(const f32x4*)(p + (long long)h * a.qs + min(16 * (k0 + ks) + 8 * half + 4 * u, a.kd - 4));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) f[4 * u + e] = 0.f;
-        }
+        for (int ks = 0; ks < KB; ++ks)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) qn = __builtin_fmaf(f[4 * u + e], f[4 * u + e], qn);
+          for (int e = 0; e < 8; ++e) s[ks][e] += v[ks][e >> 2][e & 3];
       }
-      halves8(f, q[ks]);
+#pragma unroll
+      for (int ks = 0; ks < KB; ++ks) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          f[e] = 16 * (k0 + ks) + 8 * half + 4 * (e >> 2) < a.kd ? (float)s[ks][e] : 0.f;
+          qn = __builtin_fmaf(f[e], f[e], qn);
+        }
+        halves8(f, q[k0 + ks]);
+      }
     }
     qn += __shfl_xor(qn, 32);
     const bool fine = qn >= 0x1p-80f && qn <= 0x1p80f && kn >= 0x1p-80f && kn <= 0x1p80f;
@@ -608,7 +630,7 @@ __global__ __launch_bounds__(256) void select_tile_kernel(const SelectArgs a) {
     for (int n = count; n < a.selected; ++n) out[n] = -1;
   for (unsigned long long todo = __ballot(mine && !exact && slot >= 0); todo; todo &= todo - 1) {
     const int x = __builtin_ctzll(todo);
-    select_among(a, b, i0 + x, g, lane, qsum[wave], pool[wave][__builtin_amdgcn_readlane(slot, x)],
+    select_among(a, b, i0 + x, g, lane, qsum[wave], keys[wave], pool[wave][__builtin_amdgcn_readlane(slot, x)],
                  __builtin_amdgcn_readlane(count, x));
   }
   for (unsigned long long todo = __ballot(mine && exact); todo; todo &= todo - 1)
