@@ -445,6 +445,8 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
     return __builtin_bit_cast(f16x8, frag[KF * 64 + ((st * DT + d) * 2 + m) * 64 + lane]);
   };
 
+  // (Results pass the caches by, written here and read by the join, and so do the join's outputs: 287 -> 234 us on two
+  // 160x160 maps, 659 -> 585 on 8,192 causal tokens, whose queries and keys they would push out.)
   // The queries are here before the loop: in it they are waited for with the stores behind them still under way.
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   const float cs = s.scale * 1.4426950408889634f;
@@ -573,7 +575,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
       char* base = (char*)(a.part + 32 * d);
       if (WHOLE || 32 * d + r32 < s.hd)
 #pragma unroll
-        for (int x = 0; x < 16; ++x) *(float*)(base + row_at[x]) = acc[x];
+        for (int x = 0; x < 16; ++x) __builtin_nontemporal_store(acc[x], (float*)(base + row_at[x]));
     }
   }
 }
@@ -807,7 +809,8 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         w[u] = __shfl(fv, (lane & ~(L - 1)) + min(u0 + u, L - 1));
-        v[u] = *(const f32x4*)(part + (long long)__shfl(at, (lane & ~(L - 1)) + min(u0 + u, L - 1)) * s.hd);
+        const int row = __shfl(at, (lane & ~(L - 1)) + min(u0 + u, L - 1));
+        v[u] = __builtin_nontemporal_load((const f32x4*)(part + (long long)row * s.hd));
       }
 #pragma unroll
       for (int u = 0; u < 8; ++u)
@@ -827,7 +830,8 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
     y[e] = any ? __builtin_ldexpf(y[e] / sum, power) : 0.f;
     again |= live && c < s.hd && !(__builtin_fabsf(y[e]) <= FLT_MAX);
   }
-  if (live && c < s.hd) *(f32x4*)(a.o + ((long long)b * s.tq + i) * a.ldo + (long long)(g * s.group + h) * s.hd + c) = y;
+  if (live && c < s.hd)
+    __builtin_nontemporal_store(y, (f32x4*)(a.o + ((long long)b * s.tq + i) * a.ldo + (long long)(g * s.group + h) * s.hd + c));
   for (unsigned long long todo = __ballot(again); todo;) {
     const int from = __builtin_ctzll(todo) & ~(L - 1);
     const int rb = __shfl(b, from), ri = __shfl(i, from), rh = __shfl(g * s.group + h, from);
