@@ -2,11 +2,16 @@
 //
 // A query's blocks are its own choice, so neighbouring queries share few of them, and a matrix
 // instruction wants 32 queries on the same keys.  The work is therefore done block by block: the
-// (query, slot) pairs are sorted by the block they name, a workgroup takes up to 128 rows (a query times a
+// (query, slot) pairs are sorted by the block they name, a workgroup takes up to 512 rows (a query times a
 // head of the group that shares the key head) of one block's list, and leaves for each its maximum score,
-// sum of weights and weighted sum of values (split over the long axis as in flash-decoding, Dao et al., 2023).
-// A last kernel joins a query's slots.  With few queries (a token against a cache) the pairs are taken as
-// they stand.
+// sum of weights and weighted sum of values, split over the long axis as flash-decoding does (Dao, Haziza, Massa and
+// Sizov, 2023).  A last kernel joins a query's slots.  With few queries (a token against a cache) the pairs are
+// taken as they stand.
+//
+// Measured, us (sort + tiles + join): two 160x160 maps, 4 heads of 32 / 64 channels, 8 of 400 blocks of 64 keys
+// 25 + 113 + 89; 8,192 causal tokens, 16 heads and 4 key heads of 128, 16 of 128 blocks 20 + 356 + 195; plain float32,
+// a wave to a query, 14,900 and 61,700.  The results are written and read once, 0.43 and 1.0 GB, and bound both:
+// without matrix instructions the first took 284 where it took 287 with them.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -586,7 +591,8 @@ constexpr int kFewRows = 4;
 
 // One (query, slot) pair and part of its block per workgroup, in plain float32: the keys are read once, for the few
 // heads that share them, and the time is their way from memory.  Four lanes score a key (16 keys to a wave), then
-// a lane takes two channels over the same 16 keys; the four waves' results meet in LDS.
+// a lane takes two channels over the same 16 keys; the four waves' results meet in LDS.  One token against 16 caches, 16
+// blocks of 64 keys for 4 heads of 128 channels (67 MB): 18 us, 3.7 TB/s; as a tile on the matrix cores 33 us.
 template <int KS>
 __global__ __launch_bounds__(256) void block_few_kernel(const BlockArgs a) {
   __shared__ float weight[kFewRows][kKeys], q[kFewRows][128], out[4][kFewRows][128];
@@ -749,7 +755,7 @@ __device__ __forceinline__ void block_row(const BlockArgs& a, int b, int i, int 
   y[1] = acc[1];
 }
 
-// Joins the slots of each row: L lanes of 4 channels to a row.  The lanes first take a slot each (which block it
+// Joins the slots of each row: L lanes of 4 channels to a row, at 5.4 TB/s.  The lanes first take a slot each (which block it
 // names, its statistics), then all of them go through the slots' values, whose loads depend on nothing.  A row
 // that comes out infinite or NaN (operands that are, sums that overflow, hidden keys of a tile that are not
 // finite) is computed again in plain float32.

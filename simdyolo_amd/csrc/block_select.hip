@@ -69,7 +69,9 @@ struct MeansArgs {
 };
 
 // One workgroup per image, block (with `tokens`: that may hold some) and 128 channels.  A lane sums four channels over
-// every (256 / lanes)-th key, eight keys under way at a time; the partial sums meet in LDS in one order.
+// every (256 / lanes)-th key, eight keys under way at a time; the partial sums meet in LDS in one order.  Bound by
+// memory: four 160x160 maps of 128 channels (52 MB) in 11 us, 4.8 TB/s; one token's block of 16 caches 4 us, the latency of
+// a launch and its loads.
 __global__ __launch_bounds__(256) void means_kernel(const MeansArgs a) {
   __shared__ double part[256][4];
   const int piece = blockIdx.x % a.pieces, bs = blockIdx.x / a.pieces, b = bs / a.slots, slot = bs % a.slots;
@@ -399,6 +401,7 @@ __device__ __forceinline__ void halves8(const float (&x)[8], bf16x8 (&p)[2]) {
   p[1] = __builtin_bit_cast(bf16x8, w[1]);
 }
 
+constexpr int kPools = 8;      // doubtful queries of a wave whose candidates are kept
 constexpr int kPartTiles = 8;  // 32-block tiles of a workgroup below
 
 // The means of one key head as the A operands of the matrix instructions (32 blocks x 16 channels, two parts
@@ -461,9 +464,13 @@ __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
 // instructions with 16 products each, and q rounded from 64 bits, stay below 2^-18.  sum |q||m| <= |q||m| in norms,
 // which sums in float32 and two roots change by less than 2^-16 of themselves: e = 3.5 x 2^-16 |q| max|m|.  Norms
 // outside 2^-40 .. 2^40 could lose parts to underflow: all blocks of those queries are scored in 64 bits.
-constexpr int kPools = 8;  // doubtful queries of a wave whose candidates are kept
+//
+// Bound by vector work: of 4,700 operations per wave (32 queries, 400 blocks of 32 channels, 8 wanted) 1,900 are medians and
+// 1,400 the second pass; the matrix cores are busy a fifth of the time.  Scores in 64 bits throughout took 9.9 ms where this
+// takes 130 us (four maps of 25,600 queries, 4 heads).  64 queries to a wave, which halves the reads of the means, 154;
+// a second pass that ranks doubtful queries against all blocks 184.
 template <int KS, int SMAX>
-__global__ __launch_bounds__(256) void select_tile_kernel(const SelectArgs a) {
+__global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1) void select_tile_kernel(const SelectArgs a) {
   __shared__ double qsum[4][128];
   __shared__ int pool[4][kPools][64];
   __shared__ long long keys[4][64];
@@ -639,7 +646,8 @@ __global__ __launch_bounds__(256) void select_tile_kernel(const SelectArgs a) {
 
 constexpr int kScoreQueries = 8;
 
-// Scores of 64 blocks and up to eight queries in 64 bits, four lanes to a block.
+// Scores of 64 blocks and up to eight queries in 64 bits, four lanes to a block.  For one token against caches the time is
+// that of the means' way from memory (34 MB in 7 us).
 template <int KS>
 __global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
   __shared__ double qsum[kScoreQueries][128];
@@ -675,7 +683,8 @@ __global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
   }
 }
 
-// One query per workgroup: each wave ranks a quarter of its blocks, then every candidate counts those before it.
+// One query per workgroup: each wave ranks a quarter of its blocks, then every candidate counts those before it.  Bound by
+// the chain of its steps: 11 us for 16 of 1,024 blocks, however many queries there are up to the number of CUs.
 __global__ __launch_bounds__(256) void rank_kernel(const SelectArgs a) {
   __shared__ long long key[256];
   __shared__ int id[256], chosen[64];
