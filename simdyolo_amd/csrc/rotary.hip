@@ -1,6 +1,7 @@
 // Rotary positions (Su et al., 2021): channels of every query and key head in pairs (a, b), each turned
 // by the token's position times the pair's frequency, y = (a c - b s, b c + a s).
 #include <cmath>
+#include <new>
 
 #include "sy_internal.h"
 
@@ -157,7 +158,9 @@ int op_rotary_create(sy_ctx* ctx, const sy_rotary_config* c, uint64_t* rotary) {
   if (c->scaling == SY_ROTARY_PARTS)
     SY_CHECK(c->original > 0 && std::isfinite(c->low) && std::isfinite(c->high) && c->low >= 0 && c->high > c->low,
              SY_EINVAL, "rotary scaling by parts needs original > 0 and 0 <= low < high");
-  auto p = std::make_unique<RotaryPlan>();
+  SY_CHECK(ctx, SY_EINVAL, "null context");
+  std::unique_ptr<RotaryPlan> p(new (std::nothrow) RotaryPlan);
+  SY_CHECK(p, SY_ENOMEM, "no memory for a rotary plan");
   p->cfg = *c;
   p->half = part / 2;
   p->amplitude = 1.f;
@@ -175,8 +178,11 @@ int op_rotary_create(sy_ctx* ctx, const sy_rotary_config* c, uint64_t* rotary) {
     }
     p->turns[i] = f / pi2;
   }
-  SY_CHECK(ctx, SY_EINVAL, "null context");
-  ctx->rotaries.push_back(std::move(p));
+  try {
+    ctx->rotaries.push_back(std::move(p));
+  } catch (const std::bad_alloc&) {
+    SY_CHECK(false, SY_ENOMEM, "no memory for a rotary plan");
+  }
   *rotary = ctx->rotaries.size();
   return SY_OK;
 }
@@ -193,6 +199,7 @@ int op_rotary_run(sy_ctx* ctx, uint64_t rotary, const sy_rotary_heads* parts, in
     SY_TRY(check_view(&h.x, "rotary input"));
     SY_TRY(check_view(&h.y, "rotary output"));
     SY_CHECK(h.heads > 0, SY_EINVAL, "rotary needs a head");
+    SY_CHECK((long long)h.heads * p.cfg.head_dim < (1LL << 27), SY_EUNSUPPORTED, "rotary over %d heads", h.heads);
     const int xs = h.x_stride ? h.x_stride : p.cfg.head_dim, ys = h.y_stride ? h.y_stride : p.cfg.head_dim;
     for (const auto& v : {std::make_pair(&h.x, xs), std::make_pair(&h.y, ys)}) {
       SY_CHECK(v.second >= p.cfg.head_dim && v.second % 4 == 0, SY_EINVAL, "rotary head stride %d", v.second);
