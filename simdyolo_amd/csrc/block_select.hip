@@ -405,12 +405,15 @@ constexpr int kPools = 8;      // doubtful queries of a wave whose candidates ar
 constexpr int kPartTiles = 8;  // 32-block tiles of a workgroup below
 
 // The means of one key head as the A operands of the matrix instructions (32 blocks x 16 channels, two parts
-// each), and the largest norm among them.
+// each), and the largest norm among them.  Means that no query sees (a cache's, behind the last token) are taken as 0,
+// so that what stands there does not widen the bound or send every query through 64 bits.
 template <int KS>
 __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
   __shared__ float top[4];
   const int plane = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, b = plane / a.kv, g = plane % a.kv;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  int forced;
+  const int seen = seen_blocks(a, b, a.tq - 1, &forced);
   float most = 0.f;
   for (int t = wave; t < kPartTiles; t += 4) {
     const int tile = chunk * kPartTiles + t, j = tile * 32 + (lane & 31);
@@ -423,7 +426,7 @@ __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int c = 16 * ks + 8 * half + 4 * u;
-        const f32x4 v = c < a.kd && j < a.blocks ? *(const f32x4*)(m + c) : f32x4{0.f, 0.f, 0.f, 0.f};
+        const f32x4 v = c < a.kd && j < seen ? *(const f32x4*)(m + c) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           f[4 * u + e] = v[e];
@@ -735,6 +738,7 @@ int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q,
   SY_CHECK(m->n == q->n, SY_EINVAL, "%d images of queries, %d of block means", q->n, m->n);
   SY_CHECK((m->h == 1 && s.bh == 1) || (!lengths && !s.causal), SY_EINVAL,
            "lengths and causal need keys and blocks one pixel high");
+  SY_CHECK((long long)q->n * s.kv < (1 << 24), SY_EUNSUPPORTED, "block select over %d x %d key heads", q->n, s.kv);
   SY_CHECK(ctx, SY_EINVAL, "null context");
   SelectArgs a{};
   a.q = q->data;

@@ -238,6 +238,27 @@ def test_long_causal_rows(hip, kd, selected):
         np.testing.assert_array_equal(got[:, i:i + 1], exp)
 
 
+def test_means_behind_the_sequence_are_not_read(hip):
+    """Whatever a cache's means hold behind the last query or the length: nothing of it in the choice."""
+    cfg, kd, w, tq = R.shape(4, 2, 1, 4, 5, causal=1), 32, 1600, 1030
+    q, k = tensors(2, w, tq, cfg, kd, 5)
+    m = R.means(cfg, k, 1, w).astype(np.float32)
+    starts, lengths = (100, 400), (1130, 1300)
+    whole = run_select(hip, cfg, q, m, 1, w, starts, lengths, many=True)
+    for value in (np.nan, np.inf, 1e30):
+        far = m.copy()
+        far[0, -(-1130 // 4):] = value
+        far[1, -(-1300 // 4):] = value
+        np.testing.assert_array_equal(run_select(hip, cfg, q, far, 1, w, starts, lengths, many=True), whole)
+        far[1, -(-1300 // 4):] = m[1, -(-1300 // 4):]
+        far[1, -(-1430 // 4):] = value  # no lengths: behind the last query
+        np.testing.assert_array_equal(run_select(hip, cfg, q, far, 1, w, starts, None, many=True),
+                                      run_select(hip, cfg, q, m, 1, w, starts, None, many=True))
+    keep = np.arange(0, tq, 41)
+    for i in keep:
+        np.testing.assert_array_equal(whole[:, i:i + 1], R.select(cfg, q[:, i:i + 1], m, [x + i for x in starts], lengths))
+
+
 def test_one_image_too_many(hip):
     cfg, kd = R.shape(2, 2, 1, 4, 2), 8
     with R.Device(hip) as d:
