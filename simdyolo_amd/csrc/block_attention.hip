@@ -489,7 +489,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
 #pragma unroll
     for (int x = 0; x < 32; ++x) w[x] = sc[x >> 4][x & 15] + rest[x >> 4][x & 15];
     if (k_flat) {
-      c = __builtin_ldexpf(cs, k_one + q_power);
+      c = fmaxf(__builtin_ldexpf(cs, k_one + q_power), FLT_MIN);  // not 0, which would make hidden keys' scores NaN
     } else {
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
@@ -875,6 +875,8 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
            "lengths and causal need keys and blocks one pixel high");
   SY_CHECK(!views_overlap(o, q) && !views_overlap(o, k) && !views_overlap(o, v), SY_EINVAL,
            "block attention output overlaps an input");
+  SY_CHECK((long long)q->n * s.kv < (1 << 24) && (long long)q->h * q->w * s.selected < (1LL << 31), SY_EUNSUPPORTED,
+           "block attention over %d x %dx%d queries", q->n, q->h, q->w);
   SY_CHECK(ctx, SY_EINVAL, "null context");
   s.n = q->n;
   s.tq = q->h * q->w;
@@ -897,8 +899,6 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   a.ldo = o->ldc;
   a.parts = (int)(((long long)s.bh * s.bw + kKeys - 1) / kKeys);
   const int planes = s.n * s.kv;
-  SY_CHECK((long long)s.n * s.kv < (1 << 24) && (long long)s.tq * s.selected < (1LL << 31), SY_EUNSUPPORTED,
-           "block attention over %d x %d queries", s.n, s.tq);
   // Segments: as many queries as keep the results of one in kPartials bytes
   // (and, pair by pair, its workgroups in 2^23), and as many segments to a launch.
   const double per_query = std::max((sizeof(float) * s.hd + sizeof(Stat)) * (double)s.selected * a.parts * s.group / kPartials,
@@ -925,7 +925,9 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   const long long result_rows = together * pairs * a.parts * s.group;
   SY_CHECK((result_rows + 1) * s.hd < (1LL << 30) - 128 && tile_cap * together < (1LL << 24), SY_EUNSUPPORTED,
            "block attention over %d heads to a key head", s.group);
-  SY_CHECK((double)s.bh * s.kw * std::max(k->ldc, v->ldc) < 4294967296.0, SY_EUNSUPPORTED,
+  SY_CHECK(!sorted || segments * a.chunks * kSortThreads < (1LL << 32), SY_EUNSUPPORTED,
+           "block attention over %lld lists", segments);
+  SY_CHECK(((s.bh - 1.0) * s.kw + s.bw) * std::max(k->ldc, v->ldc) < 4294967296.0, SY_EUNSUPPORTED,
            "block windows that span 2^32 floats and more");
   a.tile_cap = (int)tile_cap;
   a.trash = (unsigned)result_rows;

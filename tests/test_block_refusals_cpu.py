@@ -125,6 +125,19 @@ def test_outputs_overlap():
     assert "overlap" in why()
 
 
+def test_more_heads_and_queries_than_lists():
+    one = dict(h=1, w=1, data=far(1))
+    many = cfg(heads=4096, kv_heads=4096, key_dim=4, head_dim=4, block_h=1, block_w=1, selected=1)
+    n = 1 << 13  # 2^25 key heads
+    q, k, v = (view(4 * 4096, n=n, **{**one, "data": AT + (i << 40)}) for i in (1, 2, 3))
+    assert select(many, q=q, m=k) == N.SY_EUNSUPPORTED
+    assert attention(many, q=q, k=k, v=v, o=view(4 * 4096, n=n, h=1, w=1, data=AT + (4 << 40))) == N.SY_EUNSUPPORTED
+    q, o = (view(c, h=1 << 14, w=1 << 15, n=1, data=AT + (i << 44)) for c, i in ((64, 1), (128, 2)))
+    assert attention(cfg(selected=4), q=q, o=o, k=view(32, n=1, data=far(2)), v=view(64, n=1, data=far(3))) == \
+        N.SY_EUNSUPPORTED
+    assert why() != "null context"
+
+
 ROTARY = dict(head_dim=32, dim=16, axes=1, interleaved=0, base=10000.0, scaling=0, factor=1.0, low=1.0, high=32.0,
               original=4096)
 

@@ -256,6 +256,70 @@ def test_neighbours_do_not_change_a_row(hip):
     np.testing.assert_array_equal(moved, whole[:, turn])
 
 
+@pytest.mark.parametrize("tq,cfg,w,dim,sort", [(40000, R.shape(2, 2, 1, 2, 64), 400, 128, True),
+                                               (140000, R.shape(1, 1, 1, 1, 64), 13000, 4, False)], ids=["sorted", "few"])
+def test_more_results_than_one_launch_holds(hip, tq, cfg, w, dim, sort):
+    """1.34 GB of results for each head, in two launches; 9.0 million pairs of query and block, in two."""
+    q, k, v = tensors(1, tq, w, cfg, 32, dim, 9)
+    g, count = R.rng(10), R.count_blocks(cfg, 1, w)
+    blocks = (g.integers(0, count, (1, tq, cfg["kv_heads"], 1)) + np.arange(64) * 3) % count
+    got = run(hip, cfg, q, k, v, blocks, 1, w, pads=False, sort=sort)
+    assert np.isfinite(got).all()
+    keep = np.unique(np.concatenate([[0, tq - 1], g.integers(0, tq, 200), np.arange(tq // 2 - 20, tq // 2 + 20)]))
+    exp, bound = R.attend(cfg, q[:, keep], k, v, blocks[:, keep], 1, w, 32 ** -0.5)
+    check(got[:, keep], exp, bound)
+
+
+@pytest.mark.parametrize("tq,sort", [(3, False), (4000, True)])
+def test_offsets_past_32_bits(hip, tq, sort):
+    """A cache whose last keys lie 17 GB behind its first: rotation in place, means of the last block, selection and
+    attention there."""
+    cfg, kd, hd, w, ldc, last = R.shape(4, 2, 1, 128, 4, causal=1), 32, 64, (1 << 20) + 6400, 4160, 6400
+    _, k, v = tensors(1, 1, last, cfg, kd, hd, 21)
+    q = R.rng(22).standard_normal((1, tq, 4, kd)).astype(np.float32)
+    blocks, tail = w // 128, last // 128
+    with R.Device(hip) as d:
+        base = hip.malloc(4 * w * ldc)
+        d.ptrs.append(base)
+        slab = np.zeros((last, ldc), np.float32)
+        slab[:, :64], slab[:, 64:192] = k[0].reshape(last, 64), v[0].reshape(last, 128)
+        end = base + 4 * ldc * (w - last)
+        hip.h2d(end, slab)
+        vk, vv = N.Tensor(base, 1, 64, 1, w, ldc, 0), N.Tensor(base + 256, 1, 128, 1, w, ldc, 0)
+        hip.rotary(hip.rotary_create(kd, kd), [N.RotaryHeads(vk, vk, 2, 0, 0)])
+        hip.flush()
+        rk = hip.d2h(end, (last, ldc))[:, :64].reshape(1, last, 2, kd)
+        f, _ = R.frequencies(kd, 10000.0, 0, 1, 1, 32, 0)
+        exp, near = R.rotate(k, np.arange(w - last, w).reshape(1, last, 1), kd, False, f, 1.0)
+        assert (np.abs(rk - exp) <= near * 2.0 ** -21).all()
+        m = np.zeros((1, blocks, 2, kd), np.float32)
+        m[:, -tail:] = R.means(cfg, rk, 1, last)  # in front of them: zeros
+        vm, _, read_m = d.view(m.reshape(1, blocks, 1, 64), 1, blocks)
+        at = d.ints([w - tq])
+        cf = R.config(cfg, kd, hd)
+        hip.h2d(vm.data + 4 * 64 * (blocks - tail), np.full((tail, 64), np.nan, np.float32))
+        hip.block_means(cf, vk, vm, d.ints([w - last]), last)
+        got_m = read_m().reshape(1, blocks, 2, kd)
+        assert (np.abs(got_m - m)[:, -tail:] <= np.abs(m)[:, -tail:] * 2.0 ** -23 + np.abs(rk).max() * 2.0 ** -45).all()
+        vq, _, _ = d.view(q, 1, tq)
+        lists = d.put(np.zeros((1, tq, 2, 4), np.int32))
+        hip.block_select(cf, vq, vm, lists, at)
+        chosen = hip.d2h(lists, (1, tq, 2, 4), np.int32)
+        np.testing.assert_array_equal(chosen[:, ::37], np.concatenate(
+            [R.select(cfg, q[:, i:i + 1], got_m, [w - tq + i]) for i in range(0, tq, 37)], 1))
+        near_end = np.maximum(chosen, blocks - tail)  # blocks whose keys were written; named twice they count twice
+        vo, _, read = d.view(np.full((1, tq, 4, hd), np.nan, np.float32), 1, tq)
+        hip.profile_enable(True)
+        try:
+            hip.block_attention(cf, vq, vk, vv, d.put(near_end), vo, at)
+            hip.flush()
+            assert ("block_sort" in hip.profile_read()) == sort
+        finally:
+            hip.profile_enable(False)
+        exp, bound = R.attend(cfg, q, rk, v, near_end - (blocks - tail), 1, last, kd ** -0.5, [last - tq])
+        check(read(), exp, bound)
+
+
 # ------------------------------------------------------------------ in a row
 
 class Chain:
