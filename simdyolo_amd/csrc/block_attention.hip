@@ -123,80 +123,107 @@ __global__ __launch_bounds__(kSortThreads) void block_count_kernel(const BlockAr
   for (int j = threadIdx.x; j < a.s.blocks; j += kSortThreads) out[j] = hist[j];
 }
 
+__device__ __forceinline__ int3 operator+(int3 a, int3 b) { return make_int3(a.x + b.x, a.y + b.y, a.z + b.z); }
+
 // Exclusive sum over the workgroup's threads; *total: of all.
-__device__ __forceinline__ int2 scan_threads(int2 v, int2* lds, int2* total) {
+__device__ __forceinline__ int3 scan_threads(int3 v, int3* lds, int3* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int2 x = v;
+  int3 x = v;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const int ax = __shfl_up(x.x, off), ay = __shfl_up(x.y, off);
-    if (lane >= off) {
-      x.x += ax;
-      x.y += ay;
-    }
+    const int3 o = make_int3(__shfl_up(x.x, off), __shfl_up(x.y, off), __shfl_up(x.z, off));
+    if (lane >= off) x = x + o;
   }
   if (lane == 63) lds[wave] = x;
   __syncthreads();
-  int2 before = make_int2(0, 0), all = make_int2(0, 0);
+  int3 before = make_int3(0, 0, 0), all = before;
 #pragma unroll
   for (int w = 0; w < kSortThreads / 64; ++w) {
-    const int2 t = lds[w];
-    if (w < wave) before = make_int2(before.x + t.x, before.y + t.y);
-    all = make_int2(all.x + t.x, all.y + t.y);
+    if (w < wave) before = before + lds[w];
+    all = all + lds[w];
   }
   __syncthreads();
   *total = all;
-  return make_int2(before.x + x.x - v.x, before.y + x.y - v.y);
+  return make_int3(before.x + x.x - v.x, before.y + x.y - v.y, before.z + x.z - v.z);
 }
 
-// Puts the pairs in the order of their blocks (within a block in no certain order: a row's result does not
-// depend on its neighbours in a tile).  Every chunk's workgroup sums the counts of its segment for itself and
-// writes the tiles of some blocks.  With one chunk it does the counting, too.
+// Rows of each tile of a block's list of `all`: equal shares, in 32s.
+__device__ __forceinline__ int tile_share(const BlockArgs& a, int all) {
+  const int tiles = (all + a.rows - 1) / a.rows;
+  return ((all + tiles - 1) / max(tiles, 1) + 31) & ~31;
+}
+
+// Puts the pairs in the order of their blocks (within a block by chunk, within a chunk in no certain order: a row's
+// result does not depend on its neighbours in a tile).  Every chunk's workgroup sums the counts of its segment for itself and
+// writes the tiles that begin among its own pairs, so that tiles stand in the order of their first queries: those
+// under way together read the same queries (8,192 causal tokens, whose queries are 17 MB to a key head, block by block).
+// With one chunk it does the counting, too.
 __global__ __launch_bounds__(kSortThreads) void block_scatter_kernel(const BlockArgs a) {
   extern __shared__ int hist[];
-  __shared__ int2 lds[kSortThreads / 64];
-  __shared__ int4 work[kSortThreads];
+  __shared__ int3 lds[kSortThreads / 64];
   const BlockShape& s = a.s;
-  const int seg = blockIdx.x / a.chunks, chunk = blockIdx.x - seg * a.chunks;
+  const int seg = blockIdx.x / a.chunks, chunk = blockIdx.x - seg * a.chunks, lane = threadIdx.x & 63;
   const int* counts = a.counts + (long long)seg * a.chunks * s.blocks;
   int4* tiles = a.tiles + (long long)seg * a.tile_cap;
-  int2 base = make_int2(0, 0);
   if (a.chunks == 1) {
     for (int j = threadIdx.x; j < s.blocks; j += kSortThreads) hist[j] = 0;
     __syncthreads();
     for_pairs(a, seg, chunk, [&](int, int j) { atomicAdd(&hist[j], 1); });
     __syncthreads();
   }
-  for (int j0 = 0; j0 < s.blocks; j0 += kSortThreads) {
-    const int j = j0 + threadIdx.x;
-    int n = 0, before = 0;  // pairs of block j, those of earlier chunks
+  // Block j's pairs, those of earlier chunks, and its tiles that begin before this chunk's pairs and behind them.
+  struct Count {
+    int n, before, from, to;
+  };
+  auto count = [&](int j) {
+    Count c{0, 0, 0, 0};
+    int own = 0;
     if (j < s.blocks) {
       if (a.chunks == 1)
-        n = hist[j];
+        c.n = own = hist[j];
       else
 #pragma unroll 8
-        for (int c = 0; c < a.chunks; ++c) {
-          const int m = counts[(long long)c * s.blocks + j];
-          n += m;
-          if (c < chunk) before += m;
+        for (int x = 0; x < a.chunks; ++x) {
+          const int m = counts[(long long)x * s.blocks + j];
+          c.n += m;
+          if (x < chunk) c.before += m;
+          if (x == chunk) own = m;
         }
     }
-    const int t = (int)(((long long)n * s.group + a.rows - 1) / a.rows);
-    int2 total;
-    const int2 at = scan_threads(make_int2(n, t * a.parts), lds, &total);
-    if (j < s.blocks) hist[j] = base.x + at.x + before;
-    work[threadIdx.x] = make_int4(base.x + at.x, n, base.y + at.y, t);
-    __syncthreads();
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int u = wave * a.chunks + chunk; u < min(kSortThreads, s.blocks - j0); u += kSortThreads / 64 * a.chunks) {
-      const int4 w = work[u];
-      for (int x = lane; x < w.w * a.parts; x += 64)
-        tiles[w.z + x] = make_int4(j0 + u, x % a.parts | (x / a.parts) << 8, w.x, w.y);
+    if (c.n) {
+      const int share = tile_share(a, c.n * s.group);
+      c.from = (c.before * s.group + share - 1) / share;
+      c.to = ((c.before + own) * s.group + share - 1) / share;
     }
-    __syncthreads();
-    base = make_int2(base.x + total.x, base.y + total.y);
+    return c;
+  };
+  int3 base = make_int3(0, 0, 0), total;  // pairs, this chunk's tiles, earlier chunks' tiles
+  if (a.chunks > 1 && s.blocks > kSortThreads) {
+    for (int j = threadIdx.x; j < s.blocks; j += kSortThreads) base.z += count(j).from * a.parts;
+    (void)scan_threads(base, lds, &total);
+    base = make_int3(0, total.z, 0);
   }
-  if (chunk == 0 && threadIdx.x == 0) a.tile_count[seg] = base.y;
+  for (int j0 = 0; j0 < s.blocks; j0 += kSortThreads) {
+    const int j = j0 + threadIdx.x;
+    const Count c = count(j);
+    const int items = (c.to - c.from) * a.parts;
+    const int3 at = scan_threads(make_int3(c.n, items, s.blocks > kSortThreads ? 0 : c.from * a.parts), lds, &total);
+    if (j < s.blocks) hist[j] = base.x + at.x + c.before;
+    const int list_at = base.x + at.x, tile_at = base.y + total.z + at.y;
+    auto put = [&](int j, int x, int from, int first, int n, int to) {
+      tiles[to + x] = make_int4(j, x % a.parts | (from + x / a.parts) << 8, first, n);
+    };
+    constexpr int kAlone = 16;  // items that a thread writes; a wave together, beyond
+    if (items <= kAlone)
+      for (int x = 0; x < items; ++x) put(j, x, c.from, list_at, c.n, tile_at);
+    for (unsigned long long todo = __ballot(items > kAlone); todo; todo &= todo - 1) {
+      const int l = __builtin_ctzll(todo), many = __shfl(items, l), from = __shfl(c.from, l), first = __shfl(list_at, l),
+                n = __shfl(c.n, l), to = __shfl(tile_at, l);
+      for (int x = lane; x < many; x += 64) put(j - lane + l, x, from, first, n, to);
+    }
+    base = make_int3(base.x + total.x, base.y + total.z + total.y, 0);
+  }
+  if (chunk == a.chunks - 1 && threadIdx.x == 0) a.tile_count[seg] = base.y;
   __syncthreads();
   int* list = a.list + (long long)seg * a.span * s.selected;
   int* pos = a.pos + (long long)seg * a.span * s.selected;
@@ -295,7 +322,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
   const int4 rec = a.tiles[(long long)seg * a.tile_cap + t];  // under way with the count
   if (t >= a.tile_count[seg]) return;
   // Its share of the block's rows: as many as the other tiles', in 32s.
-  const int all = rec.w * s.group, tiles = (all + a.rows - 1) / a.rows, share = ((all + tiles - 1) / tiles + 31) & ~31;
+  const int all = rec.w * s.group, share = tile_share(a, all);
   const int j = rec.x, part = rec.y & 255, row0 = (rec.y >> 8) * share;
   const int rows = min(all - row0, share);
   if (rows <= 0) return;

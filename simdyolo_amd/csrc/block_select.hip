@@ -12,6 +12,7 @@
 namespace sy {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // The config alone; the views' part is filled in by the callers.
@@ -648,6 +649,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
 }
 
 constexpr int kScoreQueries = 8;
+constexpr int kCandidates = 256;  // of a ranking
 
 // Scores of 64 blocks and up to eight queries in 64 bits, four lanes to a block.  For one token against caches the time is
 // that of the means' way from memory (34 MB in 7 us).
@@ -686,39 +688,78 @@ __global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
   }
 }
 
-// One query per workgroup: each wave ranks a quarter of its blocks, then every candidate counts those before it.  Bound by
-// the chain of its steps: 11 us for 16 of 1,024 blocks, however many queries there are up to the number of CUs.
+// One query per workgroup.  The n-th largest of the threads' own largest scores (their upper 32 bits) is no more than the n-th
+// largest of all: the blocks from there up, a few more than wanted, are ranked by counting those before each.  Where they
+// do not fit (many blocks alike), one wave ranks all.
 __global__ __launch_bounds__(256) void rank_kernel(const SelectArgs a) {
-  __shared__ long long key[256];
-  __shared__ int id[256], chosen[64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ __align__(16) int top[256];
+  __shared__ int bound, count, chosen[64];
+  __shared__ long long key[kCandidates];
+  __shared__ int id[kCandidates];
+  const int tid = threadIdx.x, lane = tid & 63;
   const long long* keys = a.keys + (long long)blockIdx.x * a.blocks;
-  const int part = (a.blocks + 3) / 4, from = min(wave * part, a.blocks), count = min(part, a.blocks - from);
-  long long bk;
-  int bi;
-  const int kept = rank_wave(count, a.selected, lane, [&](int j) { return keys[from + j]; }, &bk, &bi);
-  key[threadIdx.x] = lane < kept ? bk : kHidden;
-  id[threadIdx.x] = lane < kept ? from + bi : 0x7fffffff;
-  if (threadIdx.x < 64) chosen[threadIdx.x] = 0x7fffffff;
+  const int row = blockIdx.x % a.tq, plane = blockIdx.x / a.tq;  // keys are [plane][query]
+  int* out = a.out + (((long long)(plane / a.kv) * a.tq + row) * a.kv + plane % a.kv) * a.selected;
+  long long k[4];  // of the first 1024 blocks, the others are read twice
+  int most = INT_MIN;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    k[u] = tid + 256 * u < a.blocks ? keys[tid + 256 * u] : kHidden;
+    most = max(most, (int)(k[u] >> 32));
+  }
+#pragma unroll 4
+  for (int j = tid + 1024; j < a.blocks; j += 256) most = max(most, (int)(keys[j] >> 32));
+  most = (most & ~255) | (255 - tid);  // each its own
+  top[tid] = most;
+  if (tid == 0) count = 0;
+  if (tid < 64) chosen[tid] = INT_MAX;
   __syncthreads();
-  if (lane < kept) {
-    int before = lane;  // of its own wave
-    for (int w = 1; w < 4; ++w) {
-      const int other = 64 * ((wave + w) & 3);
+  int before = 0;
 #pragma unroll 8
-      for (int n = 0; n < a.selected; ++n)
-        before += key[other + n] > bk || (key[other + n] == bk && id[other + n] < from + bi);
+  for (int n = 0; n < 64; ++n) {
+    const i32x4 t = *(const i32x4*)&top[4 * n];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) before += t[e] > most;
+  }
+  if (before == a.selected - 1) bound = most & ~255;
+  __syncthreads();
+  const int least = bound;
+  auto offer = [&](int j, long long x) {
+    if (x == kHidden || (int)(x >> 32) < least) return;
+    const int at = atomicAdd(&count, 1);
+    if (at < kCandidates) {
+      key[at] = x;
+      id[at] = j;
     }
-    if (before < a.selected) chosen[before] = id[threadIdx.x];
+  };
+#pragma unroll
+  for (int u = 0; u < 4; ++u) offer(tid + 256 * u, k[u]);
+  for (int j = tid + 1024; j < a.blocks; j += 256) offer(j, keys[j]);
+  __syncthreads();
+  const int found = count;
+  if (found > kCandidates) {
+    if (tid >= 64) return;
+    long long bk;
+    int bi;
+    const int kept = rank_wave(a.blocks, a.selected, lane, [&](int j) { return keys[j]; }, &bk, &bi);
+    write_row(out, a.selected, kept, lane, bi);
+    return;
+  }
+  if (tid < found) {
+    const long long mine = key[tid];
+    const int j = id[tid];
+    int rank = 0;
+#pragma unroll 4
+    for (int n = 0; n < found; ++n) rank += key[n] > mine || (key[n] == mine && id[n] < j);
+    if (rank < a.selected) chosen[rank] = j;
   }
   __syncthreads();
-  if (wave == 0) {
+  if (tid < 64) {
     const int mine = chosen[lane];
     int place = 0;
+#pragma unroll 8
     for (int n = 0; n < a.selected; ++n) place += chosen[n] < mine;
-    const int row = blockIdx.x % a.tq, plane = blockIdx.x / a.tq;  // keys are [plane][query]
-    int* out = a.out + (((long long)(plane / a.kv) * a.tq + row) * a.kv + plane % a.kv) * a.selected;
-    if (lane < a.selected) out[mine != 0x7fffffff ? place : lane] = mine != 0x7fffffff ? mine : -1;
+    if (lane < a.selected) out[mine != INT_MAX ? place : lane] = mine != INT_MAX ? mine : -1;
   }
 }
 
