@@ -199,6 +199,8 @@ struct SelectArgs {
   u32x4* parts;
   float* norm;
   int tiles, chunks;
+  int tag_bits;      // of a block's number in its scores
+  float tag_error;   // twice what they cost, of a score
   // few queries: scores, and how many of them a workgroup takes
   long long* keys;
   int queries;
@@ -347,8 +349,7 @@ __device__ __forceinline__ void select_exact(const SelectArgs& a, int b, int i, 
   __builtin_amdgcn_wave_barrier();
 }
 
-// The same among `count` candidates (up to 64, more than wanted) in ascending order: four lanes score one, then each
-// counts those before it.
+// The same among `count` candidates (up to 64, more than wanted): four lanes score one, then each counts those before it.
 __device__ __forceinline__ void select_among(const SelectArgs& a, int b, int i, int g, int lane, double* qsum,
                                              long long* keys, const int* pool, int count) {
   query_sums(a, b, i, g, lane, qsum);
@@ -372,17 +373,19 @@ __device__ __forceinline__ void select_among(const SelectArgs& a, int b, int i, 
     if ((lane & 3) == 0 && n < count) keys[n] = j == forced ? LLONG_MAX : score_key(s);
   }
   __builtin_amdgcn_wave_barrier();
-  const int mine = min(lane, count - 1);
-  const long long key = keys[mine];
+  const int mine = pool[min(lane, count - 1)];
+  const long long key = keys[min(lane, count - 1)];
   int before = 0;
 #pragma unroll 8
   for (int n = 0; n < count; ++n) {
     const long long k = keys[n];
-    before += k > key || (k == key && n < lane);
+    before += k > key || (k == key && pool[n] < mine);
   }
   const unsigned long long chosen = __ballot(lane < count && before < a.selected);
-  if (chosen >> lane & 1)
-    a.out[(((long long)b * a.tq + i) * a.kv + g) * a.selected + __builtin_popcountll(chosen & ((1ull << lane) - 1))] = pool[mine];
+  int place = 0;
+#pragma unroll 8
+  for (int n = 0; n < count; ++n) place += (chosen >> n & 1) && pool[n] < mine;
+  if (chosen >> lane & 1) a.out[(((long long)b * a.tq + i) * a.kv + g) * a.selected + place] = mine;
   __builtin_amdgcn_wave_barrier();
 }
 
@@ -473,10 +476,11 @@ __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
 // 1,400 the second pass; the matrix cores are busy a fifth of the time.  Scores in 64 bits throughout took 9.9 ms where this
 // takes 130 us (four maps of 25,600 queries, 4 heads).  64 queries to a wave, which halves the reads of the means, 154;
 // a second pass that ranks doubtful queries against all blocks 184.
-template <int KS, int SMAX>
+template <int KS, int SMAX, bool TAGS>
 __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1) void select_tile_kernel(const SelectArgs a) {
   __shared__ double qsum[4][128];
-  __shared__ int pool[4][kPools][64];
+  constexpr int kRow = 2 * SMAX + 3;  // candidates of a query (odd: its lanes' banks differ)
+  __shared__ int pool[TAGS ? 4 * 32 * kRow : 4 * kPools * 64];
   __shared__ long long keys[4][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, r32 = lane & 31;
@@ -538,7 +542,9 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
   }
   const u32x4* parts = a.parts + (long long)plane * a.tiles * KS * 2 * 64 + lane;
 
-  // Scores of tile n, whose parts are under way, with what is not seen at -inf and what is forced at +inf.
+  // Scores of tile n, whose parts are under way, with what is not seen at -inf and what is forced at +inf (with tags, which
+  // have no room beside an infinity, it is left out).
+  const unsigned keep = ~0u << a.tag_bits;
   u32x4 m[KS][2];
   auto load = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
@@ -558,19 +564,26 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
       sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m0, q[ks][0], sc, 0, 0, 0);
     }
     load(min(n + 1, last - 1));
+    if (TAGS)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = sc[r];
+        sc[r] = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, x) & keep) | (unsigned)(16 * n + r));
+      }
     const int room = seen - 32 * n - 4 * half, own = forced - 32 * n - 4 * half;
     if (__any(room < 32 || (own >= 0 && own < 32)))
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int at = 8 * (r >> 2) + (r & 3);
-        sc[r] = at >= room ? -INFINITY : at == own ? INFINITY : sc[r];
+        sc[r] = at >= room ? -INFINITY : at == own ? (TAGS ? -INFINITY : INFINITY) : sc[r];
       }
     return sc;
   };
 
+  const int wanted = a.selected - (TAGS && forced >= 0);
   float list[SMAX + 1];
 #pragma unroll
-  for (int n = 0; n <= SMAX; ++n) list[n] = n < SMAX - a.selected && half == 0 ? INFINITY : -INFINITY;
+  for (int n = 0; n <= SMAX; ++n) list[n] = n < SMAX - wanted && half == 0 ? INFINITY : -INFINITY;
   if (last > 0) load(0);
   for (int n = 0; n < last; ++n) {
     const f32x16 sc = scores(n);
@@ -594,8 +607,53 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
   for (int n = 0; n < SMAX; ++n) nth = fminf(nth, fmaxf(list[n], other[SMAX - 1 - n]));
 #pragma unroll
   for (int n = 0; n <= SMAX; ++n) after = fminf(after, fmaxf(list[n], other[SMAX - n]));
-  const float from = nth - slack;  // scores from here up are written
+  // Scores from here up are candidates.
+  const float from = __builtin_fabsf(nth) == INFINITY ? nth : nth - (TAGS ? slack + a.tag_error * __builtin_fabsf(nth) : slack);
   const bool doubt = !exact && i < a.tq && seen > a.selected && !(after < from);
+  const bool mine = half == 0 && i < a.tq;
+  int* out = a.out + (((long long)b * a.tq + i) * a.kv + g) * a.selected;
+
+  if constexpr (TAGS) {
+    // Candidates of both halves side by side, the lower half's first, then the block that is always taken.
+    exact |= doubt && (list[SMAX] >= from || other[SMAX] >= from);  // maybe more than the lists hold
+    int own = 0;
+#pragma unroll
+    for (int n = 0; n <= SMAX; ++n) own += list[n] >= from && __builtin_fabsf(list[n]) < INFINITY;
+    const int others = __shfl_xor(own, 32), count = own + others + (forced >= 0);
+    int* row = pool + (wave * 32 + r32) * kRow;
+    int to = half ? others : 0;
+#pragma unroll
+    for (int n = 0; n <= SMAX; ++n)
+      if (list[n] >= from && __builtin_fabsf(list[n]) < INFINITY) {
+        const int tag = __builtin_bit_cast(unsigned, list[n]) & ~keep;
+        row[to++] = (tag >> 4) * 32 + (tag & 12) * 2 + 4 * half + (tag & 3);
+      }
+    if (half && forced >= 0) row[count - 1] = forced;
+    __builtin_amdgcn_wave_barrier();
+    if (i < a.tq && !exact && !doubt) {
+      int id[SMAX];
+#pragma unroll
+      for (int n = 0; n < SMAX; ++n) id[n] = n < count ? row[n] : INT_MAX;
+#pragma unroll
+      for (int e = 0; e < SMAX; e += 2) {  // every second one for each half
+        const int one = half ? id[e + 1] : id[e];
+        int place = 0;
+#pragma unroll
+        for (int n = 0; n < SMAX; ++n) place += id[n] < one;
+        if (e + half < a.selected) out[e + half < count ? place : e + half] = e + half < count ? one : -1;
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    for (unsigned long long todo = __ballot(mine && doubt && !exact); todo; todo &= todo - 1) {
+      const int x = __builtin_ctzll(todo);
+      select_among(a, b, i0 + x, g, lane, qsum[wave], keys[wave], pool + (wave * 32 + x) * kRow,
+                   __builtin_amdgcn_readlane(count, x));
+    }
+    for (unsigned long long todo = __ballot(mine && exact); todo; todo &= todo - 1)
+      select_exact(a, b, i0 + __builtin_ctzll(todo), g, lane, qsum[wave]);
+    return;
+  }
+
   const unsigned doubts = (unsigned)__ballot(doubt);  // of the lower half; the upper one agrees
   int slot = doubt ? __builtin_popcount(doubts & ((1u << r32) - 1)) : -1;  // of a doubtful query's candidates
   if (slot >= kPools) {
@@ -603,8 +661,6 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
     exact = true;
   }
 
-  int* out = a.out + (((long long)b * a.tq + i) * a.kv + g) * a.selected;
-  const bool mine = half == 0 && i < a.tq;
   int count = 0;
   if (last > 0) load(0);
   for (int n = 0; n < last; ++n) {
@@ -626,7 +682,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
         w &= w - 1;
         if (mine && !exact) {
           if (slot >= 0) {
-            if (count < 64) pool[wave][slot][count] = j;
+            if (count < 64) pool[(wave * kPools + slot) * 64 + count] = j;
           } else if (count < a.selected) {
             out[count] = j;
           }
@@ -641,7 +697,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
     for (int n = count; n < a.selected; ++n) out[n] = -1;
   for (unsigned long long todo = __ballot(mine && !exact && slot >= 0); todo; todo &= todo - 1) {
     const int x = __builtin_ctzll(todo);
-    select_among(a, b, i0 + x, g, lane, qsum[wave], keys[wave], pool[wave][__builtin_amdgcn_readlane(slot, x)],
+    select_among(a, b, i0 + x, g, lane, qsum[wave], keys[wave], pool + (wave * kPools + __builtin_amdgcn_readlane(slot, x)) * 64,
                  __builtin_amdgcn_readlane(count, x));
   }
   for (unsigned long long todo = __ballot(mine && exact); todo; todo &= todo - 1)
@@ -768,6 +824,7 @@ __global__ __launch_bounds__(256) void rank_kernel(const SelectArgs a) {
 // queries 50 / 57 / 67 us against 14 / 16 / 22; 4,096 blocks, 8 key heads, 128 queries 366 against 152; but 128 blocks of 64
 // channels, 32 key heads, 128 queries 28 against 33.
 constexpr int kManyRows = 2048, kFewBlocks = 64;
+constexpr int kTagBits = 11;
 
 int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q, const sy_tensor* m,
                     const int32_t* starts, const int32_t* lengths, int32_t* blocks) {
@@ -847,34 +904,25 @@ int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q,
   ProfScope prof(ctx, "block_select", flops, bytes);
   const dim3 g((unsigned)(planes * groups));
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, dim3(256), 0, ctx->stream, a); };
-  if (steps == 2) {
-    if (s.selected <= 8)
-      launch(select_tile_kernel<2, 8>);
-    else if (s.selected <= 16)
-      launch(select_tile_kernel<2, 16>);
-    else if (s.selected <= 32)
-      launch(select_tile_kernel<2, 32>);
+  int bits = 4;
+  while (16LL << (bits - 4) < 16LL * a.tiles) ++bits;
+  a.tag_bits = bits;
+  a.tag_error = 2.125f * std::ldexp(1.f, bits - 23);
+  auto pick = [&](auto tags8, auto tags16, auto twice8, auto twice16, auto twice32, auto twice64) {
+    if (bits <= kTagBits && s.selected <= 16)
+      launch(s.selected <= 8 ? tags8 : tags16);
     else
-      launch(select_tile_kernel<2, 64>);
-  } else if (steps == 4) {
-    if (s.selected <= 8)
-      launch(select_tile_kernel<4, 8>);
-    else if (s.selected <= 16)
-      launch(select_tile_kernel<4, 16>);
-    else if (s.selected <= 32)
-      launch(select_tile_kernel<4, 32>);
-    else
-      launch(select_tile_kernel<4, 64>);
-  } else {
-    if (s.selected <= 8)
-      launch(select_tile_kernel<8, 8>);
-    else if (s.selected <= 16)
-      launch(select_tile_kernel<8, 16>);
-    else if (s.selected <= 32)
-      launch(select_tile_kernel<8, 32>);
-    else
-      launch(select_tile_kernel<8, 64>);
-  }
+      launch(s.selected <= 8 ? twice8 : s.selected <= 16 ? twice16 : s.selected <= 32 ? twice32 : twice64);
+  };
+  if (steps == 2)
+    pick(select_tile_kernel<2, 8, true>, select_tile_kernel<2, 16, true>, select_tile_kernel<2, 8, false>,
+         select_tile_kernel<2, 16, false>, select_tile_kernel<2, 32, false>, select_tile_kernel<2, 64, false>);
+  else if (steps == 4)
+    pick(select_tile_kernel<4, 8, true>, select_tile_kernel<4, 16, true>, select_tile_kernel<4, 8, false>,
+         select_tile_kernel<4, 16, false>, select_tile_kernel<4, 32, false>, select_tile_kernel<4, 64, false>);
+  else
+    pick(select_tile_kernel<8, 8, true>, select_tile_kernel<8, 16, true>, select_tile_kernel<8, 8, false>,
+         select_tile_kernel<8, 16, false>, select_tile_kernel<8, 32, false>, select_tile_kernel<8, 64, false>);
   return check_launch("block_select");
 }
 
