@@ -480,10 +480,13 @@ template <int KS, int SMAX, bool TAGS>
 __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1) void select_tile_kernel(const SelectArgs a) {
   __shared__ double qsum[4][128];
   constexpr int kRow = 2 * SMAX + 3;  // candidates of a query (odd: its lanes' banks differ)
-  __shared__ int pool[TAGS ? 4 * 32 * kRow : 4 * kPools * 64];
   __shared__ long long keys[4][64];
+  constexpr int KB = KS < 4 ? KS : 4, kStage = 32 * (16 * KB + 4);
+  __shared__ __align__(16) float stage[4][kStage];  // query sums; candidates
+  static_assert(kStage >= (TAGS ? 32 * kRow : kPools * 64), "candidates of a wave");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, r32 = lane & 31;
+  int* pool = (int*)stage[wave];
   const int groups = (a.tq + 127) / 128;
   const int plane = blockIdx.x / groups, b = plane / a.kv, g = plane - b * a.kv;
   const int i0 = (blockIdx.x - plane * groups) * 128 + wave * 32;
@@ -502,38 +505,55 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
   const int seen = seen_blocks(a, b, min(i, a.tq - 1), &forced);
   const int last = __builtin_amdgcn_readfirstlane((wave_max_i32(seen) + 31) / 32);
   {
-    // A head's channels are under way together, up to 32 to a lane.
-    constexpr int KB = KS < 4 ? KS : 4;
-    const float* p = a.q + ((long long)b * a.tq + min(i, a.tq - 1)) * a.ldq + (long long)g * a.group * a.qs;
+    // Up to 64 channels of a head at a time, in whole lines: a lane sums four channels of every STEP-th row over the heads,
+    // and the sums change their layout in LDS.
+    constexpr int kLanes = 4 * KB, kStep = 64 / kLanes, kSteps = 32 / kStep;
+    float* sums = stage[wave];
+    const int sub = lane % kLanes, first = lane / kLanes;
+    const float* p = a.q + (long long)b * a.tq * a.ldq + (long long)g * a.group * a.qs;
     float qn = 0.f;
 #pragma unroll
     for (int k0 = 0; k0 < KS; k0 += KB) {
-      double s[KB][8];
+      const int c = 16 * k0 + 4 * sub;
+      const float* from[kSteps];
+      double s[kSteps][4];
 #pragma unroll
-      for (int ks = 0; ks < KB; ++ks)
+      for (int t = 0; t < kSteps; ++t) {
+        from[t] = p + (long long)min(i0 + t * kStep + first, a.tq - 1) * a.ldq + min(c, a.kd - 4);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[ks][e] = 0.0;
-      for (int h = 0; h < a.group; ++h) {
-        f32x4 v[KB][2];
-#pragma unroll
-        for (int ks = 0; ks < KB; ++ks)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) v[ks][u] = *(const f32x4*)(p + (long long)h * a.qs + min(16 * (k0 + ks) + 8 * half + 4 * u, a.kd - 4));
-#pragma unroll
-        for (int ks = 0; ks < KB; ++ks)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) s[ks][e] += v[ks][e >> 2][e & 3];
+        for (int e = 0; e < 4; ++e) s[t][e] = 0.0;
       }
+      for (int h = 0; h < a.group; ++h) {
+        f32x4 v[kSteps];
+#pragma unroll
+        for (int t = 0; t < kSteps; ++t) v[t] = *(const f32x4*)(from[t] + (long long)h * a.qs);
+#pragma unroll
+        for (int t = 0; t < kSteps; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[t][e] += v[t][e];
+      }
+#pragma unroll
+      for (int t = 0; t < kSteps; ++t) {
+        f32x4 f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = c < a.kd ? (float)s[t][e] : 0.f;
+        *(f32x4*)&sums[(t * kStep + first) * (16 * KB + 4) + 4 * sub] = f;
+      }
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int ks = 0; ks < KB; ++ks) {
         float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          f[e] = 16 * (k0 + ks) + 8 * half + 4 * (e >> 2) < a.kd ? (float)s[ks][e] : 0.f;
-          qn = __builtin_fmaf(f[e], f[e], qn);
+        for (int u = 0; u < 2; ++u) {
+          const f32x4 v = *(const f32x4*)&sums[r32 * (16 * KB + 4) + 16 * ks + 8 * half + 4 * u];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[4 * u + e] = v[e];
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qn = __builtin_fmaf(f[e], f[e], qn);
         halves8(f, q[k0 + ks]);
       }
+      __builtin_amdgcn_wave_barrier();
     }
     qn += __shfl_xor(qn, 32);
     const bool fine = qn >= 0x1p-80f && qn <= 0x1p80f && kn >= 0x1p-80f && kn <= 0x1p80f;
@@ -620,7 +640,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
 #pragma unroll
     for (int n = 0; n <= SMAX; ++n) own += list[n] >= from && __builtin_fabsf(list[n]) < INFINITY;
     const int others = __shfl_xor(own, 32), count = own + others + (forced >= 0);
-    int* row = pool + (wave * 32 + r32) * kRow;
+    int* row = pool + r32 * kRow;
     int to = half ? others : 0;
 #pragma unroll
     for (int n = 0; n <= SMAX; ++n)
@@ -646,7 +666,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
     __builtin_amdgcn_wave_barrier();
     for (unsigned long long todo = __ballot(mine && doubt && !exact); todo; todo &= todo - 1) {
       const int x = __builtin_ctzll(todo);
-      select_among(a, b, i0 + x, g, lane, qsum[wave], keys[wave], pool + (wave * 32 + x) * kRow,
+      select_among(a, b, i0 + x, g, lane, qsum[wave], keys[wave], pool + x * kRow,
                    __builtin_amdgcn_readlane(count, x));
     }
     for (unsigned long long todo = __ballot(mine && exact); todo; todo &= todo - 1)
@@ -682,7 +702,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
         w &= w - 1;
         if (mine && !exact) {
           if (slot >= 0) {
-            if (count < 64) pool[(wave * kPools + slot) * 64 + count] = j;
+            if (count < 64) pool[slot * 64 + count] = j;
           } else if (count < a.selected) {
             out[count] = j;
           }
@@ -697,7 +717,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
     for (int n = count; n < a.selected; ++n) out[n] = -1;
   for (unsigned long long todo = __ballot(mine && !exact && slot >= 0); todo; todo &= todo - 1) {
     const int x = __builtin_ctzll(todo);
-    select_among(a, b, i0 + x, g, lane, qsum[wave], keys[wave], pool + (wave * kPools + __builtin_amdgcn_readlane(slot, x)) * 64,
+    select_among(a, b, i0 + x, g, lane, qsum[wave], keys[wave], pool + __builtin_amdgcn_readlane(slot, x) * 64,
                  __builtin_amdgcn_readlane(count, x));
   }
   for (unsigned long long todo = __ballot(mine && exact); todo; todo &= todo - 1)
