@@ -195,7 +195,7 @@ struct SelectArgs {
   int* out;
   long long ldq, ldm, rows;
   int tq, blocks, bw, kv, group, kd, qs, selected, causal;
-  // many queries: the means' parts, their largest norm for each of `chunks` of them
+  // many queries: the means' parts, made by `chunks` workgroups for each key head, and their norms
   u32x4* parts;
   float* norm;
   int tiles, chunks;
@@ -317,10 +317,20 @@ __device__ __forceinline__ double query_sum(const SelectArgs& a, const float* q,
   return s;
 }
 
-// The sum of query i's heads of group g, in 64 bits, for all lanes of a wave.
+// The sum of query i's heads of group g, in 64 bits, for all lanes of a wave: two channels to a lane.
 __device__ __forceinline__ void query_sums(const SelectArgs& a, int b, int i, int g, int lane, double* qsum) {
-  const float* q = a.q + ((long long)b * a.tq + i) * a.ldq + (long long)g * a.group * a.qs;
-  for (int c = lane; c < a.kd; c += 64) qsum[c] = query_sum(a, q, c);
+  const float* q = a.q + ((long long)b * a.tq + i) * a.ldq + (long long)g * a.group * a.qs + min(2 * lane, a.kd - 2);
+  double s0 = 0, s1 = 0;
+#pragma unroll 8
+  for (int h = 0; h < a.group; ++h) {
+    const f32x2v v = *(const f32x2v*)(q + (long long)h * a.qs);
+    s0 += v[0];
+    s1 += v[1];
+  }
+  if (2 * lane < a.kd) {
+    qsum[2 * lane] = s0;
+    qsum[2 * lane + 1] = s1;
+  }
   __builtin_amdgcn_wave_barrier();
 }
 
@@ -349,44 +359,65 @@ __device__ __forceinline__ void select_exact(const SelectArgs& a, int b, int i, 
   __builtin_amdgcn_wave_barrier();
 }
 
-// The same among `count` candidates (up to 64, more than wanted): four lanes score one, then each counts those before it.
-__device__ __forceinline__ void select_among(const SelectArgs& a, int b, int i, int g, int lane, double* qsum,
-                                             long long* keys, const int* pool, int count) {
-  query_sums(a, b, i, g, lane, qsum);
-  int forced;
-  (void)seen_blocks(a, b, i, &forced);
-  const int quarter = 4 * (lane & 3);
-  for (int n0 = 0; n0 < count; n0 += 16) {
-    const int n = n0 + (lane >> 2), j = pool[min(n, count - 1)];
-    const float* m = a.m + ((long long)b * a.blocks + j) * a.ldm + g * a.kd;
-    f32x4 v[8];
+// The same among `count` candidates (up to 64, more than wanted), of which those marked kDoubtful are scored: sixteen
+// lanes to one, KS channels to a lane, four at a time.
+constexpr int kDoubtful = 1 << 30;
+template <int KS>
+__device__ __forceinline__ void select_among(const SelectArgs& a, int b, int i, int g, int lane, const int* pool, int count) {
+  const int entry = lane < count ? pool[lane] : 0, id = lane < count ? entry & ~kDoubtful : INT_MAX;
+  const unsigned long long doubtful = __ballot(entry & kDoubtful);
+  const int c = KS * (lane & 15);
+  f32x2v m[KS / 2];
+  double qsum[KS];
+  long long key = kHidden;
+  for (unsigned long long todo = doubtful; todo;) {
+    int at[4];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) v[x] = *(const f32x4*)(m + min(16 * x + quarter, a.kd - 4));
+    for (int u = 0; u < 4; ++u) {
+      at[u] = todo ? __builtin_ctzll(todo) : -1;
+      todo &= todo - 1;
+    }
+    const int mine = lane < 32 ? (lane < 16 ? at[0] : at[1]) : (lane < 48 ? at[2] : at[3]);
+    const float* from = a.m + ((long long)b * a.blocks + __shfl(id, max(mine, at[0]))) * a.ldm + g * a.kd;
+#pragma unroll
+    for (int x = 0; x < KS / 2; ++x) m[x] = *(const f32x2v*)(from + min(c + 2 * x, a.kd - 2));
+    if (at[0] == __builtin_ctzll(doubtful)) {  // the first time
+      const float* q = a.q + ((long long)b * a.tq + i) * a.ldq + (long long)g * a.group * a.qs;
+#pragma unroll
+      for (int x = 0; x < KS; ++x) qsum[x] = 0;
+#pragma unroll 4
+      for (int h = 0; h < a.group; ++h)
+#pragma unroll
+        for (int x = 0; x < KS / 2; ++x) {
+          const f32x2v v = *(const f32x2v*)(q + (long long)h * a.qs + min(c + 2 * x, a.kd - 2));
+          qsum[2 * x] += v[0];
+          qsum[2 * x + 1] += v[1];
+        }
+    }
     double s = 0;
 #pragma unroll
-    for (int x = 0; x < 8; ++x)
-      if (16 * x + quarter < a.kd)
+    for (int x = 0; x < KS / 2; ++x)
+      if (c + 2 * x < a.kd) s = __builtin_fma(qsum[2 * x + 1], (double)m[x][1], __builtin_fma(qsum[2 * x], (double)m[x][0], s));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s = __builtin_fma(qsum[16 * x + quarter + e], (double)v[x][e], s);
-    s += __shfl_xor(s, 1);
-    s += __shfl_xor(s, 2);
-    if ((lane & 3) == 0 && n < count) keys[n] = j == forced ? LLONG_MAX : score_key(s);
+    for (int off = 1; off < 16; off <<= 1) s += __shfl_xor(s, off);
+    const long long k = score_key(s);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long long of = __shfl(k, 16 * u);
+      if (lane == at[u]) key = of;
+    }
   }
-  __builtin_amdgcn_wave_barrier();
-  const int mine = pool[min(lane, count - 1)];
-  const long long key = keys[min(lane, count - 1)];
-  int before = 0;
-#pragma unroll 8
-  for (int n = 0; n < count; ++n) {
-    const long long k = keys[n];
-    before += k > key || (k == key && pool[n] < mine);
+  int before = count - __builtin_popcountll(doubtful);
+  for (unsigned long long todo = doubtful; todo; todo &= todo - 1) {
+    const int n = __builtin_ctzll(todo);
+    const long long k = __shfl(key, n);
+    before += k > key || (k == key && __shfl(id, n) < id);
   }
-  const unsigned long long chosen = __ballot(lane < count && before < a.selected);
+  const unsigned long long chosen = __ballot(lane < count && (!(doubtful >> lane & 1) || before < a.selected));
   int place = 0;
-#pragma unroll 8
-  for (int n = 0; n < count; ++n) place += (chosen >> n & 1) && pool[n] < mine;
-  if (chosen >> lane & 1) a.out[(((long long)b * a.tq + i) * a.kv + g) * a.selected + place] = mine;
-  __builtin_amdgcn_wave_barrier();
+  for (unsigned long long todo = chosen; todo; todo &= todo - 1)
+    place += __builtin_amdgcn_readlane(id, __builtin_ctzll(todo)) < id;
+  if ((chosen >> lane & 1) && place < a.selected) a.out[(((long long)b * a.tq + i) * a.kv + g) * a.selected + place] = id;
 }
 
 // Eight floats as two bf16 parts, v = p[0] + p[1] up to 2^-18 of v.
@@ -409,16 +440,14 @@ constexpr int kPools = 8;      // doubtful queries of a wave whose candidates ar
 constexpr int kPartTiles = 8;  // 32-block tiles of a workgroup below
 
 // The means of one key head as the A operands of the matrix instructions (32 blocks x 16 channels, two parts
-// each), and the largest norm among them.  Means that no query sees (a cache's, behind the last token) are taken as 0,
+// each), and their norms, squared.  Means that no query sees (a cache's, behind the last token) are taken as 0,
 // so that what stands there does not widen the bound or send every query through 64 bits.
 template <int KS>
 __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
-  __shared__ float top[4];
   const int plane = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, b = plane / a.kv, g = plane % a.kv;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   int forced;
   const int seen = seen_blocks(a, b, a.tq - 1, &forced);
-  float most = 0.f;
   for (int t = wave; t < kPartTiles; t += 4) {
     const int tile = chunk * kPartTiles + t, j = tile * 32 + (lane & 31);
     if (tile >= a.tiles) break;
@@ -444,19 +473,7 @@ __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
       to[64] = __builtin_bit_cast(u32x4, p[1]);
     }
     norm += __shfl_xor(norm, 32);
-    most = norm <= most ? most : norm;  // a NaN stays
-    if (norm != norm) most = norm;
-  }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    const float o = __shfl_xor(most, off);
-    most = o <= most || most != most ? most : o;
-  }
-  if (lane == 0) top[wave] = most;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 4; ++w) most = top[w] <= most || most != most ? most : top[w];
-    a.norm[blockIdx.x] = most;
+    if (half == 0 && j < a.blocks) a.norm[(long long)plane * a.blocks + j] = norm;
   }
 }
 
@@ -480,7 +497,6 @@ template <int KS, int SMAX, bool TAGS>
 __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1) void select_tile_kernel(const SelectArgs a) {
   __shared__ double qsum[4][128];
   constexpr int kRow = 2 * SMAX + 3;  // candidates of a query (odd: its lanes' banks differ)
-  __shared__ long long keys[4][64];
   constexpr int KB = KS < 4 ? KS : 4, kStage = 32 * (16 * KB + 4);
   __shared__ __align__(16) float stage[4][kStage];  // query sums; candidates
   static_assert(kStage >= (TAGS ? 32 * kRow : kPools * 64), "candidates of a wave");
@@ -492,11 +508,6 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
   const int i0 = (blockIdx.x - plane * groups) * 128 + wave * 32;
   if (i0 >= a.tq) return;
 
-  float kn = 0.f;
-  for (int c = 0; c < a.chunks; ++c) {
-    const float o = a.norm[plane * a.chunks + c];
-    kn = o <= kn || kn != kn ? kn : o;
-  }
   bf16x8 q[KS][2];
   float slack;  // 2 e
   bool exact;   // all blocks of this lane's query are scored in 64 bits
@@ -504,6 +515,13 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
   const int i = i0 + r32;
   const int seen = seen_blocks(a, b, min(i, a.tq - 1), &forced);
   const int last = __builtin_amdgcn_readfirstlane((wave_max_i32(seen) + 31) / 32);
+  // The largest norm of the means whose scores count: not of the block that holds the last token, whose mean, of few keys,
+  // may be many times as long as the others (NaN above all).
+  const int scored = wave_max_i32(forced >= 0 ? forced : seen);
+  int top = 0;
+  for (int j = lane; j < scored; j += 64)
+    top = max(top, __builtin_bit_cast(int, a.norm[(long long)plane * a.blocks + j]) & 0x7fffffff);
+  const float kn = scored ? __builtin_bit_cast(float, wave_max_i32(top)) : 1.f;
   {
     // Up to 64 channels of a head at a time, in whole lines: a lane sums four channels of every STEP-th row over the heads,
     // and the sums change their layout in LDS.
@@ -629,6 +647,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
   for (int n = 0; n <= SMAX; ++n) after = fminf(after, fmaxf(list[n], other[SMAX - n]));
   // Scores from here up are candidates.
   const float from = __builtin_fabsf(nth) == INFINITY ? nth : nth - (TAGS ? slack + a.tag_error * __builtin_fabsf(nth) : slack);
+  const float sure = nth + (nth - from);  // scores above are chosen, whatever their errors (NaN: there is no doubt)
   const bool doubt = !exact && i < a.tq && seen > a.selected && !(after < from);
   const bool mine = half == 0 && i < a.tq;
   int* out = a.out + (((long long)b * a.tq + i) * a.kv + g) * a.selected;
@@ -636,6 +655,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
   if constexpr (TAGS) {
     // Candidates of both halves side by side, the lower half's first, then the block that is always taken.
     exact |= doubt && (list[SMAX] >= from || other[SMAX] >= from);  // maybe more than the lists hold
+    const int mark = doubt ? kDoubtful : 0;
     int own = 0;
 #pragma unroll
     for (int n = 0; n <= SMAX; ++n) own += list[n] >= from && __builtin_fabsf(list[n]) < INFINITY;
@@ -646,7 +666,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
     for (int n = 0; n <= SMAX; ++n)
       if (list[n] >= from && __builtin_fabsf(list[n]) < INFINITY) {
         const int tag = __builtin_bit_cast(unsigned, list[n]) & ~keep;
-        row[to++] = (tag >> 4) * 32 + (tag & 12) * 2 + 4 * half + (tag & 3);
+        row[to++] = ((tag >> 4) * 32 + (tag & 12) * 2 + 4 * half + (tag & 3)) | (list[n] > sure ? 0 : mark);
       }
     if (half && forced >= 0) row[count - 1] = forced;
     __builtin_amdgcn_wave_barrier();
@@ -666,8 +686,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
     __builtin_amdgcn_wave_barrier();
     for (unsigned long long todo = __ballot(mine && doubt && !exact); todo; todo &= todo - 1) {
       const int x = __builtin_ctzll(todo);
-      select_among(a, b, i0 + x, g, lane, qsum[wave], keys[wave], pool + x * kRow,
-                   __builtin_amdgcn_readlane(count, x));
+      select_among<KS>(a, b, i0 + x, g, lane, pool + x * kRow, __builtin_amdgcn_readlane(count, x));
     }
     for (unsigned long long todo = __ballot(mine && exact); todo; todo &= todo - 1)
       select_exact(a, b, i0 + __builtin_ctzll(todo), g, lane, qsum[wave]);
@@ -685,24 +704,33 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
   if (last > 0) load(0);
   for (int n = 0; n < last; ++n) {
     const f32x16 sc = scores(n);
-    unsigned w = 0;
+    unsigned w = 0, near = 0;
 #pragma unroll
     for (int r = 15; r >= 0; --r) w = w + w + (sc[r] >= from);
     if (!__any(w != 0)) continue;
     // Four blocks of this half, four of the other, and so on.
-    w = (w | w << 8) & 0x00ff00ffu;
-    w = (w | w << 4) & 0x0f0f0f0fu;
-    const unsigned o = (unsigned)__shfl_xor((int)w, 32);
-    w = half ? o | w << 4 : w | o << 4;
+    auto both = [&](unsigned w) {
+      w = (w | w << 8) & 0x00ff00ffu;
+      w = (w | w << 4) & 0x0f0f0f0fu;
+      const unsigned o = (unsigned)__shfl_xor((int)w, 32);
+      return half ? o | w << 4 : w | o << 4;
+    };
+    w = both(w);
+    if (doubts) {
+#pragma unroll
+      for (int r = 15; r >= 0; --r) near = near + near + !(sc[r] > sure);
+      near = both(near);
+    }
     const int room = seen - 32 * n;
     if (room < 32) w &= room > 0 ? (1u << room) - 1 : 0u;
     while (__any(w != 0)) {
       if (w) {
         const int j = 32 * n + __builtin_ctz(w);
+        const int mark = near & (w & -w) ? kDoubtful : 0;
         w &= w - 1;
         if (mine && !exact) {
           if (slot >= 0) {
-            if (count < 64) pool[slot * 64 + count] = j;
+            if (count < 64) pool[slot * 64 + count] = j | mark;
           } else if (count < a.selected) {
             out[count] = j;
           }
@@ -717,8 +745,8 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
     for (int n = count; n < a.selected; ++n) out[n] = -1;
   for (unsigned long long todo = __ballot(mine && !exact && slot >= 0); todo; todo &= todo - 1) {
     const int x = __builtin_ctzll(todo);
-    select_among(a, b, i0 + x, g, lane, qsum[wave], keys[wave], pool + __builtin_amdgcn_readlane(slot, x) * 64,
-                 __builtin_amdgcn_readlane(count, x));
+    select_among<KS>(a, b, i0 + x, g, lane, pool + __builtin_amdgcn_readlane(slot, x) * 64,
+                     __builtin_amdgcn_readlane(count, x));
   }
   for (unsigned long long todo = __ballot(mine && exact); todo; todo &= todo - 1)
     select_exact(a, b, i0 + __builtin_ctzll(todo), g, lane, qsum[wave]);
@@ -907,7 +935,7 @@ int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q,
   const long long groups = (a.tq + 127) / 128;
   SY_CHECK((long long)planes * groups * 256 < (1LL << 32) && (long long)planes * a.chunks * 256 < (1LL << 32),
            SY_EUNSUPPORTED, "block select grid too large");
-  SY_TRY(ensure_scratch(ctx, parts + sizeof(float) * planes * a.chunks));
+  SY_TRY(ensure_scratch(ctx, parts + sizeof(float) * planes * (size_t)a.blocks));
   a.parts = (u32x4*)ctx->scratch;
   a.norm = (float*)(ctx->scratch + parts);
   {
