@@ -183,10 +183,11 @@ int op_block_means(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* k, 
 
 // ----------------------------------------------------------------- selection
 //
-// Many queries: scores in float32 from the matrix cores with a bound e on their error, twice over.  The first pass
-// keeps the largest ones of each query, so that the `selected`-th, t, is known; no block further than 2 e below t is
-// chosen, whatever the rounding.  The second pass writes the blocks from t - 2 e up.  Where more than `selected`
-// lie there, some queries in a hundred, those blocks are scored again in 64 bits and ranked.
+// Many queries: scores in float32 from the matrix cores with a bound e on their error.  The largest ones of each query are
+// kept, so that the `selected`-th, t, is known; no block further than 2 e below t is chosen, whatever the rounding, and
+// every block further than 2 e above it is.  Up to 16 of 4,096 blocks are kept with their numbers; of more, the scores are
+// formed again and compared with t - 2 e.  Where more than `selected` lie there, some queries in a hundred, those within
+// 2 e of t are scored again in 64 bits.
 // Few queries: scores in 64 bits, then a ranking.
 
 struct SelectArgs {
@@ -436,7 +437,7 @@ __device__ __forceinline__ void halves8(const float (&x)[8], bf16x8 (&p)[2]) {
   p[1] = __builtin_bit_cast(bf16x8, w[1]);
 }
 
-constexpr int kPools = 8;      // doubtful queries of a wave whose candidates are kept
+constexpr int kPools = 8;      // doubtful queries of a wave whose candidates are kept (second pass)
 constexpr int kPartTiles = 8;  // 32-block tiles of a workgroup below
 
 // The means of one key head as the A operands of the matrix instructions (32 blocks x 16 channels, two parts
@@ -483,16 +484,22 @@ __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
 // so far stay sorted in registers: a new score moves through them by one median of three each.  (Fewer wanted:
 // the list starts with infinities.)  The two halves' lists meet at the end.
 //
+// TAGS: the lowest tag_bits of a score are the tile and r, so that the lists name their blocks.  That moves a score by up to
+// u = 2^(tag_bits - 23) of itself: 2 u |t| more between two of them at the border, taken with 2.125 u for the scores near t
+// that are a little larger than it.  (Otherwise: a second pass over all scores.)
+//
 // Error of a score: a part is off by 2^-8 of what it stands for, so two of them by 2^-16, twice (operands), and the
 // product of the second parts is left out, 2^-16 again: 3 x 2^-16 of sum |q||m|.  Sums of at most 24 matrix
 // instructions with 16 products each, and q rounded from 64 bits, stay below 2^-18.  sum |q||m| <= |q||m| in norms,
 // which sums in float32 and two roots change by less than 2^-16 of themselves: e = 3.5 x 2^-16 |q| max|m|.  Norms
 // outside 2^-40 .. 2^40 could lose parts to underflow: all blocks of those queries are scored in 64 bits.
 //
-// Bound by vector work: of 4,700 operations per wave (32 queries, 400 blocks of 32 channels, 8 wanted) 1,900 are medians and
-// 1,400 the second pass; the matrix cores are busy a fifth of the time.  Scores in 64 bits throughout took 9.9 ms where this
-// takes 130 us (four maps of 25,600 queries, 4 heads).  64 queries to a wave, which halves the reads of the means, 154;
-// a second pass that ranks doubtful queries against all blocks 184.
+// Bound by vector work, which keeps the SIMDs busy nine tenths of the time: 3,600 operations per wave (32 queries, 400 blocks
+// of 32 channels, 8 wanted), of them 1,900 medians; the matrix cores work a sixth of it.  Four maps of 25,600 queries, 4
+// heads: 105 us; with a second pass over the scores 140; in 64 bits throughout 9,900; 64 queries to a wave, which halves the
+// reads of the means, 154.  Two causal rows of 16,001 tokens, 16 / 4 heads of 128 channels, 16 of 251 blocks: 91 us, of them
+// 50 the queries' way from memory; with all candidates of doubtful queries scored again 117, their heads read in 32-byte
+// pieces besides 126.
 template <int KS, int SMAX, bool TAGS>
 __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1) void select_tile_kernel(const SelectArgs a) {
   __shared__ double qsum[4][128];
@@ -519,8 +526,13 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
   // may be many times as long as the others (NaN above all).
   const int scored = wave_max_i32(forced >= 0 ? forced : seen);
   int top = 0;
-  for (int j = lane; j < scored; j += 64)
-    top = max(top, __builtin_bit_cast(int, a.norm[(long long)plane * a.blocks + j]) & 0x7fffffff);
+  for (int j = lane; j < scored + lane; j += 512) {
+    int v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = ((const int*)a.norm)[(long long)plane * a.blocks + min(j + 64 * u, scored - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) top = max(top, v[u] & 0x7fffffff);
+  }
   const float kn = scored ? __builtin_bit_cast(float, wave_max_i32(top)) : 1.f;
   {
     // Up to 64 channels of a head at a time, in whole lines: a lane sums four channels of every STEP-th row over the heads,
@@ -792,9 +804,10 @@ __global__ __launch_bounds__(256) void score_kernel(const SelectArgs a) {
   }
 }
 
-// One query per workgroup.  The n-th largest of the threads' own largest scores (their upper 32 bits) is no more than the n-th
+// One query per workgroup.  The n-th largest of the threads' own largest scores (their upper bits) is no more than the n-th
 // largest of all: the blocks from there up, a few more than wanted, are ranked by counting those before each.  Where they
-// do not fit (many blocks alike), one wave ranks all.
+// do not fit (many blocks alike), one wave ranks all.  Bound by its steps one after another: 7.5 us for 16 of 1,024 blocks,
+// however many queries there are up to the number of CUs; taking the largest of all heads of four waves' lists 11.
 __global__ __launch_bounds__(256) void rank_kernel(const SelectArgs a) {
   __shared__ __align__(16) int top[256];
   __shared__ int bound, count, chosen[64];
@@ -868,10 +881,12 @@ __global__ __launch_bounds__(256) void rank_kernel(const SelectArgs a) {
 }
 
 // The matrix cores from here on, and where there are few blocks (both take 10 us then).  Below, a wave's walk through all
-// blocks, twice, takes longer than all scores in 64 bits: 512 blocks of 128 channels, 16 of them, 4 key heads and 1 / 32 / 128
-// queries 50 / 57 / 67 us against 14 / 16 / 22; 4,096 blocks, 8 key heads, 128 queries 366 against 152; but 128 blocks of 64
-// channels, 32 key heads, 128 queries 28 against 33.
+// blocks takes longer than all scores in 64 bits: 512 blocks of 128 channels, 16 of them, 4 key heads and 1 / 128 / 512 queries
+// 34 / 41 / 43 us against 11 / 18 / 39; 128 blocks of 64 channels, 32 key heads, 8 / 32 / 64 queries 15 / 15 / 17 against
+// 10 / 15 / 20.
 constexpr int kManyRows = 2048, kFewBlocks = 64;
+// Numbers of up to 11 bits (128 tiles, 4,096 blocks) in the scores of lists of up to 16: 8 / 16 of 400 blocks of 32 channels 112 /
+// 150 us, with a second pass 149 / 190; of 128 channels 111 and 180.  More blocks would cost the scores too many bits.
 constexpr int kTagBits = 11;
 
 int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q, const sy_tensor* m,

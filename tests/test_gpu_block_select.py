@@ -198,6 +198,33 @@ def test_pairs_of_blocks_that_are_alike(hip, tq):
     np.testing.assert_array_equal(got, R.select(cfg, few, m))
 
 
+@pytest.mark.parametrize("blocks", [4096, 4097])
+@pytest.mark.parametrize("kd,selected", [(32, 5), (64, 16), (128, 8), (128, 16), (32, 33)])
+def test_many_blocks(hip, blocks, kd, selected):
+    """Up to and past the blocks whose numbers fit into their scores; pairs of them 2^-18 apart."""
+    cfg = R.shape(2, 1, 1, 1, selected)
+    q, _ = tensors(1, 1, MANY, cfg, kd, 8)
+    m = R.rng(3).standard_normal((1, blocks, 1, kd)).astype(np.float32)
+    m[:, 1::2] = m[:, :blocks // 2 * 2:2] * np.float32(1 + 2.0 ** -18)
+    got = run_select(hip, cfg, q, m, 1, blocks, many=True)
+    few, got = some(q, got)
+    np.testing.assert_array_equal(got, R.select(cfg, few, m))
+
+
+@pytest.mark.parametrize("tq", [FEW, MANY])
+@pytest.mark.parametrize("selected", [1, 8, 16])
+def test_negative_and_tiny_scores(hip, tq, selected):
+    """No score above zero, and blocks with scores of zero or far below the others' among them."""
+    cfg, kd, blocks = R.shape(2, 2, 1, 1, selected), 40, 333
+    q, _ = tensors(1, 1, tq, cfg, kd, 8)
+    q, m = np.abs(q), -np.abs(R.rng(3).standard_normal((1, blocks, 2, kd))).astype(np.float32)
+    m[:, ::60] = 0
+    m[:, 1::70] *= np.float32(2.0 ** -120)
+    got = run_select(hip, cfg, q, m, 1, blocks, many=tq == MANY)
+    few, got = some(q, got)
+    np.testing.assert_array_equal(got, R.select(cfg, few, m))
+
+
 @pytest.mark.parametrize("tq", [FEW, MANY])
 @pytest.mark.parametrize("scales", [(1e-30, 1e-12), (1e25, 1e20), (1e-42, 1.0), (0.0, 1.0), (1.0, 0.0), (1e12, 1e-12)], ids=str)
 def test_far_scaled(hip, tq, scales):
