@@ -484,7 +484,7 @@ __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
 // so far stay sorted in registers: a new score moves through them by one median of three each.  (Fewer wanted:
 // the list starts with infinities.)  The two halves' lists meet at the end.
 //
-// TAGS: the lowest tag_bits of a score are the tile and r, so that the lists name their blocks.  That moves a score by up to
+// Tags: the lowest tag_bits of a score are the tile and r, so that the lists name their blocks.  That moves a score by up to
 // u = 2^(tag_bits - 23) of itself: 2 u |t| more between two of them at the border, taken with 2.125 u for the scores near t
 // that are a little larger than it.  (Otherwise: a second pass over all scores.)
 //
@@ -500,9 +500,12 @@ __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
 // reads of the means, 154.  Two causal rows of 16,001 tokens, 16 / 4 heads of 128 channels, 16 of 251 blocks: 91 us, of them
 // 50 the queries' way from memory; with all candidates of doubtful queries scored again 117, their heads read in 32-byte
 // pieces besides 126.
-template <int KS, int SMAX, bool TAGS>
+// kTwice: a second pass over the scores; kTags: their blocks' numbers in them; kRaw: that, on the means as they are.
+enum { kTwice, kTags, kRaw };
+template <int KS, int SMAX, int MODE>
 __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1) void select_tile_kernel(const SelectArgs a) {
   __shared__ double qsum[4][128];
+  constexpr bool TAGS = MODE != kTwice;
   constexpr int kRow = 2 * SMAX + 3;  // candidates of a query (odd: its lanes' banks differ)
   constexpr int KB = KS < 4 ? KS : 4, kStage = 32 * (16 * KB + 4);
   __shared__ __align__(16) float stage[4][kStage];  // query sums; candidates
@@ -516,8 +519,6 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
   if (i0 >= a.tq) return;
 
   bf16x8 q[KS][2];
-  float slack;  // 2 e
-  bool exact;   // all blocks of this lane's query are scored in 64 bits
   int forced;
   const int i = i0 + r32;
   const int seen = seen_blocks(a, b, min(i, a.tq - 1), &forced);
@@ -526,14 +527,14 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
   // may be many times as long as the others (NaN above all).
   const int scored = wave_max_i32(forced >= 0 ? forced : seen);
   int top = 0;
-  for (int j = lane; j < scored + lane; j += 512) {
+  for (int j = lane; MODE != kRaw && j < scored + lane; j += 512) {
     int v[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) v[u] = ((const int*)a.norm)[(long long)plane * a.blocks + min(j + 64 * u, scored - 1)];
 #pragma unroll
     for (int u = 0; u < 8; ++u) top = max(top, v[u] & 0x7fffffff);
   }
-  const float kn = scored ? __builtin_bit_cast(float, wave_max_i32(top)) : 1.f;
+  float qn = 0.f;
   {
     // Up to 64 channels of a head at a time, in whole lines: a lane sums four channels of every STEP-th row over the heads,
     // and the sums change their layout in LDS.
@@ -541,7 +542,6 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
     float* sums = stage[wave];
     const int sub = lane % kLanes, first = lane / kLanes;
     const float* p = a.q + (long long)b * a.tq * a.ldq + (long long)g * a.group * a.qs;
-    float qn = 0.f;
 #pragma unroll
     for (int k0 = 0; k0 < KS; k0 += KB) {
       const int c = 16 * k0 + 4 * sub;
@@ -586,9 +586,6 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
       __builtin_amdgcn_wave_barrier();
     }
     qn += __shfl_xor(qn, 32);
-    const bool fine = qn >= 0x1p-80f && qn <= 0x1p80f && kn >= 0x1p-80f && kn <= 0x1p80f;
-    exact = !fine;
-    slack = 7.f / 65536 * (__builtin_sqrtf(qn) * __builtin_sqrtf(kn));
   }
   const u32x4* parts = a.parts + (long long)plane * a.tiles * KS * 2 * 64 + lane;
 
@@ -596,7 +593,16 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
   // have no room beside an infinity, it is left out).
   const unsigned keep = ~0u << a.tag_bits;
   u32x4 m[KS][2];
+  const float* means = a.m + (long long)b * a.blocks * a.ldm + g * a.kd;
   auto load = [&](int n) __attribute__((always_inline)) {
+    if (MODE == kRaw) {
+      const float* from = means + min(32 * n + r32, a.blocks - 1) * a.ldm;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) m[ks][u] = *(const u32x4*)(from + min(16 * ks + 8 * half + 4 * u, a.kd - 4));
+      return;
+    }
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -606,14 +612,32 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
     f32x16 sc;
 #pragma unroll
     for (int r = 0; r < 16; ++r) sc[r] = 0.f;
+    float norm = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const bf16x8 m0 = __builtin_bit_cast(bf16x8, m[ks][0]), m1 = __builtin_bit_cast(bf16x8, m[ks][1]);
-      sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m1, q[ks][0], sc, 0, 0, 0);
-      sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m0, q[ks][1], sc, 0, 0, 0);
-      sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m0, q[ks][0], sc, 0, 0, 0);
+      bf16x8 p[2] = {__builtin_bit_cast(bf16x8, m[ks][0]), __builtin_bit_cast(bf16x8, m[ks][1])};
+      if (MODE == kRaw) {
+        float f[8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const f32x4 v = __builtin_bit_cast(f32x4, m[ks][u]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f[4 * u + e] = 16 * ks + 8 * half + 4 * u < a.kd ? v[e] : 0.f;
+            norm = __builtin_fmaf(f[4 * u + e], f[4 * u + e], norm);
+          }
+        }
+        halves8(f, p);
+      }
+      sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[1], q[ks][0], sc, 0, 0, 0);
+      sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[0], q[ks][1], sc, 0, 0, 0);
+      sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[0], q[ks][0], sc, 0, 0, 0);
     }
     load(min(n + 1, last - 1));
+    if (MODE == kRaw) {
+      norm += __shfl_xor(norm, 32);
+      if (32 * n + r32 < scored) top = max(top, __builtin_bit_cast(int, norm) & 0x7fffffff);
+    }
     if (TAGS)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -657,6 +681,10 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
   for (int n = 0; n < SMAX; ++n) nth = fminf(nth, fmaxf(list[n], other[SMAX - 1 - n]));
 #pragma unroll
   for (int n = 0; n <= SMAX; ++n) after = fminf(after, fmaxf(list[n], other[SMAX - n]));
+  const float kn = scored ? __builtin_bit_cast(float, wave_max_i32(top)) : 1.f;
+  // Whether all blocks of this lane's query are scored in 64 bits.
+  bool exact = !(qn >= 0x1p-80f && qn <= 0x1p80f && kn >= 0x1p-80f && kn <= 0x1p80f);
+  const float slack = 7.f / 65536 * (__builtin_sqrtf(qn) * __builtin_sqrtf(kn));  // 2 e
   // Scores from here up are candidates.
   const float from = __builtin_fabsf(nth) == INFINITY ? nth : nth - (TAGS ? slack + a.tag_error * __builtin_fabsf(nth) : slack);
   const float sure = nth + (nth - from);  // scores above are chosen, whatever their errors (NaN: there is no doubt)
@@ -888,6 +916,10 @@ constexpr int kManyRows = 2048, kFewBlocks = 64;
 // Numbers of up to 11 bits (128 tiles, 4,096 blocks) in the scores of lists of up to 16: 8 / 16 of 400 blocks of 32 channels 112 /
 // 150 us, with a second pass 149 / 190; of 128 channels 111 and 180.  More blocks would cost the scores too many bits.
 constexpr int kTagBits = 11;
+// Means split by every wave for itself, up to so many tiles x steps of all waves (beyond, the waves' 40 operations each take
+// longer than the launch that would do it once): a 20x20 map 7.0 us against 9.9, a 48x48 one of four images and 4 heads 11.3
+// against 13.8, 160x160 of 32 channels 30.4 against 30.7 (at 41,600), eight 88x88 of 64 53 against 47 (at 125,000).
+constexpr long long kRawSteps = 1 << 15;
 
 int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q, const sy_tensor* m,
                     const int32_t* starts, const int32_t* lengths, int32_t* blocks) {
@@ -950,10 +982,15 @@ int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q,
   const long long groups = (a.tq + 127) / 128;
   SY_CHECK((long long)planes * groups * 256 < (1LL << 32) && (long long)planes * a.chunks * 256 < (1LL << 32),
            SY_EUNSUPPORTED, "block select grid too large");
-  SY_TRY(ensure_scratch(ctx, parts + sizeof(float) * planes * (size_t)a.blocks));
-  a.parts = (u32x4*)ctx->scratch;
-  a.norm = (float*)(ctx->scratch + parts);
-  {
+  int bits = 4;
+  while (1LL << (bits - 4) < a.tiles) ++bits;
+  a.tag_bits = bits;
+  a.tag_error = 2.125f * std::ldexp(1.f, bits - 23);
+  const bool raw = s.selected <= 16 && bits <= kTagBits && 4LL * planes * groups * a.tiles * steps <= kRawSteps;
+  if (!raw) {
+    SY_TRY(ensure_scratch(ctx, parts + sizeof(float) * planes * (size_t)a.blocks));
+    a.parts = (u32x4*)ctx->scratch;
+    a.norm = (float*)(ctx->scratch + parts);
     ProfScope prof(ctx, "block_parts", 0, 8.0 * planes * (double)a.blocks * s.kd);
     const dim3 g((unsigned)(planes * a.chunks));
     if (steps == 2)
@@ -967,25 +1004,26 @@ int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q,
   ProfScope prof(ctx, "block_select", flops, bytes);
   const dim3 g((unsigned)(planes * groups));
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, dim3(256), 0, ctx->stream, a); };
-  int bits = 4;
-  while (16LL << (bits - 4) < 16LL * a.tiles) ++bits;
-  a.tag_bits = bits;
-  a.tag_error = 2.125f * std::ldexp(1.f, bits - 23);
-  auto pick = [&](auto tags8, auto tags16, auto twice8, auto twice16, auto twice32, auto twice64) {
-    if (bits <= kTagBits && s.selected <= 16)
+  auto pick = [&](auto raw8, auto raw16, auto tags8, auto tags16, auto twice8, auto twice16, auto twice32, auto twice64) {
+    if (raw)
+      launch(s.selected <= 8 ? raw8 : raw16);
+    else if (bits <= kTagBits && s.selected <= 16)
       launch(s.selected <= 8 ? tags8 : tags16);
     else
       launch(s.selected <= 8 ? twice8 : s.selected <= 16 ? twice16 : s.selected <= 32 ? twice32 : twice64);
   };
   if (steps == 2)
-    pick(select_tile_kernel<2, 8, true>, select_tile_kernel<2, 16, true>, select_tile_kernel<2, 8, false>,
-         select_tile_kernel<2, 16, false>, select_tile_kernel<2, 32, false>, select_tile_kernel<2, 64, false>);
+    pick(select_tile_kernel<2, 8, kRaw>, select_tile_kernel<2, 16, kRaw>, select_tile_kernel<2, 8, kTags>,
+         select_tile_kernel<2, 16, kTags>, select_tile_kernel<2, 8, kTwice>, select_tile_kernel<2, 16, kTwice>,
+         select_tile_kernel<2, 32, kTwice>, select_tile_kernel<2, 64, kTwice>);
   else if (steps == 4)
-    pick(select_tile_kernel<4, 8, true>, select_tile_kernel<4, 16, true>, select_tile_kernel<4, 8, false>,
-         select_tile_kernel<4, 16, false>, select_tile_kernel<4, 32, false>, select_tile_kernel<4, 64, false>);
+    pick(select_tile_kernel<4, 8, kRaw>, select_tile_kernel<4, 16, kRaw>, select_tile_kernel<4, 8, kTags>,
+         select_tile_kernel<4, 16, kTags>, select_tile_kernel<4, 8, kTwice>, select_tile_kernel<4, 16, kTwice>,
+         select_tile_kernel<4, 32, kTwice>, select_tile_kernel<4, 64, kTwice>);
   else
-    pick(select_tile_kernel<8, 8, true>, select_tile_kernel<8, 16, true>, select_tile_kernel<8, 8, false>,
-         select_tile_kernel<8, 16, false>, select_tile_kernel<8, 32, false>, select_tile_kernel<8, 64, false>);
+    pick(select_tile_kernel<8, 8, kRaw>, select_tile_kernel<8, 16, kRaw>, select_tile_kernel<8, 8, kTags>,
+         select_tile_kernel<8, 16, kTags>, select_tile_kernel<8, 8, kTwice>, select_tile_kernel<8, 16, kTwice>,
+         select_tile_kernel<8, 32, kTwice>, select_tile_kernel<8, 64, kTwice>);
   return check_launch("block_select");
 }
 
