@@ -9,9 +9,10 @@
 // taken as they stand.
 //
 // Measured, us (sort + tiles + join): two 160x160 maps, 4 heads of 32 / 64 channels, 8 of 400 blocks of 64 keys
-// 25 + 113 + 89; 8,192 causal tokens, 16 heads and 4 key heads of 128, 16 of 128 blocks 20 + 356 + 195; plain float32,
-// a wave to a query, 14,900 and 61,700.  The results are written and read once, 0.43 and 1.0 GB, and bound both:
-// without matrix instructions the first took 284 where it took 287 with them.
+// 24 + 113 + 89; 8,192 causal tokens, 16 heads and 4 key heads of 128, 16 of 128 blocks 17 + 340 + 194; plain float32,
+// a wave to a query, 14,900 and 61,700.  The results are written and read once, 0.43 and 1.0 GB: the join is bound by them,
+// and the tiles of 64 channels (3.8 TB/s); those of 128 by two waves per SIMD that share it between vector work (44% of the
+// time) and matrix products (30%).
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -27,6 +28,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr int kFlat = 8;
 constexpr int kKeys = 64;    // keys of a tile; longer blocks are so many tiles ("parts" of the block)
 constexpr int kTileRows = 512;  // rows of a tile at most
+constexpr int kScan = 2048;  // pairs of an image and key head that a tile's workgroup goes through itself
 constexpr int kMaxBlocks = 12288;  // of a sorted list: counters in LDS
 
 // What a tile leaves for a row beside its weighted values: the maximum (as a power of two), the sum of weights, and the
@@ -319,15 +321,44 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
   const int t = item - seg * a.tile_cap;
   if (seg >= a.now) return;
   seg += a.first;
-  const int4 rec = a.tiles[(long long)seg * a.tile_cap + t];  // under way with the count
-  if (t >= a.tile_count[seg]) return;
+  const int plane = seg / a.segs, b = plane / s.kv, g = plane - b * s.kv, i0 = (seg - plane * a.segs) * a.span;
+  const bool scan = !a.list;
+  int4 rec;  // block, part of it and number of the tile, first entry of its list, length of the list
+  unsigned long long named[kScan / 256];
+  int before = 0;
+  if (scan) {
+    // A small call without lists: those of all queries are gone through here for the ones that name the block.
+    const int j = t / a.parts % s.blocks;
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < kScan / 256; ++u) {
+      const int pair = wave * (kScan / 4) + 64 * u + lane, d = min(pair, s.tq * s.selected - 1) / s.selected;
+      const int is = list_of(a, b, d, g)[min(pair, s.tq * s.selected - 1) - d * s.selected];
+      named[u] = __ballot(pair < s.tq * s.selected && is == j && block_seen(a, j, visible(a, b, d)));
+      n += __builtin_popcountll(named[u]);
+    }
+    if (lane == 0) place[0][wave] = n;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int m = place[0][w];
+      before += w < wave ? m : 0;
+      all += m;
+    }
+    __syncthreads();
+    rec = make_int4(j, t % a.parts | t / (a.parts * s.blocks) << 8, 0, all);
+    if (all == 0) return;
+  } else {
+    rec = a.tiles[(long long)seg * a.tile_cap + t];  // under way with the count
+    if (t >= a.tile_count[seg]) return;
+  }
   // Its share of the block's rows: as many as the other tiles', in 32s.
   const int all = rec.w * s.group, share = tile_share(a, all);
   const int j = rec.x, part = rec.y & 255, row0 = (rec.y >> 8) * share;
   const int rows = min(all - row0, share);
   if (rows <= 0) return;
-  const int plane = seg / a.segs, b = plane / s.kv, g = plane - b * s.kv, i0 = (seg - plane * a.segs) * a.span;
-  const int* list = a.list + (long long)seg * a.span * s.selected + rec.z;
+  const int* list = scan ? nullptr : a.list + (long long)seg * a.span * s.selected + rec.z;
   const int y0 = j / s.bx * s.bh, x0 = j % s.bx * s.bw;
   const int cols = min(s.bw, s.kw - x0), size = min(s.bh, s.kh - y0) * cols;
   const int origin = y0 * s.kw + x0;
@@ -352,7 +383,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
       const long long end = min((long long)length, max(start + i0 + d + 1, 0LL));
       limit = min(keys, (int)end - origin - part * kKeys);
     }
-    const unsigned slot = (unsigned)((seg - a.first) * a.span * s.selected + rec.z + e0 + e) * a.parts + part;
+    const unsigned slot = (unsigned)((seg - a.first) * a.span * s.selected + (scan ? pair : rec.z + e0 + e)) * a.parts + part;
     to = r + r32 < rows ? slot * s.group + h : a.trash;
     const float* p = qb + (long long)d * a.ldq + h * s.qs;
 #pragma unroll
@@ -370,7 +401,14 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
   const int entries = (h0 + rows + s.group - 1) / s.group;
   int first_pair[2];
 #pragma unroll
-  for (int n = 0; n < 2; ++n) first_pair[n] = list[e0 + min(tid + 256 * n, entries - 1)];
+  for (int n = 0; n < 2; ++n) first_pair[n] = scan ? 0 : list[e0 + min(tid + 256 * n, entries - 1)];
+  if (scan)
+#pragma unroll
+    for (int u = 0; u < kScan / 256; ++u) {
+      const int at = before + __builtin_popcountll(named[u] & ((1ull << lane) - 1)) - e0;
+      if ((named[u] >> lane & 1) && at >= 0 && at < entries) pair_at[at] = wave * (kScan / 4) + 64 * u + lane;
+      before += __builtin_popcountll(named[u]);
+    }
 
   int r = wave * 32, k_one, v_most;
   bool k_flat, v_flat;
@@ -399,7 +437,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
     }
 #pragma unroll
     for (int n = 0; n < 2; ++n)
-      if (tid + 256 * n < kTileRows) pair_at[tid + 256 * n] = first_pair[n];
+      if (!scan && tid + 256 * n < kTileRows) pair_at[tid + 256 * n] = first_pair[n];
     if (tid < kKeys) v_at[tid] = key_at(tid, a.ldv);
     __syncthreads();
     load_q(r);
@@ -878,6 +916,11 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
   }
 }
 
+// Tiles find their rows themselves, without the sort, where there are up to so many (every block of each image and key head
+// may be named by all pairs) and lists of up to kScan: attention on one 20x20 map, 2 / 4 heads of 32 / 64 channels, 4 of 25
+// blocks 15.5 / 15.3 us against 19 / 19.5; with 1,300 tiles of 64 / 64 channels 26 against 23.
+constexpr int kScanTiles = 512;
+
 // Bytes of results that one launch leaves and the next one joins.  Fewer would stay in the 256 MiB cache in front of
 // memory, but cost more in half-filled launches: 8,192 causal tokens of 16 heads (1.0 GB) 950 us in pieces of 256 MB, 695 of
 // 400 MB, 687 in one.
@@ -948,7 +991,13 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   a.chunk = std::max(std::max(1, 2048 / s.selected), (a.span + 31) / 32);
   a.chunks = (a.span + a.chunk - 1) / a.chunk;
   const long long pairs = (long long)a.span * s.selected;
-  const long long tile_cap = a.parts * (std::min<long long>(s.blocks, pairs) + pairs * s.group / a.rows + 1);
+  auto scan_tiles = [&](long long rows) {
+    return planes * (long long)a.parts * s.blocks * ((pairs * s.group + rows - 1) / rows);
+  };
+  const bool scan = sorted && a.segs == 1 && pairs <= kScan && scan_tiles(kTileRows) <= kScanTiles;
+  while (scan && scan_tiles(a.rows) > kScanTiles) a.rows *= 2;
+  const long long tile_cap =
+      scan ? scan_tiles(a.rows) / planes : a.parts * (std::min<long long>(s.blocks, pairs) + pairs * s.group / a.rows + 1);
   const long long result_rows = together * pairs * a.parts * s.group;
   SY_CHECK((result_rows + 1) * s.hd < (1LL << 30) - 128 && tile_cap * together < (1LL << 24), SY_EUNSUPPORTED,
            "block attention over %d heads to a key head", s.group);
@@ -967,22 +1016,22 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   };
   const size_t part_at = take(sizeof(float) * ((result_rows + 1) * s.hd + 128)),
                stat_at = take(sizeof(Stat) * (result_rows + 1));
-  const size_t count_at = sorted ? take(sizeof(int) * segments * a.chunks * s.blocks) : 0;
-  const size_t list_at = sorted ? take(sizeof(int) * segments * pairs) : 0;
-  const size_t pos_at = sorted ? take(sizeof(int) * segments * pairs) : 0;
-  const size_t tile_at = sorted ? take(sizeof(int4) * segments * tile_cap) : 0;
-  const size_t number_at = sorted ? take(sizeof(int) * segments) : 0;
+  const size_t count_at = sorted && !scan ? take(sizeof(int) * segments * a.chunks * s.blocks) : 0;
+  const size_t list_at = sorted && !scan ? take(sizeof(int) * segments * pairs) : 0;
+  const size_t pos_at = sorted && !scan ? take(sizeof(int) * segments * pairs) : 0;
+  const size_t tile_at = sorted && !scan ? take(sizeof(int4) * segments * tile_cap) : 0;
+  const size_t number_at = sorted && !scan ? take(sizeof(int) * segments) : 0;
   DeviceScope device(ctx);
   SY_TRY(ensure_scratch(ctx, at));
   a.part = (float*)(ctx->scratch + part_at);
   a.stat = (Stat*)(ctx->scratch + stat_at);
   a.counts = (int*)(ctx->scratch + count_at);
-  a.list = (int*)(ctx->scratch + list_at);
-  a.pos = sorted ? (int*)(ctx->scratch + pos_at) : nullptr;
+  a.list = sorted && !scan ? (int*)(ctx->scratch + list_at) : nullptr;
+  a.pos = sorted && !scan ? (int*)(ctx->scratch + pos_at) : nullptr;
   a.tiles = (int4*)(ctx->scratch + tile_at);
   a.tile_count = (int*)(ctx->scratch + number_at);
   const double keys = std::min((double)s.selected * s.bh * s.bw, (double)s.tk);
-  if (sorted) {
+  if (sorted && !scan) {
     ProfScope prof(ctx, "block_sort", 0, 8.0 * s.n * (double)s.tq * s.kv * s.selected);
     const size_t lds = sizeof(int) * s.blocks;
     const dim3 grid((unsigned)(segments * a.chunks)), threads(kSortThreads);
@@ -996,7 +1045,7 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
     a.first = (int)first;
     a.now = now;
     {
-      ProfScope prof(ctx, "block_attention", share * 2.0 * s.n * s.tq * s.heads * keys * (s.kd + s.hd),
+      ProfScope prof(ctx, sorted ? "block_attention" : "block_few", share * 2.0 * s.n * s.tq * s.heads * keys * (s.kd + s.hd),
                      share * 4.0 * s.n * ((double)s.tq * s.heads * (s.kd + s.hd) + (double)s.tk * s.kv * (s.kd + s.hd)));
       if (sorted) {
         const unsigned grid = (unsigned)((now * tile_cap + 7) / 8 * 8);
