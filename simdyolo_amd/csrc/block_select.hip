@@ -496,7 +496,7 @@ __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
 //
 // Bound by vector work, which keeps the SIMDs busy nine tenths of the time: 3,600 operations per wave (32 queries, 400 blocks
 // of 32 channels, 8 wanted), of them 1,900 medians; the matrix cores work a sixth of it.  Four maps of 25,600 queries, 4
-// heads: 105 us; with a second pass over the scores 140; in 64 bits throughout 9,900; 64 queries to a wave, which halves the
+// heads: 106 us with the means' parts; with a second pass over the scores 140; in 64 bits throughout 9,900; 64 queries to a wave, which halves the
 // reads of the means, 154.  Two causal rows of 16,001 tokens, 16 / 4 heads of 128 channels, 16 of 251 blocks: 91 us, of them
 // 50 the queries' way from memory; with all candidates of doubtful queries scored again 117, their heads read in 32-byte
 // pieces besides 126.
