@@ -264,10 +264,10 @@ def test_uneven_channels(hip, tq):
     np.testing.assert_array_equal(got, R.select(cfg, few, m))
 
 
-@pytest.mark.parametrize("kd,selected", [(32, 8), (64, 20), (128, 64)])
-def test_long_causal_rows(hip, kd, selected):
+@pytest.mark.parametrize("kv,kd,selected", [(2, 32, 8), (2, 64, 20), (2, 128, 64), (2, 64, 1), (20, 32, 1), (20, 32, 9), (20, 64, 16)])
+def test_long_causal_rows(hip, kv, kd, selected):
     """More blocks than a wave's tile, a few of them seen by the first queries and all by the last."""
-    cfg = R.shape(6, 2, 1, 4, selected, causal=1)
+    cfg = R.shape(3 * kv, kv, 1, 4, selected, causal=1)
     tq, w, starts, lengths = 1500, 1600, (0, 100), (1490, 1600)
     q, k = tensors(2, w, tq, cfg, kd, 3)
     m = R.means(cfg, k, 1, w, lengths).astype(np.float32)
