@@ -37,6 +37,7 @@ struct Stat {
   float top, sum;
   int scale;
 };
+constexpr int kNoPower = -4096;  // below every power of a product
 
 struct BlockArgs {
   const float *q, *k, *v;
@@ -584,32 +585,28 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
       sum += w[x];
     }
     sum += __shfl_xor(sum, 32);
-    // Where values differ in size: weights times their powers, from the largest of those that the row sees, and under a
-    // power of the row.  (One power for all: weights are at most 1.)
+    // Where values differ in size: weights times their powers, under the power of the largest such product (below 1 then; a
+    // key without weight has no say in it, whatever its values).  One power for all: weights are at most 1.
     int most = v_most, w_field = 127 + 14;
     if (!v_flat) {
-      if (partly) {
-        most = -127;
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const i32x4 power = *(const i32x4*)&v_power[8 * n + 4 * half];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (8 * n + 4 * half + e < seen) most = max(most, power[e]);
-        }
-        most = max(most, __shfl_xor(most, 32));
-      }
-      float tm = 0.f;
+      w_field = 127 + 15;
+      most = 2 * kNoPower;
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
         const i32x4 power = *(const i32x4*)&v_power[8 * n + 4 * half];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          w[4 * n + e] = __builtin_ldexpf(w[4 * n + e], min(power[e] - most, 0));
-          tm = fmaxf(tm, w[4 * n + e]);
+          const int bits = __builtin_bit_cast(int, w[4 * n + e]);  // not negative; its exponent, or far below for 0
+          most = max(most, power[e] + (bits >> 23) + ((bits - 1) >> 31 & kNoPower));
         }
       }
-      w_field = pair_field(fmaxf(tm, __shfl_xor(tm, 32)));
+      most = max(most, __shfl_xor(most, 32)) - 126;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const i32x4 power = *(const i32x4*)&v_power[8 * n + 4 * half];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[4 * n + e] = __builtin_ldexpf(w[4 * n + e], power[e] - most);
+      }
     }
     const float w_scale = exp_float(w_field);
     a.stat[half ? a.trash : mine] = Stat{mx, sum, most + 127 - w_field};
@@ -847,7 +844,7 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
     const int n = n0 + sub;
     const bool on = n < slots && block_seen(a, list[min(n, slots - 1) / a.parts], end);
     any |= on;
-    Stat st = {-INFINITY, 0.f, INT_MIN};
+    Stat st = {-INFINITY, 0.f, 0};
     int at = 0;
     if (on) {
       const int p = n / a.parts;
@@ -856,23 +853,26 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
       st = a.stat[at];
     }
     float mx = st.top;
-    int most = st.scale;
 #pragma unroll
-    for (int off = 1; off < L; off <<= 1) {
-      mx = fmaxf(mx, __shfl_xor(mx, off));
-      most = max(most, __shfl_xor(most, off));
-    }
+    for (int off = 1; off < L; off <<= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
     mx = fmaxf(mx, top);
-    most = max(most, power);
-    // Negative: there is nothing to read.  A slot without weight is read all the same: a NaN in it is the row's.
-    const float f = !on ? -1.f : st.top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.top - mx);
-    const float old = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - mx);
+    // A slot's weight is 2^(its maximum - mx) as mantissa and exponent, which joins the power that its values want: the largest
+    // of these powers takes the sum, so a slot without weight leaves the others' bits alone, whatever its values.
+    const bool weighs = st.top != -INFINITY, had = top != -INFINITY;
+    const float x = weighs ? st.top - mx : 0.f, low = fmaxf(floorf(x), kNoPower), f = weighs ? __builtin_amdgcn_exp2f(x) : 0.f;
+    const float ox = had ? top - mx : 0.f, olow = fmaxf(floorf(ox), kNoPower);
+    sum = __builtin_fmaf(sum, had ? __builtin_amdgcn_exp2f(ox) : 0.f, st.sum * f);
     top = mx;
-    sum = __builtin_fmaf(sum, old, st.sum * f);
+    const int at_power = st.scale + (int)low, old_power = power + (int)olow;
+    int most = max(weighs ? at_power : INT_MIN, had ? old_power : INT_MIN);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = power == INT_MIN ? 0.f : __builtin_ldexpf(y[e] * old, power - most);
+    for (int off = 1; off < L; off <<= 1) most = max(most, __shfl_xor(most, off));
+    const float old = had ? __builtin_ldexpf(__builtin_amdgcn_exp2f(ox - floorf(ox)), old_power - most) : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] *= old;
     power = most;
-    const float fv = on ? __builtin_ldexpf(f, st.scale - most) : -1.f;
+    // Negative: there is nothing to read.  A slot without weight is read all the same: a NaN in it is the row's.
+    const float fv = !on ? -1.f : weighs ? __builtin_ldexpf(__builtin_amdgcn_exp2f(x - floorf(x)), at_power - most) : 0.f;
     const int count = min(L, slots - n0);
     for (int u0 = 0; u0 < count; u0 += 8) {
       f32x4 v[8];
