@@ -26,6 +26,7 @@ namespace sy {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kFlat = 8;
+constexpr float kWide = 0x1p-8f, kFine = 0x1p-14f;  // largest factor of a score, least value of a channel (their powers apart)
 constexpr int kKeys = 64;    // keys of a tile; longer blocks are so many tiles ("parts" of the block)
 constexpr int kTileRows = 512;  // rows of a tile at most
 constexpr int kScan = 2048;  // pairs of an image and key head that a tile's workgroup goes through itself
@@ -240,8 +241,8 @@ __global__ __launch_bounds__(kSortThreads) void block_scatter_kernel(const Block
 // ---------------------------------------------------------------------- tiles
 
 // Exponent field of the power of two that takes a largest magnitude m into [2^14, 2^15): a row in that range splits
-// into f16 pairs h + l within 2^-22 of each element, or 2^-39 of m where that is more.  Rows below 2^-113 keep
-// the largest scale there is, and with it every bit of a float.
+// into pairs of f16, h + l / 2048, within 2^-22 of each element, or 2^-36 (2^-50 of m) where that is more.  Rows below
+// 2^-113 keep the largest scale there is, and with it every bit of a float.
 __device__ __forceinline__ int pair_field(float m) { return min(268 - (int)(__builtin_bit_cast(unsigned, m) >> 23), 254); }
 
 __device__ __forceinline__ void pairs8(const float (&x)[8], float s, f16x8& h, f16x8& l) {
@@ -252,7 +253,7 @@ __device__ __forceinline__ void pairs8(const float (&x)[8], float s, f16x8& h, f
     const f16x2 hi = __builtin_convertvector((f32x2v{a * s, b * s}), f16x2);
     const f32x2v r = {__builtin_fmaf(a, s, -(float)hi[0]), __builtin_fmaf(b, s, -(float)hi[1])};
     hw[i] = __builtin_bit_cast(unsigned, hi);
-    lw[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(r, f16x2));
+    lw[i] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2v{r[0] * 2048.f, r[1] * 2048.f}), f16x2));
   }
   h = __builtin_bit_cast(f16x8, hw);
   l = __builtin_bit_cast(f16x8, lw);
@@ -283,13 +284,18 @@ __device__ __forceinline__ unsigned item_of(unsigned block, unsigned grid) { ret
 
 // One tile: up to 64 keys of a block and a.rows rows of its list, 32 at a time for each of four waves.
 //
-// Products of float32 on the f16 matrix cores: an operand is a pair h + l of f16 values under a power of two of its own
-// row (a query, a key, the values of a key, the weights of a query), and h h + h l + l h is taken: 3 x 2^-22 of
-// each product at most, whatever the other rows hold.  The powers of queries and keys come back onto the scores;
-// those of the values meet the weights before these are split, so that a key's weight counts as much as what it
-// brings; the last one, of the weights' row, is left to the join.  Where the largest elements of all keys (of all
-// values) of a tile are within 2^kFlat of each other they share one power, which keeps 2^(kFlat - 39) of a
-// row's largest element and needs no power per score (per weight).
+// Products of float32 on the f16 matrix cores: an operand is a pair h + l / 2048 of f16 values under a power of two of
+// its own row (a query, a key, the values of a key, the weights of a query), and h h + (h l + l h) / 2048 is taken:
+// 3 x 2^-22 of each product at most, whatever the other rows hold, as long as elements are not below 2^-29 of their
+// row's largest.  The powers of queries and keys come back onto the scores; those of the values meet the weights
+// before these are split, so that a key's weight counts as much as what it brings; the last one, of the weights' row, is
+// left to the join.  Where the largest elements of all keys (of all values) of a tile are within 2^kFlat of each other
+// they share one power, which needs none per score (per weight); 2^-29 becomes 2^-21 of a smaller row's then.
+//
+// Elements below that keep an absolute precision, 2^-36 under their power: for a score 1.5 x 2^-20 under both powers from
+// each channel and so, as long as its factor is at most kWide, less than 2^-20 of its exponent.  Rows past that
+// (|q||k| scale of 2^20 and more), and those of a tile whose values have a channel so far below the others in eight
+// keys at once, leave NaN for their sum: the join computes them in plain float32.
 //
 // Keys and values stand in LDS as pairs, in the order in which the matrix instruction's lanes take them, so that a
 // fragment is one 16-byte read without bank conflicts.  Once they stand there the waves run on their own: no
@@ -312,7 +318,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
   __shared__ float k_top[kKeys], v_top[kKeys];     // largest magnitude of a key, of its values
   __shared__ __align__(16) int k_power[kKeys], v_power[kKeys];
   __shared__ unsigned place[4][32];
-  __shared__ int pair_at[kTileRows];
+  __shared__ int pair_at[kTileRows], uneven;
   const BlockShape& s = a.s;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, r32 = lane & 31;
@@ -411,7 +417,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
       before += __builtin_popcountll(named[u]);
     }
 
-  int r = wave * 32, k_one, v_most;
+  int r = wave * 32, k_most, v_most;
   bool k_flat, v_flat;
   {
     const float* kb = a.k + ((long long)b * s.tk + origin) * a.ldk + (long long)g * s.ks;
@@ -440,6 +446,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
     for (int n = 0; n < 2; ++n)
       if (!scan && tid + 256 * n < kTileRows) pair_at[tid + 256 * n] = first_pair[n];
     if (tid < kKeys) v_at[tid] = key_at(tid, a.ldv);
+    if (tid == 0) uneven = 0;
     __syncthreads();
     load_q(r);
 #pragma unroll
@@ -465,11 +472,11 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
     __syncthreads();
     // One power for the whole tile where its rows are of one size.
     const float kt = k_top[lane], vt = v_top[lane];
-    const int kp = 127 - pair_field(kt), vp = 127 - pair_field(vt), k_most = wave_max_i32(kp);
+    const int kp = 127 - pair_field(kt), vp = 127 - pair_field(vt);
+    k_most = wave_max_i32(kp);
     v_most = wave_max_i32(vp);
     k_flat = !__any(kt != 0.f && kp < k_most - kFlat);
     v_flat = !__any(vt != 0.f && vp < v_most - kFlat);
-    k_one = k_most;
     if (wave == 0) {
       k_power[lane] = kp;
       v_power[lane] = vp;
@@ -499,6 +506,8 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (first + 8 * (e >> 2) + (e & 3) >= keys) vr[n][e] = 0.f;
+      const float top = max8(vr[n]);
+      if (top != 0.f && top * scale < kFine) uneven = 1;
       f16x8 p[2];
       pairs8(vr[n], scale, p[0], p[1]);
 #pragma unroll
@@ -516,6 +525,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
     return __builtin_bit_cast(f16x8, frag[KF * 64 + ((st * DT + d) * 2 + m) * 64 + lane]);
   };
 
+  const bool plain = uneven;
   // (Results pass the caches by, written here and read by the join, and so do the join's outputs: 287 -> 234 us on two
   // 160x160 maps, 659 -> 585 on 8,192 causal tokens, whose queries and keys they would push out.)
   // The queries are here before the loop: in it they are waited for with the stores behind them still under way.
@@ -552,10 +562,12 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
     load_q(min(r + 128, rows - 1));  // the last turn: something, to keep the count of loads
     // Key 4 n + e of those that a lane holds is 8 n + 4 half + e.
     float w[32], c = cs;
+    int k_top_power = k_most;
+    const bool partly = __any(seen < keys);
 #pragma unroll
-    for (int x = 0; x < 32; ++x) w[x] = sc[x >> 4][x & 15] + rest[x >> 4][x & 15];
+    for (int x = 0; x < 32; ++x) w[x] = __builtin_fmaf(rest[x >> 4][x & 15], 1.f / 2048, sc[x >> 4][x & 15]);
     if (k_flat) {
-      c = fmaxf(__builtin_ldexpf(cs, k_one + q_power), FLT_MIN);  // not 0, which would make hidden keys' scores NaN
+      c = fmaxf(__builtin_ldexpf(cs, k_most + q_power), FLT_MIN);  // not 0, which would make hidden keys' scores NaN
     } else {
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
@@ -563,9 +575,14 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[4 * n + e] = __builtin_ldexpf(w[4 * n + e], power[e] + q_power);
       }
+      if (partly) {  // hidden keys have no say
+        k_top_power = kNoPower;
+        for (int t = half; t < seen; t += 2) k_top_power = max(k_top_power, k_power[t]);
+        k_top_power = max(k_top_power, __shfl_xor(k_top_power, 32));
+      }
     }
+    const bool wide = plain || !(__builtin_ldexpf(cs, k_top_power + q_power) <= kWide);
     // Keys that do not exist, and in a causal tile those that some rows do not see.
-    const bool partly = __any(seen < keys);
     if (keys < kKeys && !partly)
 #pragma unroll
       for (int x = 0; x < 32; ++x)
@@ -609,7 +626,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
       }
     }
     const float w_scale = exp_float(w_field);
-    a.stat[half ? a.trash : mine] = Stat{mx, sum, most + 127 - w_field};
+    a.stat[half ? a.trash : mine] = Stat{mx, wide ? NAN : sum, most + 127 - w_field};
     f16x8 wp[4][2];
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
@@ -637,6 +654,8 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
         acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(wp[st][1], lead[st], acc, 0, 0, 0);
         acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(wp[st][0], v1, acc, 0, 0, 0);
       }
+#pragma unroll
+      for (int x = 0; x < 16; ++x) acc[x] *= 1.f / 2048;
 #pragma unroll
       for (int st = 0; st < 4; ++st) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(wp[st][0], lead[st], acc, 0, 0, 0);
       char* base = (char*)(a.part + 32 * d);
@@ -820,7 +839,7 @@ __device__ __forceinline__ void block_row(const BlockArgs& a, int b, int i, int 
 // Joins the slots of each row: L lanes of 4 channels to a row, at 5.4 TB/s.  The lanes first take a slot each (which block it
 // names, its statistics), then all of them go through the slots' values, whose loads depend on nothing.  A row
 // that comes out infinite or NaN (operands that are, sums that overflow, hidden keys of a tile that are not
-// finite) is computed again in plain float32.
+// finite, rows too uneven for f16 pairs) is computed again in plain float32.
 template <int L>
 __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long long rows) {
   const BlockShape& s = a.s;

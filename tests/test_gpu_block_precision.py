@@ -47,3 +47,59 @@ def test_far_values_of_little_weight(hip, tq, selected, gap):
     blocks = choice(1, tq, cfg, 1, w, 8, 0.0)
     exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5)
     check(run(hip, cfg, q, k, v, blocks, 1, w, sort=tq == MANY), exp, bound)
+
+
+@pytest.mark.parametrize("tq", [FEW, MANY])
+@pytest.mark.parametrize("far", ["q", "k"])
+@pytest.mark.parametrize("dims", [(32, 64), (64, 32), (128, 128)], ids=str)
+@pytest.mark.parametrize("r", [8, 12, 16, 20, 40])
+def test_uneven_channels_of_queries_and_keys(hip, tq, far, dims, r):
+    """One channel of the queries 2^r above the others and of the keys as far below, another the other way round: their
+    products are of the others' size.  far: the same on one side alone, whose products decide."""
+    (kd, hd), w = dims, 96
+    cfg = R.shape(2, 2, 1, 16, 4)
+    q, k, v = tensors(1, tq, w, cfg, kd, hd, 5)
+    up, down = np.float32(2.0 ** r), np.float32(2.0 ** -r)
+    q[..., 0] *= up
+    k[..., 0] *= down
+    if far == "q":
+        q[..., kd // 2] *= down
+        k[..., kd // 2] *= up
+    else:  # what is small on one side meets what is small on the other: nothing is lost with it
+        k[..., kd // 2] *= down
+    blocks = choice(1, tq, cfg, 1, w, 8, 0.0)
+    exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5)
+    check(run(hip, cfg, q, k, v, blocks, 1, w, sort=tq == MANY), exp, bound)
+
+
+@pytest.mark.parametrize("tq", [FEW, MANY])
+@pytest.mark.parametrize("keys", ["alike", "of many sizes"])
+@pytest.mark.parametrize("r", [8, 16, 20, 24, 28, 32, 60])
+def test_uneven_channels_of_values(hip, tq, keys, r):
+    """Channels of the values 2^r below the others, in every key: as precise as the others."""
+    cfg, kd, hd, w = R.shape(4, 2, 1, 48, 3, causal=1), 32, 64, 200
+    q, k, v = tensors(2, tq, w, cfg, kd, hd, 5)
+    v[..., 3] *= np.float32(2.0 ** -r)
+    v[..., 40:48] *= np.float32(2.0 ** -(r // 2))
+    v[..., 63] = 0
+    if keys == "of many sizes":
+        v *= np.exp2(5.0 * (np.arange(w) % 7)).astype(np.float32)[:, None, None]
+    blocks = choice(2, tq, cfg, 1, w, 8, 0.0)
+    exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5)
+    check(run(hip, cfg, q, k, v, blocks, 1, w, sort=tq == MANY), exp, bound)
+
+
+@pytest.mark.parametrize("tq", [FEW, MANY])
+@pytest.mark.parametrize("size", [2.0 ** 8, 2.0 ** 11, 2.0 ** 14])
+def test_large_scores(hip, tq, size):
+    """Queries and keys whose products come to 2^16 and more, on both sides of where the matrix cores are left, cancelled
+    to ordinary scores by a second channel; garbage behind the last token, far above the keys, that no row sees."""
+    cfg, kd, hd, w = R.shape(2, 1, 1, 32, 3, causal=1), 16, 16, 1000
+    q, k, v = tensors(1, tq, w, cfg, kd, hd, 5)
+    q[..., 0] = q[..., 1] = k[..., 0] = np.float32(size)
+    k[..., 1] = np.float32(-size)
+    blocks = choice(1, tq, cfg, 1, w, 8, 0.0)
+    blocks[..., 0] = 0
+    exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5)
+    k[:, max(tq, 32):] *= np.float32(2.0 ** 60)
+    check(run(hip, cfg, q, k, v, blocks, 1, w, sort=tq == MANY), exp, bound)
