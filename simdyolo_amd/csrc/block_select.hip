@@ -3,6 +3,7 @@
 //
 // The choice is made on scores in 64 bits: a product of floats is exact there and 128 of them sum within
 // 2^-46, so it does not hang on the order of a sum as it would in 32 bits.
+#include <cfloat>
 #include <climits>
 #include <cmath>
 
@@ -187,7 +188,7 @@ int op_block_means(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* k, 
 // kept, so that the `selected`-th, t, is known; no block further than 2 e below t is chosen, whatever the rounding, and
 // every block further than 2 e above it is.  Up to 16 of 4,096 blocks are kept with their numbers; of more, the scores are
 // formed again and compared with t - 2 e.  Where more than `selected` lie there, some queries in a hundred, those within
-// 2 e of t are scored again in 64 bits.
+// 2 e of t are scored again in 64 bits.  Queries of zeros (padding), and all where the means are zeros, need no scores.
 // Few queries: scores in 64 bits, then a ranking.
 
 struct SelectArgs {
@@ -437,6 +438,11 @@ __device__ __forceinline__ void halves8(const float (&x)[8], bf16x8 (&p)[2]) {
   p[1] = __builtin_bit_cast(bf16x8, w[1]);
 }
 
+// A sum of squares, not 0 unless all of what was squared is (bits: or'ed over it).
+__device__ __forceinline__ float norm_of(float squares, unsigned bits) {
+  return (bits & 0x7fffffffu) && squares == 0.f ? FLT_MIN : squares;
+}
+
 constexpr int kPools = 8;      // doubtful queries of a wave whose candidates are kept (second pass)
 constexpr int kPartTiles = 8;  // 32-block tiles of a workgroup below
 
@@ -454,6 +460,7 @@ __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
     if (tile >= a.tiles) break;
     const float* m = a.m + ((long long)b * a.blocks + min(j, a.blocks - 1)) * a.ldm + g * a.kd;
     float norm = 0.f;
+    unsigned bits = 0;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       float f[8];
@@ -466,6 +473,7 @@ __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
           f[4 * u + e] = v[e];
           norm = __builtin_fmaf(v[e], v[e], norm);
         }
+        bits |= magnitude_bits(v);
       }
       bf16x8 p[2];
       halves8(f, p);
@@ -473,6 +481,7 @@ __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
       to[0] = __builtin_bit_cast(u32x4, p[0]);
       to[64] = __builtin_bit_cast(u32x4, p[1]);
     }
+    norm = norm_of(norm, bits);
     norm += __shfl_xor(norm, 32);
     if (half == 0 && j < a.blocks) a.norm[(long long)plane * a.blocks + j] = norm;
   }
@@ -535,6 +544,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
     for (int u = 0; u < 8; ++u) top = max(top, v[u] & 0x7fffffff);
   }
   float qn = 0.f;
+  unsigned q_bits = 0;
   {
     // Up to 64 channels of a head at a time, in whole lines: a lane sums four channels of every STEP-th row over the heads,
     // and the sums change their layout in LDS.
@@ -578,6 +588,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
           const f32x4 v = *(const f32x4*)&sums[r32 * (16 * KB + 4) + 16 * ks + 8 * half + 4 * u];
 #pragma unroll
           for (int e = 0; e < 4; ++e) f[4 * u + e] = v[e];
+          q_bits |= magnitude_bits(v);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) qn = __builtin_fmaf(f[e], f[e], qn);
@@ -585,6 +596,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
       }
       __builtin_amdgcn_wave_barrier();
     }
+    qn = norm_of(qn, q_bits);
     qn += __shfl_xor(qn, 32);
   }
   const u32x4* parts = a.parts + (long long)plane * a.tiles * KS * 2 * 64 + lane;
@@ -613,6 +625,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
 #pragma unroll
     for (int r = 0; r < 16; ++r) sc[r] = 0.f;
     float norm = 0.f;
+    unsigned bits = 0;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       bf16x8 p[2] = {__builtin_bit_cast(bf16x8, m[ks][0]), __builtin_bit_cast(bf16x8, m[ks][1])};
@@ -625,6 +638,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
           for (int e = 0; e < 4; ++e) {
             f[4 * u + e] = 16 * ks + 8 * half + 4 * u < a.kd ? v[e] : 0.f;
             norm = __builtin_fmaf(f[4 * u + e], f[4 * u + e], norm);
+            bits |= __builtin_bit_cast(unsigned, f[4 * u + e]);
           }
         }
         halves8(f, p);
@@ -635,6 +649,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
     }
     load(min(n + 1, last - 1));
     if (MODE == kRaw) {
+      norm = norm_of(norm, bits);
       norm += __shfl_xor(norm, 32);
       if (32 * n + r32 < scored) top = max(top, __builtin_bit_cast(int, norm) & 0x7fffffff);
     }
@@ -682,15 +697,21 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
 #pragma unroll
   for (int n = 0; n <= SMAX; ++n) after = fminf(after, fmaxf(list[n], other[SMAX - n]));
   const float kn = scored ? __builtin_bit_cast(float, wave_max_i32(top)) : 1.f;
+  // A query of zeros (padding), or means of zeros, has scores that are all 0 if the others are finite: the lowest blocks.
+  const bool zero = (qn == 0.f && kn < INFINITY) || (kn == 0.f && qn < INFINITY);
   // Whether all blocks of this lane's query are scored in 64 bits.
-  bool exact = !(qn >= 0x1p-80f && qn <= 0x1p80f && kn >= 0x1p-80f && kn <= 0x1p80f);
+  bool exact = !zero && !(qn >= 0x1p-80f && qn <= 0x1p80f && kn >= 0x1p-80f && kn <= 0x1p80f);
   const float slack = 7.f / 65536 * (__builtin_sqrtf(qn) * __builtin_sqrtf(kn));  // 2 e
   // Scores from here up are candidates.
   const float from = __builtin_fabsf(nth) == INFINITY ? nth : nth - (TAGS ? slack + a.tag_error * __builtin_fabsf(nth) : slack);
   const float sure = nth + (nth - from);  // scores above are chosen, whatever their errors (NaN: there is no doubt)
-  const bool doubt = !exact && i < a.tq && seen > a.selected && !(after < from);
+  const bool doubt = !exact && !zero && i < a.tq && seen > a.selected && !(after < from);
   const bool mine = half == 0 && i < a.tq;
   int* out = a.out + (((long long)b * a.tq + i) * a.kv + g) * a.selected;
+  if (zero && mine) {  // (the block that is always taken is the last one seen)
+    const int count = min(seen, a.selected);
+    for (int n = 0; n < a.selected; ++n) out[n] = n >= count ? -1 : n == count - 1 && forced >= 0 ? forced : n;
+  }
 
   if constexpr (TAGS) {
     // Candidates of both halves side by side, the lower half's first, then the block that is always taken.
@@ -710,7 +731,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
       }
     if (half && forced >= 0) row[count - 1] = forced;
     __builtin_amdgcn_wave_barrier();
-    if (i < a.tq && !exact && !doubt) {
+    if (i < a.tq && !exact && !doubt && !zero) {
       int id[SMAX];
 #pragma unroll
       for (int n = 0; n < SMAX; ++n) id[n] = n < count ? row[n] : INT_MAX;
@@ -768,7 +789,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
         const int j = 32 * n + __builtin_ctz(w);
         const int mark = near & (w & -w) ? kDoubtful : 0;
         w &= w - 1;
-        if (mine && !exact) {
+        if (mine && !exact && !zero) {
           if (slot >= 0) {
             if (count < 64) pool[slot * 64 + count] = j | mark;
           } else if (count < a.selected) {
@@ -781,7 +802,7 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
   }
   __builtin_amdgcn_wave_barrier();
   if (slot >= 0 && count > 64) exact = true;
-  if (mine && !exact && slot < 0)
+  if (mine && !exact && !zero && slot < 0)
     for (int n = count; n < a.selected; ++n) out[n] = -1;
   for (unsigned long long todo = __ballot(mine && !exact && slot >= 0); todo; todo &= todo - 1) {
     const int x = __builtin_ctzll(todo);
