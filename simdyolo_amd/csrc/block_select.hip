@@ -319,21 +319,16 @@ __device__ __forceinline__ double query_sum(const SelectArgs& a, const float* q,
   return s;
 }
 
-// The sum of query i's heads of group g, in 64 bits, for all lanes of a wave: two channels to a lane.
-__device__ __forceinline__ void query_sums(const SelectArgs& a, int b, int i, int g, int lane, double* qsum) {
+// The sum of query i's heads of group g, in 64 bits, two channels to a lane.
+__device__ __forceinline__ void query_sums(const SelectArgs& a, int b, int i, int g, int lane, double (&s)[2]) {
   const float* q = a.q + ((long long)b * a.tq + i) * a.ldq + (long long)g * a.group * a.qs + min(2 * lane, a.kd - 2);
-  double s0 = 0, s1 = 0;
+  s[0] = s[1] = 0;
 #pragma unroll 8
   for (int h = 0; h < a.group; ++h) {
     const f32x2v v = *(const f32x2v*)(q + (long long)h * a.qs);
-    s0 += v[0];
-    s1 += v[1];
+    s[0] += v[0];
+    s[1] += v[1];
   }
-  if (2 * lane < a.kd) {
-    qsum[2 * lane] = s0;
-    qsum[2 * lane + 1] = s1;
-  }
-  __builtin_amdgcn_wave_barrier();
 }
 
 __device__ __forceinline__ long long exact_key(const SelectArgs& a, int b, int g, int j, const double* qsum) {
@@ -348,17 +343,36 @@ __device__ __forceinline__ long long exact_key(const SelectArgs& a, int b, int g
   return score_key(s);
 }
 
-// One query in 64 bits by one wave: a lane scores a block of 64.
-__device__ __forceinline__ void select_exact(const SelectArgs& a, int b, int i, int g, int lane, double* qsum) {
-  query_sums(a, b, i, g, lane, qsum);
+// The last query that a wave has ranked so, and its choice.
+struct Ranked {
+  double q[2];
+  int seen = -1, forced, kept, id;
+};
+
+// One query in 64 bits by one wave: a lane scores a block of 64.  Where many blocks are alike (a constant area of a map),
+// so are the queries there, one after the other: the choice of the one before is theirs.
+__device__ __forceinline__ void select_exact(const SelectArgs& a, int b, int i, int g, int lane, double* qsum, Ranked& last) {
+  double q[2];
+  query_sums(a, b, i, g, lane, q);
   int forced;
   const int seen = seen_blocks(a, b, i, &forced);
-  long long bk;
-  int bi;
-  const int kept = rank_wave(seen, a.selected, lane,
-                             [&](int j) { return j == forced ? (long long)LLONG_MAX : exact_key(a, b, g, j, qsum); }, &bk, &bi);
-  write_row(a.out + (((long long)b * a.tq + i) * a.kv + g) * a.selected, a.selected, kept, lane, bi);
-  __builtin_amdgcn_wave_barrier();
+  // (A NaN differs from itself: such a query is ranked.)
+  if (seen != last.seen || forced != last.forced || !__all(q[0] == last.q[0] && q[1] == last.q[1])) {
+    if (2 * lane < a.kd) {
+      qsum[2 * lane] = q[0];
+      qsum[2 * lane + 1] = q[1];
+    }
+    __builtin_amdgcn_wave_barrier();
+    long long bk;
+    last.kept = rank_wave(seen, a.selected, lane,
+                          [&](int j) { return j == forced ? (long long)LLONG_MAX : exact_key(a, b, g, j, qsum); }, &bk, &last.id);
+    __builtin_amdgcn_wave_barrier();
+    last.q[0] = q[0];
+    last.q[1] = q[1];
+    last.seen = seen;
+    last.forced = forced;
+  }
+  write_row(a.out + (((long long)b * a.tq + i) * a.kv + g) * a.selected, a.selected, last.kept, lane, last.id);
 }
 
 // The same among `count` candidates (up to 64, more than wanted), of which those marked kDoubtful are scored: sixteen
@@ -749,8 +763,9 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
       const int x = __builtin_ctzll(todo);
       select_among<KS>(a, b, i0 + x, g, lane, pool + x * kRow, __builtin_amdgcn_readlane(count, x));
     }
+    Ranked ranked;
     for (unsigned long long todo = __ballot(mine && exact); todo; todo &= todo - 1)
-      select_exact(a, b, i0 + __builtin_ctzll(todo), g, lane, qsum[wave]);
+      select_exact(a, b, i0 + __builtin_ctzll(todo), g, lane, qsum[wave], ranked);
     return;
   }
 
@@ -809,8 +824,9 @@ __global__ __launch_bounds__(256, SMAX > 16 ? 1 : KS == 2 ? 4 : KS == 4 ? 3 : 1)
     select_among<KS>(a, b, i0 + x, g, lane, pool + __builtin_amdgcn_readlane(slot, x) * 64,
                      __builtin_amdgcn_readlane(count, x));
   }
+  Ranked ranked;
   for (unsigned long long todo = __ballot(mine && exact); todo; todo &= todo - 1)
-    select_exact(a, b, i0 + __builtin_ctzll(todo), g, lane, qsum[wave]);
+    select_exact(a, b, i0 + __builtin_ctzll(todo), g, lane, qsum[wave], ranked);
 }
 
 constexpr int kScoreQueries = 8;

@@ -97,3 +97,26 @@ def test_one_long_mean(hip, size):
     got = run_select(hip, cfg, q, m, 1, blocks, many=True)
     few, got = some(q, got)
     np.testing.assert_array_equal(got, R.select(cfg, few, m))
+
+
+@pytest.mark.parametrize("kd,selected", [(32, 8), (128, 16), (64, 40)])
+def test_alike_queries_of_a_row(hip, kd, selected):
+    """Causal queries of a few kinds, alike in runs, on means that are nearly all alike: each sees another end."""
+    cfg, tq, blocks = R.shape(4, 2, 1, 4, selected, causal=1), 1300, 330
+    q = R.rng(1).standard_normal((2, 6, 4, kd)).astype(np.float32)[:, (np.arange(tq) // 9) % 6]
+    q[:, ::50] = np.nan
+    m = np.repeat(R.rng(2).standard_normal((2, 1, 2, kd)), blocks, 1).astype(np.float32)
+    m[:, 100::45] = R.rng(3).standard_normal((2, len(range(100, blocks, 45)), 2, kd))
+    compare(hip, cfg, q, m, (0, 13), (1290, 1200), 10)
+
+
+def test_bars_cost_little_more(hip):
+    """Bars above and below the picture, a third of the map, where keys and queries are constants: the queries there, in
+    doubt between blocks that are alike, are ranked once for a run of them (one by one 9 times the ordinary call)."""
+    cfg, n, h, w, kd = R.shape(4, 4, 8, 8, 8), 2, 160, 160, 32
+    q = R.rng(1).standard_normal((n, h, w, 4, kd)).astype(np.float32)
+    m = R.rng(2).standard_normal((n, 400, 4, kd)).astype(np.float32)
+    plain = least_ms(hip, cfg, q.reshape(n, h * w, 4, kd), m, h, w, 20, 20, kd)
+    q[:, :24] = q[:, 136:] = q[:, :1, :1]
+    m[:, :60] = m[:, 340:] = q[:, 0, :1]
+    assert least_ms(hip, cfg, q.reshape(n, h * w, 4, kd), m, h, w, 20, 20, kd) < 3 * plain
