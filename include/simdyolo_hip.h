@@ -551,8 +551,9 @@ int sy_model_set_graph(sy_model* model, int use_graph);
  * the neck: level 0 = one chain, 1 = the P3 head as a branch, 2 = the P3 and
  * P4 heads.  By default (-1) each planned shape captures every level, times
  * a few replays of each and keeps the fastest, as the convolutions are
- * autotuned; a level set here is used as given (existing graphs are
- * recaptured).  Outputs do not depend on the level.  The reference runs its
+ * autotuned (a chunk that sy_model_predict_raw or _seg has run before as a
+ * part of a batch: one chain); a level set here is used as given (existing
+ * graphs are recaptured).  Outputs do not depend on the level.  The reference runs its
  * recorded command buffer in order (VulkanReplay.cs); this has no
  * counterpart there.  sy_model_branch_level reports the level of a captured
  * shape (-1 before its first graph run). */

@@ -1276,7 +1276,7 @@ int run_plan_chain(sy_model* m, Plan* plan) {
     SY_TRY(run_ops(ctx, plan, 0));
     SY_HIP(hipStreamSynchronize(ctx->stream));
     plan->warmed = true;
-    plan->level = m->branch_level;  // run_plan still picks its branch level by timing
+    plan->level = m->branch_level;
   }
   if (!plan->graph0) {
     SY_TRY(ensure_scratch(ctx, plan->scratch));
@@ -1301,6 +1301,9 @@ int run_plan(sy_model* m, Plan* plan) {
     plan->warmed = true;
     plan->level = m->branch_level;
   }
+  // A chunk plan of the host pipeline stays one chain.  (A process once ended in a host segmentation fault where
+  // such a plan captured, timed and destroyed its branched graphs; the cause is not known.)
+  if (plan->level < 0 && plan->graph0) plan->level = 0;
   if (!plan->graph) {
     // The branch ops run on the side stream with its own scratch buffer,
     // which must not grow during capture.

@@ -90,6 +90,22 @@ def test_predict_raw_default_chunks_match_resident(v8n, hip, batch, h, w):
     np.testing.assert_array_equal(det.predict_raw(x), got)
 
 
+def test_chunk_plans_stay_one_chain(v8n, hip):
+    """The plan of a chunk that predict_raw ran as one chain does not try branched graphs when it is run by itself, a
+    batch that it ran as a whole does; the rows are the same."""
+    det, _ = v8n
+    x = synth.images(18, 160, 192, seed=4)
+    got = det.predict_raw(x)
+    inp, out = det.buffers(9, 160, 192)
+    hip.h2d(inp, x[9:])
+    det.run(9, 160, 192)
+    hip.flush()
+    np.testing.assert_array_equal(got[9:], hip.d2h(out, det.output_shape(9, 160, 192)))
+    assert det.branch_level(9, 160, 192) == 0
+    det.predict_raw(x[:3])
+    assert det.branch_level(3, 160, 192) >= 0
+
+
 def test_predict_seg_default_chunks_match_resident(hip):
     """The same for a Segment model: two chunks of eight images, the head rows
     and then the prototypes of each chunk coming down through the staging,
