@@ -27,10 +27,12 @@ struct Status {
   int code;
 };
 
+// The error that HIP keeps is taken with it: the next launch, which asks for it, has not failed.
 #define SY_HIP(call)                                                         \
   do {                                                                       \
     hipError_t e_ = (call);                                                  \
     if (e_ != hipSuccess) {                                                  \
+      (void)hipGetLastError();                                               \
       ::sy::set_error("%s failed: %s (%d) at %s:%d", #call,                  \
                       hipGetErrorString(e_), (int)e_, __FILE__, __LINE__);   \
       return e_ == hipErrorOutOfMemory ? SY_ENOMEM : SY_EDEVICE;             \

@@ -1,0 +1,44 @@
+"""A call that the device has no memory for fails by itself, and nothing after it."""
+import numpy as np
+import pytest
+
+import _blocks as R
+from simdyolo_amd import SyError, Tensor
+from simdyolo_amd import _native as N
+from simdyolo_amd.device import HipContext
+
+pytestmark = pytest.mark.gpu
+
+
+def beyond_memory(ctx):
+    """Lists of 2^39 pairs of query and block, 4.4 TB: refused when they are asked for, before anything is launched (the
+    addresses stand for nothing)."""
+    far = [Tensor((i + 1) << 44, 64, 32, 1, w, 32, 0) for i, w in enumerate((1 << 24, 1024, 1024, 1 << 24))]
+    with pytest.raises(SyError) as e:
+        ctx.block_attention(R.config(R.shape(8, 8, 1, 16, 64), 4, 4), far[0], far[1], far[2], 5 << 44, far[3])
+    assert e.value.code == N.SY_ENOMEM
+
+
+def attention(ctx, d):
+    cfg = R.shape(2, 2, 4, 4, 3)
+    q, k, v = (R.rng(i).standard_normal((1, 400, 2, 32)).astype(np.float32) for i in range(3))
+    blocks = np.tile(np.array([0, 7, 24], np.int32), (1, 400, 2, 1))
+    vq, vk, vv = (d.view(a, 20, 20)[0] for a in (q, k, v))
+    vo, _, read = d.view(np.full((1, 400, 2, 32), np.nan, np.float32), 20, 20)
+    p = d.put(blocks)
+    exp, bound = R.attend(cfg, q, k, v, blocks, 20, 20, 32 ** -0.5)
+
+    def run():
+        ctx.block_attention(R.config(cfg, 32, 32), vq, vk, vv, p, vo)
+
+    def check():
+        assert (np.abs(read() - exp) <= bound).all()
+    return run, check
+
+
+def test_next_call_works():
+    with HipContext(0) as ctx, R.Device(ctx) as d:
+        run, check = attention(ctx, d)
+        beyond_memory(ctx)
+        run()
+        check()
