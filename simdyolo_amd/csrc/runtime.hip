@@ -71,11 +71,12 @@ int ensure_scratch(sy_ctx* ctx, size_t bytes) {
     SY_HIP(hipFree(ctx->scratch));
     ctx->scratch = nullptr;
     ctx->scratch_size = 0;
+    ++ctx->scratch_gen;  // graphs captured before now hold its address, also where the next allocation fails
   }
   size_t sz = (bytes + (1u << 20) - 1) & ~size_t((1u << 20) - 1);
   SY_HIP(hipMalloc((void**)&ctx->scratch, sz));
   ctx->scratch_size = sz;
-  ++ctx->scratch_gen;  // graphs captured before now hold the old address
+  ++ctx->scratch_gen;
   return SY_OK;
 }
 

@@ -42,3 +42,20 @@ def test_next_call_works():
         beyond_memory(ctx)
         run()
         check()
+
+
+def test_graphs_of_before_are_refused():
+    """The scratch that a graph was captured with is gone with the call that wanted more of it."""
+    with HipContext(0) as ctx, R.Device(ctx) as d:
+        run, check = attention(ctx, d)
+        run()
+        ctx.graph_begin()
+        run()
+        graph = ctx.graph_end()
+        ctx.graph_launch(graph)
+        check()
+        beyond_memory(ctx)
+        with pytest.raises(SyError, match="capture it again"):
+            ctx.graph_launch(graph)
+        run()
+        check()
