@@ -369,10 +369,12 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
   const int y0 = j / s.bx * s.bh, x0 = j % s.bx * s.bw;
   const int cols = min(s.bw, s.kw - x0), size = min(s.bh, s.kh - y0) * cols;
   const int origin = y0 * s.kw + x0;
-  // Keys of this part that exist: in the window and, in a sequence, before its end.
-  const int length = a.lengths ? min(max(a.lengths[b], 0), s.tk) : s.tk;
+  // Keys of this part that exist: in the window and, in a sequence, before its end.  Nor does any row see those behind the
+  // last query's: a cache may hold anything there (NaN in the block of the last of 8,100 tokens: 624 us, not 4,575).
   const long long start = a.starts ? a.starts[b] : 0;
-  int keys = a.lengths ? min(size, length - origin) : size;
+  int length = a.lengths ? min(max(a.lengths[b], 0), s.tk) : s.tk;
+  if (s.causal) length = (int)min((long long)length, max(start + s.tq, 0LL));
+  int keys = a.lengths || s.causal ? min(size, length - origin) : size;
   keys = min(max(keys - part * kKeys, 0), kKeys);
 
   // The lane's row in the wave's turn r: its query, the keys it sees, where its results go.  Channels past key_dim read

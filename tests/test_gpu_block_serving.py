@@ -88,3 +88,30 @@ def test_two_graphs_on_new_inputs():
                     chains[1 - i]()
                 ctx.graph_launch(g)
                 c.check()
+
+
+def test_garbage_behind_the_last_token_costs_nothing(hip):
+    """A causal call on a cache without lengths whose rest holds NaN: the rows of the last tokens are not computed twice (7
+    times the call's time when they were)."""
+    cfg, tq, w, dim = R.shape(16, 4, 1, 64, 8, causal=1), 4036, 4096, 64
+    q, k, v = tensors(1, tq, w, cfg, dim, dim, 7)
+    g = R.rng(8)
+    blocks = np.sort(g.integers(0, np.arange(tq)[None, :, None, None] // 64 + 1, (1, tq, 4, 8)), -1).astype(np.int32)
+    blocks[..., -1] = np.arange(tq)[:, None] // 64
+    took = []
+    for rest in (0.0, np.nan):
+        k[:, tq:], v[:, tq:] = rest, rest
+        with R.Device(hip) as d:
+            vq, vk, vv = (d.view(a, 1, a.shape[1])[0] for a in (q, k, v))
+            vo, _, read = d.view(np.full((1, tq, 16, dim), np.nan, np.float32), 1, tq)
+            p, cf, least = d.put(blocks), R.config(cfg, dim, dim), np.inf
+            for _ in range(5):
+                hip.timer_start()
+                hip.block_attention(cf, vq, vk, vv, p, vo)
+                least = min(least, hip.timer_stop())
+            got = read()
+        took.append(least)
+        keep = np.r_[g.integers(0, tq, 60), 3968:tq:5]
+        for i in keep:
+            check(got[:, i:i + 1], *R.attend(cfg, q[:, i:i + 1], k, v, blocks[:, i:i + 1], 1, w, dim ** -0.5, [i]))
+    assert took[1] < 2 * took[0]
