@@ -50,7 +50,7 @@ struct BlockArgs {
   // Segments: `span` queries of one image and key head each, `segs` of them to a plane.
   int span, segs, first;  // first: of the launch
   int now;           // segments of the launch
-  // Sorted lists of each segment.
+  // Sorted lists of each segment of the launch.
   int rows;          // of a tile
   unsigned trash;    // a row of results that nobody reads
   int chunk, chunks, tile_cap;  // queries of a workgroup of the sort, such workgroups; tiles at most
@@ -85,12 +85,12 @@ __device__ __forceinline__ const int* list_of(const BlockArgs& a, int b, int i, 
 
 // --------------------------------------------------------------- sorted lists
 
-// The pairs of one chunk of a segment, four at a time in every thread: f(pair, block) for those whose block
+// The pairs of one chunk of a launch's segment, four at a time in every thread: f(pair, block) for those whose block
 // is seen.
 template <class F>
-__device__ __forceinline__ void for_pairs(const BlockArgs& a, int seg, int chunk, F f) {
+__device__ __forceinline__ void for_pairs(const BlockArgs& a, int of_launch, int chunk, F f) {
   const BlockShape& s = a.s;
-  const int plane = seg / a.segs, b = plane / s.kv, g = plane - b * s.kv;
+  const int seg = a.first + of_launch, plane = seg / a.segs, b = plane / s.kv, g = plane - b * s.kv;
   const int i0 = seg % a.segs * a.span, i1 = min(i0 + a.span, s.tq);
   const int from = i0 + chunk * a.chunk, to = min(from + a.chunk, i1);
   const int pairs = max(to - from, 0) * s.selected, skip = (from - i0) * s.selected;
@@ -324,10 +324,9 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
   const int half = lane >> 5, r32 = lane & 31;
 
   const unsigned item = item_of(blockIdx.x, gridDim.x);
-  int seg = item / a.tile_cap;
-  const int t = item - seg * a.tile_cap;
-  if (seg >= a.now) return;
-  seg += a.first;
+  const int ls = item / a.tile_cap, seg = a.first + ls;
+  const int t = item - ls * a.tile_cap;
+  if (ls >= a.now) return;
   const int plane = seg / a.segs, b = plane / s.kv, g = plane - b * s.kv, i0 = (seg - plane * a.segs) * a.span;
   const bool scan = !a.list;
   int4 rec;  // block, part of it and number of the tile, first entry of its list, length of the list
@@ -357,15 +356,15 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
     rec = make_int4(j, t % a.parts | t / (a.parts * s.blocks) << 8, 0, all);
     if (all == 0) return;
   } else {
-    rec = a.tiles[(long long)seg * a.tile_cap + t];  // under way with the count
-    if (t >= a.tile_count[seg]) return;
+    rec = a.tiles[(long long)ls * a.tile_cap + t];  // under way with the count
+    if (t >= a.tile_count[ls]) return;
   }
   // Its share of the block's rows: as many as the other tiles', in 32s.
   const int all = rec.w * s.group, share = tile_share(a, all);
   const int j = rec.x, part = rec.y & 255, row0 = (rec.y >> 8) * share;
   const int rows = min(all - row0, share);
   if (rows <= 0) return;
-  const int* list = scan ? nullptr : a.list + (long long)seg * a.span * s.selected + rec.z;
+  const int* list = scan ? nullptr : a.list + (long long)ls * a.span * s.selected + rec.z;
   const int y0 = j / s.bx * s.bh, x0 = j % s.bx * s.bw;
   const int cols = min(s.bw, s.kw - x0), size = min(s.bh, s.kh - y0) * cols;
   const int origin = y0 * s.kw + x0;
@@ -392,7 +391,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
       const long long end = min((long long)length, max(start + i0 + d + 1, 0LL));
       limit = min(keys, (int)end - origin - part * kKeys);
     }
-    const unsigned slot = (unsigned)((seg - a.first) * a.span * s.selected + (scan ? pair : rec.z + e0 + e)) * a.parts + part;
+    const unsigned slot = (unsigned)(ls * a.span * s.selected + (scan ? pair : rec.z + e0 + e)) * a.parts + part;
     to = r + r32 < rows ? slot * s.group + h : a.trash;
     const float* p = qb + (long long)d * a.ldq + h * s.qs;
 #pragma unroll
@@ -873,7 +872,7 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
     int at = 0;
     if (on) {
       const int p = n / a.parts;
-      const long long pair = a.pos ? a.pos[(long long)a.first * a.span * s.selected + home + first + p] : first + p;
+      const long long pair = a.pos ? a.pos[home + first + p] : first + p;
       at = (int)(((home + pair) * a.parts + (n - p * a.parts)) * s.group + h);
       st = a.stat[at];
     }
@@ -1026,13 +1025,13 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   const long long result_rows = together * pairs * a.parts * s.group;
   SY_CHECK((result_rows + 1) * s.hd < (1LL << 30) - 128 && tile_cap * together < (1LL << 24), SY_EUNSUPPORTED,
            "block attention over %d heads to a key head", s.group);
-  SY_CHECK(!sorted || segments * a.chunks * kSortThreads < (1LL << 32), SY_EUNSUPPORTED,
-           "block attention over %lld lists", segments);
+  SY_CHECK(!sorted || (long long)together * a.chunks * kSortThreads < (1LL << 32), SY_EUNSUPPORTED,
+           "block attention over %d lists", together);
   SY_CHECK(((s.bh - 1.0) * s.kw + s.bw) * std::max(k->ldc, v->ldc) < 4294967296.0, SY_EUNSUPPORTED,
            "block windows that span 2^32 floats and more");
   a.tile_cap = (int)tile_cap;
   a.trash = (unsigned)result_rows;
-  // Scratch: results, then lists.
+  // Scratch, of one launch: results, then lists.
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t from = at;
@@ -1041,11 +1040,11 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   };
   const size_t part_at = take(sizeof(float) * ((result_rows + 1) * s.hd + 128)),
                stat_at = take(sizeof(Stat) * (result_rows + 1));
-  const size_t count_at = sorted && !scan ? take(sizeof(int) * segments * a.chunks * s.blocks) : 0;
-  const size_t list_at = sorted && !scan ? take(sizeof(int) * segments * pairs) : 0;
-  const size_t pos_at = sorted && !scan ? take(sizeof(int) * segments * pairs) : 0;
-  const size_t tile_at = sorted && !scan ? take(sizeof(int4) * segments * tile_cap) : 0;
-  const size_t number_at = sorted && !scan ? take(sizeof(int) * segments) : 0;
+  const size_t count_at = sorted && !scan ? take(sizeof(int) * together * a.chunks * s.blocks) : 0;
+  const size_t list_at = sorted && !scan ? take(sizeof(int) * together * pairs) : 0;
+  const size_t pos_at = sorted && !scan ? take(sizeof(int) * together * pairs) : 0;
+  const size_t tile_at = sorted && !scan ? take(sizeof(int4) * together * tile_cap) : 0;
+  const size_t number_at = sorted && !scan ? take(sizeof(int) * together) : 0;
   DeviceScope device(ctx);
   SY_TRY(ensure_scratch(ctx, at));
   a.part = (float*)(ctx->scratch + part_at);
@@ -1056,19 +1055,19 @@ int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
   a.tiles = (int4*)(ctx->scratch + tile_at);
   a.tile_count = (int*)(ctx->scratch + number_at);
   const double keys = std::min((double)s.selected * s.bh * s.bw, (double)s.tk);
-  if (sorted && !scan) {
-    ProfScope prof(ctx, "block_sort", 0, 8.0 * s.n * (double)s.tq * s.kv * s.selected);
-    const size_t lds = sizeof(int) * s.blocks;
-    const dim3 grid((unsigned)(segments * a.chunks)), threads(kSortThreads);
-    if (a.chunks > 1) hipLaunchKernelGGL(block_count_kernel, grid, threads, lds, ctx->stream, a);
-    hipLaunchKernelGGL(block_scatter_kernel, grid, threads, lds, ctx->stream, a);
-    SY_TRY(check_launch("block_sort"));
-  }
   for (long long first = 0; first < segments; first += together) {
     const int now = (int)std::min<long long>(together, segments - first);
     const double share = (double)now / segments;
     a.first = (int)first;
     a.now = now;
+    if (sorted && !scan) {
+      ProfScope prof(ctx, "block_sort", 0, share * 8.0 * s.n * (double)s.tq * s.kv * s.selected);
+      const size_t lds = sizeof(int) * s.blocks;
+      const dim3 grid((unsigned)(now * a.chunks)), threads(kSortThreads);
+      if (a.chunks > 1) hipLaunchKernelGGL(block_count_kernel, grid, threads, lds, ctx->stream, a);
+      hipLaunchKernelGGL(block_scatter_kernel, grid, threads, lds, ctx->stream, a);
+      SY_TRY(check_launch("block_sort"));
+    }
     {
       ProfScope prof(ctx, sorted ? "block_attention" : "block_few", share * 2.0 * s.n * s.tq * s.heads * keys * (s.kd + s.hd),
                      share * 4.0 * s.n * ((double)s.tq * s.heads * (s.kd + s.hd) + (double)s.tk * s.kv * (s.kd + s.hd)));

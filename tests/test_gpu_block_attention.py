@@ -451,3 +451,20 @@ def test_token_by_token(hip):
     check(out, exp, bound)
     whole = run(hip, cfg, q, k, v, lists, 1, w, pads=False)
     check(whole, exp, bound)
+
+
+def test_lists_of_each_launch(hip):
+    """Five sequences of 0.31 GB of results each: three and two to a launch, which sorts its own pairs."""
+    cfg, n, tq, dim = R.shape(1, 1, 1, 16, 30, causal=1), 5, 20000, 128
+    lengths, starts = (20000, 19000, 5, 20000, 12345), (0, -700, 10, 0, 60)
+    q, k, v = tensors(n, tq, tq, cfg, dim, dim, 9)
+    g = R.rng(10)
+    last = np.clip((np.asarray(starts)[:, None, None, None] + np.arange(tq)[:, None, None]) // 16, 0, 1249)
+    blocks = np.minimum(g.integers(0, 1250, (n, tq, 1, 30)), last).astype(np.int32)
+    got = run(hip, cfg, q, k, v, blocks, 1, tq, 1, starts, lengths, pads=False, sort=True)
+    assert np.isfinite(got).all()
+    for b in range(n):
+        for i in np.unique(np.r_[0, 1, tq - 1, g.integers(0, tq, 25)]):
+            one = slice(b, b + 1)
+            check(got[one, i:i + 1], *R.attend(cfg, q[one, i:i + 1], k[one], v[one], blocks[one, i:i + 1], 1, tq, dim ** -0.5,
+                                               [starts[b] + i], [lengths[b]]))

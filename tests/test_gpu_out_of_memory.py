@@ -11,11 +11,12 @@ pytestmark = pytest.mark.gpu
 
 
 def beyond_memory(ctx):
-    """Lists of 2^39 pairs of query and block, 4.4 TB: refused when they are asked for, before anything is launched (the
-    addresses stand for nothing)."""
-    far = [Tensor((i + 1) << 44, 64, 32, 1, w, 32, 0) for i, w in enumerate((1 << 24, 1024, 1024, 1 << 24))]
+    """Means of 16 images of 8 heads of 128 channels in 2^24 - 1 blocks, whose operands take 1.1 TB: refused when that is
+    asked for, before anything is launched (the addresses stand for nothing)."""
+    q = Tensor(1 << 44, 16, 1024, 1, 64, 1024, 0)
+    m = Tensor(2 << 44, 16, 1024, 1, (1 << 24) - 1, 1024, 0)
     with pytest.raises(SyError) as e:
-        ctx.block_attention(R.config(R.shape(8, 8, 1, 16, 64), 4, 4), far[0], far[1], far[2], 5 << 44, far[3])
+        ctx.block_select(R.config(R.shape(8, 8, 1, 1, 4), 128, 4), q, m, 3 << 44)
     assert e.value.code == N.SY_ENOMEM
 
 
