@@ -33,12 +33,12 @@
  * sy_block_attention multiplies pairs of f16 values under a power of two of
  * each row's own (a query, a key, a key's values): an operand within 2^-22 of
  * itself, or 2^-42 of its row's largest where that is more, whatever other
- * rows hold, and 3 x 2^-22 of each product at most.  Queries whose scores could
- * feel more than that (|q||k| scale of 2^20 and more, elementwise largest), those
- * that meet values with a channel 2^-21 and more below the others throughout,
- * and rows that come out infinite or NaN are computed in plain float32, as all
- * are where queries are few.  With channels of one size its error against
- * float64 is 0.4 to 0.65 of plain float32's.
+ * rows hold, and 3 x 2^-22 of each product at most; channels of the values
+ * that are far below the others have a power of their own.  Queries whose
+ * scores could feel more than that (|q||k| scale of 2^20 and more, elementwise
+ * largest) and rows that come out infinite or NaN are computed in plain
+ * float32, as all are where queries are few.  With channels of one size its
+ * error against float64 is 0.4 to 0.65 of plain float32's.
  *
  * Errors.  Every int-returning call returns SY_OK (0) or one of the SY_E*
  * codes; sy_last_error() returns a thread-local message.  The C# binding maps

@@ -294,8 +294,9 @@ __device__ __forceinline__ unsigned item_of(unsigned block, unsigned grid) { ret
 //
 // Elements below that keep an absolute precision, 2^-36 under their power: for a score 1.5 x 2^-20 under both powers from
 // each channel and so, as long as its factor is at most kWide, less than 2^-20 of its exponent.  Rows past that
-// (|q||k| scale of 2^20 and more), and those of a tile whose values have a channel so far below the others in eight
-// keys at once, leave NaN for their sum: the join computes them in plain float32.
+// (|q||k| scale of 2^20 and more) leave NaN for their sum: the join computes them in plain float32.  A tile whose values
+// have a channel so far below the others, in eight keys at once, gives every channel a power of its own, which comes
+// off the results (2^-90 and less: plain float32, too).
 //
 // Keys and values stand in LDS as pairs, in the order in which the matrix instruction's lanes take them, so that a
 // fragment is one 16-byte read without bank conflicts.  Once they stand there the waves run on their own: no
@@ -318,7 +319,8 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
   __shared__ float k_top[kKeys], v_top[kKeys];     // largest magnitude of a key, of its values
   __shared__ __align__(16) int k_power[kKeys], v_power[kKeys];
   __shared__ unsigned place[4][32];
-  __shared__ int pair_at[kTileRows], uneven;
+  __shared__ int pair_at[kTileRows];
+  __shared__ int uneven, c_power[32 * DT];         // whether channels have powers of their own; these, 14 above
   const BlockShape& s = a.s;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, r32 = lane & 31;
@@ -383,6 +385,11 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
   f32x4 qr[KS][2];
   int limit;
   unsigned to;  // row of the results
+  auto result_row = [&](int x) __attribute__((always_inline)) {
+    const int e = x / s.group;
+    const unsigned slot = (unsigned)(ls * a.span * s.selected + (scan ? pair_at[e] : rec.z + e0 + e)) * a.parts + part;
+    return slot * s.group + (x - e * s.group);
+  };
   auto load_q = [&](int r) __attribute__((always_inline)) {
     const int x = h0 + min(r + r32, rows - 1), e = x / s.group, h = x - e * s.group;
     const int pair = pair_at[e], d = pair / s.selected;
@@ -391,13 +398,22 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
       const long long end = min((long long)length, max(start + i0 + d + 1, 0LL));
       limit = min(keys, (int)end - origin - part * kKeys);
     }
-    const unsigned slot = (unsigned)(ls * a.span * s.selected + (scan ? pair : rec.z + e0 + e)) * a.parts + part;
-    to = r + r32 < rows ? slot * s.group + h : a.trash;
+    to = r + r32 < rows ? result_row(x) : a.trash;
     const float* p = qb + (long long)d * a.ldq + h * s.qs;
+    constexpr bool kOften = KS * DT < 16;  // whether offsets kept for the loop would be spilled
+    if (kOften && s.kd == 16 * KS) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) qr[ks][u] = *(const f32x4*)(p + 8 * half + 16 * ks + 4 * u);
+      return;
+    }
+    int at = 8 * half;
+    if (kOften) asm("" : "+v"(at));  // made here
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) qr[ks][u] = *(const f32x4*)(p + min(16 * ks + 8 * half + 4 * u, s.kd - 4));
+      for (int u = 0; u < 2; ++u) qr[ks][u] = *(const f32x4*)(p + min(at + 16 * ks + 4 * u, s.kd - 4));
   };
   // The key's place in floats from the block's first one; a quotient of numbers below 2^11, exact in float32.
   const float per_row = 1.f / cols;
@@ -448,6 +464,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
       if (!scan && tid + 256 * n < kTileRows) pair_at[tid + 256 * n] = first_pair[n];
     if (tid < kKeys) v_at[tid] = key_at(tid, a.ldv);
     if (tid == 0) uneven = 0;
+    if (tid < 32 * DT) c_power[tid] = kNoPower;
     __syncthreads();
     load_q(r);
 #pragma unroll
@@ -516,8 +533,31 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
         frag[KF * 64 + (((piece >> 1) * DT + (c >> 5)) * 2 + m) * 64 + (piece & 1) * 32 + (c & 31)] =
             __builtin_bit_cast(u32x4, p[m]);
     }
+    __syncthreads();
+    if (uneven) {
+      const int power = v_flat ? -v_most : 0;
+#pragma unroll
+      for (int n = 0; n < VI; ++n) {
+        const float top = max8(vr[n]);
+        if (top > 0.f && top <= FLT_MAX) atomicMax(&c_power[(tid + 256 * n) % (32 * DT)], __builtin_amdgcn_frexp_expf(top) - 1 + power);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < VI; ++n) {
+        const int x = tid + 256 * n, ch = x % (32 * DT), piece = x / (32 * DT), own = c_power[ch];
+        if (own < 14 - 90 && own != kNoPower) uneven = 2;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) vr[n][e] = __builtin_ldexpf(vr[n][e], power + 14 - max(own, 14 - 90));
+        f16x8 p[2];
+        pairs8(vr[n], 1.f, p[0], p[1]);
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+          frag[KF * 64 + (((piece >> 1) * DT + (ch >> 5)) * 2 + m) * 64 + (piece & 1) * 32 + (ch & 31)] =
+              __builtin_bit_cast(u32x4, p[m]);
+      }
+      __syncthreads();
+    }
   }
-  __syncthreads();
 
   auto k_at = [&](int t, int ks, int m) __attribute__((always_inline)) {
     return __builtin_bit_cast(f16x8, frag[((t * KS + ks) * 2 + m) * 64 + half * 32 + ((r32 + 2 * ks + half) & 31)]);
@@ -526,7 +566,6 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
     return __builtin_bit_cast(f16x8, frag[KF * 64 + ((st * DT + d) * 2 + m) * 64 + lane]);
   };
 
-  const bool plain = uneven;
   // (Results pass the caches by, written here and read by the join, and so do the join's outputs: 287 -> 234 us on two
   // 160x160 maps, 659 -> 585 on 8,192 causal tokens, whose queries and keys they would push out.)
   // The queries are here before the loop: in it they are waited for with the stores behind them still under way.
@@ -582,7 +621,7 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
         k_top_power = max(k_top_power, __shfl_xor(k_top_power, 32));
       }
     }
-    const bool wide = plain || !(__builtin_ldexpf(cs, k_top_power + q_power) <= kWide);
+    const bool wide = !(__builtin_ldexpf(cs, k_top_power + q_power) <= kWide);
     // Keys that do not exist, and in a causal tile those that some rows do not see.
     if (keys < kKeys && !partly) {
       int end = keys;
@@ -667,6 +706,33 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
       if (WHOLE || 32 * d + r32 < s.hd)
 #pragma unroll
         for (int x = 0; x < 16; ++x) __builtin_nontemporal_store(acc[x], (float*)(base + row_at[x]));
+    }
+  }
+  if (!uneven) return;
+  // The channels' own powers come off afterwards, so that the loop does not know of them.  (All channels of one size, and one
+  // 1e-12 of the others: two 160x160 maps 232 and 395 us.)
+  __threadfence_block();  // results of the wave's other lanes
+  const int quads = s.hd / 4;
+  for (r = wave * 32; r < rows; r += 128) {
+    const int count = min(32, rows - r) * quads;
+    for (int n0 = lane; n0 < count; n0 += 4 * 64) {
+      f32x4* of[4];
+      f32x4 y[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int n = min(n0 + 64 * u, count - 1), x = n / quads;
+        const unsigned row = result_row(h0 + r + x);
+        of[u] = (f32x4*)(a.part + (size_t)row * s.hd) + (n - x * quads);
+        y[u] = *of[u];
+        if (uneven == 2 && n == x * quads) a.stat[row].sum = NAN;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int c = min(n0 + 64 * u, count - 1) % quads * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[u][e] = __builtin_ldexpf(y[u][e], max(c_power[c + e] - 14, -90));
+        if (n0 + 64 * u < count) *of[u] = y[u];
+      }
     }
   }
 }

@@ -103,3 +103,51 @@ def test_large_scores(hip, tq, size):
     exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5)
     k[:, max(tq, 32):] *= np.float32(2.0 ** 60)
     check(run(hip, cfg, q, k, v, blocks, 1, w, sort=tq == MANY), exp, bound)
+
+
+@pytest.mark.parametrize("dims", [(32, 20), (64, 64), (128, 128)], ids=str)
+@pytest.mark.parametrize("group", [1, 3])
+def test_channels_of_values_with_powers_of_their_own(hip, dims, group):
+    """Channels from 2^-21 to 2^-115 of the others, one that is so in the keys of one block alone, one of zeros, one with
+    an infinity in a key that some rows see."""
+    (kd, hd), w = dims, 300
+    cfg = R.shape(2 * group, 2, 1, 70, 3, causal=1)
+    q, k, v = tensors(2, 500, w, cfg, kd, hd, 5)
+    for c, r in enumerate((21, 30, 44, 60, 76, 92, 103, 115)):
+        v[..., c] *= np.float32(2.0 ** -r)
+    v[:, 70:140, :, 8] *= np.float32(2.0 ** -50)
+    v[..., 9] = 0
+    blocks = choice(2, 500, cfg, 1, w, 8, 0.0)
+    exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5, (0, -40))
+    check(run(hip, cfg, q, k, v, blocks, 1, w, starts=(0, -40), sort=True), exp, bound + 2.0 ** -140)
+    v[0, 75, 1, 3] = np.inf
+    with np.errstate(invalid="ignore"):
+        exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5, (0, -40))
+    got = run(hip, cfg, q, k, v, blocks, 1, w, starts=(0, -40), sort=True)
+    np.testing.assert_array_equal(np.isfinite(got), np.isfinite(exp))
+    fine = np.isfinite(exp)
+    assert (np.abs(got[fine] - exp[fine]) <= bound[fine] + 2.0 ** -140).all()
+
+
+def test_a_dead_channel_costs_little_more(hip):
+    """A channel of the values at 1e-12 of the others in every key: 1.7 times the ordinary call, not plain float32 (170
+    times)."""
+    cfg, h, w, kd, hd = R.shape(2, 2, 8, 8, 8), 120, 120, 32, 64
+    q, k, v = tensors(1, h * w, h * w, cfg, kd, hd, 5)
+    blocks = R.rng(3).integers(0, 225, (1, h * w, 2, 8)).astype(np.int32)
+    took = []
+    for size in (1.0, 1e-12):
+        v[..., 7] *= np.float32(size)
+        with R.Device(hip) as d:
+            vq, vk, vv = (d.view(a, h, w)[0] for a in (q, k, v))
+            vo, _, read = d.view(np.full((1, h * w, 2, hd), np.nan, np.float32), h, w)
+            p, cf, least = d.put(blocks), R.config(cfg, kd, hd), np.inf
+            for _ in range(5):
+                hip.timer_start()
+                hip.block_attention(cf, vq, vk, vv, p, vo)
+                least = min(least, hip.timer_stop())
+            got = read()
+        took.append(least)
+        keep = R.rng(4).integers(0, h * w, 100)
+        check(got[:, keep], *R.attend(cfg, q[:, keep], k, v, blocks[:, keep], h, w, kd ** -0.5))
+    assert took[1] < 5 * took[0]
