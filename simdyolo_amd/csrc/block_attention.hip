@@ -8,11 +8,11 @@
 // Sizov, 2023).  A last kernel joins a query's slots.  With few queries (a token against a cache) the pairs are
 // taken as they stand.
 //
-// Measured, us (sort + tiles + join): two 160x160 maps, 4 heads of 32 / 64 channels, 8 of 400 blocks of 64 keys
-// 24 + 113 + 89; 8,192 causal tokens, 16 heads and 4 key heads of 128, 16 of 128 blocks 17 + 340 + 194; plain float32,
-// a wave to a query, 14,900 and 61,700.  The results are written and read once, 0.43 and 1.0 GB: the join is bound by them,
-// and the tiles of 64 channels (3.8 TB/s); those of 128 by two waves per SIMD that share it between vector work (44% of the
-// time) and matrix products (30%).
+// Measured, us (sort + tiles + join, under a tracer): two 160x160 maps, 4 heads of 32 / 64 channels, 8 of 400 blocks of 64
+// keys 22 + 121 + 89; 8,192 causal tokens, 16 heads and 4 key heads of 128, 16 of 128 blocks 17 + 389 + 193; plain
+// float32, a wave to a query, 14,900 and 61,700.  The results are written and read once, 0.43 and 1.0 GB: the join is bound
+// by them, and the tiles of 64 channels (3.5 TB/s); those of 128 by two waves per SIMD that share it between vector work (50%
+// of the time) and matrix products (30%).
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -26,11 +26,14 @@ namespace sy {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kFlat = 8;
-constexpr float kWide = 0x1p-8f, kFine = 0x1p-14f;  // largest factor of a score, least value of a channel (their powers apart)
+// Largest factor of a score, and least value of a channel, that f16 pairs hold (their powers of two apart).
+constexpr float kWide = 0x1p-8f, kFine = 0x1p-14f;
 constexpr int kKeys = 64;    // keys of a tile; longer blocks are so many tiles ("parts" of the block)
 constexpr int kTileRows = 512;  // rows of a tile at most
 constexpr int kScan = 2048;  // pairs of an image and key head that a tile's workgroup goes through itself
-constexpr int kMaxBlocks = 12288;  // of a sorted list: counters in LDS
+// Blocks of a sorted list: counters in LDS.  More go pair by pair, however many queries there are (4,096 of 4 heads of 64, 16
+// of 12,288 blocks of 16 keys 287 us, of 12,289 509).
+constexpr int kMaxBlocks = 12288;
 
 // What a tile leaves for a row beside its weighted values: the maximum (as a power of two), the sum of weights, and the
 // power of two that the values want.
@@ -566,8 +569,9 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
     return __builtin_bit_cast(f16x8, frag[KF * 64 + ((st * DT + d) * 2 + m) * 64 + lane]);
   };
 
-  // (Results pass the caches by, written here and read by the join, and so do the join's outputs: 287 -> 234 us on two
-  // 160x160 maps, 659 -> 585 on 8,192 causal tokens, whose queries and keys they would push out.)
+  // (Results pass the caches by, written here and read by the join, and so do the join's outputs: a whole call 258 us on two
+  // 160x160 maps, 294 with all of them cached, 615 and 676 on 8,192 causal tokens, whose queries and keys they would
+  // push out.)
   // The queries are here before the loop: in it they are waited for with the stores behind them still under way.
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   const float cs = s.scale * 1.4426950408889634f;
@@ -1012,8 +1016,8 @@ __global__ __launch_bounds__(256) void block_join_kernel(const BlockArgs a, long
 constexpr int kScanTiles = 512;
 
 // Bytes of results that one launch leaves and the next one joins.  Fewer would stay in the 256 MiB cache in front of
-// memory, but cost more in half-filled launches: 8,192 causal tokens of 16 heads (1.0 GB) 950 us in pieces of 256 MB, 695 of
-// 400 MB, 687 in one.
+// memory, but cost more in half-filled launches: 8,192 causal tokens of 16 heads (1.0 GB) 978 us in pieces of 256 MB, 681 of
+// 400 MB, 615 in one; two 160x160 maps (0.43 GB) 302, 286 and 258.
 constexpr double kPartials = 1200e6;
 
 int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q, const sy_tensor* k,

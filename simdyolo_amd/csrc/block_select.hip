@@ -1,8 +1,9 @@
 // Which key blocks each query attends to: mean keys of the blocks, and for every query the blocks whose
 // mean has the largest product with it.
 //
-// The choice is made on scores in 64 bits: a product of floats is exact there and 128 of them sum within
-// 2^-46, so it does not hang on the order of a sum as it would in 32 bits.
+// The choice is made on scores in 64 bits: products of floats are exact there (those of a sum of several heads round
+// once) and 128 of them sum within 2^-45 of their magnitudes, whatever the order, which differs between the kernels
+// below.  In 32 bits a choice would hang on it far more often.
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -519,10 +520,12 @@ __global__ __launch_bounds__(256) void means_parts_kernel(const SelectArgs a) {
 //
 // Bound by vector work, which keeps the SIMDs busy nine tenths of the time: 3,600 operations per wave (32 queries, 400 blocks
 // of 32 channels, 8 wanted), of them 1,900 medians; the matrix cores work a sixth of it.  Four maps of 25,600 queries, 4
-// heads: 106 us with the means' parts; with a second pass over the scores 140; in 64 bits throughout 9,900; 64 queries to a wave, which halves the
-// reads of the means, 154.  Two causal rows of 16,001 tokens, 16 / 4 heads of 128 channels, 16 of 251 blocks: 91 us, of them
-// 50 the queries' way from memory; with all candidates of doubtful queries scored again 117, their heads read in 32-byte
-// pieces besides 126.
+// heads: 106 to 121 us with the means' parts; with a second pass over the scores 140; 64 queries to a wave, which halves
+// the reads of the means, 154; where every query is in doubt between more blocks than the lists hold, and ranked in
+// 64 bits, 2,450 (one mean 1,000 times as long as the others, which widens the bound for all, or means all alike but
+// queries that are not; one mean 10 / 100 times as long 130 / 302).  Two causal rows of 16,001 tokens, 16 / 4 heads of
+// 128 channels, 16 of 251 blocks: 90 us, of them 50 the queries' way from memory; with all candidates of doubtful queries
+// scored again 117, their heads read in 32-byte pieces besides 126.
 // kTwice: a second pass over the scores; kTags: their blocks' numbers in them; kRaw: that, on the means as they are.
 enum { kTwice, kTags, kRaw };
 template <int KS, int SMAX, int MODE>
