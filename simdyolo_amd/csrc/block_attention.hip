@@ -26,7 +26,7 @@ namespace sy {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kFlat = 8;
-// Largest factor of a score, and least value of a channel, that f16 pairs hold (their powers of two apart).
+// Largest factor of a score, and least value, that f16 pairs hold (their powers of two apart).
 constexpr float kWide = 0x1p-8f, kFine = 0x1p-14f;
 constexpr int kKeys = 64;    // keys of a tile; longer blocks are so many tiles ("parts" of the block)
 constexpr int kTileRows = 512;  // rows of a tile at most
@@ -297,9 +297,9 @@ __device__ __forceinline__ unsigned item_of(unsigned block, unsigned grid) { ret
 //
 // Elements below that keep an absolute precision, 2^-36 under their power: for a score 1.5 x 2^-20 under both powers from
 // each channel and so, as long as its factor is at most kWide, less than 2^-20 of its exponent.  Rows past that
-// (|q||k| scale of 2^20 and more) leave NaN for their sum: the join computes them in plain float32.  A tile whose values
-// have a channel so far below the others, in eight keys at once, gives every channel a power of its own, which comes
-// off the results (2^-90 and less: plain float32, too).
+// (|q||k| scale of 2^20 and more) leave NaN for their sum: the join computes them in plain float32.  A tile that has values
+// so far below the others of their key gives every channel a power of its own, too, which comes off the results (2^-90
+// and less: plain float32).
 //
 // Keys and values stand in LDS as pairs, in the order in which the matrix instruction's lanes take them, so that a
 // fragment is one 16-byte read without bank conflicts.  Once they stand there the waves run on their own: no
@@ -527,8 +527,14 @@ __global__ __launch_bounds__(256, KS * DT >= 16 ? 2 : KS * DT == 4 ? 4 : 3) void
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (first + 8 * (e >> 2) + (e & 3) >= keys) vr[n][e] = 0.f;
-      const float top = max8(vr[n]);
-      if (top != 0.f && top * scale < kFine) uneven = 1;
+      // Any value below what pairs hold (of values of one size 1 in 10^9)?  Zeros are none.
+      float least = __builtin_fabsf(vr[n][0]);
+#pragma unroll
+      for (int e = 1; e < 8; ++e) least = fminf(least, __builtin_fabsf(vr[n][e]));
+      if (least * scale < kFine)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (vr[n][e] != 0.f && __builtin_fabsf(vr[n][e]) * scale < kFine) uneven = 1;
       f16x8 p[2];
       pairs8(vr[n], scale, p[0], p[1]);
 #pragma unroll

@@ -151,3 +151,17 @@ def test_a_dead_channel_costs_little_more(hip):
         keep = R.rng(4).integers(0, h * w, 100)
         check(got[:, keep], *R.attend(cfg, q[:, keep], k, v, blocks[:, keep], h, w, kd ** -0.5))
     assert took[1] < 5 * took[0]
+
+
+@pytest.mark.parametrize("hd", [4, 12, 64])
+@pytest.mark.parametrize("bw", [3, 64])
+def test_uneven_channels_and_uneven_keys(hip, hd, bw):
+    """A channel 2^-41 of the others, which a few keys have hardly anything of: these keys' rows are scaled up, and the small
+    channel of the other keys is as precise as without them."""
+    cfg, kd, w = R.shape(2, 1, 1, bw, 9, causal=1), 20, 8 * bw + 2
+    q, k, v = tensors(2, 700, w, cfg, kd, hd, 5)
+    v[..., 1] *= np.float32(2.0 ** -41)
+    v[..., [0, *range(2, hd)]] *= np.where(np.arange(w) % 7 == 3, np.float32(2.0 ** -16), np.float32(1))[:, None, None]
+    blocks = choice(2, 700, cfg, 1, w, 8, 0.0)
+    exp, bound = R.attend(cfg, q, k, v, blocks, 1, w, kd ** -0.5, (0, 30))
+    check(run(hip, cfg, q, k, v, blocks, 1, w, starts=(0, 30), sort=True), exp, bound)
