@@ -411,6 +411,57 @@ int sy_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor*
                        const sy_tensor* v, const int32_t* blocks, const int32_t* starts, const int32_t* lengths,
                        const sy_tensor* o);
 
+/* Normalisation, cross attention and the gated half of a feed-forward block: a
+ * decoder's layer, with sy_conv_run (1x1, residual) for its plain projections.
+ * No counterpart in the reference, whose networks fold batch norm into
+ * convolutions and attend to their own map only; for heads and necks whose
+ * queries or pixels look at other states (a text, an encoder's map). */
+#define SY_ACT_NONE 0
+#define SY_ACT_SILU 1
+#define SY_ACT_GELU 2      /* x (1 + erf(x / sqrt 2)) / 2 */
+#define SY_ACT_GELU_TANH 3 /* x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2 */
+#define SY_ACT_RELU 4
+#define SY_ACT_SIGMOID 5
+/* y = act((x - mean) / sqrt(var + eps) * gamma + beta): mean and (biased)
+ * variance over the pixels of an image and the c / groups neighbouring channels
+ * of a group, summed in 64 bits.  gamma and beta: device, c floats each, or
+ * NULL.  One group over views one pixel high and wide (n tokens) is the layer
+ * norm of each token.  y may be x itself; other overlaps are refused. */
+int sy_group_norm(sy_ctx* ctx, const sy_tensor* x, int groups, const float* gamma, const float* beta, float eps,
+                  int act, const sy_tensor* y);
+
+/* Attention of each pixel of q to the states of k and v, maps or rows of another
+ * size: o = softmax(scale q k^T) v, head by head; heads / kv_heads neighbours
+ * share a key head.  Image b's first lengths[b] states are visible (device, or
+ * NULL: all; taken between 0 and h*w of k), and of those the ones whose mask
+ * byte is not 0.  A query without a visible state gets zeros; states that a
+ * query does not see are not read into its result, whatever they hold.  o is a
+ * view of heads * head_dim channels on q's map and overlaps no input.  Products
+ * are formed as in sy_attention's fused kernel ("Precision"), sums over the
+ * states in float32. */
+typedef struct sy_cross_config {
+  int32_t heads, kv_heads;   /* heads % kv_heads == 0 */
+  int32_t key_dim, head_dim; /* channels of a query or key head, of a value head: multiples of 4 up to 128 */
+  int32_t q_stride, k_stride, v_stride; /* channels from a head to the next (0: dense) */
+  float scale;
+} sy_cross_config;
+/* A byte for each state of k: at data + image * b + head * h + query * i + state
+ * (device; strides in bytes, 0 where all share them). */
+typedef struct sy_key_mask {
+  const uint8_t* data;
+  int64_t image, head, query;
+} sy_key_mask;
+int sy_cross_attention(sy_ctx* ctx, const sy_cross_config* cfg, const sy_tensor* q, const sy_tensor* k,
+                       const sy_tensor* v, const int32_t* lengths, const sy_key_mask* mask, const sy_tensor* o);
+
+/* The two projections of a gated feed-forward block, its activation and their
+ * product: y = act(x gate^T + gate_bias) * (x up^T + up_bias), pixel by pixel.
+ * Weights (host, [oc][ic]) are packed once, as sy_conv_create does; biases
+ * (host, oc) may be NULL.  The handle lives as long as the context. */
+int sy_gated_create(sy_ctx* ctx, const float* gate, const float* up, const float* gate_bias, const float* up_bias,
+                    int oc, int ic, int act, uint64_t* gated);
+int sy_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tensor* y);
+
 /* Per-instance mask geometry returned by sy_mask_decode: the crop in source
  * pixels and the offset (in floats) of its width*height probabilities in the
  * output buffer. */

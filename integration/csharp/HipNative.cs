@@ -40,6 +40,12 @@ internal struct SyRotaryHeads { public SyTensor X, Y; public int Heads, XStride,
 [StructLayout(LayoutKind.Sequential)]
 internal struct SyBlockConfig { public int Heads, KvHeads, KeyDim, HeadDim, QStride, KStride, VStride, BlockH, BlockW, Selected, Causal; public float Scale; }
 
+[StructLayout(LayoutKind.Sequential)]
+internal struct SyCrossConfig { public int Heads, KvHeads, KeyDim, HeadDim, QStride, KStride, VStride; public float Scale; }
+
+[StructLayout(LayoutKind.Sequential)]
+internal struct SyKeyMask { public nint Data; public long Image, Head, Query; }
+
 internal static unsafe partial class HipNative
 {
     private const string Lib = "simdyolo_hip";
@@ -105,6 +111,17 @@ internal static unsafe partial class HipNative
     internal static partial int BlockSelect(nint ctx, in SyBlockConfig cfg, in SyTensor q, in SyTensor means, nint starts, nint lengths, nint blocks);
     [LibraryImport(Lib, EntryPoint = "sy_block_attention")]
     internal static partial int BlockAttention(nint ctx, in SyBlockConfig cfg, in SyTensor q, in SyTensor k, in SyTensor v, nint blocks, nint starts, nint lengths, in SyTensor o);
+
+    // ------------------------------------------------------------ normalisation, cross attention, gated projections
+    // (no counterpart in the reference; see include/simdyolo_hip.h); pointers but the weights' are device memory.
+    [LibraryImport(Lib, EntryPoint = "sy_group_norm")]
+    internal static partial int GroupNorm(nint ctx, in SyTensor x, int groups, nint gamma, nint beta, float eps, int act, in SyTensor y);
+    [LibraryImport(Lib, EntryPoint = "sy_cross_attention")]
+    internal static partial int CrossAttention(nint ctx, in SyCrossConfig cfg, in SyTensor q, in SyTensor k, in SyTensor v, nint lengths, SyKeyMask* mask, in SyTensor o);
+    [LibraryImport(Lib, EntryPoint = "sy_gated_create")]
+    internal static partial int GatedCreate(nint ctx, float* gate, float* up, float* gateBias, float* upBias, int oc, int ic, int act, out ulong gated);
+    [LibraryImport(Lib, EntryPoint = "sy_gated_run")]
+    internal static partial int GatedRun(nint ctx, ulong gated, in SyTensor x, in SyTensor y);
 
     // ------------------------------------------------------------ generic device ops
     // IDeviceBackend.Compute: one tensor.comp operation; inputs[3] / lengths[3] are the A, B, D bindings.

@@ -18,6 +18,7 @@ LAYOUT_NHWC, LAYOUT_NCHW = 0, 1
 CONV_AUTO, CONV_IGEMM, CONV_WINOGRAD, CONV_DIRECT, CONV_WINOGRAD3, CONV_DEPTHWISE, CONV_WINOGRAD2 = range(7)
 ARCH_YOLOV8, ARCH_YOLO11, ARCH_YOLO26 = 0, 1, 2
 ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_PARTS = range(4)
+ACT_NONE, ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_RELU, ACT_SIGMOID = range(6)
 
 # Every exported symbol declared in include/simdyolo_hip.h.
 EXPORTS = (
@@ -30,6 +31,7 @@ EXPORTS = (
     "sy_e2e_topk_noalloc",
     "sy_mask_decode", "sy_attention", "sy_compute", "sy_matmul",
     "sy_rotary_create", "sy_rotary_run", "sy_block_means", "sy_block_select", "sy_block_attention",
+    "sy_group_norm", "sy_cross_attention", "sy_gated_create", "sy_gated_run",
     "sy_graph_begin", "sy_graph_end", "sy_graph_launch", "sy_graph_destroy",
     "sy_timer_start", "sy_timer_stop", "sy_profile_enable", "sy_profile_read",
     "sy_model_layout", "sy_model_create", "sy_model_destroy", "sy_model_output_shape", "sy_model_predict_raw",
@@ -105,6 +107,17 @@ class BlockConfig(ctypes.Structure):
         [("scale", ctypes.c_float)]
 
 
+class CrossConfig(ctypes.Structure):
+    _fields_ = [(f, ctypes.c_int32) for f in ("heads", "kv_heads", "key_dim", "head_dim", "q_stride", "k_stride",
+                                              "v_stride")] + [("scale", ctypes.c_float)]
+
+
+class KeyMask(ctypes.Structure):
+    """A byte for each state of the keys; strides in bytes (0 where images, heads or queries share them)."""
+    _fields_ = [("data", ctypes.c_void_p), ("image", ctypes.c_int64), ("head", ctypes.c_int64),
+                ("query", ctypes.c_int64)]
+
+
 class DecodeOptions(ctypes.Structure):
     _fields_ = [("confidence", ctypes.c_float), ("iou", ctypes.c_float), ("max_detections", ctypes.c_int32),
                 ("max_candidates", ctypes.c_int32), ("class_count", ctypes.c_int32),
@@ -158,6 +171,10 @@ _SIGS = {
     "sy_attention": (_i, [_vp, _tp, _i, _i, _i, _f, _tp, _tp]),
     "sy_rotary_create": (_i, [_vp, ctypes.POINTER(RotaryConfig), _u64p]),
     "sy_rotary_run": (_i, [_vp, ctypes.c_uint64, ctypes.POINTER(RotaryHeads), _i, _vp]),
+    "sy_group_norm": (_i, [_vp, _tp, _i, _vp, _vp, _f, _i, _tp]),
+    "sy_cross_attention": (_i, [_vp, ctypes.POINTER(CrossConfig), _tp, _tp, _tp, _vp, ctypes.POINTER(KeyMask), _tp]),
+    "sy_gated_create": (_i, [_vp, _fp, _fp, _fp, _fp, _i, _i, _i, _u64p]),
+    "sy_gated_run": (_i, [_vp, ctypes.c_uint64, _tp, _tp]),
     "sy_block_means": (_i, [_vp, _bp, _tp, _vp, _i, _vp, _tp]),
     "sy_block_select": (_i, [_vp, _bp, _tp, _tp, _vp, _vp, _vp]),
     "sy_block_attention": (_i, [_vp, _bp, _tp, _tp, _tp, _vp, _vp, _vp, _tp]),

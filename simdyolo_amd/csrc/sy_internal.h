@@ -63,6 +63,7 @@ std::shared_timed_mutex& capture_lock();
 
 struct ConvPlan;
 struct RotaryPlan;
+struct GatedPlan;
 
 enum Algo { kAuto = 0, kIgemm = 1, kWinograd = 2, kDirect = 3, kWinograd3 = 4, kDepthwise = 5, kWinograd2 = 6 };
 
@@ -101,6 +102,7 @@ struct sy_ctx {
   std::vector<void*> owned;
   std::vector<std::unique_ptr<sy::ConvPlan>> convs;
   std::vector<std::shared_ptr<const sy::RotaryPlan>> rotaries;
+  std::vector<std::shared_ptr<const sy::GatedPlan>> gateds;
   // scratch (Winograd transforms, staging); grows outside capture only
   char* scratch = nullptr;
   size_t scratch_size = 0;
@@ -336,6 +338,15 @@ int op_block_select(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q,
 int op_block_attention(sy_ctx* ctx, const sy_block_config* cfg, const sy_tensor* q, const sy_tensor* k,
                        const sy_tensor* v, const int32_t* blocks, const int32_t* starts, const int32_t* lengths,
                        const sy_tensor* o);
+
+int op_group_norm(sy_ctx* ctx, const sy_tensor* x, int groups, const float* gamma, const float* beta, float eps,
+                  int act, const sy_tensor* y);
+int op_cross_attention(sy_ctx* ctx, const sy_cross_config* cfg, const sy_tensor* q, const sy_tensor* k,
+                       const sy_tensor* v, const int32_t* lengths, const sy_key_mask* mask, const sy_tensor* o);
+
+int op_gated_create(sy_ctx* ctx, const float* gate, const float* up, const float* gate_bias, const float* up_bias,
+                    int oc, int ic, int act, uint64_t* gated);
+int op_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tensor* y);
 
 int64_t pool_out_size(int len, int k, int s, int before, int after, int ceil_mode);
 

@@ -189,6 +189,35 @@ class HipContext:
         check(self._lib.sy_block_attention(self.handle, ctypes.byref(cfg), ctypes.byref(q), ctypes.byref(k),
                                            ctypes.byref(v), blocks_ptr, starts, lengths, ctypes.byref(o)))
 
+    def group_norm(self, x: Tensor, y: Tensor, groups: int, gamma: int | None = None, beta: int | None = None,
+                   eps: float = 1e-5, act: int = N.ACT_NONE):
+        """gamma and beta are device pointers to x.c floats."""
+        check(self._lib.sy_group_norm(self.handle, ctypes.byref(x), groups, gamma, beta, eps, act, ctypes.byref(y)))
+
+    def cross_attention(self, cfg: N.CrossConfig, q: Tensor, k: Tensor, v: Tensor, o: Tensor,
+                        lengths: int | None = None, mask: N.KeyMask | None = None):
+        """`lengths` is a device pointer to int32 [n]."""
+        check(self._lib.sy_cross_attention(self.handle, ctypes.byref(cfg), ctypes.byref(q), ctypes.byref(k),
+                                           ctypes.byref(v), lengths, ctypes.byref(mask) if mask is not None else None,
+                                           ctypes.byref(o)))
+
+    def gated_create(self, gate, up, gate_bias=None, up_bias=None, act: int = N.ACT_SILU) -> int:
+        """Weights [oc][ic] of the two projections, and their biases."""
+        gate, up, gate_bias, up_bias = (None if a is None else np.ascontiguousarray(a, dtype=np.float32)
+                                        for a in (gate, up, gate_bias, up_bias))
+        if gate.ndim != 2 or up.shape != gate.shape or any(b is not None and b.shape != gate.shape[:1]
+                                                           for b in (gate_bias, up_bias)):
+            raise ValueError("gated projections differ in shape")
+        h = ctypes.c_uint64()
+        check(self._lib.sy_gated_create(self.handle, fptr(gate), fptr(up),
+                                        fptr(gate_bias) if gate_bias is not None else None,
+                                        fptr(up_bias) if up_bias is not None else None, *gate.shape, act,
+                                        ctypes.byref(h)))
+        return h.value
+
+    def gated(self, gated: int, x: Tensor, y: Tensor):
+        check(self._lib.sy_gated_run(self.handle, gated, ctypes.byref(x), ctypes.byref(y)))
+
     def compute(self, op: int, inputs, params, work_items: int, out_ptr: int, out_len: int):
         """One tensor.comp op. `inputs` holds up to three (device_ptr, length_in_floats) pairs or None for
         the A, B and D bindings; `params` up to 32 uint32 slots (floats passed as their bit pattern)."""
