@@ -223,19 +223,19 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : 2) void cross_kernel(const C
       const unsigned some = seen[0] | seen[1] | seen[2] | seen[3];
       any |= some;
       if (__any(some != 0)) {
-        f32x16 s, c;
+        f32x16 s;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = c[r] = 0.f;
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           bf16x8 kp[3];
 #pragma unroll
           for (int p = 0; p < 3; ++p)
             kp[p] = __builtin_bit_cast(bf16x8, f[(ks * 3 + p) * 64 + half * 32 + (r32 ^ (2 * ks + half))]);
-          mfma_parts(kp, q[ks], s, c);
-        }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] += c[r];
+          for (int x = 0; x < 6; ++x)
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kp[kPairA[x]], q[ks][kPairB[x]], s, 0, 0, 0);
+        }
         if (mask) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
@@ -271,19 +271,19 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : 2) void cross_kernel(const C
         lrun += sum;
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-          bf16x8 p[3], vp[DT][3];
+          bf16x8 p[3];
           parts8(f32x4{s[8 * st], s[8 * st + 1], s[8 * st + 2], s[8 * st + 3]},
                  f32x4{s[8 * st + 4], s[8 * st + 5], s[8 * st + 6], s[8 * st + 7]}, p);
 #pragma unroll
-          for (int d = 0; d < DT; ++d)
+          for (int d = 0; d < DT; ++d) {
+            bf16x8 vp[3];
 #pragma unroll
             for (int x = 0; x < 3; ++x)
-              vp[d][x] = __builtin_bit_cast(bf16x8, f[KU * 3 + ((st * DT + d) * 3 + x) * 64 + lane]);
+              vp[x] = __builtin_bit_cast(bf16x8, f[KU * 3 + ((st * DT + d) * 3 + x) * 64 + lane]);
 #pragma unroll
-          for (int x = 0; x < 6; ++x)
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-              acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vp[d][kPairA[x]], p[kPairB[x]], acc[d], 0, 0, 0);
+            for (int x = 0; x < 6; ++x)
+              acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vp[kPairA[x]], p[kPairB[x]], acc[d], 0, 0, 0);
+          }
         }
       }
       if (more) stage(frag + (now ^ 1) * (KU + VU) * 3);
@@ -448,11 +448,12 @@ int op_cross_attention(sy_ctx* ctx, const sy_cross_config* c, const sy_tensor* q
   a.c = c->scale * 1.4426950408889634f;
   a.rows = a.tq * a.group;
   const long long planes = (long long)q->n * a.kv;
-  const int nw = a.rows <= 64 ? 1 : 4;
+  static const int kNw = getenv("NW") ? atoi(getenv("NW")) : 0;
+  const int nw = a.rows <= 64 ? 1 : kNw ? kNw : a.rows <= 128 ? 4 : 8;
   a.tiles = (a.rows + 32 * nw - 1) / (32 * nw);
   const long long whole = planes * a.tiles;
   // Pieces: where the rows alone leave CUs without work, of four tiles and more.
-  const long long want = (nw == 1 ? 2048 : 768) / whole;
+  const long long want = (nw == 1 ? 2048 : nw == 4 ? 768 : 384) / whole;
   a.splits = (int)std::max<long long>(1, std::min<long long>(want, a.tk / (4 * kCrossKeys)));
   a.piece = ((a.tk + a.splits - 1) / a.splits + kCrossKeys - 1) / kCrossKeys * kCrossKeys;
   a.splits = (a.tk + a.piece - 1) / a.piece;
@@ -471,7 +472,7 @@ int op_cross_attention(sy_ctx* ctx, const sy_cross_config* c, const sy_tensor* q
     const double scores = (double)q->n * a.heads * a.tq * a.tk;
     ProfScope prof(ctx, "cross_attention", 2 * scores * (a.kd + a.hd),
                    4.0 * q->n * ((double)a.tq * a.heads + (double)a.tk * a.kv) * (a.kd + a.hd));
-    CrossKernel kernel = nw == 1 ? pick_cross<1>(a.kd, a.hd) : pick_cross<4>(a.kd, a.hd);
+    CrossKernel kernel = nw == 1 ? pick_cross<1>(a.kd, a.hd) : nw == 4 ? pick_cross<4>(a.kd, a.hd) : pick_cross<8>(a.kd, a.hd);
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(nw * 64), 0, ctx->stream, a);
     SY_TRY(check_launch("cross_attention"));
   }

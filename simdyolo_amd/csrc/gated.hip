@@ -64,19 +64,22 @@ __device__ __forceinline__ bool uneven(unsigned largest, unsigned smallest) {
   return e == 255 || (smallest != 0x7fffffffu && (int)(smallest >> 23) < e + kUneven && smallest != 0);
 }
 
-// Eight elements from `at`, zeros from `end` on.
+// Eight elements of a row of `end` from `at`, zeros from `end` on.
 __device__ __forceinline__ void load8(const float* row, int at, int end, bool quads, float (&v)[8]) {
-  if (quads && at + 8 <= end) {
-    const f32x4 a = *(const f32x4*)(row + at), b = *(const f32x4*)(row + at + 4);
+  if (quads) {  // end is a multiple of 4
+    const f32x4 a = *(const f32x4*)(row + min(at, end - 4)), b = *(const f32x4*)(row + min(at + 4, end - 4));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[e] = a[e];
       v[4 + e] = b[e];
     }
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = at + e < end ? row[at + e] : 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = row[min(at + e, end - 1)];
+  }
+  if (at + 8 > end)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = at + e < end ? v[e] : 0.f;
 }
 
 __device__ __forceinline__ void pair8(const float (&x)[8], float s, u32x4& h, u32x4& l) {
@@ -90,58 +93,71 @@ __device__ __forceinline__ void pair8(const float (&x)[8], float s, u32x4& h, u3
   }
 }
 
-// A panel of 32 rows per workgroup, 8 lanes to a row: its largest element, then its
-// pairs.  Rows past the last are zeros.
-__global__ __launch_bounds__(256) void gated_split_kernel(const float* x, long long ldx, int rows, int ic, int steps,
+// A panel of 32 rows per workgroup, 16 lanes to a row: its largest element, then its
+// pairs; the first kHeld octets of a lane stay in registers between.  Rows past the last are zeros.
+// `more`: the panel's flag is that of an earlier call, too.
+constexpr int kHeld = 2;
+__global__ __launch_bounds__(512) void gated_split_kernel(const float* x, long long ldx, int rows, int ic, int steps,
                                                           bool quads, u32x4* out, int* words, int* plain, int stride,
-                                                          int offset) {
+                                                          int offset, bool more) {
   __shared__ int any;
-  const int r = threadIdx.x >> 3, q = threadIdx.x & 7;
+  const int r = threadIdx.x >> 4, q = threadIdx.x & 15;
   const long long row = (long long)blockIdx.x * 32 + r;
   const long long panel = (long long)blockIdx.x * stride + offset;
   const float* xr = x + min(row, (long long)rows - 1) * ldx;
-  const int end = row < rows ? ic : 0;
-  if (threadIdx.x == 0) any = 0;
+  if (threadIdx.x == 0) any = more ? plain[blockIdx.x] : 0;
   __syncthreads();
   unsigned top = 0, low = 0x7fffffffu;
-  for (int o = q; o < 2 * steps; o += 8) {
-    float v[8];
-    load8(xr, 8 * o, end, quads, v);
+  float held[kHeld][8];
+  auto look = [&](const float(&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const unsigned m = magnitude(v[e]);
       top = max(top, m);
       low = min(low, m ? m : 0x7fffffffu);
     }
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (q + 16 * i < 2 * steps) load8(xr, 8 * (q + 16 * i), ic, quads, held[i]);
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (q + 16 * i < 2 * steps) look(held[i]);
+  for (int o = q + 16 * kHeld; o < 2 * steps; o += 16) {
+    float v[8];
+    load8(xr, 8 * o, ic, quads, v);
+    look(v);
   }
 #pragma unroll
-  for (int off = 1; off < 8; off <<= 1) {
+  for (int off = 1; off < 16; off <<= 1) {
     top = max(top, (unsigned)__shfl_xor((int)top, off));
     low = min(low, (unsigned)__shfl_xor((int)low, off));
   }
+  if (row >= rows) top = 0, low = 0x7fffffffu;
   const bool bad = uneven(top, low);
   const int field = bad && top >> 23 == 255 ? 127 : gated_field(top);
   if (q == 0) {
     words[panel * 32 + r] = field | (bad ? kPlainRow : 0);
     if (bad) any = 1;
   }
-  const float s = exp_float(field);
+  const float s = row < rows ? exp_float(field) : 0.f;
   u32x4* to = out + panel * steps * kStep;
-  for (int o = q; o < 2 * steps; o += 8) {
-    float v[8];
-    load8(xr, 8 * o, end, quads, v);
+  auto put = [&](int o, const float(&v)[8]) {
     u32x4 h, l;
     pair8(v, s, h, l);
     to[(o >> 1) * kStep + (o & 1) * 32 + r] = h;
     to[(o >> 1) * kStep + 64 + (o & 1) * 32 + r] = l;
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (q + 16 * i < 2 * steps) put(q + 16 * i, held[i]);
+  for (int o = q + 16 * kHeld; o < 2 * steps; o += 16) {
+    float v[8];
+    load8(xr, 8 * o, ic, quads, v);
+    put(o, v);
   }
   __syncthreads();
-  if (threadIdx.x == 0 && any) plain[blockIdx.x] = 1;
-}
-
-__global__ void gated_clear_kernel(int* p, int n) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i < n) p[i] = 0;
+  if (threadIdx.x == 0) plain[blockIdx.x] = any;
 }
 
 // Four weights of output channel `col` (gate or up) from input channel k.
@@ -291,88 +307,143 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_kernel(const GatedArgs a
   }
 }
 
-// Few rows (up to 32): 32 output channels to a workgroup, the steps shared out over
-// its waves, weights straight from memory into the matrix instruction's
-// registers.  A wave splits its own share of x, under powers of its own, and is plain by itself.
-constexpr int kFewWaves = 8;
-__global__ __launch_bounds__(kFewWaves * 64) void gated_few_kernel(const GatedArgs a) {
-  __shared__ float sums[kFewWaves][2][32][33];
+// Few tiles: TM panels of rows and 32 output channels to a workgroup, the steps shared
+// out over its NK waves, both operands straight from memory into the matrix
+// instruction's registers, kAhead steps of them under way.  A wave splits its own share of x,
+// under powers of that share's rows, and is plain by itself.
+constexpr int kAhead = 4;
+template <int TM, int NK>
+__global__ __launch_bounds__(NK * 64) void gated_few_kernel(const GatedArgs a) {
+  __shared__ float sums[NK][2][TM * 32][33];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int half = lane >> 5, r32 = lane & 31, panel = blockIdx.x;
-  const int share = (a.steps + kFewWaves - 1) / kFewWaves, k0 = min(wave * share, a.steps), k1 = min(k0 + share, a.steps);
+  const int half = lane >> 5, r32 = lane & 31;
+  const int tile = blockIdx.x / a.panels, panel = blockIdx.x - tile * a.panels, row0 = tile * TM * 32;
+  const int share = (a.steps + NK - 1) / NK, k0 = min(wave * share, a.steps), k1 = min(k0 + share, a.steps);
   const u32x4* w = a.w + (long long)2 * panel * a.steps * kStep + lane;
   const long long up = (long long)a.steps * kStep;
-  const float* xr = a.x + min(r32, a.rows - 1) * a.ldx;
-  const int end = r32 < a.rows ? a.ic : 0;
-  f32x16 acc[2], crs[2];
+  const int w_plain = a.w_plain[panel];
+  const float* xr[TM];
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int i = 0; i < TM; ++i) xr[i] = a.x + (long long)min(row0 + 32 * i + r32, a.rows - 1) * a.ldx;
+  f16x8 wv[kAhead][2][2];
+  float xv[kAhead][TM][8];
+  auto load_w = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) acc[j][r] = crs[j][r] = 0.f;
-  unsigned top = 0, low = 0x7fffffffu;
-  for (int k = k0; k < k1; ++k) {
-    float v[8];
-    load8(xr, 16 * k + 8 * half, end, a.quads, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const unsigned m = magnitude(v[e]);
-      top = max(top, m);
-      low = min(low, m ? m : 0x7fffffffu);
-    }
-  }
-  top = max(top, (unsigned)__shfl_xor((int)top, 32));
-  low = min(low, (unsigned)__shfl_xor((int)low, 32));
-  const bool plain = __any(uneven(top, low)) || a.w_plain[panel];
-  const int field = gated_field(top);
-  if (plain) {
-    gated_plain(a, 0, panel, k0, k1, lane, acc);
-  } else {
-    const float s = exp_float(field);
-#pragma unroll 4
-    for (int k = k0; k < k1; ++k) {
-      f16x8 b[2][2], xv[2];
+    for (int u = 0; u < kAhead; ++u)
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int p = 0; p < 2; ++p) b[j][p] = __builtin_bit_cast(f16x8, w[j * up + (long long)k * kStep + 64 * p]);
-      float v[8];
-      load8(xr, 16 * k + 8 * half, end, a.quads, v);
-      u32x4 h, l;
-      pair8(v, s, h, l);
-      xv[0] = __builtin_bit_cast(f16x8, h);
-      xv[1] = __builtin_bit_cast(f16x8, l);
+        for (int p = 0; p < 2; ++p)
+          wv[u][j][p] = __builtin_bit_cast(f16x8, w[j * up + (long long)min(k + u, a.steps - 1) * kStep + 64 * p]);
+  };
+  auto load_x = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        crs[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xv[1], b[j][0], crs[j], 0, 0, 0);
-        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xv[0], b[j][0], acc[j], 0, 0, 0);
-        crs[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xv[0], b[j][1], crs[j], 0, 0, 0);
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int i = 0; i < TM; ++i) load8(xr[i], min(k + u, a.steps) * 16 + 8 * half, a.ic, a.quads, xv[u][i]);
+  };
+  f32x16 acc[TM][2], crs[TM][2];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = crs[i][j][r] = 0.f;
+  unsigned top[TM] = {}, low[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) low[i] = 0x7fffffffu;
+  if (k0 < k1) {
+    load_w(k0);
+    // The share's largest and smallest elements, from behind, so that its first steps stay in registers.
+    for (int k = k0 + (k1 - k0 - 1) / kAhead * kAhead; k >= k0; k -= kAhead) {
+      load_x(k);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const unsigned m = k + u < k1 ? magnitude(xv[u][i][e]) : 0;
+            top[i] = max(top[i], m);
+            low[i] = min(low[i], m ? m : 0x7fffffffu);
+          }
+    }
+  }
+  bool plain = w_plain != 0;
+  int field[TM];
+  float scale[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    top[i] = max(top[i], (unsigned)__shfl_xor((int)top[i], 32));
+    low[i] = min(low[i], (unsigned)__shfl_xor((int)low[i], 32));
+    plain |= uneven(top[i], low[i]);
+    field[i] = gated_field(top[i]);
+    scale[i] = exp_float(field[i]);
+  }
+  if (__any(plain)) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) gated_plain(a, row0 + 32 * i, panel, k0, k1, lane, acc[i]);
+  } else {
+    for (int k = k0; k < k1; k += kAhead) {
+      f16x8 xp[kAhead][TM][2], wp[kAhead][2][2];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          u32x4 h, l;
+          pair8(xv[u][i], k + u < k1 ? scale[i] : 0.f, h, l);
+          xp[u][i][0] = __builtin_bit_cast(f16x8, h);
+          xp[u][i][1] = __builtin_bit_cast(f16x8, l);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) wp[u][j][p] = wv[u][j][p];
       }
+      if (k + kAhead < k1) {
+        load_w(k + kAhead);
+        load_x(k + kAhead);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            crs[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xp[u][i][1], wp[u][j][0], crs[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xp[u][i][0], wp[u][j][0], acc[i][j], 0, 0, 0);
+            crs[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xp[u][i][0], wp[u][j][1], crs[i][j], 0, 0, 0);
+          }
     }
     // Lane r's field is that of row r.
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int ww = a.w_row[panel * 64 + 32 * j + r32] & 0xff;
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int f = __shfl(field, 8 * (r >> 2) + 4 * half + (r & 3));
-        acc[j][r] = __builtin_ldexpf(__builtin_fmaf(crs[j][r], 1.f / 2048, acc[j][r]), 254 - f - ww);
+        const int f = __shfl(field[i], 8 * (r >> 2) + 4 * half + (r & 3));
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          acc[i][j][r] = __builtin_ldexpf(__builtin_fmaf(crs[i][j][r], 1.f / 2048, acc[i][j][r]),
+                                          254 - f - (a.w_row[panel * 64 + 32 * j + r32] & 0xff));
       }
-    }
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sums[wave][j][8 * (r >> 2) + 4 * half + (r & 3)][r32] = acc[j][r];
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sums[wave][j][32 * i + 8 * (r >> 2) + 4 * half + (r & 3)][r32] = acc[i][j][r];
   __syncthreads();
-  for (int i = threadIdx.x; i < a.rows * 32; i += kFewWaves * 64) {
-    const int row = i >> 5, c = i & 31, col = 32 * panel + c;
+  const int rows = min(TM * 32, a.rows - row0), col = 32 * panel + r32;
+  const float gb = a.bias[col], ub = a.bias[a.panels * 32 + col];
+  for (int row = threadIdx.x >> 5; row < rows; row += NK * 2) {
     float g = 0.f, u = 0.f;
 #pragma unroll
-    for (int x = 0; x < kFewWaves; ++x) {
-      g += sums[x][0][row][c];
-      u += sums[x][1][row][c];
+    for (int x = 0; x < NK; ++x) {
+      g += sums[x][0][row][r32];
+      u += sums[x][1][row][r32];
     }
-    if (col < a.oc) a.y[row * a.ldy + col] = activate(a.act, g + a.bias[col]) * (u + a.bias[a.panels * 32 + col]);
+    if (col < a.oc) a.y[(row0 + row) * a.ldy + col] = activate(a.act, g + gb) * (u + ub);
   }
 }
 
@@ -395,11 +466,9 @@ static int gated_pack(sy_ctx* ctx, const float* gate, const float* up, const flo
   SY_TRY(sy_memcpy(ctx, p->raw, gate, values * sizeof(float), 0));
   SY_TRY(sy_memcpy(ctx, p->raw + values, up, values * sizeof(float), 0));
   SY_TRY(sy_memcpy(ctx, p->bias, bias.data(), 2 * cols * sizeof(float), 0));
-  hipLaunchKernelGGL(gated_clear_kernel, dim3((p->panels + 255) / 256), dim3(256), 0, ctx->stream, p->w_plain, p->panels);
   for (int m = 0; m < 2; ++m)
-    hipLaunchKernelGGL(gated_split_kernel, dim3(p->panels), dim3(256), 0, ctx->stream, p->raw + m * values,
-                       (long long)p->ic, p->oc, p->ic, p->steps, p->ic % 4 == 0 && values % 4 == 0, p->w, p->w_row,
-                       p->w_plain, 2, m);
+    hipLaunchKernelGGL(gated_split_kernel, dim3(p->panels), dim3(512), 0, ctx->stream, p->raw + m * values,
+                       (long long)p->ic, p->oc, p->ic, p->steps, p->ic % 4 == 0, p->w, p->w_row, p->w_plain, 2, m, m == 1);
   SY_TRY(check_launch("gated_split"));
   std::vector<int> plain;
   try {
@@ -487,13 +556,20 @@ int op_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tenso
   a.w_plain = p.w_plain;
   a.bias = p.bias;
   a.raw = p.raw;
-  a.quads = ((uintptr_t)x->data & 15) == 0 && x->ldc % 4 == 0;
+  // The last quad of a row must not pass the buffer's end.
+  a.quads = ((uintptr_t)x->data & 15) == 0 && x->ldc % 4 == 0 && p.ic % 4 == 0;
   a.xpanels = (a.rows + 31) / 32;
   DeviceScope device(ctx);
   const double flops = 4.0 * rows * p.ic * p.oc, bytes = 4.0 * ((double)rows * (p.ic + p.oc) + 2.0 * p.ic * p.oc);
-  if (a.rows <= 32) {
+  static const int kFew = getenv("FEW") ? atoi(getenv("FEW")) : 0;
+  if (a.rows <= 32 || kFew) {
     ProfScope prof(ctx, "gated_few", flops, bytes);
-    hipLaunchKernelGGL(gated_few_kernel, dim3(p.panels), dim3(kFewWaves * 64), 0, ctx->stream, a);
+    const int tm = kFew ? kFew / 10 : 1, nk = kFew ? kFew % 10 : 8;
+    const dim3 grid((unsigned)(p.panels * ((a.xpanels + tm - 1) / tm)));
+    if (tm == 1 && nk == 8) hipLaunchKernelGGL((gated_few_kernel<1, 8>), grid, dim3(nk * 64), 0, ctx->stream, a);
+    if (tm == 1 && nk == 4) hipLaunchKernelGGL((gated_few_kernel<1, 4>), grid, dim3(nk * 64), 0, ctx->stream, a);
+    if (tm == 2 && nk == 4) hipLaunchKernelGGL((gated_few_kernel<2, 4>), grid, dim3(nk * 64), 0, ctx->stream, a);
+    if (tm == 2 && nk == 8) hipLaunchKernelGGL((gated_few_kernel<2, 8>), grid, dim3(nk * 64), 0, ctx->stream, a);
     return check_launch("gated_few");
   }
   size_t at = 0;
@@ -512,9 +588,8 @@ int op_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tenso
   a.x_plain = x_plain;
   {
     ProfScope prof(ctx, "gated_split", 0, 8.0 * rows * p.ic);
-    hipLaunchKernelGGL(gated_clear_kernel, dim3((a.xpanels + 255) / 256), dim3(256), 0, ctx->stream, x_plain, a.xpanels);
-    hipLaunchKernelGGL(gated_split_kernel, dim3(a.xpanels), dim3(256), 0, ctx->stream, a.x, a.ldx, a.rows, a.ic, a.steps,
-                       a.quads, xs, x_row, x_plain, 1, 0);
+    hipLaunchKernelGGL(gated_split_kernel, dim3(a.xpanels), dim3(512), 0, ctx->stream, a.x, a.ldx, a.rows, a.ic, a.steps,
+                       a.quads, xs, x_row, x_plain, 1, 0, false);
     SY_TRY(check_launch("gated_split"));
   }
   ProfScope prof(ctx, "gated", flops, bytes);

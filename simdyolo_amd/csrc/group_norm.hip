@@ -21,13 +21,14 @@ struct NormArgs {
   long long ldx, ldy;
   int n, t, c, groups, each;  // each: channels of a group
   int act;
-  double eps;
+  double eps, share;          // share: 1 / elements of a group
   // Runs of groups (columns of a workgroup) and pieces of the pixels.
   int run, runs, cols, rows;  // groups of a run, runs; columns (of VEC channels), pixels side by side
   int blocks;                 // a run is a group's share of columns: so many to a group (1: whole groups)
   int piece, pieces;
   int lanes;                  // rows_kernel: lanes of a group
   double2* sums;              // [n][groups][blocks][pieces]
+  float* pivot;               // [n][groups]
 };
 
 template <int VEC>
@@ -50,18 +51,21 @@ struct Moments {
   }
 };
 
-// Mean (in two floats) and 1 / sqrt(var + eps).
+// Mean (in two floats) and 1 / sqrt(var + eps): the hardware's estimate (2^-23 and
+// better) and one step of Newton's, where a library's division and root would
+// cost more than the rest of a token's work.
 struct Scale {
   float hi, lo, r;
 };
-__device__ __forceinline__ Scale scale_of(const NormArgs& a, const Moments& m, double p, double count) {
-  const double d = m.s / count, mean = p + d;
-  double var = m.q / count - d * d;
-  var = var < 0 ? 0 : var;  // NaN stays
+__device__ __forceinline__ Scale scale_of(const NormArgs& a, const Moments& m, double p) {
+  const double d = m.s * a.share, mean = p + d;
+  double var = __builtin_fma(m.q, a.share, -d * d);
+  var = (var < 0 ? 0 : var) + a.eps;  // NaN stays
+  const double e = __builtin_amdgcn_rsq(var);
   Scale s;
   s.hi = (float)mean;
   s.lo = __builtin_fabsf(s.hi) < INFINITY ? (float)(mean - (double)s.hi) : 0.f;
-  s.r = (float)(1.0 / sqrt(var + a.eps));
+  s.r = (float)(e * __builtin_fma(-0.5 * var * e, e, 1.5));
   return s;
 }
 
@@ -69,7 +73,25 @@ __device__ __forceinline__ float normal(const NormArgs& a, float x, const Scale&
   return activate(a.act, __builtin_fmaf((x - s.hi) - s.lo, s.r * g, b));
 }
 
-__device__ __forceinline__ double shuffle_xor(double v, int lane) { return __shfl_xor(v, lane); }
+// v plus that of the lane that DPP control ctrl reads.
+template <int ctrl>
+__device__ __forceinline__ double plus_dpp(double v) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)b, ctrl, 0xf, 0xf, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), ctrl, 0xf, 0xf, false);
+  return v + __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+
+// Sum over aligned groups of `lanes` (a power of two), in each of them.
+__device__ __forceinline__ double plus_lanes(double v, int lanes) {
+  if (lanes > 1) v = plus_dpp<0xb1>(v);   // lane ^ 1
+  if (lanes > 2) v = plus_dpp<0x4e>(v);   // lane ^ 2
+  if (lanes > 4) v = plus_dpp<0x141>(v);  // 7 - lane
+  if (lanes > 8) v = plus_dpp<0x140>(v);  // 15 - lane
+  if (lanes > 16) v += __shfl_xor(v, 16);
+  if (lanes > 32) v += __shfl_xor(v, 32);
+  return v;
+}
 
 // A group of an image by `lanes` neighbouring lanes, its elements in their
 // registers: small images, single tokens.
@@ -94,6 +116,15 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(const NormArgs a) {
     ch[i] = (u - px[i] * units) * VEC;
     v[i] = *(const vec*)(x + px[i] * a.ldx + ch[i]);
   }
+  vec ga[V], be[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int c = g * a.each + ch[i] + e;
+      ga[i][e] = a.gamma ? a.gamma[c] : 1.f;
+      be[i][e] = a.beta ? a.beta[c] : 0.f;
+    }
   const double p = (double)x[0];
   Moments m{0, 0};
 #pragma unroll
@@ -101,20 +132,15 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(const NormArgs a) {
     if (lane + i * lanes < total)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) m.add(v[i][e], p);
-  for (int off = 1; off < lanes; off <<= 1) {
-    m.s += shuffle_xor(m.s, off);
-    m.q += shuffle_xor(m.q, off);
-  }
-  const Scale s = scale_of(a, m, p, (double)a.t * a.each);
+  m.s = plus_lanes(m.s, lanes);
+  m.q = plus_lanes(m.q, lanes);
+  const Scale s = scale_of(a, m, p);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     if (!live || lane + i * lanes >= total) continue;
     vec o;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int c = g * a.each + ch[i] + e;
-      o[e] = normal(a, v[i][e], s, a.gamma ? a.gamma[c] : 1.f, a.beta ? a.beta[c] : 0.f);
-    }
+    for (int e = 0; e < VEC; ++e) o[e] = normal(a, v[i][e], s, ga[i][e], be[i][e]);
     *(vec*)(y + px[i] * a.ldy + ch[i]) = o;
   }
 }
@@ -134,11 +160,8 @@ __device__ __forceinline__ void meet(const NormArgs& a, const Moments& m, double
       s.s += red[at].x;
       s.q += red[at].y;
     }
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      s.s += shuffle_xor(s.s, off);
-      s.q += shuffle_xor(s.q, off);
-    }
+    s.s = plus_lanes(s.s, 64);
+    s.q = plus_lanes(s.q, 64);
     if (lane == 0) out[g] = s;
   }
   __syncthreads();
@@ -146,25 +169,32 @@ __device__ __forceinline__ void meet(const NormArgs& a, const Moments& m, double
 
 constexpr int kMaxRun = 256;  // groups of a run at most: one to a column of 256 threads and more
 
-// A run of groups of one image per workgroup, its elements in registers: a thread
-// stays with its column (VEC channels) and goes down the pixels.
-template <int VEC, int V>
-__global__ __launch_bounds__(1024) void norm_run_kernel(const NormArgs a) {
+// A group of one image per workgroup, its elements in registers: a thread stays with
+// its column (VEC channels) and goes down the pixels.  Neighbouring groups, which share
+// lines of memory where they have few channels, are neighbours on one XCD.
+constexpr int kGroupVec = 4;  // vectors that a thread holds
+template <int VEC>
+__global__ __launch_bounds__(1024) void norm_group_kernel(const NormArgs a) {
+  constexpr int V = kGroupVec;
   typedef typename Vec<VEC>::type vec;
-  __shared__ double2 red[1024];
-  __shared__ Moments total[kMaxRun];
-  __shared__ Scale scale[kMaxRun];
-  const int img = blockIdx.x / a.runs, g0 = (blockIdx.x - img * a.runs) * a.run;
-  const int groups = min(a.run, a.groups - g0), cols_each = a.each / VEC, cols = groups * cols_each;
-  const int row = threadIdx.x / a.cols, col = threadIdx.x - row * a.cols;
-  const bool live = row < a.rows && col < cols;
-  const int g = min(col / cols_each, groups - 1), c = g0 * a.each + min(col, cols - 1) * VEC;
+  __shared__ double2 red[16];
+  const unsigned item = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  if (item >= (unsigned)a.n * a.groups) return;
+  const int img = item / a.groups, g = item - img * a.groups;
+  const int row = threadIdx.x / a.cols, col = threadIdx.x - row * a.cols, c = g * a.each + col * VEC;
+  const bool live = row < a.rows;
   const float* x = a.x + (long long)img * a.t * a.ldx;
   float* y = a.y + (long long)img * a.t * a.ldy;
   vec v[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = *(const vec*)(x + min(row + i * a.rows, a.t - 1) * a.ldx + c);
-  const double p = (double)x[(g0 + g) * a.each];
+  const double p = (double)x[g * a.each];
+  float ga[VEC], be[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    ga[e] = a.gamma ? a.gamma[c + e] : 1.f;
+    be[e] = a.beta ? a.beta[c + e] : 0.f;
+  }
   Moments m{0, 0};
   if (live)
 #pragma unroll
@@ -172,17 +202,17 @@ __global__ __launch_bounds__(1024) void norm_run_kernel(const NormArgs a) {
       if (row + i * a.rows < a.t)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) m.add(v[i][e], p);
-  meet(a, m, red, cols_each, a.cols, groups, total);
-  if (live && row == 0 && col % cols_each == 0) scale[g] = scale_of(a, total[g], p, (double)a.t * a.each);
+  m.s = plus_lanes(m.s, 64);
+  m.q = plus_lanes(m.q, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_double2(m.s, m.q);
   __syncthreads();
-  if (!live) return;
-  const Scale s = scale[g];
-  float ga[VEC], be[VEC];
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    ga[e] = a.gamma ? a.gamma[c + e] : 1.f;
-    be[e] = a.beta ? a.beta[c + e] : 0.f;
+  m = {red[0].x, red[0].y};
+  for (unsigned w = 1; w < blockDim.x >> 6; ++w) {
+    m.s += red[w].x;
+    m.q += red[w].y;
   }
+  if (!live) return;
+  const Scale s = scale_of(a, m, p);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     if (row + i * a.rows >= a.t) break;
@@ -229,6 +259,8 @@ __global__ __launch_bounds__(256) void norm_sums_kernel(const NormArgs a) {
     }
   }
   meet(a, m, red, cols_each, a.cols, groups, total);
+  if (piece == 0 && run % a.blocks == 0 && live && row == 0 && col % cols_each == 0)
+    a.pivot[(long long)img * a.groups + g0 + g] = (float)p;
   for (int i = threadIdx.x; i < groups; i += 256)
     a.sums[(((long long)img * a.groups + g0 + i) * a.blocks + run % a.blocks) * a.pieces + piece] =
         make_double2(total[i].s, total[i].q);
@@ -244,52 +276,54 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(const NormArgs a) {
   const int cols_each = min(a.each / VEC - first, a.cols), cols = groups * cols_each;
   const float* x = a.x + (long long)img * a.t * a.ldx;
   float* y = a.y + (long long)img * a.t * a.ldy;
-  for (int g = threadIdx.x >> 6; g < groups; g += 4) {
-    const int parts = a.blocks * a.pieces;
-    const double2* sums = a.sums + ((long long)img * a.groups + g0 + g) * parts;
-    Moments m{0, 0};
-    for (int i = lane; i < parts; i += 64) {
-      m.s += sums[i].x;
-      m.q += sums[i].y;
-    }
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      m.s += shuffle_xor(m.s, off);
-      m.q += shuffle_xor(m.q, off);
-    }
-    if (lane == 0) scale[g] = scale_of(a, m, (double)x[(g0 + g) * a.each], (double)a.t * a.each);
-  }
-  __syncthreads();
-  const int row = threadIdx.x / a.cols, col = threadIdx.x - row * a.cols;
-  if (row >= a.rows || col >= cols) return;
+  const int row = threadIdx.x / a.cols, col = min((int)threadIdx.x - row * a.cols, cols - 1);
   const int c = g0 * a.each + (first + col) * VEC;
-  const Scale s = scale[col / cols_each];
+  const int from = piece * a.piece, to = min(from + a.piece, a.t);
+  // The first pixels and the weights are under way while the moments meet.
+  int i = from + row;
+  vec v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = *(const vec*)(x + min(i + k * a.rows, to - 1) * a.ldx + c);
   float ga[VEC], be[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
     ga[e] = a.gamma ? a.gamma[c + e] : 1.f;
     be[e] = a.beta ? a.beta[c + e] : 0.f;
   }
-  const int from = piece * a.piece, to = min(from + a.piece, a.t);
-  auto put = [&](int i, const vec& v) {
-    vec o;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) o[e] = normal(a, v[e], s, ga[e], be[e]);
-    __builtin_nontemporal_store(o, (vec*)(y + i * a.ldy + c));
-  };
-  int i = from + row;
-  for (; i + 3 * a.rows < to; i += 4 * a.rows) {
-    vec v[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = *(const vec*)(x + (i + k * a.rows) * a.ldx + c);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) put(i + k * a.rows, v[k]);
+  for (int g = threadIdx.x >> 6; g < groups; g += 4) {
+    const int parts = a.blocks * a.pieces;
+    const double2* sums = a.sums + ((long long)img * a.groups + g0 + g) * parts;
+    Moments m{0, 0};
+    for (int p = lane; p < parts; p += 64) {
+      m.s += sums[p].x;
+      m.q += sums[p].y;
+    }
+    m.s = plus_lanes(m.s, 64);
+    m.q = plus_lanes(m.q, 64);
+    if (lane == 0) scale[g] = scale_of(a, m, (double)a.pivot[((long long)img * a.groups + g0 + g)]);
   }
-  for (; i < to; i += a.rows) put(i, *(const vec*)(x + i * a.ldx + c));
+  __syncthreads();
+  if (row >= a.rows || (int)threadIdx.x - row * a.cols >= cols) return;
+  const Scale s = scale[col / cols_each];
+  while (i < to) {
+    vec o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[k][e] = normal(a, v[k][e], s, ga[e], be[e]);
+    const int at = i;
+    i += 4 * a.rows;
+    if (i < to)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = *(const vec*)(x + min(i + k * a.rows, to - 1) * a.ldx + c);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (at + k * a.rows < to) __builtin_nontemporal_store(o[k], (vec*)(y + (at + k * a.rows) * a.ldy + c));
+  }
 }
 
 // Elements of a group that 64 lanes hold: kRowsVec vectors each.
-constexpr int kRowsVec = 16;
+constexpr int kRowsVec = 4;
 
 int op_group_norm(sy_ctx* ctx, const sy_tensor* x, int groups, const float* gamma, const float* beta, float eps,
                   int act, const sy_tensor* y) {
@@ -325,6 +359,7 @@ int op_group_norm(sy_ctx* ctx, const sy_tensor* x, int groups, const float* gamm
   a.each = x->c / groups;
   a.act = act;
   a.eps = eps;
+  a.share = 1.0 / ((double)a.t * a.each);
   const bool quads = a.each % 4 == 0 && a.ldx % 4 == 0 && a.ldy % 4 == 0 &&
                      (((uintptr_t)x->data | (uintptr_t)y->data) & 15) == 0;
   const int vec = quads ? 4 : 1;
@@ -340,47 +375,40 @@ int op_group_norm(sy_ctx* ctx, const sy_tensor* x, int groups, const float* gamm
     const int v = (int)((units + a.lanes - 1) / a.lanes);
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, ctx->stream, a); };
     if (quads)
-      v <= 1 ? launch(norm_rows_kernel<4, 1>) : v <= 4 ? launch(norm_rows_kernel<4, 4>) : launch(norm_rows_kernel<4, kRowsVec>);
+      v <= 1 ? launch(norm_rows_kernel<4, 1>) : launch(norm_rows_kernel<4, kRowsVec>);
     else
-      v <= 4 ? launch(norm_rows_kernel<1, 4>) : launch(norm_rows_kernel<1, kRowsVec>);
+      launch(norm_rows_kernel<1, kRowsVec>);
+    return check_launch("group_norm");
+  }
+  const int each = a.each / vec;
+  if (each <= 1024 && (a.t + 1024 / each - 1) / (1024 / each) <= kGroupVec) {
+    int threads = 256;
+    while (each > threads || (a.t + threads / each - 1) / (threads / each) > kGroupVec) threads *= 2;
+    a.cols = each;
+    a.rows = threads / each;
+    const long long grid = ((long long)a.n * groups + 7) / 8 * 8;
+    SY_CHECK(grid * threads < (1LL << 32), SY_EUNSUPPORTED, "group norm over %d images of %d groups", a.n, groups);
+    hipLaunchKernelGGL(quads ? norm_group_kernel<4> : norm_group_kernel<1>, dim3((unsigned)grid), dim3(threads), 0,
+                       ctx->stream, a);
     return check_launch("group_norm");
   }
   // A run of groups: 128 bytes of a pixel and more.
-  const int each = a.each / vec;
-  auto columns = [&](int threads) {
-    a.run = std::min({groups, std::max(1, threads / each), std::max(1, (32 / vec + each - 1) / each)});
-    a.cols = std::min(a.run * each, threads);
-    a.rows = threads / a.cols;
-    a.blocks = (each + threads - 1) / threads;
-    a.runs = a.blocks > 1 ? groups * a.blocks : (groups + a.run - 1) / a.run;
-    return (a.t + a.rows - 1) / a.rows;  // pixels of a thread
-  };
-  const int most = quads ? 16 : 64;  // vectors that a thread holds
-  if (each <= 1024 && columns(1024) <= most) {
-    int threads = 256;
-    while (threads < 1024 && (each > threads || columns(threads) > (a.n * (long long)a.runs < 512 ? most / 4 : most)))
-      threads *= 2;
-    const int v = columns(threads);
-    const long long grid = (long long)a.n * a.runs;
-    SY_CHECK(grid * threads < (1LL << 32), SY_EUNSUPPORTED, "group norm over %d images of %d groups", a.n, groups);
-    auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), 0, ctx->stream, a);
-    };
-    if (quads)
-      v <= 4 ? launch(norm_run_kernel<4, 4>) : launch(norm_run_kernel<4, 16>);
-    else
-      v <= 16 ? launch(norm_run_kernel<1, 16>) : launch(norm_run_kernel<1, 64>);
-    return check_launch("group_norm");
-  }
-  (void)columns(256);
-  // Pieces: a few workgroups to a CU, but 16 pixels of a thread and more.
+  a.run = std::min({groups, std::max(1, 256 / each), std::max(1, (32 / vec + each - 1) / each)});
+  a.cols = std::min(a.run * each, 256);
+  a.rows = 256 / a.cols;
+  a.blocks = (each + 255) / 256;
+  a.runs = a.blocks > 1 ? groups * a.blocks : (groups + a.run - 1) / a.run;
+  // Pieces: 8 pixels of a thread and more, 2 where those would leave CUs without work, up to 8192 workgroups.
   const long long runs = (long long)a.n * a.runs;
-  a.piece = (int)std::max<long long>(16 * a.rows, (a.t * runs + 2047) / 2048);
+  const int least = a.t * runs >= 256LL * 8 * a.rows ? 8 : 2;
+  a.piece = (int)std::max<long long>(least * a.rows, (a.t * runs + 8191) / 8192);
   a.pieces = (a.t + a.piece - 1) / a.piece;
   const long long grid = runs * a.pieces;
   SY_CHECK(grid * 256 < (1LL << 32), SY_EUNSUPPORTED, "group norm over %d images of %d groups", a.n, groups);
-  SY_TRY(ensure_scratch(ctx, sizeof(double2) * (size_t)a.n * groups * a.blocks * a.pieces));
+  const size_t sums = sizeof(double2) * (size_t)a.n * groups * a.blocks * a.pieces;
+  SY_TRY(ensure_scratch(ctx, sums + sizeof(float) * (size_t)a.n * groups));
   a.sums = (double2*)ctx->scratch;
+  a.pivot = (float*)(ctx->scratch + sums);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, ctx->stream, a); };
   launch(quads ? norm_sums_kernel<4> : norm_sums_kernel<1>);
   launch(quads ? norm_apply_kernel<4> : norm_apply_kernel<1>);
