@@ -28,6 +28,7 @@ struct CrossArgs {
   int tq, tk, heads, kv, group, kd, hd, qs, ks, vs;
   float scale, c;       // c: scale log2(e)
   int rows, tiles;      // rows (query, head of the group) of an image and key head, their tiles
+  int run;              // row tiles of a workgroup that goes through many
   int splits, piece;    // pieces of the states, a multiple of kCrossKeys each
   unsigned items;
   CrossStat* stat;      // [image, key head][piece][row], where there are several
@@ -90,6 +91,40 @@ __device__ __forceinline__ void cross_row(const CrossArgs& a, int b, int i, int 
 // Products of part pairs, the smallest first.
 constexpr int kPairA[6] = {2, 1, 0, 1, 0, 0}, kPairB[6] = {0, 1, 2, 0, 1, 0};
 
+// A query's channels 16 ks + 8 half .. + 7 of a head, zeros past the last.
+template <int KS>
+__device__ __forceinline__ void cross_query(const CrossArgs& a, int b, int i, int head, f32x4 (&raw)[KS][2]) {
+  const float* q = a.q + ((long long)b * a.tq + i) * a.ldq + (long long)head * a.qs;
+  const int half = (threadIdx.x & 63) >> 5;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int c = 16 * ks + 8 * half + 4 * e;
+      raw[ks][e] = c < a.kd ? *(const f32x4*)(q + c) : zero;
+    }
+}
+
+// What a wave keeps of its 32 rows: the weighted values (channel 32 d + lane % 32 of rows 8 (r / 4)
+// + 4 half + r % 4), and of row lane % 32 the maximum, the lane's share of the sum, and whether a
+// state was visible.
+template <int DT>
+struct CrossRows {
+  f32x16 acc[DT];
+  float top, sum;
+  unsigned any;
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+    top = -INFINITY;
+    sum = 0.f;
+    any = 0;
+  }
+};
+
 // 32 rows (a query and a head of the group that shares the key head) to a wave, NW
 // waves to a workgroup, over one piece of the states, 32 at a time.
 //
@@ -109,285 +144,642 @@ constexpr int kPairA[6] = {2, 1, 0, 1, 0, 0}, kPairB[6] = {0, 1, 2, 0, 1, 0};
 // where a score passes it by kSlack: weights reach 2^kSlack until then, which costs
 // bf16 parts nothing.
 constexpr float kSlack = 8.f;
-template <int KS, int DT, int NW>
-__global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : 2) void cross_kernel(const CrossArgs a) {
-  constexpr int NT = NW * 64;
-  constexpr int KU = KS * 64, VU = 2 * DT * 64;  // 8-element units of a tile's keys and values
-  constexpr int KI = (KU + NT - 1) / NT, VI = (VU + NT - 1) / NT;
-  __shared__ u32x4 frag[2 * (KU + VU) * 3];
-  const unsigned item = cross_item();
-  if (item >= a.items) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int half = lane >> 5, r32 = lane & 31;
-  const int tile = item % a.tiles, rest = item / a.tiles, split = rest % a.splits, plane = rest / a.splits;
-  const int b = plane / a.kv, g = plane - b * a.kv;
-  const int from = split * a.piece, to = min(from + a.piece, cross_end(a, b));
-  const int row = (tile * NW + wave) * 32 + r32, row1 = min(row, a.rows - 1);
-  const int qi = row1 / a.group, head = g * a.group + row1 - qi * a.group;
-  const float* kb = a.k + (long long)b * a.tk * a.ldk + (long long)g * a.ks;
-  const float* vb = a.v + (long long)b * a.tk * a.ldv + (long long)g * a.vs;
-  const uint8_t* mask = cross_mask(a, b, head, qi);
 
-  // A tile's units on their way: keys two by two quads, values eight states of a channel.
-  f32x4 kr[KI][2];
-  float vr[VI][8];
-  auto load = [&](int j0) __attribute__((always_inline)) {
-    const float* kt = kb + (long long)j0 * a.ldk;
-    const float* vt = vb + (long long)j0 * a.ldv;
-    const int last = to - 1 - j0;  // states from here on are read from the last visible one
+// A row's mask bytes of the tile at j0, the lane's states four by four; 0 past `to`.
+__device__ __forceinline__ void cross_seen(const uint8_t* mask, int j0, int to, unsigned (&seen)[4]) {
+  const int half = (threadIdx.x & 63) >> 5;
+  if (j0 + kCrossKeys <= to) {
 #pragma unroll
-    for (int i = 0; i < KI; ++i) {
-      const int u = tid + i * NT, oct = u % (2 * KS), r = min(u / (2 * KS), last);
-      if (KU % NT != 0 && u >= KU) break;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) kr[i][e] = *(const f32x4*)(kt + (unsigned)(r * a.ldk + min(8 * oct + 4 * e, a.kd - 4)));
-    }
-#pragma unroll
-    for (int i = 0; i < VI; ++i) {
-      const int u = tid + i * NT, f = u >> 6, d = f % DT, st = f / DT;
-      if (VU % NT != 0 && u >= VU) break;
-      const int c = min(32 * d + r32, a.hd - 1);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        vr[i][e] = vt[(unsigned)(min(16 * st + 8 * (e >> 2) + 4 * half + (e & 3), last) * a.ldv + c)];
-    }
-  };
-  auto stage = [&](u32x4* to_lds) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < KI; ++i) {
-      const int u = tid + i * NT, oct = u % (2 * KS), r = u / (2 * KS);
-      if (KU % NT != 0 && u >= KU) break;
-      bf16x8 p[3];
-      parts8(kr[i][0], kr[i][1], p);
-      // Lanes of one key write 16 bytes each, 1.5 KB apart: its place within the fragment goes round with them.
-      u32x4* at = to_lds + (oct >> 1) * 192 + (oct & 1) * 32 + (r ^ oct);
-#pragma unroll
-      for (int s = 0; s < 3; ++s) at[s * 64] = __builtin_bit_cast(u32x4, p[s]);
-    }
-#pragma unroll
-    for (int i = 0; i < VI; ++i) {
-      const int u = tid + i * NT;
-      if (VU % NT != 0 && u >= VU) break;
-      bf16x8 p[3];
-      parts8(f32x4{vr[i][0], vr[i][1], vr[i][2], vr[i][3]}, f32x4{vr[i][4], vr[i][5], vr[i][6], vr[i][7]}, p);
-      u32x4* at = to_lds + KU * 3 + (u >> 6) * 192 + lane;
-#pragma unroll
-      for (int s = 0; s < 3; ++s) at[s * 64] = __builtin_bit_cast(u32x4, p[s]);
-    }
-  };
-
-  f32x16 acc[DT];
-#pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
-  float mrun = -INFINITY, lrun = 0.f;
-  unsigned any = 0;  // the row has a visible state
-
-  if (from < to) {
-    load(from);
-    bf16x8 q[KS][3];
-    {
-      const float* qr = a.q + ((long long)b * a.tq + qi) * a.ldq + (long long)head * a.qs;
-      const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const int c = 16 * ks + 8 * half;
-        parts8(c < a.kd ? *(const f32x4*)(qr + c) : zero, c + 4 < a.kd ? *(const f32x4*)(qr + c + 4) : zero, q[ks]);
-      }
-    }
-    stage(frag);
-    __syncthreads();
-    int now = 0;
-    for (int j0 = from; j0 < to; j0 += kCrossKeys, now ^= 1) {
-      const bool more = j0 + kCrossKeys < to;
-      if (more) load(j0 + kCrossKeys);
-      const u32x4* f = frag + now * (KU + VU) * 3;
-      unsigned seen[4] = {~0u, ~0u, ~0u, ~0u};
-      if (mask) {
-        if (j0 + kCrossKeys <= to) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) __builtin_memcpy(&seen[x], mask + j0 + 8 * x + 4 * half, 4);
-        } else {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            seen[x] = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int j = j0 + 8 * x + 4 * half + e;
-              if (j < to) seen[x] |= (unsigned)mask[j] << 8 * e;
-            }
-          }
-        }
-      }
-      const unsigned some = seen[0] | seen[1] | seen[2] | seen[3];
-      any |= some;
-      if (__any(some != 0)) {
-        f32x16 s;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          bf16x8 kp[3];
-#pragma unroll
-          for (int p = 0; p < 3; ++p)
-            kp[p] = __builtin_bit_cast(bf16x8, f[(ks * 3 + p) * 64 + half * 32 + (r32 ^ (2 * ks + half))]);
-#pragma unroll
-          for (int x = 0; x < 6; ++x)
-            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kp[kPairA[x]], q[ks][kPairB[x]], s, 0, 0, 0);
-        }
-        if (mask) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (!(seen[r >> 2] >> 8 * (r & 3) & 0xff)) s[r] = -INFINITY;
-        }
-        if (j0 + kCrossKeys > to) {
-          asm volatile("");  // a branch, not 16 selects in every tile
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (j0 + 8 * (r >> 2) + 4 * half + (r & 3) >= to) s[r] = -INFINITY;
-        }
-        float mx = s[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.c;
-        if (__any(mx - mrun > kSlack)) {
-          mx = fmaxf(mx, mrun);
-          const float w = __builtin_amdgcn_exp2f(mrun - (mx == -INFINITY ? 0.f : mx));
-          mrun = mx;
-          lrun *= w;
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[d][r] *= w;
-        }
-        const float m = mrun == -INFINITY ? 0.f : mrun;  // no weight yet: all are 0
-        float sum = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -m));
-          sum += s[r];
-        }
-        lrun += sum;
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          bf16x8 p[3];
-          parts8(f32x4{s[8 * st], s[8 * st + 1], s[8 * st + 2], s[8 * st + 3]},
-                 f32x4{s[8 * st + 4], s[8 * st + 5], s[8 * st + 6], s[8 * st + 7]}, p);
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            bf16x8 vp[3];
-#pragma unroll
-            for (int x = 0; x < 3; ++x)
-              vp[x] = __builtin_bit_cast(bf16x8, f[KU * 3 + ((st * DT + d) * 3 + x) * 64 + lane]);
-#pragma unroll
-            for (int x = 0; x < 6; ++x)
-              acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vp[kPairA[x]], p[kPairB[x]], acc[d], 0, 0, 0);
-          }
-        }
-      }
-      if (more) stage(frag + (now ^ 1) * (KU + VU) * 3);
-      __syncthreads();
-    }
-  }
-
-  float l = lrun + __shfl_xor(lrun, 32);
-  any |= __shfl_xor((int)any, 32);
-  if (any && mrun == -INFINITY && from < to) l = NAN;  // visible, but no finite score: again, in plain float32
-  const bool live = row < a.rows;
-  if (a.splits > 1) {
-    const long long at = ((long long)plane * a.splits + split) * a.rows + row1;
-    if (live && half == 0) a.stat[at] = {mrun, l};
-    if (live && l != 0.f)
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int c = 32 * d + 8 * x + 4 * half;
-          if (c < a.hd)
-            *(f32x4*)(a.part + at * a.hd + c) = f32x4{acc[d][4 * x], acc[d][4 * x + 1], acc[d][4 * x + 2], acc[d][4 * x + 3]};
-        }
+    for (int x = 0; x < 4; ++x) __builtin_memcpy(&seen[x], mask + j0 + 8 * x + 4 * half, 4);
     return;
   }
-  float* o = a.o + ((long long)b * a.tq + qi) * a.ldo + (long long)head * a.hd;
-  bool again = false;
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
+  for (int x = 0; x < 4; ++x) {
+    seen[x] = 0;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int c = 32 * d + 8 * x + 4 * half;
-      f32x4 y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[e] = l == 0.f ? 0.f : acc[d][4 * x + e] / l;
-        again |= live && c < a.hd && !(__builtin_fabsf(y[e]) <= FLT_MAX);
-      }
-      if (live && c < a.hd) *(f32x4*)(o + c) = y;
+    for (int e = 0; e < 4; ++e) {
+      const int j = j0 + 8 * x + 4 * half + e;
+      if (j < to) seen[x] |= (unsigned)mask[j] << 8 * e;
     }
-  unsigned long long todo = __ballot(again);
-  for (todo = (todo | todo >> 32) & 0xffffffffu; todo; todo &= todo - 1) {
-    const int t = __builtin_ctzll(todo), ri = __shfl(qi, t), rh = __shfl(head, t);
+  }
+}
+
+// One tile: states j0 .. j0 + 31 up to `to`, whose parts are at f.  seen: its mask bytes, where there are any.
+template <int KS, int DT>
+__device__ __forceinline__ void cross_tile(const CrossArgs& a, const u32x4* f, int j0, int to, const unsigned (&seen)[4],
+                                           const bf16x8 (&q)[KS][3], CrossRows<DT>& w) {
+  const int lane = threadIdx.x & 63, half = lane >> 5, r32 = lane & 31;
+  if (a.mask) {
+    const unsigned some = seen[0] | seen[1] | seen[2] | seen[3];
+    w.any |= some;
+    if (!__any(some != 0)) return;
+  } else {
+    w.any = 1;
+  }
+  // Fragments are read a step ahead of the products that take them.
+  const u32x4* v = f + KS * 192 + lane;
+  auto key = [&](int ks, bf16x8(&k)[3]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 3; ++x)
+      k[x] = __builtin_bit_cast(bf16x8, f[(ks * 3 + x) * 64 + half * 32 + (r32 ^ (2 * ks + half))]);
+  };
+  auto value = [&](int i, bf16x8(&p)[3]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 3; ++x) p[x] = __builtin_bit_cast(bf16x8, v[(i * 3 + x) * 64]);
+  };
+  f32x16 s;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = 0.f;
+  bf16x8 kp[2][3];
+  key(0, kp[0]);
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    if (ks + 1 < KS) key(ks + 1, kp[(ks + 1) & 1]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int x = 0; x < 6; ++x)
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kp[ks & 1][kPairA[x]], q[ks][kPairB[x]], s, 0, 0, 0);
+  }
+  bf16x8 vp[2][3];
+  value(0, vp[0]);
+  if (a.mask) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (!(seen[r >> 2] >> 8 * (r & 3) & 0xff)) s[r] = -INFINITY;
+  }
+  if (j0 + kCrossKeys > to) {
+    asm volatile("");  // a branch, not 16 selects in every tile
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (j0 + 8 * (r >> 2) + 4 * half + (r & 3) >= to) s[r] = -INFINITY;
+  }
+  float mx = s[0];
+#pragma unroll
+  for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+  mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.c;
+  if (__any(mx - w.top > kSlack)) {
+    mx = fmaxf(mx, w.top);
+    const float x = __builtin_amdgcn_exp2f(w.top - (mx == -INFINITY ? 0.f : mx));
+    const bool before = __any(w.top != -INFINITY);
+    w.top = mx;
+    w.sum *= x;
+    if (before)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float xr = __shfl(x, 8 * (r >> 2) + 4 * half + (r & 3));
+#pragma unroll
+        for (int d = 0; d < DT; ++d) w.acc[d][r] *= xr;
+      }
+  }
+  const float m = w.top == -INFINITY ? 0.f : w.top;  // no weight yet: all are 0
+  float sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -m));
+    sum += s[r];
+  }
+  w.sum += sum;
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+    bf16x8 p[3];
+    parts8(f32x4{s[8 * st], s[8 * st + 1], s[8 * st + 2], s[8 * st + 3]},
+           f32x4{s[8 * st + 4], s[8 * st + 5], s[8 * st + 6], s[8 * st + 7]}, p);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const int i = st * DT + d;
+      if (i + 1 < 2 * DT) value(i + 1, vp[(i + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x < 6; ++x)
+        w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[kPairA[x]], vp[i & 1][kPairB[x]], w.acc[d], 0, 0, 0);
+    }
+  }
+}
+
+// The outputs of 32 rows from row0, or what a piece leaves for them, in whole lines of
+// memory.  states: the piece has any.
+template <int DT>
+__device__ __forceinline__ void cross_finish(const CrossArgs& a, const CrossRows<DT>& w, int plane, int split, int row0,
+                                             bool states) {
+  const int lane = threadIdx.x & 63, half = lane >> 5, r32 = lane & 31;
+  const int b = plane / a.kv, g = plane - b * a.kv, row1 = min(row0 + r32, a.rows - 1);
+  float l = w.sum + __shfl_xor(w.sum, 32);
+  const unsigned any = w.any | (unsigned)__shfl_xor((int)w.any, 32);
+  if (any && states && w.top == -INFINITY) l = NAN;  // visible, but no finite score: again, in plain float32
+  // Where row 0 of the tile goes, and how far row1 is from it.
+  float* out;
+  long long step, mine;  // floats from row to row; to row1, where they differ
+  if (a.splits > 1) {
+    const long long at = ((long long)plane * a.splits + split) * a.rows + row0;
+    if (half == 0 && row0 + r32 < a.rows) a.stat[at + r32] = {w.top, l};
+    out = a.part + at * a.hd;
+    step = a.hd;
+    mine = 0;
+  } else {
+    const int qi = row1 / a.group;
+    out = a.o + (long long)b * a.tq * a.ldo + (long long)g * a.group * a.hd;
+    step = a.ldo;
+    mine = qi * a.ldo + (long long)(row1 - qi * a.group) * a.hd;
+    if (a.group == 1) out += row0 * a.ldo;
+  }
+  const float factor = a.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;  // l is 1 and more, or there is nothing to weigh
+  float f[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) f[r] = __shfl(factor, 8 * (r >> 2) + 4 * half + (r & 3));
+  float odd = 0.f;  // not 0 where a value is not finite
+  if ((a.splits > 1 || a.group == 1) && row0 + 32 <= a.rows) {
+    float* at = out + 4 * half * step + r32;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      if (32 * d + r32 >= a.hd) break;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float y = w.acc[d][r] * f[r];
+        odd = __builtin_fmaf(y, 0.f, odd);
+        __builtin_nontemporal_store(y, at + (8 * (r >> 2) + (r & 3)) * step + 32 * d);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int at = 8 * (r >> 2) + (r & 3), row = at + 4 * half;
+      const long long off =
+          a.splits > 1 || a.group == 1
+              ? row * step
+              : (long long)(unsigned)__shfl((int)mine, row) | (long long)__shfl((int)(mine >> 32), row) << 32;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const float y = w.acc[d][r] * f[r];
+        if (32 * d + r32 < a.hd && row0 + row < a.rows) {
+          odd = __builtin_fmaf(y, 0.f, odd);
+          __builtin_nontemporal_store(y, out + off + 32 * d + r32);
+        }
+      }
+    }
+  }
+  if (a.splits > 1 || !__any(odd != 0.f)) return;
+  unsigned again = 0;  // rows with such a value
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int at = 8 * (r >> 2) + (r & 3);
+    bool bad = false;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) bad |= !(__builtin_fabsf(w.acc[d][r] * f[r]) <= FLT_MAX);
+    const unsigned long long who = __ballot(bad);
+    again |= ((unsigned)who != 0 ? 1u : 0u) << at | ((who >> 32) != 0 ? 1u : 0u) << (at + 4);
+  }
+  for (; again; again &= again - 1) {
+    const int t = __builtin_ctz(again);
+    if (row0 + t >= a.rows) return;
+    const int ri = (row0 + t) / a.group, rh = g * a.group + row0 + t - ri * a.group;
+    float* ro = a.o + ((long long)b * a.tq + ri) * a.ldo + (long long)rh * a.hd;
     float z[2];
     cross_row(a, b, ri, rh, lane, z);
-    float* ro = a.o + ((long long)b * a.tq + ri) * a.ldo + (long long)rh * a.hd;
 #pragma unroll
     for (int x = 0; x < 2; ++x)
       if (lane + 64 * x < a.hd) ro[lane + 64 * x] = z[x];
   }
 }
 
-// Joins the pieces of a row: L lanes to a row, four channels to a lane.
-template <int L>
+// States on their way to LDS: NT threads take 8-element units of SUB tiles, keys as two
+// quads of a row, values as eight states of a channel, split them and put them down in the
+// order in which the matrix instruction's lanes take them.
+template <int KS, int DT, int NT, int SUB>
+struct CrossStage {
+  static constexpr int TILE = (KS + 2 * DT) * 192;  // 16-byte units of a tile
+  static constexpr int KU = SUB * KS * 64, VU = SUB * 2 * DT * 64;
+  static constexpr int KI = (KU + NT - 1) / NT, VI = (VU + NT - 1) / NT;
+  f32x4 kr[KI][2];
+  float vr[VI][8];
+  // Where the keys do not keep every thread busy the values begin with those that are left.
+  static __device__ __forceinline__ int value_tid() {
+    return KU % NT ? (int)(threadIdx.x + NT - KU % NT) % NT : (int)threadIdx.x;
+  }
+  // The tiles at j0 of a head's keys and values; past `to` the last state is read again.
+  __device__ __forceinline__ void load(const CrossArgs& a, const float* kb, const float* vb, int j0, int to) {
+    const int half = (threadIdx.x & 63) >> 5, r32 = threadIdx.x & 31;
+    const float* kt = kb + (long long)j0 * a.ldk;
+    const float* vt = vb + (long long)j0 * a.ldv;
+    const int last = to - 1 - j0;
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      const int u = threadIdx.x + i * NT, oct = u % (2 * KS), r = min(u / (2 * KS), last);
+      if (KU % NT != 0 && u >= KU) break;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        kr[i][e] = *(const f32x4*)(kt + (unsigned)(r * a.ldk + min(8 * oct + 4 * e, a.kd - 4)));
+    }
+#pragma unroll
+    for (int i = 0; i < VI; ++i) {
+      const int u = value_tid() + i * NT, f = u >> 6, d = f % DT, st = f / DT;
+      if (VU % NT != 0 && u >= VU) break;
+      const int c = min(32 * d + r32, a.hd - 1);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        vr[i][e] = vt[(unsigned)(min(16 * st + 8 * (e >> 2) + 4 * half + (e & 3), last) * a.ldv + c)];
+    }
+  }
+  __device__ __forceinline__ void put(u32x4* lds) const {
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      const int u = threadIdx.x + i * NT, oct = u % (2 * KS), r = u / (2 * KS);
+      if (KU % NT != 0 && u >= KU) break;
+      bf16x8 p[3];
+      parts8(kr[i][0], kr[i][1], p);
+      // Lanes of one key write 16 bytes each, 1.5 KB apart: its place within the fragment goes round with them.
+      u32x4* at = lds + (r >> 5) * TILE + (oct >> 1) * 192 + (oct & 1) * 32 + ((r & 31) ^ oct);
+#pragma unroll
+      for (int s = 0; s < 3; ++s) at[s * 64] = __builtin_bit_cast(u32x4, p[s]);
+    }
+#pragma unroll
+    for (int i = 0; i < VI; ++i) {
+      const int u = value_tid() + i * NT, f = u >> 6, sub = f / (2 * DT);
+      if (VU % NT != 0 && u >= VU) break;
+      bf16x8 p[3];
+      parts8(f32x4{vr[i][0], vr[i][1], vr[i][2], vr[i][3]}, f32x4{vr[i][4], vr[i][5], vr[i][6], vr[i][7]}, p);
+      u32x4* at = lds + sub * TILE + KS * 192 + (f - sub * 2 * DT) * 192 + (u & 63);
+#pragma unroll
+      for (int s = 0; s < 3; ++s) at[s * 64] = __builtin_bit_cast(u32x4, p[s]);
+    }
+  }
+};
+
+template <int KS, int DT, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void cross_kernel(const CrossArgs a) {
+  typedef CrossStage<KS, DT, NW * 64, 1> Stage;
+  __shared__ u32x4 frag[2][Stage::TILE];
+  const unsigned item = cross_item();
+  if (item >= a.items) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = item % a.tiles, rest = item / a.tiles, split = rest % a.splits, plane = rest / a.splits;
+  const int b = plane / a.kv, g = plane - b * a.kv;
+  const int from = split * a.piece, to = min(from + a.piece, cross_end(a, b));
+  const int row = (tile * NW + wave) * 32 + (threadIdx.x & 31), row1 = min(row, a.rows - 1);
+  const int qi = row1 / a.group, head = g * a.group + row1 - qi * a.group;
+  const float* kb = a.k + (long long)b * a.tk * a.ldk + (long long)g * a.ks;
+  const float* vb = a.v + (long long)b * a.tk * a.ldv + (long long)g * a.vs;
+  const uint8_t* mask = cross_mask(a, b, head, qi);
+  const bool some = (tile * NW + wave) * 32 < a.rows;  // the wave has rows
+  CrossRows<DT> rows;
+  rows.clear();
+  if (from < to) {
+    Stage stage;
+    stage.load(a, kb, vb, from, to);
+    bf16x8 q[KS][3];
+    {
+      f32x4 raw[KS][2];
+      cross_query<KS>(a, b, qi, head, raw);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) parts8(raw[ks][0], raw[ks][1], q[ks]);
+    }
+    stage.put(frag[0]);
+    // Mask bytes are loaded ahead, too, where there are registers for them.
+    constexpr bool AHEAD = KS + 2 * DT < 16;
+    unsigned next[4];
+    if (AHEAD && mask) cross_seen(mask, from, to, next);
+    __syncthreads();
+    int now = 0;
+    for (int j0 = from; j0 < to; j0 += kCrossKeys, now ^= 1) {
+      const bool more = j0 + kCrossKeys < to;
+      if (!AHEAD && mask) cross_seen(mask, j0, to, next);
+      unsigned seen[4] = {next[0], next[1], next[2], next[3]};
+      if (more) {
+        if (AHEAD && mask) cross_seen(mask, j0 + kCrossKeys, to, next);
+        stage.load(a, kb, vb, j0 + kCrossKeys, to);
+      }
+      if (some) cross_tile<KS, DT>(a, frag[now], j0, to, seen, q, rows);
+      if (more) stage.put(frag[now ^ 1]);
+      __syncthreads();
+    }
+  }
+  cross_finish<DT>(a, rows, plane, split, (tile * NW + wave) * 32, from < to);
+}
+
+// Few states: a workgroup splits all of them once and goes through many rows, its
+// waves on their own, the next rows' queries under way.
+constexpr int kShortLds = 150 * 1024, kShortWaves = 4;
+constexpr int short_bytes(int ks, int dt) { return (ks + 2 * dt) * 3072; }  // of a tile
+template <int KS, int DT>
+__global__ __launch_bounds__(kShortWaves * 64, 2) void cross_short_kernel(const CrossArgs a) {
+  constexpr int NW = kShortWaves;
+  typedef CrossStage<KS, DT, NW * 64, 1> Stage;
+  extern __shared__ u32x4 frag[];
+  // Images' lengths differ: every XCD takes workgroups of all of them.
+  const int planes = a.items / a.tiles;  // tiles: runs of row tiles here
+  if (blockIdx.x >= a.items) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = threadIdx.x & 31;
+  const int run = blockIdx.x / planes, plane = blockIdx.x - run * planes;
+  const int b = plane / a.kv, g = plane - b * a.kv, to = cross_end(a, b);
+  const float* kb = a.k + (long long)b * a.tk * a.ldk + (long long)g * a.ks;
+  const float* vb = a.v + (long long)b * a.tk * a.ldv + (long long)g * a.vs;
+  const int first = run * a.run, last = min(first + a.run, (a.rows + 31) / 32);
+  auto place = [&](int tile, int& qi, int& head) {
+    const int row = min(tile * 32 + r32, a.rows - 1);
+    qi = row / a.group;
+    head = g * a.group + row - qi * a.group;
+  };
+  int qi, head;
+  f32x4 raw[KS][2];
+  place(min(first + wave, last - 1), qi, head);
+  {
+    Stage stage;
+    if (to > 0) stage.load(a, kb, vb, 0, to);
+    cross_query<KS>(a, b, qi, head, raw);
+    for (int j0 = 0; j0 < to; j0 += kCrossKeys) {
+      stage.put(frag + j0 / kCrossKeys * Stage::TILE);
+      if (j0 + kCrossKeys < to) stage.load(a, kb, vb, j0 + kCrossKeys, to);
+    }
+  }
+  __syncthreads();
+  bf16x8 q[KS][3];
+  auto split = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) parts8(raw[ks][0], raw[ks][1], q[ks]);
+  };
+  split();
+  for (int tile = first + wave; tile < last; tile += NW) {
+    const uint8_t* mask = cross_mask(a, b, head, qi);
+    if (tile + NW < last) {
+      place(tile + NW, qi, head);
+      cross_query<KS>(a, b, qi, head, raw);
+    }
+    CrossRows<DT> rows;
+    rows.clear();
+    for (int j0 = 0; j0 < to; j0 += kCrossKeys) {
+      unsigned seen[4];
+      if (mask) cross_seen(mask, j0, to, seen);
+      cross_tile<KS, DT>(a, frag + j0 / kCrossKeys * Stage::TILE, j0, to, seen, q, rows);
+    }
+    split();  // before the stores: waiting for loads behind them would wait for them, too
+    cross_finish<DT>(a, rows, plane, 0, tile * 32, to > 0);
+  }
+}
+
+// v summed over aligned groups of 16 lanes, in each of them.
+__device__ __forceinline__ float plus16(float v) {
+#define SY_PLUS(ctrl) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, false))
+  SY_PLUS(0xb1);   // lane ^ 1
+  SY_PLUS(0x4e);   // lane ^ 2
+  SY_PLUS(0x141);  // 7 - lane
+  SY_PLUS(0x140);  // 15 - lane
+#undef SY_PLUS
+  return v;
+}
+
+// Few rows (a token's query): up to G rows of an image and key head, in plain float32.
+// 16 lanes take a state, 4 C channels each, and go through every 16th state of
+// the piece with a maximum and sums of their own; the workgroup's 16 meet at the end.
+template <int C, int G>
+__global__ __launch_bounds__(256) void cross_few_kernel(const CrossArgs a) {
+  constexpr int U = G * C >= 8 ? 4 : 8;  // states under way
+  __shared__ f32x4 O[4][G][16 * C];
+  __shared__ CrossStat S[4][G];
+  const unsigned item = cross_item();
+  if (item >= a.items) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = tid & 15;
+  const int split = item % a.splits, plane = item / a.splits, b = plane / a.kv, g = plane - b * a.kv;
+  const int from = split * a.piece, to = min(from + a.piece, cross_end(a, b));
+  const float* kb = a.k + (long long)b * a.tk * a.ldk + (long long)g * a.ks;
+  const float* vb = a.v + (long long)b * a.tk * a.ldv + (long long)g * a.vs;
+  int kc[C], vc[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    kc[c] = min(64 * c + 4 * l16, a.kd - 4);
+    vc[c] = min(64 * c + 4 * l16, a.hd - 4);
+  }
+  f32x4 q[G][C], acc[G][C];
+  float top[G], sum[G];
+  const uint8_t* mask[G];
+#pragma unroll
+  for (int r = 0; r < G; ++r) {
+    const int row = min(r, a.rows - 1), qi = row / a.group, head = g * a.group + row - qi * a.group;
+    const float* qr = a.q + ((long long)b * a.tq + qi) * a.ldq + (long long)head * a.qs;
+    mask[r] = cross_mask(a, b, head, qi);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      q[r][c] = 64 * c + 4 * l16 < a.kd ? *(const f32x4*)(qr + kc[c]) : f32x4{0.f, 0.f, 0.f, 0.f};
+      acc[r][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    top[r] = -INFINITY;
+    sum[r] = 0.f;
+  }
+  unsigned any = 0;
+  for (int j0 = from + (tid >> 4); j0 < to; j0 += 16 * U) {
+    f32x4 k[U][C], v[U][C];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const long long j = min(j0 + 16 * u, to - 1);
+        k[u][c] = *(const f32x4*)(kb + j * a.ldk + kc[c]);
+        v[u][c] = *(const f32x4*)(vb + j * a.ldv + vc[c]);
+      }
+#pragma unroll
+    for (int r = 0; r < G; ++r) {
+      float s[U], mx = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float t = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t = __builtin_fmaf(q[r][c][e], k[u][c][e], t);
+        t = plus16(t);
+        bool sees = j0 + 16 * u < to;
+        if (a.mask && sees) sees = mask[r][j0 + 16 * u] != 0;
+        any |= (unsigned)sees << r;
+        s[u] = sees ? t : -INFINITY;
+        mx = fmaxf(mx, s[u]);
+      }
+      mx *= a.c;
+      if (mx > top[r]) {
+        const float x = __builtin_amdgcn_exp2f(top[r] - mx);
+        top[r] = mx;
+        sum[r] *= x;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[r][c][e] *= x;
+      }
+      const float m = top[r] == -INFINITY ? 0.f : top[r];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u], a.c, -m));
+        sum[r] += p;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[r][c][e] = __builtin_fmaf(p, v[u][c][e], acc[r][c][e]);
+      }
+    }
+  }
+  // The wave's four, then the workgroup's waves.
+#pragma unroll
+  for (int r = 0; r < G; ++r) {
+    float t = fmaxf(top[r], __shfl_xor(top[r], 16));
+    t = fmaxf(t, __shfl_xor(t, 32));
+    const float x = top[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[r] - t);
+    // A NaN keeps its place in the sum: x is 1 then or NaN itself.
+    sum[r] *= x;
+    sum[r] += __shfl_xor(sum[r], 16);
+    sum[r] += __shfl_xor(sum[r], 32);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc[r][c][e] *= x;
+        acc[r][c][e] += __shfl_xor(acc[r][c][e], 16);
+        acc[r][c][e] += __shfl_xor(acc[r][c][e], 32);
+      }
+      if (lane < 16) O[wave][r][16 * c + l16] = acc[r][c];
+    }
+    const bool seen = __any(any >> r & 1);
+    if (lane == 0) S[wave][r] = {t, seen && t == -INFINITY ? NAN : sum[r]};
+  }
+  __syncthreads();
+  for (int r = wave; r < min(G, a.rows); r += 4) {
+    const int qi = r / a.group, head = g * a.group + r - qi * a.group;
+    float t = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) t = fmaxf(t, S[w][r].top);
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (S[w][r].sum == 0.f) continue;
+      const float x = __builtin_amdgcn_exp2f(S[w][r].top - t);
+      l = __builtin_fmaf(S[w][r].sum, x, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(O[w][r][min(lane, 16 * C - 1)][e], x, y[e]);
+    }
+    const bool live = lane < 16 * C && 4 * lane < a.hd;
+    if (a.splits > 1) {
+      const long long at = ((long long)plane * a.splits + split) * a.rows + r;
+      if (lane == 0) a.stat[at] = {t, l};
+      if (live) *(f32x4*)(a.part + at * a.hd + 4 * lane) = y;
+      continue;
+    }
+    float* o = a.o + ((long long)b * a.tq + qi) * a.ldo + (long long)head * a.hd;
+    bool again = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      y[e] = l == 0.f ? 0.f : y[e] / l;
+      again |= live && !(__builtin_fabsf(y[e]) <= FLT_MAX);
+    }
+    if (live) *(f32x4*)(o + 4 * lane) = y;
+    if (__any(again)) {
+      float z[2];
+      cross_row(a, b, qi, head, lane, z);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (lane + 64 * x < a.hd) o[lane + 64 * x] = z[x];
+    }
+  }
+}
+
+// Joins the pieces of a row, W lanes to a row: L of them take four channels each of
+// every (W / L)-th piece.
+template <int L, int W>
 __global__ __launch_bounds__(256) void cross_join_kernel(const CrossArgs a, long long rows) {
-  const int lane = threadIdx.x & 63, c = 4 * (threadIdx.x % L);
-  const long long at = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
-  const bool live = at < rows;
-  const long long plane = min(at, rows - 1) / a.rows;
-  const int row = (int)(min(at, rows - 1) - plane * a.rows);
+  constexpr int SG = W / L;
+  const int lane = threadIdx.x & 63, l = lane & (W - 1), c = 4 * (l % L), sg = l / L;
+  const long long at = (long long)blockIdx.x * (256 / W) + threadIdx.x / W;
+  const bool here = at < rows;
+  const long long at1 = here ? at : rows - 1, plane = at1 / a.rows;
+  const int row = (int)(at1 - plane * a.rows);
   const int b = (int)(plane / a.kv), g = (int)(plane - (long long)b * a.kv), qi = row / a.group;
   const int head = g * a.group + row - qi * a.group;
   const CrossStat* stat = a.stat + plane * a.splits * a.rows + row;
   const float* part = a.part + (plane * a.splits * a.rows + row) * a.hd + min(c, a.hd - 4);
   float top = -INFINITY;
-  for (int x = 0; x < a.splits; ++x) top = fmaxf(top, stat[(long long)x * a.rows].top);
+  for (int x = l; x < a.splits; x += W) top = fmaxf(top, stat[(long long)x * a.rows].top);
+#pragma unroll
+  for (int off = W / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
   float sum = 0.f;
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
-  for (int x = 0; x < a.splits; ++x) {
+#pragma unroll 4
+  for (int x = sg; x < a.splits; x += SG) {
     const CrossStat s = stat[(long long)x * a.rows];
-    if (s.sum == 0.f) continue;
-    const float w = __builtin_amdgcn_exp2f(s.top - top);
     const f32x4 p = *(const f32x4*)(part + (long long)x * a.rows * a.hd);
-    sum = __builtin_fmaf(s.sum, w, sum);
+    const bool none = s.sum == 0.f;  // nothing was left there then
+    const float w = __builtin_amdgcn_exp2f(s.top - top);
+    sum = none ? sum : __builtin_fmaf(s.sum, w, sum);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(p[e], w, y[e]);
+    for (int e = 0; e < 4; ++e) y[e] = none ? y[e] : __builtin_fmaf(p[e], w, y[e]);
   }
+#pragma unroll
+  for (int off = L; off < W; off <<= 1) {
+    sum += __shfl_xor(sum, off);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], off);
+  }
+  const bool live = here && l < L && c < a.hd;
   bool again = false;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     y[e] = sum == 0.f ? 0.f : y[e] / sum;
-    again |= live && c < a.hd && !(__builtin_fabsf(y[e]) <= FLT_MAX);
+    again |= live && !(__builtin_fabsf(y[e]) <= FLT_MAX);
   }
-  if (live && c < a.hd) *(f32x4*)(a.o + ((long long)b * a.tq + qi) * a.ldo + (long long)head * a.hd + c) = y;
+  if (live) *(f32x4*)(a.o + ((long long)b * a.tq + qi) * a.ldo + (long long)head * a.hd + c) = y;
   for (unsigned long long todo = __ballot(again); todo;) {
-    const int t = __builtin_ctzll(todo) & ~(L - 1);
+    const int t = __builtin_ctzll(todo) & ~(W - 1);
     const int rb = __shfl(b, t), ri = __shfl(qi, t), rh = __shfl(head, t);
+    float* o = a.o + ((long long)rb * a.tq + ri) * a.ldo + (long long)rh * a.hd;
     float z[2];
     cross_row(a, rb, ri, rh, lane, z);
-    float* o = a.o + ((long long)rb * a.tq + ri) * a.ldo + (long long)rh * a.hd;
 #pragma unroll
     for (int x = 0; x < 2; ++x)
       if (lane + 64 * x < a.hd) o[lane + 64 * x] = z[x];
-    todo &= ~(((1ull << L) - 1) << t);
+    todo &= W == 64 ? 0 : ~(((1ull << (W & 63)) - 1) << t);
   }
 }
 
 typedef void (*CrossKernel)(const CrossArgs);
+#define SY_CROSS_PICK(kernel, ...)                                                                             \
+  ks == 2   ? (dt == 1 ? kernel<2, 1 __VA_ARGS__> : dt == 2 ? kernel<2, 2 __VA_ARGS__> : kernel<2, 4 __VA_ARGS__>) \
+  : ks == 4 ? (dt == 1 ? kernel<4, 1 __VA_ARGS__> : dt == 2 ? kernel<4, 2 __VA_ARGS__> : kernel<4, 4 __VA_ARGS__>) \
+            : (dt == 1 ? kernel<8, 1 __VA_ARGS__> : dt == 2 ? kernel<8, 2 __VA_ARGS__> : kernel<8, 4 __VA_ARGS__>)
+#define SY_COMMA ,
 template <int NW>
-static CrossKernel pick_cross(int kd, int hd) {
-  auto by_hd = [&](CrossKernel d1, CrossKernel d2, CrossKernel d4) { return hd <= 32 ? d1 : hd <= 64 ? d2 : d4; };
-  if (kd <= 32) return by_hd(cross_kernel<2, 1, NW>, cross_kernel<2, 2, NW>, cross_kernel<2, 4, NW>);
-  if (kd <= 64) return by_hd(cross_kernel<4, 1, NW>, cross_kernel<4, 2, NW>, cross_kernel<4, 4, NW>);
-  return by_hd(cross_kernel<8, 1, NW>, cross_kernel<8, 2, NW>, cross_kernel<8, 4, NW>);
+static CrossKernel pick_cross(int ks, int dt) {
+  return SY_CROSS_PICK(cross_kernel, SY_COMMA NW);
+}
+static CrossKernel pick_short(int ks, int dt) { return SY_CROSS_PICK(cross_short_kernel); }
+#undef SY_COMMA
+#undef SY_CROSS_PICK
+static CrossKernel pick_few(int kd, int hd, int rows) {
+  if (std::max(kd, hd) <= 64)
+    return rows == 1 ? cross_few_kernel<1, 1> : rows == 2 ? cross_few_kernel<1, 2>
+           : rows <= 4 ? cross_few_kernel<1, 4> : cross_few_kernel<1, 8>;
+  return rows == 1 ? cross_few_kernel<2, 1> : rows == 2 ? cross_few_kernel<2, 2>
+         : rows <= 4 ? cross_few_kernel<2, 4> : cross_few_kernel<2, 8>;
+}
+
+// Waves of a workgroup and pieces of the states: the least estimated time, in cycles.  A wave's
+// tile takes 192 (ks + 2 dt) of the matrix cores, about 850 of other vector work and its share of
+// splitting the states; the waves of a SIMD overlap by a quarter; loads and barrier take 2,500 (of eight waves 3,200) anyway.
+static void cross_plan(CrossArgs& a, int ks, int dt, long long planes, long long row_tiles, int* nw) {
+  const int cus = 256, s = ks + 2 * dt;
+  const long long key_tiles = (a.tk + kCrossKeys - 1) / kCrossKeys;
+  double best = INFINITY;
+  for (int w : {4, 8}) {
+    // Workgroups to a CU, as their registers allow.
+    const int there = w == 8 || s == 16 ? 1 : s <= 6 && ks == 2 ? 3 : 2;
+    const long long whole = planes * ((row_tiles + w - 1) / w);
+    for (long long x = 1; x <= std::max<long long>(1, std::min<long long>(64, key_tiles / 2)); ++x) {
+      const long long rounds = (whole * x + cus * there - 1) / (cus * there);
+      const long long together = std::min<long long>(there, (whole * x + cus - 1) / cus);
+      const double tile =
+          std::max(w == 8 ? 3200.0 : 2500.0, 0.75 * together * w / 4 * (192.0 * s + 850 + 200.0 * s / w));
+      const double join = x > 1 ? 10000 + 0.5 * planes * a.rows * x / 256 : 0;
+      const double time = rounds * ((key_tiles + x - 1) / x + 3) * tile + join;
+      if (time < best) {
+        best = time;
+        *nw = w;
+        a.tiles = (int)((row_tiles + w - 1) / w);
+        a.splits = (int)x;
+      }
+    }
+  }
 }
 
 int op_cross_attention(sy_ctx* ctx, const sy_cross_config* c, const sy_tensor* q, const sy_tensor* k,
@@ -448,17 +840,26 @@ int op_cross_attention(sy_ctx* ctx, const sy_cross_config* c, const sy_tensor* q
   a.c = c->scale * 1.4426950408889634f;
   a.rows = a.tq * a.group;
   const long long planes = (long long)q->n * a.kv;
-  static const int kNw = getenv("NW") ? atoi(getenv("NW")) : 0;
-  const int nw = a.rows <= 64 ? 1 : kNw ? kNw : a.rows <= 128 ? 4 : 8;
-  a.tiles = (a.rows + 32 * nw - 1) / (32 * nw);
-  const long long whole = planes * a.tiles;
-  // Pieces: where the rows alone leave CUs without work, of four tiles and more.
-  const long long want = (nw == 1 ? 2048 : nw == 4 ? 768 : 384) / whole;
-  a.splits = (int)std::max<long long>(1, std::min<long long>(want, a.tk / (4 * kCrossKeys)));
+  const int ks = a.kd <= 32 ? 2 : a.kd <= 64 ? 4 : 8, dt = a.hd <= 32 ? 1 : a.hd <= 64 ? 2 : 4;
+  int nw = 0;  // waves that share a tile's states; 0: few rows, or few states
+  const long long row_tiles = (a.rows + 31) / 32;
+  const bool few = a.rows <= 8;
+  const bool brief = !few && (a.tk + kCrossKeys - 1) / kCrossKeys * short_bytes(ks, dt) <= kShortLds && row_tiles * planes >= 2048;
+  a.splits = 1;
+  if (few) {
+    a.tiles = 1;
+    a.splits = (int)std::max<long long>(1, std::min<long long>(256 / planes, a.tk / 256));
+  } else if (brief) {
+    a.run = (int)std::max<long long>(8, (row_tiles * planes + 511) / 512);
+    a.run = (a.run + kShortWaves - 1) / kShortWaves * kShortWaves;
+    a.tiles = (int)((row_tiles + a.run - 1) / a.run);
+  } else {
+    cross_plan(a, ks, dt, planes, row_tiles, &nw);
+  }
   a.piece = ((a.tk + a.splits - 1) / a.splits + kCrossKeys - 1) / kCrossKeys * kCrossKeys;
   a.splits = (a.tk + a.piece - 1) / a.piece;
-  const long long items = whole * a.splits, grid = (items + 7) / 8 * 8;
-  SY_CHECK(grid * nw * 64 < (1LL << 32), SY_EUNSUPPORTED, "cross attention over %lld rows", planes * a.rows);
+  const long long items = planes * a.tiles * a.splits, grid = (items + 7) / 8 * 8;
+  SY_CHECK(grid * 512 < (1LL << 32), SY_EUNSUPPORTED, "cross attention over %lld rows", planes * a.rows);
   a.items = (unsigned)items;
   DeviceScope device(ctx);
   if (a.splits > 1) {
@@ -472,17 +873,27 @@ int op_cross_attention(sy_ctx* ctx, const sy_cross_config* c, const sy_tensor* q
     const double scores = (double)q->n * a.heads * a.tq * a.tk;
     ProfScope prof(ctx, "cross_attention", 2 * scores * (a.kd + a.hd),
                    4.0 * q->n * ((double)a.tq * a.heads + (double)a.tk * a.kv) * (a.kd + a.hd));
-    CrossKernel kernel = nw == 1 ? pick_cross<1>(a.kd, a.hd) : nw == 4 ? pick_cross<4>(a.kd, a.hd) : pick_cross<8>(a.kd, a.hd);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(nw * 64), 0, ctx->stream, a);
+    CrossKernel kernel = few     ? pick_few(a.kd, a.hd, a.rows)
+                         : brief ? pick_short(ks, dt)
+                         : nw == 4 ? pick_cross<4>(ks, dt)
+                                   : pick_cross<8>(ks, dt);
+    const int threads = few ? 256 : brief ? kShortWaves * 64 : nw * 64;
+    const size_t lds = brief ? (size_t)(a.tk + kCrossKeys - 1) / kCrossKeys * short_bytes(ks, dt) : 0;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, ctx->stream, a);
     SY_TRY(check_launch("cross_attention"));
   }
   if (a.splits > 1) {
     const long long rows = planes * a.rows;
     ProfScope prof(ctx, "cross_join", 0, 4.0 * rows * a.hd * (a.splits + 1));
-    if (a.hd <= 64)
-      hipLaunchKernelGGL(cross_join_kernel<16>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, ctx->stream, a, rows);
-    else
-      hipLaunchKernelGGL(cross_join_kernel<32>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, ctx->stream, a, rows);
+    // A wave to a row from 8 pieces on: 2,400 rows of 32 pieces 3.9 us against 10 of 16 lanes to a row.
+    auto join = a.splits < 8 ? (a.hd <= 32   ? cross_join_kernel<8, 8>
+                                : a.hd <= 64 ? cross_join_kernel<16, 16>
+                                             : cross_join_kernel<32, 32>)
+                             : (a.hd <= 32   ? cross_join_kernel<8, 64>
+                                : a.hd <= 64 ? cross_join_kernel<16, 64>
+                                             : cross_join_kernel<32, 64>);
+    const int each = a.splits >= 8 ? 4 : a.hd <= 32 ? 32 : a.hd <= 64 ? 16 : 8;  // rows of a workgroup
+    hipLaunchKernelGGL(join, dim3((unsigned)((rows + each - 1) / each)), dim3(256), 0, ctx->stream, a, rows);
     SY_TRY(check_launch("cross_join"));
   }
   return SY_OK;
