@@ -93,68 +93,102 @@ __device__ __forceinline__ void pair8(const float (&x)[8], float s, u32x4& h, u3
   }
 }
 
-// A panel of 32 rows per workgroup, 16 lanes to a row: its largest element, then its
-// pairs; the first kHeld octets of a lane stay in registers between.  Rows past the last are zeros.
-// `more`: the panel's flag is that of an earlier call, too.
-constexpr int kHeld = 2;
+// A panel of 32 rows per workgroup, in lots of kLot elements: a wave takes every eighth row in
+// whole lines, a lane four elements; the first kHeld lots stay in registers between the search for
+// the rows' largest and the split.  Fragments leave through LDS, in whole lines too.  Rows past the last are
+// zeros.  `more`: the panel's flag is that of an earlier call, too.
+constexpr int kLot = 256, kLotSteps = kLot / 16, kHeld = 4;
 __global__ __launch_bounds__(512) void gated_split_kernel(const float* x, long long ldx, int rows, int ic, int steps,
                                                           bool quads, u32x4* out, int* words, int* plain, int stride,
                                                           int offset, bool more) {
+  __shared__ u32x4 lds[2][kLotSteps * kStep];
   __shared__ int any;
-  const int r = threadIdx.x >> 4, q = threadIdx.x & 15;
-  const long long row = (long long)blockIdx.x * 32 + r;
-  const long long panel = (long long)blockIdx.x * stride + offset;
-  const float* xr = x + min(row, (long long)rows - 1) * ldx;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long row0 = (long long)blockIdx.x * 32, panel = (long long)blockIdx.x * stride + offset;
+  const int lots = (steps + kLotSteps - 1) / kLotSteps;
   if (threadIdx.x == 0) any = more ? plain[blockIdx.x] : 0;
-  __syncthreads();
-  unsigned top = 0, low = 0x7fffffffu;
-  float held[kHeld][8];
-  auto look = [&](const float(&v)[8]) {
+  auto load = [&](int lot, float (&v)[4][4]) __attribute__((always_inline)) {
+    const int c = lot * kLot + 4 * lane;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const unsigned m = magnitude(v[e]);
-      top = max(top, m);
-      low = min(low, m ? m : 0x7fffffffu);
+    for (int i = 0; i < 4; ++i) {
+      const float* xr = x + min(row0 + wave + 8 * i, (long long)rows - 1) * ldx;
+      if (quads) {
+        const f32x4 t = *(const f32x4*)(xr + min(c, ic - 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][e] = t[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][e] = xr[min(c + e, ic - 1)];
+      }
     }
+    if (c + 4 > ic)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][e] = c + e < ic ? v[i][e] : 0.f;
   };
+  unsigned top[4] = {}, low[4];
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i)
-    if (q + 16 * i < 2 * steps) load8(xr, 8 * (q + 16 * i), ic, quads, held[i]);
+  for (int i = 0; i < 4; ++i) low[i] = 0x7fffffffu;
+  auto look = [&](const float(&v)[4][4]) __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i)
-    if (q + 16 * i < 2 * steps) look(held[i]);
-  for (int o = q + 16 * kHeld; o < 2 * steps; o += 16) {
-    float v[8];
-    load8(xr, 8 * o, ic, quads, v);
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned m = magnitude(v[i][e]);
+        top[i] = max(top[i], m);
+        low[i] = min(low[i], m ? m : 0x7fffffffu);
+      }
+  };
+  float held[kHeld][4][4];
+#pragma unroll
+  for (int l = 0; l < kHeld; ++l)
+    if (l < lots) load(l, held[l]);
+#pragma unroll
+  for (int l = 0; l < kHeld; ++l)
+    if (l < lots) look(held[l]);
+  for (int l = kHeld; l < lots; ++l) {
+    float v[4][4];
+    load(l, v);
     look(v);
   }
+  __syncthreads();  // `any` stands
+  float scale[4];
 #pragma unroll
-  for (int off = 1; off < 16; off <<= 1) {
-    top = max(top, (unsigned)__shfl_xor((int)top, off));
-    low = min(low, (unsigned)__shfl_xor((int)low, off));
+  for (int i = 0; i < 4; ++i) {
+    const unsigned t = (unsigned)wave_max_i32((int)top[i]);
+    const unsigned l = 0x7fffffffu - (unsigned)wave_max_i32((int)(0x7fffffffu - low[i]));
+    const bool here = row0 + wave + 8 * i < rows, bad = here && uneven(t, l);
+    const int field = gated_field(t);
+    scale[i] = here ? exp_float(field) : 0.f;
+    if (lane == 0) {
+      words[panel * 32 + wave + 8 * i] = field | (bad ? kPlainRow : 0);
+      if (bad) any = 1;
+    }
   }
-  if (row >= rows) top = 0, low = 0x7fffffffu;
-  const bool bad = uneven(top, low);
-  const int field = bad && top >> 23 == 255 ? 127 : gated_field(top);
-  if (q == 0) {
-    words[panel * 32 + r] = field | (bad ? kPlainRow : 0);
-    if (bad) any = 1;
-  }
-  const float s = row < rows ? exp_float(field) : 0.f;
   u32x4* to = out + panel * steps * kStep;
-  auto put = [&](int o, const float(&v)[8]) {
-    u32x4 h, l;
-    pair8(v, s, h, l);
-    to[(o >> 1) * kStep + (o & 1) * 32 + r] = h;
-    to[(o >> 1) * kStep + 64 + (o & 1) * 32 + r] = l;
+  auto put = [&](int lot, const float(&v)[4][4]) __attribute__((always_inline)) {
+    u32x4* at_lds = lds[lot & 1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u32x2 h, l;
+      split4(f32x4{v[i][0], v[i][1], v[i][2], v[i][3]}, scale[i], h, l);
+      // Elements 4 lane .. + 3: step lane / 4, half (lane / 2) % 2, its first or second four.
+      u32x2* at = (u32x2*)(at_lds + (lane >> 2) * kStep + ((lane >> 1) & 1) * 32 + wave + 8 * i) + (lane & 1);
+      at[0] = h;
+      at[128] = l;
+    }
+    __syncthreads();
+    const int units = min(kLotSteps, steps - lot * kLotSteps) * kStep;
+    for (int u = threadIdx.x; u < units; u += 512) to[lot * kLotSteps * kStep + u] = at_lds[u];
   };
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i)
-    if (q + 16 * i < 2 * steps) put(q + 16 * i, held[i]);
-  for (int o = q + 16 * kHeld; o < 2 * steps; o += 16) {
-    float v[8];
-    load8(xr, 8 * o, ic, quads, v);
-    put(o, v);
+  for (int l = 0; l < kHeld; ++l)
+    if (l < lots) put(l, held[l]);
+  for (int l = kHeld; l < lots; ++l) {
+    float v[4][4];
+    load(l, v);
+    put(l, v);
   }
   __syncthreads();
   if (threadIdx.x == 0) plain[blockIdx.x] = any;
@@ -201,13 +235,15 @@ __device__ __forceinline__ void gated_plain(const GatedArgs& a, long long row0, 
   }
 }
 
-// WM x WN waves, each 64 rows by 32 output channels (gate and up): x and the weights
-// arrive split, in the order of the matrix instruction's lanes; two steps at a time
-// go through LDS, two stages in turn with one barrier between.
+// WM x WN waves, each two panels of rows by 32 output channels (gate and up): x and the weights
+// arrive split, in the order of the matrix instruction's lanes.  x goes through LDS, two
+// steps at a time, two stages in turn; the weights straight into registers, a stage ahead: with both in LDS
+// its ports are busy as long as the matrix cores.  A step's fragments of x are read while the one before it
+// is multiplied, over the barrier too: it stands before a stage's last products.
 template <int WM, int WN>
 __global__ __launch_bounds__(WM* WN * 64, 2) void gated_kernel(const GatedArgs a) {
-  constexpr int NW = WM * WN, PA = 2 * WM, PB = 2 * WN;  // panels of x and of the weights
-  constexpr int CHUNKS = 4 * (PA + PB), IT = CHUNKS / NW;   // 1 KB each
+  constexpr int TM = 2, NW = WM * WN, PA = TM * WM;
+  constexpr int CHUNKS = 4 * PA, IT = CHUNKS / NW;  // of x, 1 KB each
   static_assert(CHUNKS % NW == 0, "whole chunks to a wave");
   __shared__ u32x4 frag[2][CHUNKS][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -221,14 +257,14 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_kernel(const GatedArgs a
   const u32x4* src[IT];
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    const int c = wave + i * NW, p = c >> 2;
-    const u32x4* base = p < PA ? a.xs + (long long)min(rt * PA + p, a.xpanels - 1) * a.steps * kStep
-                               : a.w + (long long)min(ct * PB + p - PA, 2 * a.panels - 1) * a.steps * kStep;
-    src[i] = base + (c & 3) * 64 + lane;
+    const int c = wave + i * NW;
+    src[i] = a.xs + (long long)min(rt * PA + (c >> 2), a.xpanels - 1) * a.steps * kStep + (c & 3) * 64 + lane;
   }
-  f32x16 acc[2][2], crs[2][2];
+  const u32x4* w = a.w + 2LL * min(ct * WN + wn, a.panels - 1) * a.steps * kStep + lane;
+  const long long up = (long long)a.steps * kStep;
+  f32x16 acc[TM][2], crs[TM][2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -242,38 +278,55 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_kernel(const GatedArgs a
 #pragma unroll
     for (int i = 0; i < IT; ++i) frag[buf][wave + i * NW][lane] = reg[i];
   };
+  f16x8 av[2][TM][2], bv[2][2][2];
+  auto wload = [&](int s, int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) bv[k][j][p] = __builtin_bit_cast(f16x8, w[j * up + (2 * s + k) * kStep + 64 * p]);
+  };
+  auto fetch = [&](int buf, int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+        av[k][i][p] = __builtin_bit_cast(f16x8, frag[buf][(wm * TM + i) * 4 + 2 * k + p][lane]);
+  };
+  auto multiply = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        crs[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av[k][i][1], bv[k][j][0], crs[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av[k][i][0], bv[k][j][0], acc[i][j], 0, 0, 0);
+      }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        crs[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av[k][i][0], bv[k][j][1], crs[i][j], 0, 0, 0);
+  };
   const int stages = a.steps / 2;
   gload(0);
+  wload(0, 0);
+  wload(0, 1);
   put(0);
+  gload(min(1, stages - 1));
   __syncthreads();
+  fetch(0, 0);
   for (int s = 0; s < stages; ++s) {
-    if (s + 1 < stages) gload(s + 1);
-    const u32x4(*f)[64] = frag[s & 1];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      f16x8 av[2][2], bv[2][2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          av[i][p] = __builtin_bit_cast(f16x8, f[(wm * 2 + i) * 4 + 2 * k + p][lane]);
-          bv[i][p] = __builtin_bit_cast(f16x8, f[(PA + wn * 2 + i) * 4 + 2 * k + p][lane]);
-        }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          crs[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av[i][1], bv[j][0], crs[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av[i][0], bv[j][0], acc[i][j], 0, 0, 0);
-        }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          crs[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av[i][0], bv[j][1], crs[i][j], 0, 0, 0);
-    }
-    if (s + 1 < stages) put((s + 1) & 1);
+    const int buf = s & 1, next = min(s + 1, stages - 1);
+    fetch(buf, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(0);
+    wload(next, 0);
+    put(buf ^ 1);  // the last stage's again, past the end
+    gload(min(s + 2, stages - 1));
     __syncthreads();
+    fetch(buf ^ 1, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(1);
+    wload(next, 1);
   }
 
   const int panel = ct * WN + wn, col = 32 * panel + r32;
@@ -282,8 +335,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_kernel(const GatedArgs a
   const float gb = a.bias[col], ub = a.bias[a.panels * 32 + col];
   const int gw = a.w_row[panel * 64 + r32] & 0xff, uw = a.w_row[panel * 64 + 32 + r32] & 0xff;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int xp = (rt * WM + wm) * 2 + i;
+  for (int i = 0; i < TM; ++i) {
+    const int xp = (rt * WM + wm) * TM + i;
     if (xp >= a.xpanels) return;
     f32x16 g, u;
     if (a.x_plain[xp] | a.w_plain[panel]) {
@@ -307,143 +360,264 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_kernel(const GatedArgs a
   }
 }
 
-// Few tiles: TM panels of rows and 32 output channels to a workgroup, the steps shared
-// out over its NK waves, both operands straight from memory into the matrix
-// instruction's registers, kAhead steps of them under way.  A wave splits its own share of x,
-// under powers of that share's rows, and is plain by itself.
-constexpr int kAhead = 4;
-template <int TM, int NK>
-__global__ __launch_bounds__(NK * 64) void gated_few_kernel(const GatedArgs a) {
-  __shared__ float sums[NK][2][TM * 32][33];
+// 16 x 16 gate and up sums of a wave in plain float32, over elements k0 .. k0 + 31 of the
+// rows from row0 and the channels from col0, added to acc.
+__device__ __forceinline__ void gated_plain16(const GatedArgs& a, int row0, int col0, int k0, int lane, f32x4 (&acc)[2]) {
+  const int row = row0 + (lane & 15), col = col0 + (lane & 15);
+  const float* x = a.x + (long long)min(row, a.rows - 1) * a.ldx;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int c = k0 + 16 * h + 4 * (lane >> 4);
+    f32x4 xv;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) xv[e] = row < a.rows && c + e < a.ic ? x[c + e] : 0.f;
+    const f32x4 g = gated_weights(a, 0, col, c), u = gated_weights(a, 1, col, c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      acc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[e], g[e], acc[0], 0, 0, 0);
+      acc[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[e], u[e], acc[1], 0, 0, 0);
+    }
+  }
+}
+
+// Few rows: 16 of them by 16 output channels to a workgroup, the steps shared out over its eight
+// waves, both operands straight from memory into the matrix instruction's registers, kAhead
+// pairs of steps at once.  A wave splits x itself, under powers of the pairs of steps it has in
+// hand, and brings each lot's sums to their true scale; a lot with an uneven row is plain by itself.
+constexpr int kFewWaves = 8, kAhead = 4;
+__global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const GatedArgs a) {
+  __shared__ float sums[kFewWaves][2][16][17];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int half = lane >> 5, r32 = lane & 31;
-  const int tile = blockIdx.x / a.panels, panel = blockIdx.x - tile * a.panels, row0 = tile * TM * 32;
-  const int share = (a.steps + NK - 1) / NK, k0 = min(wave * share, a.steps), k1 = min(k0 + share, a.steps);
-  const u32x4* w = a.w + (long long)2 * panel * a.steps * kStep + lane;
+  const int r16 = lane & 15, oct = lane >> 4;  // row or channel; elements 8 oct .. 8 oct + 7 of a pair of steps
+  const int tile = blockIdx.x / (2 * a.panels), rest = blockIdx.x - tile * 2 * a.panels, row0 = 16 * tile;
+  const int panel = rest >> 1, sub = (rest & 1) * 16, pairs = a.steps / 2;
+  const int share = (pairs + kFewWaves - 1) / kFewWaves, p0 = min(wave * share, pairs), p1 = min(p0 + share, pairs);
+  // A fragment's unit: step oct / 2, half oct % 2, channel sub + r16.
+  const u32x4* w = a.w + (long long)2 * panel * a.steps * kStep + (oct >> 1) * kStep + (oct & 1) * 32 + sub + r16;
   const long long up = (long long)a.steps * kStep;
+  const float* xr = a.x + (long long)min(row0 + r16, a.rows - 1) * a.ldx;
   const int w_plain = a.w_plain[panel];
-  const float* xr[TM];
+  const int wf[2] = {a.w_row[panel * 64 + sub + r16] & 0xff, a.w_row[panel * 64 + 32 + sub + r16] & 0xff};
+  f32x4 total[2] = {};
+  for (int p = p0; p < p1; p += kAhead) {
+    f16x8 wv[kAhead][2][2];
+    float xv[kAhead][8];
 #pragma unroll
-  for (int i = 0; i < TM; ++i) xr[i] = a.x + (long long)min(row0 + 32 * i + r32, a.rows - 1) * a.ldx;
-  f16x8 wv[kAhead][2][2];
-  float xv[kAhead][TM][8];
-  auto load_w = [&](int k) __attribute__((always_inline)) {
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u)
+    for (int u = 0; u < kAhead; ++u) {
+      const long long at = (long long)min(p + u, pairs - 1) * 2 * kStep;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int p = 0; p < 2; ++p)
-          wv[u][j][p] = __builtin_bit_cast(f16x8, w[j * up + (long long)min(k + u, a.steps - 1) * kStep + 64 * p]);
-  };
-  auto load_x = [&](int k) __attribute__((always_inline)) {
+        for (int s = 0; s < 2; ++s) wv[u][j][s] = __builtin_bit_cast(f16x8, w[j * up + at + 64 * s]);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) load8(xr, min(p + u, pairs) * 32 + 8 * oct, a.ic, a.quads, xv[u]);
+    unsigned top = 0, low = 0x7fffffffu;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-      for (int i = 0; i < TM; ++i) load8(xr[i], min(k + u, a.steps) * 16 + 8 * half, a.ic, a.quads, xv[u][i]);
-  };
-  f32x16 acc[TM][2], crs[TM][2];
+      for (int e = 0; e < 8; ++e) {
+        const unsigned m = p + u < p1 ? magnitude(xv[u][e]) : 0;
+        top = max(top, m);
+        low = min(low, m ? m : 0x7fffffffu);
+      }
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
+    for (int off = 16; off < 64; off <<= 1) {
+      top = max(top, (unsigned)__shfl_xor((int)top, off));
+      low = min(low, (unsigned)__shfl_xor((int)low, off));
+    }
+    if (__any(w_plain != 0 || uneven(top, low))) {
+      for (int u = p; u < min(p + kAhead, p1); ++u) gated_plain16(a, row0, 32 * panel + sub, 32 * u, lane, total);
+      continue;
+    }
+    const int field = gated_field(top);
+    const float scale = exp_float(field);
+    f32x4 acc[2] = {}, crs[2] = {};
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int u = 0; u < kAhead; ++u) {
+      u32x4 h, l;
+      pair8(xv[u], p + u < p1 ? scale : 0.f, h, l);
+      const f16x8 xh = __builtin_bit_cast(f16x8, h), xl = __builtin_bit_cast(f16x8, l);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = crs[i][j][r] = 0.f;
-  unsigned top[TM] = {}, low[TM];
+      for (int j = 0; j < 2; ++j) {
+        crs[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, wv[u][j][0], crs[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, wv[u][j][0], acc[j], 0, 0, 0);
+        crs[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, wv[u][j][1], crs[j], 0, 0, 0);
+      }
+    }
+    // Lane r's field is that of row r; the lane's sums are rows 4 oct .. 4 oct + 3 of channel r16.
 #pragma unroll
-  for (int i = 0; i < TM; ++i) low[i] = 0x7fffffffu;
-  if (k0 < k1) {
-    load_w(k0);
-    // The share's largest and smallest elements, from behind, so that its first steps stay in registers.
-    for (int k = k0 + (k1 - k0 - 1) / kAhead * kAhead; k >= k0; k -= kAhead) {
-      load_x(k);
+    for (int r = 0; r < 4; ++r) {
+      const int f = __shfl(field, 4 * oct + r);
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const unsigned m = k + u < k1 ? magnitude(xv[u][i][e]) : 0;
-            top[i] = max(top[i], m);
-            low[i] = min(low[i], m ? m : 0x7fffffffu);
-          }
+      for (int j = 0; j < 2; ++j)
+        total[j][r] += __builtin_ldexpf(__builtin_fmaf(crs[j][r], 1.f / 2048, acc[j][r]), 254 - f - wf[j]);
     }
   }
-  bool plain = w_plain != 0;
-  int field[TM];
-  float scale[TM];
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    top[i] = max(top[i], (unsigned)__shfl_xor((int)top[i], 32));
-    low[i] = min(low[i], (unsigned)__shfl_xor((int)low[i], 32));
-    plain |= uneven(top[i], low[i]);
-    field[i] = gated_field(top[i]);
-    scale[i] = exp_float(field[i]);
-  }
-  if (__any(plain)) {
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int i = 0; i < TM; ++i) gated_plain(a, row0 + 32 * i, panel, k0, k1, lane, acc[i]);
-  } else {
-    for (int k = k0; k < k1; k += kAhead) {
-      f16x8 xp[kAhead][TM][2], wp[kAhead][2][2];
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          u32x4 h, l;
-          pair8(xv[u][i], k + u < k1 ? scale[i] : 0.f, h, l);
-          xp[u][i][0] = __builtin_bit_cast(f16x8, h);
-          xp[u][i][1] = __builtin_bit_cast(f16x8, l);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int p = 0; p < 2; ++p) wp[u][j][p] = wv[u][j][p];
-      }
-      if (k + kAhead < k1) {
-        load_w(k + kAhead);
-        load_x(k + kAhead);
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            crs[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xp[u][i][1], wp[u][j][0], crs[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xp[u][i][0], wp[u][j][0], acc[i][j], 0, 0, 0);
-            crs[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xp[u][i][0], wp[u][j][1], crs[i][j], 0, 0, 0);
-          }
-    }
-    // Lane r's field is that of row r.
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int f = __shfl(field[i], 8 * (r >> 2) + 4 * half + (r & 3));
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          acc[i][j][r] = __builtin_ldexpf(__builtin_fmaf(crs[i][j][r], 1.f / 2048, acc[i][j][r]),
-                                          254 - f - (a.w_row[panel * 64 + 32 * j + r32] & 0xff));
-      }
-  }
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sums[wave][j][32 * i + 8 * (r >> 2) + 4 * half + (r & 3)][r32] = acc[i][j][r];
+    for (int r = 0; r < 4; ++r) sums[wave][j][4 * oct + r][r16] = total[j][r];
   __syncthreads();
-  const int rows = min(TM * 32, a.rows - row0), col = 32 * panel + r32;
+  const int row = threadIdx.x >> 4, col = 32 * panel + sub + r16;
+  if (row >= 16 || row0 + row >= a.rows) return;
+  float g = 0.f, u = 0.f;
+#pragma unroll
+  for (int x = 0; x < kFewWaves; ++x) {
+    g += sums[x][0][row][r16];
+    u += sums[x][1][row][r16];
+  }
+  if (col < a.oc) a.y[(row0 + row) * a.ldy + col] = activate(a.act, g + a.bias[col]) * (u + a.bias[a.panels * 32 + col]);
+}
+
+// A middling number of tiles: a panel of rows by PAN panels of output channels to a workgroup, each
+// panel's steps shared out over 8 / PAN waves.  x goes through LDS in lots of kLot elements, two
+// in turn, loaded row by row in whole lines and split by the workgroup itself (a kernel of its own would
+// cost more than the products); weights come straight from memory.
+template <int PAN>
+__global__ __launch_bounds__(512, 2) void gated_mid_kernel(const GatedArgs a) {
+  constexpr int KW = 8 / PAN, SH = kLotSteps / KW;  // waves of a panel, their steps of a lot
+  constexpr int LOT = kLotSteps * kStep;
+  __shared__ u32x4 lds[2][LOT];
+  __shared__ float sums[8][2][32][33];
+  __shared__ int fields[32];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, r32 = lane & 31, part = wave % KW;
+  const int cols = (a.panels + PAN - 1) / PAN, tile = blockIdx.x / cols, first = (blockIdx.x - tile * cols) * PAN;
+  const int panel = min(first + wave / KW, a.panels - 1), row0 = tile * 32;
+  const u32x4* w = a.w + (long long)2 * panel * a.steps * kStep + lane;
+  const long long up = (long long)a.steps * kStep;
+  // A wave takes every eighth row, a lane four elements of it.
+  float v[4][4];
+  auto load = [&](int k0) __attribute__((always_inline)) {
+    const int c = 16 * k0 + 4 * lane;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float* x = a.x + (long long)min(row0 + wave + 8 * i, a.rows - 1) * a.ldx;
+      if (a.quads) {
+        const f32x4 t = *(const f32x4*)(x + min(c, a.ic - 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][e] = t[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][e] = x[min(c + e, a.ic - 1)];
+      }
+    }
+    if (c + 4 > a.ic)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][e] = c + e < a.ic ? v[i][e] : 0.f;
+  };
+  // Weights of steps k and on, four at a time.
+  f16x8 wv[4][2][2];
+  auto load_w = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          wv[u][j][s] = __builtin_bit_cast(f16x8, w[j * up + (long long)min(k + u, a.steps - 1) * kStep + 64 * s]);
+  };
+  // The rows' powers, from their last lot to the first, which stays in registers.
+  unsigned top[4] = {}, low[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) low[i] = 0x7fffffffu;
+  for (int k0 = (a.steps - 1) / kLotSteps * kLotSteps; k0 >= 0; k0 -= kLotSteps) {
+    load(k0);
+    if (k0 == 0) load_w(part * SH);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned m = magnitude(v[i][e]);
+        top[i] = max(top[i], m);
+        low[i] = min(low[i], m ? m : 0x7fffffffu);
+      }
+  }
+  float scale[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned t = (unsigned)wave_max_i32((int)top[i]);
+    const unsigned l = 0x7fffffffu - (unsigned)wave_max_i32((int)(0x7fffffffu - low[i]));
+    const int field = gated_field(t);
+    scale[i] = exp_float(field);
+    if (lane == 0) fields[wave + 8 * i] = field | (uneven(t, l) ? kPlainRow : 0);
+  }
+  auto put = [&](u32x4* to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u32x2 h, l;
+      split4(f32x4{v[i][0], v[i][1], v[i][2], v[i][3]}, scale[i], h, l);
+      // Elements 4 lane .. + 3: step lane / 4, half (lane / 2) % 2, its first or second four.
+      u32x2* at = (u32x2*)(to + (lane >> 2) * kStep + ((lane >> 1) & 1) * 32 + wave + 8 * i) + (lane & 1);
+      at[0] = h;
+      at[128] = l;
+    }
+  };
+  put(lds[0]);
+  f32x16 acc[2], crs[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[j][r] = crs[j][r] = 0.f;
+  __syncthreads();
+  int now = 0;
+  for (int k0 = 0; k0 < a.steps; k0 += kLotSteps, now ^= 1) {
+    const bool more = k0 + kLotSteps < a.steps;
+    if (more) load(k0 + kLotSteps);
+#pragma unroll
+    for (int u = 0; u < SH; ++u) {
+      const int k = part * SH + u;
+      if (k0 + k < a.steps) {
+        const u32x4* f = lds[now] + k * kStep + lane;
+        const f16x8 xh = __builtin_bit_cast(f16x8, f[0]), xl = __builtin_bit_cast(f16x8, f[64]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          crs[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xl, wv[u & 3][j][0], crs[j], 0, 0, 0);
+          acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, wv[u & 3][j][0], acc[j], 0, 0, 0);
+          crs[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, wv[u & 3][j][1], crs[j], 0, 0, 0);
+        }
+      }
+      if ((u & 3) == 3) load_w(u + 1 < SH ? k0 + k + 1 : k0 + kLotSteps + part * SH);
+    }
+    if (more) put(lds[now ^ 1]);
+    __syncthreads();
+  }
+  if (__any(fields[r32] & kPlainRow) || a.w_plain[panel]) {
+    const int share = (a.steps + KW - 1) / KW;
+    gated_plain(a, row0, panel, min(part * share, a.steps), min((part + 1) * share, a.steps), lane, acc);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int f = fields[8 * (r >> 2) + 4 * half + (r & 3)];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        acc[j][r] = __builtin_ldexpf(__builtin_fmaf(crs[j][r], 1.f / 2048, acc[j][r]),
+                                     254 - f - (a.w_row[panel * 64 + 32 * j + r32] & 0xff));
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sums[wave][j][8 * (r >> 2) + 4 * half + (r & 3)][r32] = acc[j][r];
+  __syncthreads();
+  if (first + wave / KW >= a.panels) return;
+  const int col = 32 * panel + r32;
+  if (col >= a.oc) return;
   const float gb = a.bias[col], ub = a.bias[a.panels * 32 + col];
-  for (int row = threadIdx.x >> 5; row < rows; row += NK * 2) {
+#pragma unroll
+  for (int i = 0; i < 16 / KW; ++i) {
+    const int row = 2 * (KW * i + part) + half;
+    if (row0 + row >= a.rows) break;
     float g = 0.f, u = 0.f;
 #pragma unroll
-    for (int x = 0; x < NK; ++x) {
-      g += sums[x][0][row][r32];
-      u += sums[x][1][row][r32];
+    for (int x = 0; x < KW; ++x) {
+      g += sums[wave - part + x][0][row][r32];
+      u += sums[wave - part + x][1][row][r32];
     }
-    if (col < a.oc) a.y[(row0 + row) * a.ldy + col] = activate(a.act, g + gb) * (u + ub);
+    a.y[(row0 + row) * a.ldy + col] = activate(a.act, g + gb) * (u + ub);
   }
 }
 
@@ -561,16 +735,23 @@ int op_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tenso
   a.xpanels = (a.rows + 31) / 32;
   DeviceScope device(ctx);
   const double flops = 4.0 * rows * p.ic * p.oc, bytes = 4.0 * ((double)rows * (p.ic + p.oc) + 2.0 * p.ic * p.oc);
-  static const int kFew = getenv("FEW") ? atoi(getenv("FEW")) : 0;
-  if (a.rows <= 32 || kFew) {
+  // 32 rows of 1024 to 2816 channels 13.3 us here, 17.6 as a middling number of tiles; 33 of 2048 to 4096 47.7 and 32.4.
+  if (a.rows <= 32) {
     ProfScope prof(ctx, "gated_few", flops, bytes);
-    const int tm = kFew ? kFew / 10 : 1, nk = kFew ? kFew % 10 : 8;
-    const dim3 grid((unsigned)(p.panels * ((a.xpanels + tm - 1) / tm)));
-    if (tm == 1 && nk == 8) hipLaunchKernelGGL((gated_few_kernel<1, 8>), grid, dim3(nk * 64), 0, ctx->stream, a);
-    if (tm == 1 && nk == 4) hipLaunchKernelGGL((gated_few_kernel<1, 4>), grid, dim3(nk * 64), 0, ctx->stream, a);
-    if (tm == 2 && nk == 4) hipLaunchKernelGGL((gated_few_kernel<2, 4>), grid, dim3(nk * 64), 0, ctx->stream, a);
-    if (tm == 2 && nk == 8) hipLaunchKernelGGL((gated_few_kernel<2, 8>), grid, dim3(nk * 64), 0, ctx->stream, a);
+    const dim3 grid((unsigned)(2 * p.panels * ((a.rows + 15) / 16)));
+    hipLaunchKernelGGL(gated_few_kernel, grid, dim3(kFewWaves * 64), 0, ctx->stream, a);
     return check_launch("gated_few");
+  }
+  // One workgroup to a CU: 1200 rows of 256 to 690 channels (228 of them) 13.1 us here, 20.4 split beforehand; to 2048
+  // channels (608) 32.8 and 25.8.
+  const long long mids = a.xpanels * ((p.panels + 3LL) / 4), wide = a.xpanels * ((p.panels + 1LL) / 2);
+  if (mids <= 256) {
+    ProfScope prof(ctx, "gated_mid", flops, bytes);
+    if (wide <= 256)
+      hipLaunchKernelGGL(gated_mid_kernel<2>, dim3((unsigned)wide), dim3(512), 0, ctx->stream, a);
+    else
+      hipLaunchKernelGGL(gated_mid_kernel<4>, dim3((unsigned)mids), dim3(512), 0, ctx->stream, a);
+    return check_launch("gated_mid");
   }
   size_t at = 0;
   auto take = [&](size_t size) {
@@ -593,19 +774,19 @@ int op_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tenso
     SY_TRY(check_launch("gated_split"));
   }
   ProfScope prof(ctx, "gated", flops, bytes);
-  auto tiles = [&](int wm, int wn) {
-    a.row_tiles = (a.xpanels + 2 * wm - 1) / (2 * wm);
-    a.col_tiles = (a.panels + wn - 1) / wn;
+  auto tiles = [&](int rows, int cols) {
+    a.row_tiles = (a.xpanels + rows - 1) / rows;
+    a.col_tiles = (a.panels + cols - 1) / cols;
     return (long long)a.row_tiles * a.col_tiles;
   };
-  auto launch = [&](auto kernel, int wm, int wn) {
-    const long long grid = tiles(wm, wn);
-    SY_CHECK(grid * wm * wn * 64 < (1LL << 32), SY_EUNSUPPORTED, "gated grid too large");
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(wm * wn * 64), 0, ctx->stream, a);
+  auto launch = [&](auto kernel, int rows, int cols, int waves) {
+    const long long grid = tiles(rows, cols);
+    SY_CHECK(grid * waves * 64 < (1LL << 32), SY_EUNSUPPORTED, "gated grid too large");
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(waves * 64), 0, ctx->stream, a);
     return check_launch("gated");
   };
-  if (tiles(4, 2) >= 512) return launch(gated_kernel<4, 2>, 4, 2);
-  return launch(gated_kernel<2, 1>, 2, 1);
+  if (a.panels <= 2) return launch(gated_kernel<1, 2>, 2, 2, 2);
+  return launch(gated_kernel<1, 4>, 2, 4, 4);
 }
 
 }  // namespace sy
