@@ -217,11 +217,11 @@ __device__ __forceinline__ void cross_tile(const CrossArgs& a, const u32x4* f, i
 #pragma unroll
   for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
   mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.c;
-  if (__any(mx - w.top > kSlack)) {
-    mx = fmaxf(mx, w.top);
-    const float x = __builtin_amdgcn_exp2f(w.top - (mx == -INFINITY ? 0.f : mx));
+  const bool move = mx - w.top > kSlack;  // row by row, so that no row's bits hang on another's scores
+  if (__any(move)) {
+    const float x = move ? __builtin_amdgcn_exp2f(w.top - mx) : 1.f;
     const bool before = __any(w.top != -INFINITY);
-    w.top = mx;
+    w.top = move ? mx : w.top;
     w.sum *= x;
     if (before)
 #pragma unroll
@@ -812,10 +812,20 @@ int op_cross_attention(sy_ctx* ctx, const sy_cross_config* c, const sy_tensor* q
   SY_CHECK(!views_overlap(o, q) && !views_overlap(o, k) && !views_overlap(o, v), SY_EINVAL,
            "cross attention output overlaps an input");
   SY_CHECK(k->ldc < (1 << 24) && v->ldc < (1 << 24), SY_EUNSUPPORTED, "cross attention states of 2^24 channels and more");
+  // Whether `bytes` bytes at p share memory with o (or lie between its pixels).
+  auto meets = [&](const void* p, long double bytes) {
+    const long double from = (long double)(uintptr_t)p, at = (long double)(uintptr_t)o->data;
+    const long double size = 4.0L * (((long double)pixels(*o) - 1) * o->ldc + o->c);
+    return from < at + size && at < from + bytes;
+  };
   if (mask) {
     SY_CHECK(mask->data, SY_EINVAL, "null mask data");
     SY_CHECK(mask->image >= 0 && mask->head >= 0 && mask->query >= 0, SY_EINVAL, "negative mask stride");
+    SY_CHECK(!meets(mask->data, (long double)mask->image * (q->n - 1) + (long double)mask->head * (a.heads - 1) +
+                                    (long double)mask->query * ((double)q->h * q->w - 1) + (double)k->h * k->w),
+             SY_EINVAL, "cross attention output overlaps the mask");
   }
+  SY_CHECK(!lengths || !meets(lengths, 4.0L * q->n), SY_EINVAL, "cross attention output overlaps the lengths");
   SY_CHECK((long long)q->n * a.kv < (1 << 24) && (long long)q->h * q->w * a.group < (1LL << 31) - 1024, SY_EUNSUPPORTED,
            "cross attention over %d x %dx%d queries", q->n, q->h, q->w);
   SY_CHECK(ctx, SY_EINVAL, "null context");
@@ -859,7 +869,8 @@ int op_cross_attention(sy_ctx* ctx, const sy_cross_config* c, const sy_tensor* q
   a.piece = ((a.tk + a.splits - 1) / a.splits + kCrossKeys - 1) / kCrossKeys * kCrossKeys;
   a.splits = (a.tk + a.piece - 1) / a.piece;
   const long long items = planes * a.tiles * a.splits, grid = (items + 7) / 8 * 8;
-  SY_CHECK(grid * 512 < (1LL << 32), SY_EUNSUPPORTED, "cross attention over %lld rows", planes * a.rows);
+  const int threads = few ? 256 : brief ? kShortWaves * 64 : nw * 64;
+  SY_CHECK(grid * threads < (1LL << 32), SY_EUNSUPPORTED, "cross attention over %lld rows", planes * a.rows);
   a.items = (unsigned)items;
   DeviceScope device(ctx);
   if (a.splits > 1) {
@@ -877,7 +888,6 @@ int op_cross_attention(sy_ctx* ctx, const sy_cross_config* c, const sy_tensor* q
                          : brief ? pick_short(ks, dt)
                          : nw == 4 ? pick_cross<4>(ks, dt)
                                    : pick_cross<8>(ks, dt);
-    const int threads = few ? 256 : brief ? kShortWaves * 64 : nw * 64;
     const size_t lds = brief ? (size_t)(a.tk + kCrossKeys - 1) / kCrossKeys * short_bytes(ks, dt) : 0;
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, ctx->stream, a);
     SY_TRY(check_launch("cross_attention"));

@@ -123,6 +123,46 @@ def test_hidden_states_hold_anything(hip, tk, what):
     check(got[:, :35], clean[0][:, :35], clean[1][:, :35])
 
 
+# n, queries, states, heads, key heads, key dim, head dim: enough rows for a state's parts to be used many times
+MANY = [(8, 1100, 77, 8, 8, 64, 64), (16, 700, 40, 24, 8, 32, 36), (4, 2500, 33, 8, 8, 100, 128), (40, 300, 1, 6, 6, 20, 8),
+        (2, 2100, 1100, 8, 8, 64, 64), (1, 3000, 1300, 12, 4, 128, 128), (2, 2000, 500, 8, 4, 32, 20)]
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("case", MANY, ids=str)
+def test_many_rows(hip, case, masked):
+    """Ragged lengths, with and without a mask for each query, states behind them NaN; some of the rows, from every
+    image, are compared, and the rest must be as finite."""
+    n, tq, tk, heads, kv, kd, hd = case
+    q, k, v = tensors(*case, seed=12)
+    g = R.rng(13)
+    lengths = g.integers(tk // 2, tk + 1, n)
+    lengths[0] = tk
+    if n > 2:
+        lengths[2] = 0
+    mask = (g.random((n, 1, tq, tk)) < 0.3).astype(np.uint8) if masked else None
+    for b in range(n):
+        k[b, lengths[b]:], v[b, lengths[b]:] = np.nan, np.nan
+    got = run(hip, q, k, v, lengths, mask)
+    assert np.isfinite(got).all()
+    rows = np.unique(np.r_[0:3, tq - 3:tq, g.integers(0, tq, 12)])
+    exp, bound = L.cross(q[:, rows], k, v, scaled(q, k), lengths, None if mask is None else mask[:, :, rows])
+    check(got[:, rows], exp, bound)
+
+
+@pytest.mark.parametrize("case", MANY[:2] + MANY[4:6], ids=str)
+def test_rows_beside_odd_ones(hip, case):
+    """A row whose query is infinite, and one whose query is huge, leave every other row's bits alone."""
+    q, k, v = tensors(*case, seed=14)
+    one = run(hip, q, k, v)
+    q[0, 40, 0, 3], q[0, 77, 1] = np.inf, 1e30
+    two = run(hip, q, k, v)
+    keep = np.ones(one.shape[:3], bool)
+    keep[0, 40, 0] = keep[0, 77, 1] = False
+    np.testing.assert_array_equal(one[keep], two[keep])
+    assert np.isnan(two[0, 40, 0]).all() and np.isfinite(two[0, 77, 1]).all()
+
+
 @pytest.mark.parametrize("scale", [1e-30, 1e-3, 1.0, 30.0])
 @pytest.mark.parametrize("tk", [50, 1500])
 def test_scales(hip, tk, scale):

@@ -42,7 +42,8 @@ def rows_of(rows, ic, seed):
 
 SIZES = [(1, 1, 1), (1, 64, 32), (2, 15, 33), (3, 16, 31), (5, 257, 100), (16, 100, 65), (31, 300, 40), (32, 512, 96),
          (33, 1, 2), (34, 32, 64), (64, 33, 32), (65, 64, 97), (127, 31, 5), (128, 128, 128), (129, 200, 130),
-         (300, 255, 690), (1000, 17, 33), (257, 600, 64), (4100, 48, 1100)]
+         (300, 255, 690), (1000, 17, 33), (257, 600, 64), (4100, 48, 1100), (3000, 1100, 300), (9000, 40, 33), (12, 1500, 20),
+         (40, 1500, 100)]
 
 
 @pytest.mark.parametrize("pad,before", [(0, 0), (4, 8), (3, 1)])
@@ -61,22 +62,22 @@ def test_activations(hip, rows, act):
     check(run(hip, x, w, L.ACTS[act]), *L.gated(x, *w, L.ACTS[act]))
 
 
-@pytest.mark.parametrize("rows", [7, 200])
+@pytest.mark.parametrize("rows", [7, 200, 3000])
 @pytest.mark.parametrize("size", [1e-30, 1e-12, 1e12, 1e25])
 def test_rows_of_any_size(hip, rows, size):
     """Rows far apart beside each other, against weights that bring them back."""
-    x, w = rows_of(rows, 96, 5), weights(70, 96, 6, bias=False)
+    x, w = rows_of(rows, 96, 5), weights(70 if rows < 1000 else 400, 96, 6, bias=False)
     x[::2] *= np.float32(size)
     w[0] *= np.float32(min(1 / size, 1e12))
     check(run(hip, x, w, N.ACT_NONE), *L.gated(x, *w, N.ACT_NONE))
 
 
-@pytest.mark.parametrize("rows", [7, 200])
+@pytest.mark.parametrize("rows", [7, 200, 3000])
 @pytest.mark.parametrize("far", [20, 27, 32, 40, 60])
 def test_uneven_channels(hip, rows, far):
     """Channels 2^far below the others of their row, whose weights are as far above the others of theirs; and such rows
     alone, where the large channels' weights are 0."""
-    x, w = rows_of(rows, 64, 7), weights(40, 64, 8)
+    x, w = rows_of(rows, 64, 7), weights(40 if rows < 1000 else 400, 64, 8)
     x[:, ::2] *= np.float32(2.0 ** -far)
     w[0][:, ::2] *= np.float32(2.0 ** far)
     w[1][:, 1::2] = 0
@@ -91,11 +92,11 @@ def test_uneven_channels(hip, rows, far):
     assert (np.abs(got - exp) <= bound).all(), (np.abs(got - exp) / bound).max()
 
 
-@pytest.mark.parametrize("rows", [7, 200])
+@pytest.mark.parametrize("rows", [7, 200, 3000])
 @pytest.mark.parametrize("what", [np.nan, np.inf])
 def test_non_finite(hip, rows, what):
     """An infinity or NaN in a row spoils that row alone, in the weights that channel alone."""
-    x, w = rows_of(rows, 64, 9), weights(70, 64, 10)
+    x, w = rows_of(rows, 64, 9), weights(70 if rows < 1000 else 400, 64, 10)
     exp, bound = L.gated(x, *w, N.ACT_NONE)
     x[5, 3] = what
     w[1][40, 6] = what
@@ -123,14 +124,16 @@ def test_maps(hip, shape):
     check(run(hip, x, p, N.ACT_GELU, shape, pad=4), *L.gated(x, *p, N.ACT_GELU))
 
 
-def test_a_row_does_not_depend_on_the_others(hip):
-    x, w = rows_of(200, 96, 15), weights(64, 96, 16)
+@pytest.mark.parametrize("rows,oc", [(200, 64), (3000, 400)])
+def test_a_row_does_not_depend_on_the_others(hip, rows, oc):
+    """Rows of other sizes beside it, and plain ones in another panel."""
+    x, w = rows_of(rows, 96, 15), weights(oc, 96, 16)
     layer = hip.gated_create(*w)
     one = run(hip, x, w, layer=layer)
     x[::2] *= np.float32(1e8)
     x[7, 3] = np.nan
     two = run(hip, x, w, layer=layer)
-    keep = np.r_[33:200:2]
+    keep = np.r_[33:rows:2]
     np.testing.assert_array_equal(one[keep], two[keep])
 
 

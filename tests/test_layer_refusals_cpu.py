@@ -86,6 +86,10 @@ def test_cross_views(name, good, bad):
 def test_cross_others():
     for mask in (N.KeyMask(0, 0, 0, 0), N.KeyMask(far(9), -1, 0, 0), N.KeyMask(far(9), 0, -1, 0), N.KeyMask(far(9), 0, 0, -1)):
         assert cross(mask=mask) == N.SY_EINVAL and why() != "null context"
+    for at in (far(4), far(4) - 20, far(4) + 2 * 128 * 4 * 32 - 1):
+        assert cross(mask=N.KeyMask(at, 24, 0, 0)) == N.SY_EINVAL and "mask" in why()
+    assert cross(mask=N.KeyMask(far(3) + 8, 0, 0, 1 << 40)) == N.SY_EINVAL and "mask" in why()
+    assert cross(lengths=far(4) + 64) == N.SY_EINVAL and "lengths" in why()
     for at in (1, 2, 3):
         assert cross(o=view(128, data=far(at))) == N.SY_EINVAL and "overlaps" in why()
     assert cross(k=view(32, h=3, ldc=1 << 24, data=far(100)), v=view(64, h=3, data=far(40))) == N.SY_EUNSUPPORTED
