@@ -35,7 +35,7 @@ template <int VEC>
 struct Vec;
 template <>
 struct Vec<4> {
-  typedef f32x4 type;
+  typedef f32x4 type __attribute__((aligned(4)));  // the memory takes quads at any multiple of four bytes
 };
 template <>
 struct Vec<1> {
@@ -145,12 +145,14 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(const NormArgs a) {
   }
 }
 
-// The moments of the run's groups from every thread's own (VEC channels of one
-// group): a wave adds up a group's threads, in one order.
-__device__ __forceinline__ void meet(const NormArgs& a, const Moments& m, double2* red, int cols_each, int used,
+// The moments of the run's groups from every thread's own, E of them, each of one group: a
+// wave adds up a group's, in one order.  cols_each and used: of a group and of all, side by side.
+template <int E>
+__device__ __forceinline__ void meet(const NormArgs& a, const Moments (&m)[E], double2* red, int cols_each, int used,
                                      int groups, Moments* out) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  red[threadIdx.x] = make_double2(m.s, m.q);
+#pragma unroll
+  for (int e = 0; e < E; ++e) red[threadIdx.x * E + e] = make_double2(m[e].s, m[e].q);
   __syncthreads();
   const int per = a.rows * cols_each;
   for (int g = wave; g < groups; g += waves) {
@@ -223,57 +225,63 @@ __global__ __launch_bounds__(1024) void norm_group_kernel(const NormArgs a) {
   }
 }
 
+constexpr int kDeep = 4;  // pixels of a thread under way
+
 // Larger images: the moments of a piece of the pixels and a run of groups, then
-// every piece normalised by the moments of all.
-template <int VEC>
+// every piece normalised by the moments of all.  MIX: a column's four channels may be of
+// several groups, and have moments each.
+template <int VEC, bool MIX>
 __global__ __launch_bounds__(256) void norm_sums_kernel(const NormArgs a) {
   typedef typename Vec<VEC>::type vec;
-  __shared__ double2 red[256];
+  constexpr int E = MIX ? VEC : 1, W = MIX ? 1 : VEC;  // moments of a thread; channels of one
+  __shared__ double2 red[256 * E];
   __shared__ Moments total[kMaxRun];
   const int piece = blockIdx.x % a.pieces, rest = blockIdx.x / a.pieces, img = rest / a.runs, run = rest - img * a.runs;
   const int g0 = run / a.blocks * a.run, first = run % a.blocks * a.cols;  // group, its column
   const int groups = min(a.run, a.groups - g0);
-  const int cols_each = min(a.each / VEC - first, a.cols), cols = groups * cols_each;
-  const int row = threadIdx.x / a.cols, col = threadIdx.x - row * a.cols;
+  const int cols_each = min(a.each / W - first, a.cols * E), cols = groups * cols_each / E;
+  const int row = threadIdx.x / a.cols, col = threadIdx.x - row * a.cols, col1 = min(col, cols - 1);
   const bool live = row < a.rows && col < cols;
-  const int g = min(col / cols_each, groups - 1), c = g0 * a.each + (first + min(col, cols - 1)) * VEC;
+  const int c = g0 * a.each + (first + col1) * VEC;
   const float* x = a.x + (long long)img * a.t * a.ldx;
   const int from = piece * a.piece, to = min(from + a.piece, a.t);
-  const double p = (double)x[(g0 + g) * a.each];
-  Moments m{0, 0};
+  double p[E];
+  Moments m[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    p[e] = (double)x[(g0 + (col1 * E + e) / cols_each) * a.each];
+    m[e] = {0, 0};
+  }
   if (live) {
-    int i = from + row;
-    for (; i + 3 * a.rows < to; i += 4 * a.rows) {
-      vec v[4];
+    for (int i = from + row; i < to; i += kDeep * a.rows) {
+      vec v[kDeep];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = *(const vec*)(x + (i + k * a.rows) * a.ldx + c);
+      for (int k = 0; k < kDeep; ++k) v[k] = *(const vec*)(x + min(i + k * a.rows, to - 1) * a.ldx + c);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < kDeep; ++k)
+        if (i + k * a.rows < to)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) m.add(v[k][e], p);
-    }
-    for (; i < to; i += a.rows) {
-      const vec v = *(const vec*)(x + i * a.ldx + c);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) m.add(v[e], p);
+          for (int e = 0; e < VEC; ++e) m[e % E].add(v[k][e], p[e % E]);
     }
   }
-  meet(a, m, red, cols_each, a.cols, groups, total);
-  if (piece == 0 && run % a.blocks == 0 && live && row == 0 && col % cols_each == 0)
-    a.pivot[(long long)img * a.groups + g0 + g] = (float)p;
+  meet<E>(a, m, red, cols_each, a.cols * E, groups, total);
+  if (piece == 0 && run % a.blocks == 0)
+    for (int i = threadIdx.x; i < groups; i += 256)
+      a.pivot[(long long)img * a.groups + g0 + i] = x[(g0 + i) * a.each];
   for (int i = threadIdx.x; i < groups; i += 256)
     a.sums[(((long long)img * a.groups + g0 + i) * a.blocks + run % a.blocks) * a.pieces + piece] =
         make_double2(total[i].s, total[i].q);
 }
 
-template <int VEC>
+template <int VEC, bool MIX>
 __global__ __launch_bounds__(256) void norm_apply_kernel(const NormArgs a) {
   typedef typename Vec<VEC>::type vec;
+  constexpr int E = MIX ? VEC : 1, W = MIX ? 1 : VEC;
   __shared__ Scale scale[kMaxRun];
   const int piece = blockIdx.x % a.pieces, rest = blockIdx.x / a.pieces, img = rest / a.runs, run = rest - img * a.runs;
   const int g0 = run / a.blocks * a.run, first = run % a.blocks * a.cols, lane = threadIdx.x & 63;
   const int groups = min(a.run, a.groups - g0);
-  const int cols_each = min(a.each / VEC - first, a.cols), cols = groups * cols_each;
+  const int cols_each = min(a.each / W - first, a.cols * E), cols = groups * cols_each / E;
   const float* x = a.x + (long long)img * a.t * a.ldx;
   float* y = a.y + (long long)img * a.t * a.ldy;
   const int row = threadIdx.x / a.cols, col = min((int)threadIdx.x - row * a.cols, cols - 1);
@@ -281,9 +289,9 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(const NormArgs a) {
   const int from = piece * a.piece, to = min(from + a.piece, a.t);
   // The first pixels and the weights are under way while the moments meet.
   int i = from + row;
-  vec v[4];
+  vec v[kDeep];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) v[k] = *(const vec*)(x + min(i + k * a.rows, to - 1) * a.ldx + c);
+  for (int k = 0; k < kDeep; ++k) v[k] = *(const vec*)(x + min(i + k * a.rows, to - 1) * a.ldx + c);
   float ga[VEC], be[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
@@ -304,20 +312,22 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(const NormArgs a) {
   }
   __syncthreads();
   if (row >= a.rows || (int)threadIdx.x - row * a.cols >= cols) return;
-  const Scale s = scale[col / cols_each];
+  Scale s[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) s[e] = scale[(col * E + e) / cols_each];
   while (i < to) {
-    vec o[4];
+    vec o[kDeep];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < kDeep; ++k)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o[k][e] = normal(a, v[k][e], s, ga[e], be[e]);
+      for (int e = 0; e < VEC; ++e) o[k][e] = normal(a, v[k][e], s[e % E], ga[e], be[e]);
     const int at = i;
-    i += 4 * a.rows;
+    i += kDeep * a.rows;
     if (i < to)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = *(const vec*)(x + min(i + k * a.rows, to - 1) * a.ldx + c);
+      for (int k = 0; k < kDeep; ++k) v[k] = *(const vec*)(x + min(i + k * a.rows, to - 1) * a.ldx + c);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < kDeep; ++k)
       if (at + k * a.rows < to) __builtin_nontemporal_store(o[k], (vec*)(y + (at + k * a.rows) * a.ldy + c));
   }
 }
@@ -360,8 +370,7 @@ int op_group_norm(sy_ctx* ctx, const sy_tensor* x, int groups, const float* gamm
   a.act = act;
   a.eps = eps;
   a.share = 1.0 / ((double)a.t * a.each);
-  const bool quads = a.each % 4 == 0 && a.ldx % 4 == 0 && a.ldy % 4 == 0 &&
-                     (((uintptr_t)x->data | (uintptr_t)y->data) & 15) == 0;
+  const bool quads = a.each % 4 == 0;
   const int vec = quads ? 4 : 1;
   const long long units = (long long)a.t * (a.each / vec);  // of a group
   const double bytes = 8.0 * a.n * (double)a.t * a.c, flops = 8.0 * a.n * (double)a.t * a.c;
@@ -392,15 +401,28 @@ int op_group_norm(sy_ctx* ctx, const sy_tensor* x, int groups, const float* gamm
                        ctx->stream, a);
     return check_launch("group_norm");
   }
-  // A run of groups: 128 bytes of a pixel and more.
-  a.run = std::min({groups, std::max(1, 256 / each), std::max(1, (32 / vec + each - 1) / each)});
-  a.cols = std::min(a.run * each, 256);
+  // A run of groups: 128 bytes of a pixel and more.  Where groups are not of whole quads but a pixel is, runs of two or
+  // four groups are, too; their columns have four moments each, which pays for large maps: eight 160x160 maps of 60
+  // channels, 4 groups 45.5 us, 66.5 channel by channel, of 180, 12 groups 112 and 128, sixteen 45x75 of 108, 12 groups
+  // 21.8 and 25.3, but five of those 13.2 and 11.9.
+  const int whole = a.each % 2 ? 4 : 2;
+  const bool mix = !quads && a.c % 4 == 0 && whole * a.each <= 1024 && (double)a.n * a.t * a.c >= 4e6;
+  if (mix) {
+    a.run = std::min(groups, (32 / a.each + whole - 1) / whole * whole + (a.each > 32 ? whole : 0));
+    a.cols = a.run * a.each / 4;
+    a.blocks = 1;
+  } else {
+    a.run = std::min({groups, std::max(1, 256 / each), std::max(1, (32 / vec + each - 1) / each)});
+    a.cols = std::min(a.run * each, 256);
+    a.blocks = (each + 255) / 256;
+  }
   a.rows = 256 / a.cols;
-  a.blocks = (each + 255) / 256;
   a.runs = a.blocks > 1 ? groups * a.blocks : (groups + a.run - 1) / a.run;
-  // Pieces: 8 pixels of a thread and more, 2 where those would leave CUs without work, up to 8192 workgroups.
+  // Pieces: 8 pixels of a thread and more in up to 8192 workgroups, 4 where those would be fewer than 1024: one 80x80 map
+  // of 64 channels 9.2 us with 4, 11.9 with 8, 16.7 with 16 (its few waves work through them one by one); eight 160x160
+  // maps of 256 channels 108 with 4 and 104 with 8.
   const long long runs = (long long)a.n * a.runs;
-  const int least = a.t * runs >= 256LL * 8 * a.rows ? 8 : 2;
+  const int least = a.t * runs >= 1024LL * 4 * a.rows ? 8 : 4;
   a.piece = (int)std::max<long long>(least * a.rows, (a.t * runs + 8191) / 8192);
   a.pieces = (a.t + a.piece - 1) / a.piece;
   const long long grid = runs * a.pieces;
@@ -410,8 +432,8 @@ int op_group_norm(sy_ctx* ctx, const sy_tensor* x, int groups, const float* gamm
   a.sums = (double2*)ctx->scratch;
   a.pivot = (float*)(ctx->scratch + sums);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, ctx->stream, a); };
-  launch(quads ? norm_sums_kernel<4> : norm_sums_kernel<1>);
-  launch(quads ? norm_apply_kernel<4> : norm_apply_kernel<1>);
+  launch(quads ? norm_sums_kernel<4, false> : mix ? norm_sums_kernel<4, true> : norm_sums_kernel<1, false>);
+  launch(quads ? norm_apply_kernel<4, false> : mix ? norm_apply_kernel<4, true> : norm_apply_kernel<1, false>);
   return check_launch("group_norm");
 }
 

@@ -41,7 +41,8 @@ SHAPES = [
     (2, 1, 1, 4096, 1), (2, 1, 1, 4097, 1), (2, 1, 1, 9000, 2), (3, 4, 4, 32, 8), (1, 7, 9, 40, 5), (2, 7, 9, 35, 7),
     (1, 20, 20, 256, 32), (2, 20, 20, 512, 32), (2, 13, 17, 108, 12), (1, 45, 75, 27, 3), (1, 40, 40, 64, 1),
     (1, 60, 60, 96, 96), (1, 80, 80, 64, 8), (2, 65, 63, 24, 2), (1, 70, 70, 1040, 2), (1, 100, 100, 10, 1),
-    (1, 80, 80, 7, 7), (1, 3, 5, 8200, 1), (1, 1, 3000, 512, 512), (2, 33, 31, 640, 20),
+    (1, 80, 80, 7, 7), (1, 3, 5, 8200, 1), (1, 1, 3000, 512, 512), (2, 33, 31, 640, 20), (3, 60, 50, 36, 6), (1, 90, 80, 20, 20), (2, 70, 61, 140, 4), (1, 70, 80, 72, 24),
+    (1, 64, 70, 1020, 4), (2, 50, 90, 44, 4), (1, 61, 70, 12, 2), (9, 100, 90, 60, 4), (3, 130, 120, 100, 20),
 ]
 
 
