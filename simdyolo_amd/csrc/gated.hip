@@ -49,7 +49,6 @@ struct GatedArgs {
   const int *x_row, *x_plain;
   int xpanels;
   int row_tiles, col_tiles;
-  bool quads;  // x can be read 16 bytes at a time
 };
 
 // Exponent field of the power of two that takes a largest magnitude m into [2^14,
@@ -64,22 +63,33 @@ __device__ __forceinline__ bool uneven(unsigned largest, unsigned smallest) {
   return e == 255 || (smallest != 0x7fffffffu && (int)(smallest >> 23) < e + kUneven && smallest != 0);
 }
 
-// Eight elements of a row of `end` from `at`, zeros from `end` on.
-__device__ __forceinline__ void load8(const float* row, int at, int end, bool quads, float (&v)[8]) {
-  if (quads) {  // end is a multiple of 4
-    const f32x4 a = *(const f32x4*)(row + min(at, end - 4)), b = *(const f32x4*)(row + min(at + 4, end - 4));
+// Four elements of a row of `end` from `at`, zeros from `end` on.  The memory takes quads at any
+// multiple of four bytes; the one that meets the row's end is read from within the row.
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+__device__ __forceinline__ f32x4 load4(const float* row, int at, int end) {
+  if (end < 4) {
+    f32x4 t;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = a[e];
-      v[4 + e] = b[e];
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = row[min(at + e, end - 1)];
+    for (int e = 0; e < 4; ++e) t[e] = at + e < end ? row[at + e] : 0.f;
+    return t;
   }
-  if (at + 8 > end)
+  const int from = min(at, end - 4), d = at - from;
+  f32x4 t = *(const f32x4_any*)(row + from);
+  if (d > 0) {
+    t[0] = d == 1 ? t[1] : d == 2 ? t[2] : d == 3 ? t[3] : 0.f;
+    t[1] = d == 1 ? t[2] : d == 2 ? t[3] : 0.f;
+    t[2] = d == 1 ? t[3] : 0.f;
+    t[3] = 0.f;
+  }
+  return t;
+}
+__device__ __forceinline__ void load8(const float* row, int at, int end, float (&v)[8]) {
+  const f32x4 a = load4(row, at, end), b = load4(row, at + 4, end);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = at + e < end ? v[e] : 0.f;
+  for (int e = 0; e < 4; ++e) {
+    v[e] = a[e];
+    v[4 + e] = b[e];
+  }
 }
 
 __device__ __forceinline__ void pair8(const float (&x)[8], float s, u32x4& h, u32x4& l) {
@@ -99,7 +109,7 @@ __device__ __forceinline__ void pair8(const float (&x)[8], float s, u32x4& h, u3
 // zeros.  `more`: the panel's flag is that of an earlier call, too.
 constexpr int kLot = 256, kLotSteps = kLot / 16, kHeld = 4;
 __global__ __launch_bounds__(512) void gated_split_kernel(const float* x, long long ldx, int rows, int ic, int steps,
-                                                          bool quads, u32x4* out, int* words, int* plain, int stride,
+                                                          u32x4* out, int* words, int* plain, int stride,
                                                           int offset, bool more) {
   __shared__ u32x4 lds[2][kLotSteps * kStep];
   __shared__ int any;
@@ -111,21 +121,10 @@ __global__ __launch_bounds__(512) void gated_split_kernel(const float* x, long l
     const int c = lot * kLot + 4 * lane;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float* xr = x + min(row0 + wave + 8 * i, (long long)rows - 1) * ldx;
-      if (quads) {
-        const f32x4 t = *(const f32x4*)(xr + min(c, ic - 4));
+      const f32x4 t = load4(x + min(row0 + wave + 8 * i, (long long)rows - 1) * ldx, c, ic);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = t[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = xr[min(c + e, ic - 1)];
-      }
+      for (int e = 0; e < 4; ++e) v[i][e] = t[e];
     }
-    if (c + 4 > ic)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = c + e < ic ? v[i][e] : 0.f;
   };
   unsigned top[4] = {}, low[4];
 #pragma unroll
@@ -411,7 +410,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const Gate
         for (int s = 0; s < 2; ++s) wv[u][j][s] = __builtin_bit_cast(f16x8, w[j * up + at + 64 * s]);
     }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) load8(xr, min(p + u, pairs) * 32 + 8 * oct, a.ic, a.quads, xv[u]);
+    for (int u = 0; u < kAhead; ++u) load8(xr, min(p + u, pairs) * 32 + 8 * oct, a.ic, xv[u]);
     unsigned top = 0, low = 0x7fffffffu;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
@@ -489,25 +488,14 @@ __global__ __launch_bounds__(512, 2) void gated_mid_kernel(const GatedArgs a) {
   const long long up = (long long)a.steps * kStep;
   // A wave takes every eighth row, a lane four elements of it.
   float v[4][4];
-  auto load = [&](int k0) __attribute__((always_inline)) {
+  auto load = [&](int k0, float(&v)[4][4]) __attribute__((always_inline)) {
     const int c = 16 * k0 + 4 * lane;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float* x = a.x + (long long)min(row0 + wave + 8 * i, a.rows - 1) * a.ldx;
-      if (a.quads) {
-        const f32x4 t = *(const f32x4*)(x + min(c, a.ic - 4));
+      const f32x4 t = load4(a.x + (long long)min(row0 + wave + 8 * i, a.rows - 1) * a.ldx, c, a.ic);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = t[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = x[min(c + e, a.ic - 1)];
-      }
+      for (int e = 0; e < 4; ++e) v[i][e] = t[e];
     }
-    if (c + 4 > a.ic)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = c + e < a.ic ? v[i][e] : 0.f;
   };
   // Weights of steps k and on, four at a time.
   f16x8 wv[4][2][2];
@@ -520,22 +508,30 @@ __global__ __launch_bounds__(512, 2) void gated_mid_kernel(const GatedArgs a) {
         for (int s = 0; s < 2; ++s)
           wv[u][j][s] = __builtin_bit_cast(f16x8, w[j * up + (long long)min(k + u, a.steps - 1) * kStep + 64 * s]);
   };
-  // The rows' powers, from their last lot to the first, which stays in registers.
+  // The rows' powers: the first lot stays in registers, the others come four at a time.
   unsigned top[4] = {}, low[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) low[i] = 0x7fffffffu;
-  for (int k0 = (a.steps - 1) / kLotSteps * kLotSteps; k0 >= 0; k0 -= kLotSteps) {
-    load(k0);
-    if (k0 == 0) load_w(part * SH);
+  auto look = [&](const float(&t)[4][4]) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const unsigned m = magnitude(v[i][e]);
+        const unsigned m = magnitude(t[i][e]);
         top[i] = max(top[i], m);
         low[i] = min(low[i], m ? m : 0x7fffffffu);
       }
+  };
+  load(0, v);
+  for (int k0 = kLotSteps; k0 < a.steps; k0 += 4 * kLotSteps) {
+    float t[4][4][4];
+#pragma unroll
+    for (int l = 0; l < 4; ++l) load(min(k0 + l * kLotSteps, (a.steps - 1) / kLotSteps * kLotSteps), t[l]);
+#pragma unroll
+    for (int l = 0; l < 4; ++l) look(t[l]);
   }
+  load_w(part * SH);
+  look(v);
   float scale[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -566,7 +562,7 @@ __global__ __launch_bounds__(512, 2) void gated_mid_kernel(const GatedArgs a) {
   int now = 0;
   for (int k0 = 0; k0 < a.steps; k0 += kLotSteps, now ^= 1) {
     const bool more = k0 + kLotSteps < a.steps;
-    if (more) load(k0 + kLotSteps);
+    if (more) load(k0 + kLotSteps, v);
 #pragma unroll
     for (int u = 0; u < SH; ++u) {
       const int k = part * SH + u;
@@ -642,7 +638,7 @@ static int gated_pack(sy_ctx* ctx, const float* gate, const float* up, const flo
   SY_TRY(sy_memcpy(ctx, p->bias, bias.data(), 2 * cols * sizeof(float), 0));
   for (int m = 0; m < 2; ++m)
     hipLaunchKernelGGL(gated_split_kernel, dim3(p->panels), dim3(512), 0, ctx->stream, p->raw + m * values,
-                       (long long)p->ic, p->oc, p->ic, p->steps, p->ic % 4 == 0, p->w, p->w_row, p->w_plain, 2, m, m == 1);
+                       (long long)p->ic, p->oc, p->ic, p->steps, p->w, p->w_row, p->w_plain, 2, m, m == 1);
   SY_TRY(check_launch("gated_split"));
   std::vector<int> plain;
   try {
@@ -730,13 +726,12 @@ int op_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tenso
   a.w_plain = p.w_plain;
   a.bias = p.bias;
   a.raw = p.raw;
-  // The last quad of a row must not pass the buffer's end.
-  a.quads = ((uintptr_t)x->data & 15) == 0 && x->ldc % 4 == 0 && p.ic % 4 == 0;
   a.xpanels = (a.rows + 31) / 32;
   DeviceScope device(ctx);
   const double flops = 4.0 * rows * p.ic * p.oc, bytes = 4.0 * ((double)rows * (p.ic + p.oc) + 2.0 * p.ic * p.oc);
-  // 32 rows of 1024 to 2816 channels 13.3 us here, 17.6 as a middling number of tiles; 33 of 2048 to 4096 47.7 and 32.4.
-  if (a.rows <= 32) {
+  // 32 rows of 1024 to 2816 channels 13.3 us here, 17.6 as a middling number of tiles; 64 of 256 to 688 (176 workgroups)
+  // 6.7 and 7.8, 256 of 128 to 256 (256) 5.4 and 7.7, 100 of 255 to 690 (308) 11.9 and 8.4, 33 of 2048 to 4096 (768) 40 and 33.
+  if (a.rows <= 32 || 2LL * p.panels * ((a.rows + 15) / 16) <= 256) {
     ProfScope prof(ctx, "gated_few", flops, bytes);
     const dim3 grid((unsigned)(2 * p.panels * ((a.rows + 15) / 16)));
     hipLaunchKernelGGL(gated_few_kernel, grid, dim3(kFewWaves * 64), 0, ctx->stream, a);
@@ -770,7 +765,7 @@ int op_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tenso
   {
     ProfScope prof(ctx, "gated_split", 0, 8.0 * rows * p.ic);
     hipLaunchKernelGGL(gated_split_kernel, dim3(a.xpanels), dim3(512), 0, ctx->stream, a.x, a.ldx, a.rows, a.ic, a.steps,
-                       a.quads, xs, x_row, x_plain, 1, 0, false);
+                       xs, x_row, x_plain, 1, 0, false);
     SY_TRY(check_launch("gated_split"));
   }
   ProfScope prof(ctx, "gated", flops, bytes);
@@ -785,6 +780,8 @@ int op_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tenso
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(waves * 64), 0, ctx->stream, a);
     return check_launch("gated");
   };
+  // Two panels of output channels to a workgroup where there are no more: 20000 rows of 96 to 60 channels would leave half
+  // the waves of four without any.
   if (a.panels <= 2) return launch(gated_kernel<1, 2>, 2, 2, 2);
   return launch(gated_kernel<1, 4>, 2, 4, 4);
 }
