@@ -57,51 +57,69 @@ __device__ __forceinline__ int gated_field(unsigned m) { return min(268 - (int)(
 
 __device__ __forceinline__ unsigned magnitude(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
 
-// Whether a row with the largest magnitude m must be computed plainly, from its smallest nonzero one.
-__device__ __forceinline__ bool uneven(unsigned largest, unsigned smallest) {
-  const int e = (int)(largest >> 23);
-  return e == 255 || (smallest != 0x7fffffffu && (int)(smallest >> 23) < e + kUneven && smallest != 0);
-}
+// The part of a row that a thread holds: its largest magnitude, and its smallest but for zeros, less one.
+struct Range {
+  unsigned top = 0, low = ~0u;
+  __device__ void look(float v) {
+    const unsigned m = magnitude(v);
+    top = max(top, m);
+    low = min(low, m - 1);
+  }
+  // Whether the row, whose largest is `largest`, must be computed plainly for this part's sake.
+  __device__ bool uneven(unsigned largest) const {
+    const int e = (int)(largest >> 23);
+    return e == 255 || low < (unsigned)max(max(e + kUneven, 0) << 23, 1) - 1;
+  }
+};
 
-// Four elements of a row of `end` from `at`, zeros from `end` on.  The memory takes quads at any
-// multiple of four bytes; the one that meets the row's end is read from within the row.
+// Four elements of a row of `end` from `at`.  The memory takes quads at any multiple of four bytes; one that meets the
+// row's end is read from within the row, and put right where it is used: a branch between loads would have
+// every load waited for (1200 rows of 255 to 690 channels 12.9 us so, 12.5 without).
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
-__device__ __forceinline__ f32x4 load4(const float* row, int at, int end) {
-  if (end < 4) {
-    f32x4 t;
+struct Quad {
+  int from, shift, left;  // where it is read, how far that is ahead, elements that are there
+  __device__ Quad(int at, int end) : from(max(min(at, end - 4), 0)), shift(at - from), left(end - at) {}
+  // Of rows of fewer than four elements the quad is read whole, too.
+  __device__ f32x4 load(const float* row) const { return *(const f32x4_any*)(row + from); }
+  __device__ f32x4 mend(f32x4 t) const {
+    if (shift & 1) t = f32x4{t[1], t[2], t[3], t[3]};
+    if (shift & 2) t = f32x4{t[2], t[3], t[3], t[3]};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) t[e] = at + e < end ? row[at + e] : 0.f;
+    for (int e = 0; e < 4; ++e) t[e] = e < left ? t[e] : 0.f;
     return t;
   }
-  const int from = min(at, end - 4), d = at - from;
-  f32x4 t = *(const f32x4_any*)(row + from);
-  if (d > 0) {
-    t[0] = d == 1 ? t[1] : d == 2 ? t[2] : d == 3 ? t[3] : 0.f;
-    t[1] = d == 1 ? t[2] : d == 2 ? t[3] : 0.f;
-    t[2] = d == 1 ? t[3] : 0.f;
-    t[3] = 0.f;
+};
+
+// Largest value over aligned groups of 32 or 64 lanes, in each of them.
+template <int LANES>
+__device__ __forceinline__ unsigned lanes_max(unsigned m) {
+  m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0xb1, 0xf, 0xf, true));   // lane ^ 1
+  m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x4e, 0xf, 0xf, true));   // lane ^ 2
+  m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x141, 0xf, 0xf, true));  // 7 - lane
+  m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x140, 0xf, 0xf, true));  // 15 - lane
+  const auto a = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  m = max(a[0], a[1]);
+  if (LANES == 64) {
+    const auto b = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    m = max(b[0], b[1]);
   }
-  return t;
-}
-__device__ __forceinline__ void load8(const float* row, int at, int end, float (&v)[8]) {
-  const f32x4 a = load4(row, at, end), b = load4(row, at + 4, end);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    v[e] = a[e];
-    v[4 + e] = b[e];
-  }
+  return m;
 }
 
-__device__ __forceinline__ void pair8(const float (&x)[8], float s, u32x4& h, u32x4& l) {
+__device__ __forceinline__ void pair8(const f32x4 (&x)[2], float s, u32x4& h, u32x4& l) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float a = x[2 * i], b = x[2 * i + 1];
+    const float a = x[i >> 1][2 * i & 3], b = x[i >> 1][(2 * i & 3) + 1];
     const f16x2 hi = __builtin_convertvector((f32x2v{a * s, b * s}), f16x2);
     const f32x2v r = {__builtin_fmaf(a, s, -(float)hi[0]), __builtin_fmaf(b, s, -(float)hi[1])};
     h[i] = __builtin_bit_cast(unsigned, hi);
     l[i] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2v{r[0] * 2048.f, r[1] * 2048.f}), f16x2));
   }
 }
+
+// Unit of row r in a step of a panel in LDS: a wave that splits a row writes a quad of it to every half step, 512 bytes
+// apart, and the rows change places there so that these go to all banks.
+__device__ __forceinline__ int place(int step, int half, int r) { return half * 32 + (r ^ ((2 * step + half) & 31)); }
 
 // A panel of 32 rows per workgroup, in lots of kLot elements: a wave takes every eighth row in
 // whole lines, a lane four elements; the first kHeld lots stay in registers between the search for
@@ -117,47 +135,39 @@ __global__ __launch_bounds__(512) void gated_split_kernel(const float* x, long l
   const long long row0 = (long long)blockIdx.x * 32, panel = (long long)blockIdx.x * stride + offset;
   const int lots = (steps + kLotSteps - 1) / kLotSteps;
   if (threadIdx.x == 0) any = more ? plain[blockIdx.x] : 0;
-  auto load = [&](int lot, float (&v)[4][4]) __attribute__((always_inline)) {
-    const int c = lot * kLot + 4 * lane;
+  auto load = [&](int lot, f32x4(&v)[4]) __attribute__((always_inline)) {
+    const Quad q(lot * kLot + 4 * lane, ic);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = q.load(x + min(row0 + wave + 8 * i, (long long)rows - 1) * ldx);
+  };
+  Range range[4];
+  auto look = [&](int lot, f32x4(&v)[4]) __attribute__((always_inline)) {
+    const Quad q(lot * kLot + 4 * lane, ic);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const f32x4 t = load4(x + min(row0 + wave + 8 * i, (long long)rows - 1) * ldx, c, ic);
+      v[i] = q.mend(v[i]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[i][e] = t[e];
+      for (int e = 0; e < 4; ++e) range[i].look(v[i][e]);
     }
   };
-  unsigned top[4] = {}, low[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) low[i] = 0x7fffffffu;
-  auto look = [&](const float(&v)[4][4]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const unsigned m = magnitude(v[i][e]);
-        top[i] = max(top[i], m);
-        low[i] = min(low[i], m ? m : 0x7fffffffu);
-      }
-  };
-  float held[kHeld][4][4];
+  f32x4 held[kHeld][4];
 #pragma unroll
   for (int l = 0; l < kHeld; ++l)
     if (l < lots) load(l, held[l]);
 #pragma unroll
   for (int l = 0; l < kHeld; ++l)
-    if (l < lots) look(held[l]);
+    if (l < lots) look(l, held[l]);
   for (int l = kHeld; l < lots; ++l) {
-    float v[4][4];
+    f32x4 v[4];
     load(l, v);
-    look(v);
+    look(l, v);
   }
   __syncthreads();  // `any` stands
   float scale[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const unsigned t = (unsigned)wave_max_i32((int)top[i]);
-    const unsigned l = 0x7fffffffu - (unsigned)wave_max_i32((int)(0x7fffffffu - low[i]));
-    const bool here = row0 + wave + 8 * i < rows, bad = here && uneven(t, l);
+    const unsigned t = lanes_max<64>(range[i].top);
+    const bool here = row0 + wave + 8 * i < rows, bad = here && __any(range[i].uneven(t));
     const int field = gated_field(t);
     scale[i] = here ? exp_float(field) : 0.f;
     if (lane == 0) {
@@ -166,27 +176,33 @@ __global__ __launch_bounds__(512) void gated_split_kernel(const float* x, long l
     }
   }
   u32x4* to = out + panel * steps * kStep;
-  auto put = [&](int lot, const float(&v)[4][4]) __attribute__((always_inline)) {
+  auto put = [&](int lot, const f32x4(&v)[4]) __attribute__((always_inline)) {
     u32x4* at_lds = lds[lot & 1];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       u32x2 h, l;
-      split4(f32x4{v[i][0], v[i][1], v[i][2], v[i][3]}, scale[i], h, l);
+      split4(v[i], scale[i], h, l);
       // Elements 4 lane .. + 3: step lane / 4, half (lane / 2) % 2, its first or second four.
-      u32x2* at = (u32x2*)(at_lds + (lane >> 2) * kStep + ((lane >> 1) & 1) * 32 + wave + 8 * i) + (lane & 1);
+      u32x2* at = (u32x2*)(at_lds + (lane >> 2) * kStep + place(lane >> 2, (lane >> 1) & 1, wave + 8 * i)) + (lane & 1);
       at[0] = h;
       at[128] = l;
     }
     __syncthreads();
     const int units = min(kLotSteps, steps - lot * kLotSteps) * kStep;
-    for (int u = threadIdx.x; u < units; u += 512) to[lot * kLotSteps * kStep + u] = at_lds[u];
+    for (int u = threadIdx.x; u < units; u += 512) {
+      const int step = u / kStep, part = u & 64, half = (u >> 5) & 1;
+      to[lot * kLotSteps * kStep + u] = at_lds[step * kStep + part + place(step, half, u & 31)];
+    }
   };
 #pragma unroll
   for (int l = 0; l < kHeld; ++l)
     if (l < lots) put(l, held[l]);
   for (int l = kHeld; l < lots; ++l) {
-    float v[4][4];
+    const Quad q(l * kLot + 4 * lane, ic);
+    f32x4 v[4];
     load(l, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = q.mend(v[i]);
     put(l, v);
   }
   __syncthreads();
@@ -231,6 +247,26 @@ __device__ __forceinline__ void gated_plain(const GatedArgs& a, long long row0, 
       acc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(xv[e], g[e], acc[0], 0, 0, 0);
       acc[1] = __builtin_amdgcn_mfma_f32_32x32x2f32(xv[e], u[e], acc[1], 0, 0, 0);
     }
+  }
+}
+
+// A wave's 32 x 32 sums, gate and up, to the output: rows from row0, channel `col` of lane r32.
+__device__ __forceinline__ void gated_out(const GatedArgs& a, int row0, int col, int half, float (&g)[16], float (&u)[16]) {
+  const float gb = a.bias[col], ub = a.bias[a.panels * 32 + col];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) g[r] += gb;
+  activate(a.act, g);
+  if (col >= a.oc) return;
+  float* y = a.y + (row0 + 4 * half) * a.ldy + col;
+  if (row0 + 32 <= a.rows) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) y[(8 * (r >> 2) + (r & 3)) * a.ldy] = g[r] * (u[r] + ub);
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int row = 8 * (r >> 2) + (r & 3);
+    if (row0 + 4 * half + row < a.rows) y[row * a.ldy] = g[r] * (u[r] + ub);
   }
 }
 
@@ -330,19 +366,20 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_kernel(const GatedArgs a
 
   const int panel = ct * WN + wn, col = 32 * panel + r32;
   if (panel >= a.panels) return;
-  const bool live = col < a.oc;
-  const float gb = a.bias[col], ub = a.bias[a.panels * 32 + col];
   const int gw = a.w_row[panel * 64 + r32] & 0xff, uw = a.w_row[panel * 64 + 32 + r32] & 0xff;
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const int xp = (rt * WM + wm) * TM + i;
     if (xp >= a.xpanels) return;
-    f32x16 g, u;
+    float g[16], u[16];
     if (a.x_plain[xp] | a.w_plain[panel]) {
       f32x16 t[2];
       gated_plain(a, (long long)xp * 32, panel, 0, a.steps, lane, t);
-      g = t[0];
-      u = t[1];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        g[r] = t[0][r];
+        u[r] = t[1][r];
+      }
     } else {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -351,11 +388,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_kernel(const GatedArgs a
         u[r] = __builtin_ldexpf(__builtin_fmaf(crs[i][1][r], 1.f / 2048, acc[i][1][r]), 254 - f - uw);
       }
     }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int row = xp * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-      if (live && row < a.rows) a.y[row * a.ldy + col] = activate(a.act, g[r] + gb) * (u[r] + ub);
-    }
+    gated_out(a, xp * 32, col, half, g, u);
   }
 }
 
@@ -400,7 +433,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const Gate
   f32x4 total[2] = {};
   for (int p = p0; p < p1; p += kAhead) {
     f16x8 wv[kAhead][2][2];
-    float xv[kAhead][8];
+    f32x4 xv[kAhead][2];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const long long at = (long long)min(p + u, pairs - 1) * 2 * kStep;
@@ -409,23 +442,32 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const Gate
 #pragma unroll
         for (int s = 0; s < 2; ++s) wv[u][j][s] = __builtin_bit_cast(f16x8, w[j * up + at + 64 * s]);
     }
+    if (a.ic >= 4) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) load8(xr, min(p + u, pairs) * 32 + 8 * oct, a.ic, xv[u]);
-    unsigned top = 0, low = 0x7fffffffu;
+      for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) xv[u][h] = Quad(min(p + u, pairs) * 32 + 8 * oct + 4 * h, a.ic).load(xr);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) xv[u][h][e] = xr[min(e, a.ic - 1)];
+    }
+    Range range;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const unsigned m = p + u < p1 ? magnitude(xv[u][e]) : 0;
-        top = max(top, m);
-        low = min(low, m ? m : 0x7fffffffu);
-      }
+      for (int h = 0; h < 2; ++h) {
+        xv[u][h] = Quad(p + u < p1 ? (p + u) * 32 + 8 * oct + 4 * h : a.ic, a.ic).mend(xv[u][h]);
 #pragma unroll
-    for (int off = 16; off < 64; off <<= 1) {
-      top = max(top, (unsigned)__shfl_xor((int)top, off));
-      low = min(low, (unsigned)__shfl_xor((int)low, off));
-    }
-    if (__any(w_plain != 0 || uneven(top, low))) {
+        for (int e = 0; e < 4; ++e) range.look(xv[u][h][e]);
+      }
+    unsigned top = range.top;
+#pragma unroll
+    for (int off = 16; off < 64; off <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, off));
+    if (__any(w_plain != 0 || range.uneven(top))) {
       for (int u = p; u < min(p + kAhead, p1); ++u) gated_plain16(a, row0, 32 * panel + sub, 32 * u, lane, total);
       continue;
     }
@@ -435,7 +477,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const Gate
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       u32x4 h, l;
-      pair8(xv[u], p + u < p1 ? scale : 0.f, h, l);
+      pair8(xv[u], scale, h, l);
       const f16x8 xh = __builtin_bit_cast(f16x8, h), xl = __builtin_bit_cast(f16x8, l);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -466,7 +508,10 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const Gate
     g += sums[x][0][row][r16];
     u += sums[x][1][row][r16];
   }
-  if (col < a.oc) a.y[(row0 + row) * a.ldy + col] = activate(a.act, g + a.bias[col]) * (u + a.bias[a.panels * 32 + col]);
+  if (col >= a.oc) return;
+  float v[1] = {g + a.bias[col]};
+  activate(a.act, v);
+  a.y[(row0 + row) * a.ldy + col] = v[0] * (u + a.bias[a.panels * 32 + col]);
 }
 
 // A middling number of tiles: a panel of rows by PAN panels of output channels to a workgroup, each
@@ -487,15 +532,15 @@ __global__ __launch_bounds__(512, 2) void gated_mid_kernel(const GatedArgs a) {
   const u32x4* w = a.w + (long long)2 * panel * a.steps * kStep + lane;
   const long long up = (long long)a.steps * kStep;
   // A wave takes every eighth row, a lane four elements of it.
-  float v[4][4];
-  auto load = [&](int k0, float(&v)[4][4]) __attribute__((always_inline)) {
-    const int c = 16 * k0 + 4 * lane;
+  auto load = [&](int k0, f32x4(&v)[4]) __attribute__((always_inline)) {
+    const Quad q(16 * k0 + 4 * lane, a.ic);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 t = load4(a.x + (long long)min(row0 + wave + 8 * i, a.rows - 1) * a.ldx, c, a.ic);
+    for (int i = 0; i < 4; ++i) v[i] = q.load(a.x + (long long)min(row0 + wave + 8 * i, a.rows - 1) * a.ldx);
+  };
+  auto mend = [&](int k0, f32x4(&v)[4]) __attribute__((always_inline)) {
+    const Quad q(16 * k0 + 4 * lane, a.ic);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[i][e] = t[e];
-    }
+    for (int i = 0; i < 4; ++i) v[i] = q.mend(v[i]);
   };
   // Weights of steps k and on, four at a time.
   f16x8 wv[4][2][2];
@@ -509,45 +554,44 @@ __global__ __launch_bounds__(512, 2) void gated_mid_kernel(const GatedArgs a) {
           wv[u][j][s] = __builtin_bit_cast(f16x8, w[j * up + (long long)min(k + u, a.steps - 1) * kStep + 64 * s]);
   };
   // The rows' powers: the first lot stays in registers, the others come four at a time.
-  unsigned top[4] = {}, low[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) low[i] = 0x7fffffffu;
-  auto look = [&](const float(&t)[4][4]) __attribute__((always_inline)) {
+  Range range[4];
+  auto look = [&](const f32x4(&t)[4]) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const unsigned m = magnitude(t[i][e]);
-        top[i] = max(top[i], m);
-        low[i] = min(low[i], m ? m : 0x7fffffffu);
-      }
+      for (int e = 0; e < 4; ++e) range[i].look(t[i][e]);
   };
+  f32x4 v[4];
   load(0, v);
-  for (int k0 = kLotSteps; k0 < a.steps; k0 += 4 * kLotSteps) {
-    float t[4][4][4];
-#pragma unroll
-    for (int l = 0; l < 4; ++l) load(min(k0 + l * kLotSteps, (a.steps - 1) / kLotSteps * kLotSteps), t[l]);
-#pragma unroll
-    for (int l = 0; l < 4; ++l) look(t[l]);
-  }
   load_w(part * SH);
+  for (int k0 = kLotSteps; k0 < a.steps; k0 += 4 * kLotSteps) {
+    f32x4 t[4][4];
+    auto at = [&](int l) { return min(k0 + l * kLotSteps, (a.steps - 1) / kLotSteps * kLotSteps); };
+#pragma unroll
+    for (int l = 0; l < 4; ++l) load(at(l), t[l]);
+#pragma unroll
+    for (int l = 0; l < 4; ++l) {
+      mend(at(l), t[l]);
+      look(t[l]);
+    }
+  }
+  mend(0, v);
   look(v);
   float scale[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const unsigned t = (unsigned)wave_max_i32((int)top[i]);
-    const unsigned l = 0x7fffffffu - (unsigned)wave_max_i32((int)(0x7fffffffu - low[i]));
-    const int field = gated_field(t);
+    const unsigned t = lanes_max<64>(range[i].top);
+    const int field = gated_field(t), bad = __any(range[i].uneven(t)) ? kPlainRow : 0;
     scale[i] = exp_float(field);
-    if (lane == 0) fields[wave + 8 * i] = field | (uneven(t, l) ? kPlainRow : 0);
+    if (lane == 0) fields[wave + 8 * i] = field | bad;
   }
   auto put = [&](u32x4* to) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       u32x2 h, l;
-      split4(f32x4{v[i][0], v[i][1], v[i][2], v[i][3]}, scale[i], h, l);
+      split4(v[i], scale[i], h, l);
       // Elements 4 lane .. + 3: step lane / 4, half (lane / 2) % 2, its first or second four.
-      u32x2* at = (u32x2*)(to + (lane >> 2) * kStep + ((lane >> 1) & 1) * 32 + wave + 8 * i) + (lane & 1);
+      u32x2* at = (u32x2*)(to + (lane >> 2) * kStep + place(lane >> 2, (lane >> 1) & 1, wave + 8 * i)) + (lane & 1);
       at[0] = h;
       at[128] = l;
     }
@@ -567,7 +611,7 @@ __global__ __launch_bounds__(512, 2) void gated_mid_kernel(const GatedArgs a) {
     for (int u = 0; u < SH; ++u) {
       const int k = part * SH + u;
       if (k0 + k < a.steps) {
-        const u32x4* f = lds[now] + k * kStep + lane;
+        const u32x4* f = lds[now] + k * kStep + place(k, half, r32);
         const f16x8 xh = __builtin_bit_cast(f16x8, f[0]), xl = __builtin_bit_cast(f16x8, f[64]);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -578,7 +622,10 @@ __global__ __launch_bounds__(512, 2) void gated_mid_kernel(const GatedArgs a) {
       }
       if ((u & 3) == 3) load_w(u + 1 < SH ? k0 + k + 1 : k0 + kLotSteps + part * SH);
     }
-    if (more) put(lds[now ^ 1]);
+    if (more) {
+      mend(k0 + kLotSteps, v);
+      put(lds[now ^ 1]);
+    }
     __syncthreads();
   }
   if (__any(fields[r32] & kPlainRow) || a.w_plain[panel]) {
@@ -603,17 +650,174 @@ __global__ __launch_bounds__(512, 2) void gated_mid_kernel(const GatedArgs a) {
   const int col = 32 * panel + r32;
   if (col >= a.oc) return;
   const float gb = a.bias[col], ub = a.bias[a.panels * 32 + col];
+  float g[16 / KW], u[16 / KW];
 #pragma unroll
   for (int i = 0; i < 16 / KW; ++i) {
     const int row = 2 * (KW * i + part) + half;
-    if (row0 + row >= a.rows) break;
-    float g = 0.f, u = 0.f;
+    g[i] = gb;
+    u[i] = ub;
 #pragma unroll
     for (int x = 0; x < KW; ++x) {
-      g += sums[wave - part + x][0][row][r32];
-      u += sums[wave - part + x][1][row][r32];
+      g[i] += sums[wave - part + x][0][row][r32];
+      u[i] += sums[wave - part + x][1][row][r32];
     }
-    a.y[(row0 + row) * a.ldy + col] = activate(a.act, g + gb) * (u + ub);
+  }
+  activate(a.act, g);
+#pragma unroll
+  for (int i = 0; i < 16 / KW; ++i) {
+    const int row = row0 + 2 * (KW * i + part) + half;
+    if (row < a.rows) a.y[row * a.ldy + col] = g[i] * u[i];
+  }
+}
+
+// Short rows (up to 256 elements) and many: 32 PX rows by panels of output channels, one to a wave, to a
+// workgroup.  It loads its rows at once, in whole lines, splits them into LDS, where they stay, and
+// goes through a column of tiles (every col_tiles-th) with the weights straight from memory and no
+// further barrier.  LANES lanes hold a row, a quad each.
+template <int PX, int LANES>
+__global__ __launch_bounds__(256, 2) void gated_short_kernel(const GatedArgs a) {
+  constexpr int SIDE = 64 / LANES, LOADS = 8 * PX / SIDE;  // rows side by side in a wave's load; loads of a wave
+  extern __shared__ u32x4 xs[];                            // [PX][steps] fragments
+  __shared__ __align__(16) int words[32 * PX];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, r32 = lane & 31, l = lane % LANES, side = lane / LANES;
+  const int tile = blockIdx.x / a.col_tiles, first = blockIdx.x - tile * a.col_tiles, row0 = tile * 32 * PX;
+  const long long up = (long long)a.steps * kStep;
+  constexpr int AHEAD = PX == 1 ? 4 : 2;  // steps of weights under way
+  f16x8 wv[AHEAD][2][2];
+  auto load_w = [&](int panel, int k, int u) __attribute__((always_inline)) {
+    const u32x4* w = a.w + (long long)2 * panel * a.steps * kStep + lane + min(k, a.steps - 1) * kStep;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) wv[u][j][s] = __builtin_bit_cast(f16x8, w[j * up + 64 * s]);
+  };
+  {
+    const Quad q(4 * l, a.ic);
+    const int mine = wave * 8 * PX + side;  // the first of a lane's rows
+    f32x4 v[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+      v[i] = q.load(a.x + (unsigned long long)(unsigned)min(row0 + mine + i * SIDE, a.rows - 1) * (unsigned)a.ldx);
+    const int panel = min(first * 4 + wave, a.panels - 1);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) load_w(panel, u, u);
+    unsigned top[LOADS], low[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      v[i] = q.mend(v[i]);
+      Range range;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) range.look(v[i][e]);
+      low[i] = range.low;
+      top[i] = lanes_max<LANES>(range.top);
+    }
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      Range range;
+      range.low = low[i];
+      const unsigned long long bad = __ballot(range.uneven(top[i])) >> (side * LANES & 63);
+      low[i] = (LANES == 64 ? bad : (unsigned)bad) != 0 ? kPlainRow : 0;
+    }
+    if (l == 0)
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) words[mine + i * SIDE] = gated_field(top[i]) | low[i];
+    const int step = l >> 2;
+    if (step < a.steps)
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int r = mine + i * SIDE;
+        u32x2 h, lo;
+        split4(v[i], exp_float(gated_field(top[i])), h, lo);
+        u32x2* at = (u32x2*)(xs + ((r >> 5) * a.steps + step) * kStep + place(step, (l >> 1) & 1, r & 31)) + (l & 1);
+        at[0] = h;
+        at[128] = lo;
+      }
+  }
+  __syncthreads();
+  bool plain[PX], again = false;
+#pragma unroll
+  for (int i = 0; i < PX; ++i) plain[i] = __any(words[32 * i + r32] & kPlainRow);
+  for (int ct = first; 4 * ct < a.panels; ct += a.col_tiles) {
+    const int panel = min(4 * ct + wave, a.panels - 1), next = min(4 * (ct + a.col_tiles) + wave, a.panels - 1);
+    f32x16 acc[PX][2], crs[PX][2];
+#pragma unroll
+    for (int i = 0; i < PX; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = crs[i][j][r] = 0.f;
+    for (int k0 = 0; k0 < a.steps; k0 += AHEAD)
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int k = k0 + u;
+        if (k < a.steps) {
+          f16x8 av[PX][2];
+#pragma unroll
+          for (int i = 0; i < PX; ++i)
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+              av[i][p] = __builtin_bit_cast(f16x8, xs[(i * a.steps + k) * kStep + 64 * p + place(k, half, r32)]);
+#pragma unroll
+          for (int i = 0; i < PX; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              crs[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av[i][1], wv[u][j][0], crs[i][j], 0, 0, 0);
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av[i][0], wv[u][j][0], acc[i][j], 0, 0, 0);
+            }
+#pragma unroll
+          for (int i = 0; i < PX; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              crs[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av[i][0], wv[u][j][1], crs[i][j], 0, 0, 0);
+        }
+        load_w(panel, k + AHEAD, u);
+      }
+    if (4 * ct + wave >= a.panels) break;
+    const int col = 32 * panel + r32;
+    const int gw = a.w_row[panel * 64 + r32] & 0xff, uw = a.w_row[panel * 64 + 32 + r32] & 0xff;
+    const bool w_plain = a.w_plain[panel];
+#pragma unroll
+    for (int i = 0; i < PX; ++i) {
+      float g[16], u[16];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int4 f = *(const int4*)&words[32 * i + 8 * q + 4 * half];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * q + e, to = 254 - ((&f.x)[e] & 0xff);
+          g[r] = __builtin_ldexpf(__builtin_fmaf(crs[i][0][r], 1.f / 2048, acc[i][0][r]), to - gw);
+          u[r] = __builtin_ldexpf(__builtin_fmaf(crs[i][1][r], 1.f / 2048, acc[i][1][r]), to - uw);
+        }
+      }
+      if (i == PX - 1)
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) load_w(next, u, u);
+      if (plain[i] || w_plain) {
+        again = true;
+        continue;
+      }
+      gated_out(a, row0 + 32 * i, col, half, g, u);
+    }
+  }
+  if (!again) return;
+  // The tiles that were left out, in plain float32 (inside the loop above they would cost it its registers).
+  for (int ct = first; 4 * ct + wave < a.panels; ct += a.col_tiles) {
+    const int panel = 4 * ct + wave, col = 32 * panel + r32;
+    const bool w_plain = a.w_plain[panel];
+#pragma unroll 1
+    for (int i = 0; i < PX; ++i) {
+      if (!w_plain && !__any(words[32 * i + r32] & kPlainRow)) continue;
+      f32x16 t[2];
+      gated_plain(a, row0 + 32 * i, panel, 0, a.steps, lane, t);
+      float g[16], u[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        g[r] = t[0][r];
+        u[r] = t[1][r];
+      }
+      gated_out(a, row0 + 32 * i, col, half, g, u);
+    }
   }
 }
 
@@ -632,7 +836,7 @@ static int gated_pack(sy_ctx* ctx, const float* gate, const float* up, const flo
   SY_HIP(hipMalloc((void**)&p->w_row, cols * 2 * sizeof(int)));
   SY_HIP(hipMalloc((void**)&p->w_plain, p->panels * sizeof(int)));
   SY_HIP(hipMalloc((void**)&p->bias, 2 * cols * sizeof(float)));
-  SY_HIP(hipMalloc((void**)&p->raw, 2 * values * sizeof(float)));
+  SY_HIP(hipMalloc((void**)&p->raw, (2 * values + 4) * sizeof(float)));  // rows are read by quads
   SY_TRY(sy_memcpy(ctx, p->raw, gate, values * sizeof(float), 0));
   SY_TRY(sy_memcpy(ctx, p->raw + values, up, values * sizeof(float), 0));
   SY_TRY(sy_memcpy(ctx, p->bias, bias.data(), 2 * cols * sizeof(float), 0));
@@ -731,13 +935,38 @@ int op_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tenso
   const double flops = 4.0 * rows * p.ic * p.oc, bytes = 4.0 * ((double)rows * (p.ic + p.oc) + 2.0 * p.ic * p.oc);
   // 32 rows of 1024 to 2816 channels 13.3 us here, 17.6 as a middling number of tiles; 64 of 256 to 688 (176 workgroups)
   // 6.7 and 7.8, 256 of 128 to 256 (256) 5.4 and 7.7, 100 of 255 to 690 (308) 11.9 and 8.4, 33 of 2048 to 4096 (768) 40 and 33.
-  if (a.rows <= 32 || 2LL * p.panels * ((a.rows + 15) / 16) <= 256) {
+  if (a.rows <= 32 || a.ic < 4 || 2LL * p.panels * ((a.rows + 15) / 16) <= 256) {
     ProfScope prof(ctx, "gated_few", flops, bytes);
-    const dim3 grid((unsigned)(2 * p.panels * ((a.rows + 15) / 16)));
-    hipLaunchKernelGGL(gated_few_kernel, grid, dim3(kFewWaves * 64), 0, ctx->stream, a);
+    const long long grid = 2LL * p.panels * ((a.rows + 15) / 16);
+    SY_CHECK(grid * kFewWaves * 64 < (1LL << 32), SY_EUNSUPPORTED, "gated grid too large");
+    hipLaunchKernelGGL(gated_few_kernel, dim3((unsigned)grid), dim3(kFewWaves * 64), 0, ctx->stream, a);
     return check_launch("gated_few");
   }
-  // One workgroup to a CU: 1200 rows of 256 to 690 channels (228 of them) 13.1 us here, 20.4 split beforehand; to 2048
+  if (a.ic <= 4 * 64) {
+    // Short rows: three column tiles (of 128 channels) or four at most, or a thousand tiles; else the products are so
+    // many that splitting x beforehand pays (20000 rows of 256 to 512 channels 58 us here, 53 so; to 256 33.7 and 38).
+    // Where 64 rows to a workgroup make 512 of them, that, and every column tile in turn: 60000 rows of 256 to 384 channels
+    // 104 us, 122 with 32 rows, 123 split beforehand; 9471 of 90 to 360 15.5 to 24, 17.9, 19.7.  With 32 rows, every
+    // column tile in turn where there are 400 workgroups: 14161 of 137 to 377 26.4 us, a tile to each 30.4; 9471 of 90 to
+    // 360 21.6 and 17.9.
+    const int cols = (a.panels + 3) / 4, wide = (a.rows + 63) / 64;
+    auto go = [&](auto kernel, int tiles, int px) {
+      ProfScope prof(ctx, "gated_short", flops, bytes);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * a.col_tiles)), dim3(256), (size_t)px * a.steps * kStep * 16,
+                         ctx->stream, a);
+      return check_launch("gated_short");
+    };
+    if (wide >= 512 && cols <= 4) {
+      SY_CHECK(wide * 256LL < (1LL << 32), SY_EUNSUPPORTED, "gated grid too large");
+      a.col_tiles = 1;
+      return a.steps <= 8 ? go(gated_short_kernel<2, 32>, wide, 2) : go(gated_short_kernel<2, 64>, wide, 2);
+    }
+    if (cols <= 3 || (long long)a.xpanels * cols <= 1024) {
+      a.col_tiles = a.xpanels >= 400 ? 1 : cols;
+      return a.steps <= 8 ? go(gated_short_kernel<1, 32>, a.xpanels, 1) : go(gated_short_kernel<1, 64>, a.xpanels, 1);
+    }
+  }
+  // One workgroup to a CU: 1200 rows of 256 to 690 channels (228 of them) 12.2 us here, 20.4 split beforehand; to 2048
   // channels (608) 32.8 and 25.8.
   const long long mids = a.xpanels * ((p.panels + 3LL) / 4), wide = a.xpanels * ((p.panels + 1LL) / 2);
   if (mids <= 256) {
@@ -780,8 +1009,8 @@ int op_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tenso
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(waves * 64), 0, ctx->stream, a);
     return check_launch("gated");
   };
-  // Two panels of output channels to a workgroup where there are no more: 20000 rows of 96 to 60 channels would leave half
-  // the waves of four without any.
+  // Two panels of output channels to a workgroup where there are no more: 60000 rows of 512 to 64 channels 83 us, 99 where
+  // half the waves have none.
   if (a.panels <= 2) return launch(gated_kernel<1, 2>, 2, 2, 2);
   return launch(gated_kernel<1, 4>, 2, 4, 4);
 }

@@ -69,8 +69,18 @@ __device__ __forceinline__ Scale scale_of(const NormArgs& a, const Moments& m, d
   return s;
 }
 
-__device__ __forceinline__ float normal(const NormArgs& a, float x, const Scale& s, float g, float b) {
-  return activate(a.act, __builtin_fmaf((x - s.hi) - s.lo, s.r * g, b));
+// Before the activation.
+__device__ __forceinline__ float normal(float x, const Scale& s, float g, float b) {
+  return __builtin_fmaf((x - s.hi) - s.lo, s.r * g, b);
+}
+
+template <int VEC>
+__device__ __forceinline__ void put(float* to, const float* from) {
+  typedef typename Vec<VEC>::type vec;
+  vec t;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) t[e] = from[e];
+  *(vec*)to = t;
 }
 
 // v plus that of the lane that DPP control ctrl reads.
@@ -135,14 +145,15 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(const NormArgs a) {
   m.s = plus_lanes(m.s, lanes);
   m.q = plus_lanes(m.q, lanes);
   const Scale s = scale_of(a, m, p);
+  float o[V * VEC];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (!live || lane + i * lanes >= total) continue;
-    vec o;
+  for (int i = 0; i < V; ++i)
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) o[e] = normal(a, v[i][e], s, ga[i][e], be[i][e]);
-    *(vec*)(y + px[i] * a.ldy + ch[i]) = o;
-  }
+    for (int e = 0; e < VEC; ++e) o[i * VEC + e] = normal(v[i][e], s, ga[i][e], be[i][e]);
+  activate(a.act, o);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (live && lane + i * lanes < total) put<VEC>(y + px[i] * a.ldy + ch[i], &o[i * VEC]);
 }
 
 // The moments of the run's groups from every thread's own, E of them, each of one group: a
@@ -215,14 +226,15 @@ __global__ __launch_bounds__(1024) void norm_group_kernel(const NormArgs a) {
   }
   if (!live) return;
   const Scale s = scale_of(a, m, p);
+  float o[V * VEC];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (row + i * a.rows >= a.t) break;
-    vec o;
+  for (int i = 0; i < V; ++i)
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) o[e] = normal(a, v[i][e], s, ga[e], be[e]);
-    *(vec*)(y + (row + i * a.rows) * a.ldy + c) = o;
-  }
+    for (int e = 0; e < VEC; ++e) o[i * VEC + e] = normal(v[i][e], s, ga[e], be[e]);
+  activate(a.act, o);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (row + i * a.rows < a.t) put<VEC>(y + (row + i * a.rows) * a.ldy + c, &o[i * VEC]);
 }
 
 constexpr int kDeep = 4;  // pixels of a thread under way
@@ -316,19 +328,25 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(const NormArgs a) {
 #pragma unroll
   for (int e = 0; e < E; ++e) s[e] = scale[(col * E + e) / cols_each];
   while (i < to) {
-    vec o[kDeep];
+    float o[kDeep * VEC];
 #pragma unroll
     for (int k = 0; k < kDeep; ++k)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o[k][e] = normal(a, v[k][e], s[e % E], ga[e], be[e]);
+      for (int e = 0; e < VEC; ++e) o[k * VEC + e] = normal(v[k][e], s[e % E], ga[e], be[e]);
     const int at = i;
     i += kDeep * a.rows;
     if (i < to)
 #pragma unroll
       for (int k = 0; k < kDeep; ++k) v[k] = *(const vec*)(x + min(i + k * a.rows, to - 1) * a.ldx + c);
+    activate(a.act, o);
 #pragma unroll
     for (int k = 0; k < kDeep; ++k)
-      if (at + k * a.rows < to) __builtin_nontemporal_store(o[k], (vec*)(y + (at + k * a.rows) * a.ldy + c));
+      if (at + k * a.rows < to) {
+        vec t;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) t[e] = o[k * VEC + e];
+        __builtin_nontemporal_store(t, (vec*)(y + (at + k * a.rows) * a.ldy + c));
+      }
   }
 }
 
