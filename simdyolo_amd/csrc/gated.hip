@@ -417,6 +417,7 @@ __device__ __forceinline__ void gated_plain16(const GatedArgs& a, int row0, int 
 // pairs of steps at once.  A wave splits x itself, under powers of the pairs of steps it has in
 // hand, and brings each lot's sums to their true scale; a lot with an uneven row is plain by itself.
 constexpr int kFewWaves = 8, kAhead = 4;
+template <bool TINY>
 __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const GatedArgs a) {
   __shared__ float sums[kFewWaves][2][16][17];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -435,6 +436,17 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const Gate
     f16x8 wv[kAhead][2][2];
     f32x4 xv[kAhead][2];
 #pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (TINY) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) xv[u][h][e] = xr[min(e, a.ic - 1)];
+        } else {
+          xv[u][h] = Quad(min(p + u, pairs) * 32 + 8 * oct + 4 * h, a.ic).load(xr);
+        }
+      }
+#pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const long long at = (long long)min(p + u, pairs - 1) * 2 * kStep;
 #pragma unroll
@@ -442,28 +454,20 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const Gate
 #pragma unroll
         for (int s = 0; s < 2; ++s) wv[u][j][s] = __builtin_bit_cast(f16x8, w[j * up + at + 64 * s]);
     }
-    if (a.ic >= 4) {
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) xv[u][h] = Quad(min(p + u, pairs) * 32 + 8 * oct + 4 * h, a.ic).load(xr);
-    } else {
+    if (p + kAhead > p1 || 32 * (p + kAhead) > a.ic) {  // the row's end, or the wave's
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) xv[u][h][e] = xr[min(e, a.ic - 1)];
+          xv[u][h] = Quad(p + u < p1 ? (p + u) * 32 + 8 * oct + 4 * h : a.ic, a.ic).mend(xv[u][h]);
     }
     Range range;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        xv[u][h] = Quad(p + u < p1 ? (p + u) * 32 + 8 * oct + 4 * h : a.ic, a.ic).mend(xv[u][h]);
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) range.look(xv[u][h][e]);
-      }
     unsigned top = range.top;
 #pragma unroll
     for (int off = 16; off < 64; off <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, off));
@@ -933,13 +937,14 @@ int op_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tenso
   a.xpanels = (a.rows + 31) / 32;
   DeviceScope device(ctx);
   const double flops = 4.0 * rows * p.ic * p.oc, bytes = 4.0 * ((double)rows * (p.ic + p.oc) + 2.0 * p.ic * p.oc);
-  // 32 rows of 1024 to 2816 channels 13.3 us here, 17.6 as a middling number of tiles; 64 of 256 to 688 (176 workgroups)
-  // 6.7 and 7.8, 256 of 128 to 256 (256) 5.4 and 7.7, 100 of 255 to 690 (308) 11.9 and 8.4, 33 of 2048 to 4096 (768) 40 and 33.
+  // 32 rows of 1024 to 2816 channels 11.0 us here, 17.6 as a middling number of tiles; 64 of 256 to 688 (176 workgroups)
+  // 6.4, 7.5 as short rows; 256 of 128 to 256 (256) 5.1 and 5.7, 400 of 128 to 256 (400) 6.3 and 6.2, 33 of 2048 to 4096 (768) 40
+  // and 33 as a middling number.
   if (a.rows <= 32 || a.ic < 4 || 2LL * p.panels * ((a.rows + 15) / 16) <= 256) {
     ProfScope prof(ctx, "gated_few", flops, bytes);
     const long long grid = 2LL * p.panels * ((a.rows + 15) / 16);
     SY_CHECK(grid * kFewWaves * 64 < (1LL << 32), SY_EUNSUPPORTED, "gated grid too large");
-    hipLaunchKernelGGL(gated_few_kernel, dim3((unsigned)grid), dim3(kFewWaves * 64), 0, ctx->stream, a);
+    hipLaunchKernelGGL(a.ic < 4 ? gated_few_kernel<true> : gated_few_kernel<false>, dim3((unsigned)grid), dim3(kFewWaves * 64), 0, ctx->stream, a);
     return check_launch("gated_few");
   }
   if (a.ic <= 4 * 64) {
