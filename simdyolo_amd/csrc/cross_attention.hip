@@ -164,29 +164,20 @@ __device__ __forceinline__ void cross_seen(const uint8_t* mask, int j0, int to, 
   }
 }
 
-// One tile: states j0 .. j0 + 31 up to `to`, whose parts are at f.  seen: its mask bytes, where there are any.
-template <int KS, int DT>
-__device__ __forceinline__ void cross_tile(const CrossArgs& a, const u32x4* f, int j0, int to, const unsigned (&seen)[4],
-                                           const bf16x8 (&q)[KS][3], CrossRows<DT>& w) {
-  const int lane = threadIdx.x & 63, half = lane >> 5, r32 = lane & 31;
+// One tile: states j0 .. j0 + 31 up to `to`.  key(ks, p) and value(i, p) give their parts, then() follows the last
+// of the keys.  seen: the tile's mask bytes, where there are any.
+template <int KS, int DT, class Key, class Value, class Then>
+__device__ __forceinline__ void cross_tile(const CrossArgs& a, Key key, Value value, Then then, int j0, int to,
+                                           const unsigned (&seen)[4], const bf16x8 (&q)[KS][3], CrossRows<DT>& w) {
+  const int half = (threadIdx.x & 63) >> 5;
   if (a.mask) {
     const unsigned some = seen[0] | seen[1] | seen[2] | seen[3];
     w.any |= some;
-    if (!__any(some != 0)) return;
+    if (!__any(some != 0)) return then();
   } else {
     w.any = 1;
   }
   // Fragments are read a step ahead of the products that take them.
-  const u32x4* v = f + KS * 192 + lane;
-  auto key = [&](int ks, bf16x8(&k)[3]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int x = 0; x < 3; ++x)
-      k[x] = __builtin_bit_cast(bf16x8, f[(ks * 3 + x) * 64 + half * 32 + (r32 ^ (2 * ks + half))]);
-  };
-  auto value = [&](int i, bf16x8(&p)[3]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int x = 0; x < 3; ++x) p[x] = __builtin_bit_cast(bf16x8, v[(i * 3 + x) * 64]);
-  };
   f32x16 s;
 #pragma unroll
   for (int r = 0; r < 16; ++r) s[r] = 0.f;
@@ -200,6 +191,7 @@ __device__ __forceinline__ void cross_tile(const CrossArgs& a, const u32x4* f, i
     for (int x = 0; x < 6; ++x)
       s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kp[ks & 1][kPairA[x]], q[ks][kPairB[x]], s, 0, 0, 0);
   }
+  then();
   bf16x8 vp[2][3];
   value(0, vp[0]);
   if (a.mask) {
@@ -254,6 +246,24 @@ __device__ __forceinline__ void cross_tile(const CrossArgs& a, const u32x4* f, i
         w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[kPairA[x]], vp[i & 1][kPairB[x]], w.acc[d], 0, 0, 0);
     }
   }
+}
+
+// A tile whose parts are in LDS, at f.
+template <int KS, int DT>
+__device__ __forceinline__ void cross_tile(const CrossArgs& a, const u32x4* f, int j0, int to, const unsigned (&seen)[4],
+                                           const bf16x8 (&q)[KS][3], CrossRows<DT>& w) {
+  const int lane = threadIdx.x & 63, half = lane >> 5, r32 = lane & 31;
+  const u32x4* v = f + KS * 192 + lane;
+  auto key = [&](int ks, bf16x8(&k)[3]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 3; ++x)
+      k[x] = __builtin_bit_cast(bf16x8, f[(ks * 3 + x) * 64 + half * 32 + (r32 ^ (2 * ks + half))]);
+  };
+  auto value = [&](int i, bf16x8(&p)[3]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 3; ++x) p[x] = __builtin_bit_cast(bf16x8, v[(i * 3 + x) * 64]);
+  };
+  cross_tile<KS, DT>(a, key, value, [] {}, j0, to, seen, q, w);
 }
 
 // The outputs of 32 rows from row0, or what a piece leaves for them, in whole lines of
@@ -460,7 +470,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cross_kernel(const CrossArgs a) {
 constexpr int kShortLds = 150 * 1024, kShortWaves = 4;
 constexpr int short_bytes(int ks, int dt) { return (ks + 2 * dt) * 3072; }  // of a tile
 template <int KS, int DT>
-__global__ __launch_bounds__(kShortWaves * 64, 2) void cross_short_kernel(const CrossArgs a) {
+__global__ __launch_bounds__(kShortWaves * 64, KS == 8 ? 1 : 2) void cross_short_kernel(const CrossArgs a) {
   constexpr int NW = kShortWaves;
   typedef CrossStage<KS, DT, NW * 64, 1> Stage;
   extern __shared__ u32x4 frag[];
@@ -513,6 +523,127 @@ __global__ __launch_bounds__(kShortWaves * 64, 2) void cross_short_kernel(const 
     split();  // before the stores: waiting for loads behind them would wait for them, too
     cross_finish<DT>(a, rows, plane, 0, tile * 32, to > 0);
   }
+}
+
+// Little work: 32 rows to a workgroup, and every fourth of their tiles to each of its waves, which take the states
+// straight into the order of the matrix instruction's lanes and split them for themselves: no barrier, and
+// no tile waits for another's loads.  What the waves hold meets in LDS at the end.
+constexpr int kLoneWaves = 4;
+template <int KS, int DT>
+__global__ __launch_bounds__(kLoneWaves * 64, KS + 2 * DT <= 8 ? 2 : 1) void cross_lone_kernel(const CrossArgs a) {
+  constexpr int NW = kLoneWaves;
+  __shared__ f32x4 others[NW - 1][DT * 4][64];
+  __shared__ float tops[NW][32], sums[NW][32];
+  __shared__ unsigned seens[NW][32];
+  const unsigned item = cross_item();
+  if (item >= a.items) return;
+  const int lane = threadIdx.x & 63, half = lane >> 5, r32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = item % a.tiles, plane = item / a.tiles;
+  const int b = plane / a.kv, g = plane - b * a.kv, to = cross_end(a, b);
+  const int row1 = min(tile * 32 + r32, a.rows - 1), qi = row1 / a.group, head = g * a.group + row1 - qi * a.group;
+  const float* kb = a.k + (long long)b * a.tk * a.ldk + (long long)g * a.ks;
+  const float* vb = a.v + (long long)b * a.tk * a.ldv + (long long)g * a.vs;
+  const uint8_t* mask = cross_mask(a, b, head, qi);
+  f32x4 kr[KS][2];
+  float vr[2 * DT][8];
+  auto load_k = [&](int j0) __attribute__((always_inline)) {
+    const float* k = kb + (long long)min(j0 + r32, to - 1) * a.ldk;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) kr[ks][e] = *(const f32x4*)(k + min(16 * ks + 8 * half + 4 * e, a.kd - 4));
+  };
+  auto load_v = [&](int j0) __attribute__((always_inline)) {
+    const float* v = vb + (long long)j0 * a.ldv;
+    const int last = to - 1 - j0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float* at = v + (unsigned)(min(8 * (e >> 2) + 4 * half + (e & 3), last) * a.ldv);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) vr[(e >> 3) * DT + d][e & 7] = at[min(32 * d + r32, a.hd - 1)];
+    }
+  };
+  CrossRows<DT> rows;
+  rows.clear();
+  int j0 = wave * kCrossKeys;
+  if (j0 < to) {
+    bf16x8 q[KS][3];
+    f32x4 raw[KS][2];
+    cross_query<KS>(a, b, qi, head, raw);
+    load_k(j0);
+    load_v(j0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) parts8(raw[ks][0], raw[ks][1], q[ks]);
+    do {
+      const int next = j0 + NW * kCrossKeys;
+      unsigned seen[4];
+      if (mask) cross_seen(mask, j0, to, seen);
+      cross_tile<KS, DT>(
+          a,
+          [&](int ks, bf16x8(&p)[3]) __attribute__((always_inline)) { parts8(kr[ks][0], kr[ks][1], p); },
+          [&](int i, bf16x8(&p)[3]) __attribute__((always_inline)) {
+            parts8(f32x4{vr[i][0], vr[i][1], vr[i][2], vr[i][3]}, f32x4{vr[i][4], vr[i][5], vr[i][6], vr[i][7]}, p);
+          },
+          [&]() __attribute__((always_inline)) {
+            if (next < to) load_k(next);
+          },
+          j0, to, seen, q, rows);
+      if (next < to) load_v(next);
+      j0 = next;
+    } while (j0 < to);
+  }
+  // The waves' maxima, then their sums on the common one.
+  const unsigned any = rows.any | (unsigned)__shfl_xor((int)rows.any, 32);
+  const float sum = rows.sum + __shfl_xor(rows.sum, 32);
+  if (half == 0) {
+    tops[wave][r32] = rows.top;
+    sums[wave][r32] = sum;
+    seens[wave][r32] = any;
+  }
+  __syncthreads();
+  float top = tops[0][r32], l = 0.f;
+  unsigned all = 0;
+#pragma unroll
+  for (int w = 1; w < NW; ++w) top = fmaxf(top, tops[w][r32]);
+  // A NaN keeps its place in the sum: its factor is 0, 1 or NaN.
+  auto share = [&](float t) { return t == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t - top); };
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    l = __builtin_fmaf(sums[w][r32], share(tops[w][r32]), l);
+    all |= seens[w][r32];
+  }
+  const float x = share(rows.top);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const float xr = __shfl(x, 8 * (r >> 2) + 4 * half + (r & 3));
+#pragma unroll
+    for (int d = 0; d < DT; ++d) rows.acc[d][r] *= xr;
+  }
+  if (wave > 0) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        others[wave - 1][4 * d + i][lane] =
+            f32x4{rows.acc[d][4 * i], rows.acc[d][4 * i + 1], rows.acc[d][4 * i + 2], rows.acc[d][4 * i + 3]};
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int w = 0; w < NW - 1; ++w) {
+        const f32x4 t = others[w][4 * d + i][lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rows.acc[d][4 * i + e] += t[e];
+      }
+  rows.top = top;
+  rows.sum = half == 0 ? l : 0.f;
+  rows.any = all;
+  cross_finish<DT>(a, rows, plane, 0, tile * 32, to > 0);
 }
 
 // v summed over aligned groups of 16 lanes, in each of them.
@@ -574,6 +705,12 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossArgs a) {
         k[u][c] = *(const f32x4*)(kb + j * a.ldk + kc[c]);
         v[u][c] = *(const f32x4*)(vb + j * a.ldv + vc[c]);
       }
+    uint8_t seen[G][U];
+    if (a.mask)
+#pragma unroll
+      for (int r = 0; r < G; ++r)
+#pragma unroll
+        for (int u = 0; u < U; ++u) seen[r][u] = mask[r][min(j0 + 16 * u, to - 1)];
 #pragma unroll
     for (int r = 0; r < G; ++r) {
       float s[U], mx = -INFINITY;
@@ -585,8 +722,7 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) t = __builtin_fmaf(q[r][c][e], k[u][c][e], t);
         t = plus16(t);
-        bool sees = j0 + 16 * u < to;
-        if (a.mask && sees) sees = mask[r][j0 + 16 * u] != 0;
+        const bool sees = j0 + 16 * u < to && (!a.mask || seen[r][u] != 0);
         any |= (unsigned)sees << r;
         s[u] = sees ? t : -INFINITY;
         mx = fmaxf(mx, s[u]);
@@ -744,6 +880,7 @@ static CrossKernel pick_cross(int ks, int dt) {
   return SY_CROSS_PICK(cross_kernel, SY_COMMA NW);
 }
 static CrossKernel pick_short(int ks, int dt) { return SY_CROSS_PICK(cross_short_kernel); }
+static CrossKernel pick_lone(int ks, int dt) { return SY_CROSS_PICK(cross_lone_kernel); }
 #undef SY_COMMA
 #undef SY_CROSS_PICK
 static CrossKernel pick_few(int kd, int hd, int rows) {
@@ -754,8 +891,11 @@ static CrossKernel pick_few(int kd, int hd, int rows) {
 
 // Waves of a workgroup and pieces of the states: the least estimated time, in cycles.  A wave's
 // tile takes 192 (ks + 2 dt) of the matrix cores, about 850 of other vector work and its share of
-// splitting the states; the waves of a SIMD overlap by a quarter; loads and barrier take 2,500 (of eight waves 3,200) anyway.
-static void cross_plan(CrossArgs& a, int ks, int dt, long long planes, long long row_tiles, int* nw) {
+// splitting the states (200 (ks + 2 dt)); the waves of a SIMD overlap by a quarter; loads and barrier take 2,500 (of
+// eight waves 3,200) anyway.  Whether each wave takes tiles for itself instead (cross_lone_kernel), with no overlap:
+// 400 rows of 8 heads of 32 to 77 states 6.2 us so, 7.6 not, 450 rows of 12 key heads to 171 10.7 and 15.8, 536 rows of 12 to
+// 213 9.8 and 15.3, but 800 rows of one to 2000 35 and 16.
+static void cross_plan(CrossArgs& a, int ks, int dt, long long planes, long long row_tiles, int* nw, bool* lone) {
   const int cus = 256, s = ks + 2 * dt;
   const long long key_tiles = (a.tk + kCrossKeys - 1) / kCrossKeys;
   double best = INFINITY;
@@ -777,6 +917,16 @@ static void cross_plan(CrossArgs& a, int ks, int dt, long long planes, long long
         a.splits = (int)x;
       }
     }
+  }
+  const long long rounds = (planes * row_tiles + cus - 1) / cus;
+  // (Beside it a join costs 3,500: 300 rows of two key heads to 900 states 14.7 us so, 11.9 in pieces; of eight to 600 11.3
+  // and 13.7.)
+  if (a.splits > 1) best -= 6500;
+  *lone = rounds * ((key_tiles + kLoneWaves - 1) / kLoneWaves * (392.0 * s + 850) + 800.0 * s - 1400) < best;
+  if (*lone) {
+    *nw = kLoneWaves;
+    a.tiles = (int)row_tiles;
+    a.splits = 1;
   }
 }
 
@@ -849,7 +999,8 @@ int op_cross_attention(sy_ctx* ctx, const sy_cross_config* c, const sy_tensor* q
   a.rows = a.tq * a.group;
   const long long planes = (long long)q->n * a.kv;
   const int ks = a.kd <= 32 ? 2 : a.kd <= 64 ? 4 : 8, dt = a.hd <= 32 ? 1 : a.hd <= 64 ? 2 : 4;
-  int nw = 0;  // waves that share a tile's states; 0: few rows, or few states
+  int nw = 0;  // waves of a workgroup; 0: few rows, or few states
+  bool lone = false;  // each with tiles of its own
   const long long row_tiles = (a.rows + 31) / 32;
   // 64 heads on 8 key heads of 16 images' 4000 states, a row tile of 8 rows each: 68 us on the matrix cores, 105 in
   // plain float32; 32 heads, 4 rows each, of 8 images 103 and 55.
@@ -864,7 +1015,7 @@ int op_cross_attention(sy_ctx* ctx, const sy_cross_config* c, const sy_tensor* q
     a.run = (a.run + kShortWaves - 1) / kShortWaves * kShortWaves;
     a.tiles = (int)((row_tiles + a.run - 1) / a.run);
   } else {
-    cross_plan(a, ks, dt, planes, row_tiles, &nw);
+    cross_plan(a, ks, dt, planes, row_tiles, &nw, &lone);
   }
   a.piece = ((a.tk + a.splits - 1) / a.splits + kCrossKeys - 1) / kCrossKeys * kCrossKeys;
   a.splits = (a.tk + a.piece - 1) / a.piece;
@@ -886,6 +1037,7 @@ int op_cross_attention(sy_ctx* ctx, const sy_cross_config* c, const sy_tensor* q
                    4.0 * q->n * ((double)a.tq * a.heads + (double)a.tk * a.kv) * (a.kd + a.hd));
     CrossKernel kernel = few     ? pick_few(a.kd, a.hd, a.rows)
                          : brief ? pick_short(ks, dt)
+                         : lone ? pick_lone(ks, dt)
                          : nw == 4 ? pick_cross<4>(ks, dt)
                                    : pick_cross<8>(ks, dt);
     const size_t lds = brief ? (size_t)(a.tk + kCrossKeys - 1) / kCrossKeys * short_bytes(ks, dt) : 0;
