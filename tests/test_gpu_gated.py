@@ -183,3 +183,54 @@ def test_refusals(hip):
         hip.gated(layer, vx, Tensor(vx.data + 48, 1, 8, 2, 3, vx.ldc, 0))
     with pytest.raises(ValueError):
         hip.gated_create(np.zeros((4, 5), np.float32), np.zeros((4, 6), np.float32))
+
+
+# rows, input channels, output channels: few rows, a middling number of tiles, many of long rows, of short ones
+FORMS = [(7, 320, 70), (200, 320, 70), (3000, 320, 400), (3000, 250, 2100), (13100, 40, 300), (33000, 64, 60), (33000, 200, 70)]
+
+
+@pytest.mark.parametrize("size", [(33000, 250, 70), (33001, 120, 130), (13000, 250, 300), (3000, 200, 900), (3000, 256, 2100),
+                                  (200, 256, 40), (5000, 3, 40), (66000, 2, 20), (40000, 5, 9), (35000, 130, 500)], ids=str)
+@pytest.mark.parametrize("pad", [0, 3])
+def test_many_short_rows(hip, size, pad):
+    rows, ic, oc = size
+    x, w = rows_of(rows, ic, 31), weights(oc, ic, 32)
+    check(run(hip, x, w, N.ACT_GELU, pad=pad), *L.gated(x, *w, N.ACT_GELU))
+
+
+@pytest.mark.parametrize("size", FORMS, ids=str)
+@pytest.mark.parametrize("far", [32, 60])
+def test_uneven_channels_of_every_form(hip, size, far):
+    """As above, with some ordinary rows beside them."""
+    rows, ic, oc = size
+    x, w = rows_of(rows, ic, 33), weights(oc, ic, 34)
+    x[rows // 3:, ::2] *= np.float32(2.0 ** -far)
+    w[0][:, ::2] *= np.float32(2.0 ** far)
+    w[1][:, 1::2] = 0
+    exp, _ = L.gated(x, *w, N.ACT_NONE)
+    x64 = x.astype(np.float64)
+    near = [np.abs(x64) @ np.abs(m.astype(np.float64)).T for m in w[:2]]
+    a, b = (x64 @ w[i].astype(np.float64).T + w[2 + i] for i in range(2))
+    off = [(m * (ic + 16) * L.UNIT + m * 2.0 ** -17) + np.abs(s) * 2 * L.UNIT for m, s in zip(near, (a, b))]
+    bound = off[0] * np.abs(b) + off[1] * (np.abs(a) + off[0]) + np.abs(exp) * L.UNIT + L.TINY
+    got = run(hip, x, w, N.ACT_NONE)
+    assert (np.abs(got - exp) <= bound).all(), (np.abs(got - exp) / bound).max()
+
+
+@pytest.mark.parametrize("size", FORMS, ids=str)
+@pytest.mark.parametrize("what", [np.nan, -np.inf])
+def test_non_finite_of_every_form(hip, size, what):
+    """An infinity or NaN in the first, a middle and the last row, and in a weight of the first and the last channel."""
+    rows, ic, oc = size
+    x, w = rows_of(rows, ic, 35), weights(oc, ic, 36)
+    exp, bound = L.gated(x, *w, N.ACT_NONE)
+    bad = [0, rows // 2, rows - 1]
+    x[bad[0], 0], x[bad[1], ic // 2], x[bad[2], ic - 1] = what, what, what
+    fine = np.ones(exp.shape, bool)
+    fine[bad] = False
+    got = run(hip, x, w, N.ACT_NONE)
+    assert not np.isfinite(got[bad]).any() and (np.abs(got - exp) <= bound)[fine].all()
+    w[1][0, ic - 1] = w[0][oc - 1, 0] = what
+    fine[:, [0, oc - 1]] = False
+    got = run(hip, x, w, N.ACT_NONE)
+    assert not np.isfinite(got[:, [0, oc - 1]]).any() and (np.abs(got - exp) <= bound)[fine].all()
