@@ -475,7 +475,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cross_kernel(const CrossArgs a) {
 // waves on their own, the next rows' queries under way.  Memory bounds it: 25600 queries to 77 states of four
 // images, 8 heads of 64 channels 125 us, 3.4 TB/s (outputs go past the caches, in whole lines).
 constexpr int kShortLds = 150 * 1024, kShortWaves = 4;
-constexpr int short_bytes(int ks, int dt) { return (ks + 2 * dt) * 3072; }  // of a tile
+constexpr int short_bytes(int ks, int dt) { return (ks + 2 * dt) * 192 * 16; }  // of a tile
 template <int KS, int DT>
 __global__ __launch_bounds__(kShortWaves * 64, KS == 8 ? 1 : 2) void cross_short_kernel(const CrossArgs a) {
   constexpr int NW = kShortWaves;
