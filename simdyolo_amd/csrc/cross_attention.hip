@@ -477,7 +477,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cross_kernel(const CrossArgs a) {
 constexpr int kShortLds = 150 * 1024, kShortWaves = 4;
 constexpr int short_bytes(int ks, int dt) { return (ks + 2 * dt) * 192 * 16; }  // of a tile
 template <int KS, int DT>
-__global__ __launch_bounds__(kShortWaves * 64, KS == 8 ? 1 : 2) void cross_short_kernel(const CrossArgs a) {
+__global__ __launch_bounds__(kShortWaves * 64, KS >= 5 ? 1 : 2) void cross_short_kernel(const CrossArgs a) {
   constexpr int NW = kShortWaves;
   typedef CrossStage<KS, DT, NW * 64, 1> Stage;
   extern __shared__ u32x4 frag[];
@@ -538,7 +538,7 @@ __global__ __launch_bounds__(kShortWaves * 64, KS == 8 ? 1 : 2) void cross_short
 // states, 8 heads of 32 channels 5.8 us, 4 of them the launch.
 constexpr int kLoneWaves = 4;
 template <int KS, int DT>
-__global__ __launch_bounds__(kLoneWaves * 64, KS + 2 * DT <= 8 ? 2 : 1) void cross_lone_kernel(const CrossArgs a) {
+__global__ __launch_bounds__(kLoneWaves * 64, KS + 2 * DT <= 8 && KS < 6 ? 2 : 1) void cross_lone_kernel(const CrossArgs a) {
   constexpr int NW = kLoneWaves;
   __shared__ f32x4 others[NW - 1][DT * 4][64];
   __shared__ float tops[NW][32], sums[NW][32];
@@ -879,10 +879,18 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const CrossArgs a, long
 }
 
 typedef void (*CrossKernel)(const CrossArgs);
-#define SY_CROSS_PICK(kernel, ...)                                                                             \
-  ks == 2   ? (dt == 1 ? kernel<2, 1 __VA_ARGS__> : dt == 2 ? kernel<2, 2 __VA_ARGS__> : kernel<2, 4 __VA_ARGS__>) \
-  : ks == 4 ? (dt == 1 ? kernel<4, 1 __VA_ARGS__> : dt == 2 ? kernel<4, 2 __VA_ARGS__> : kernel<4, 4 __VA_ARGS__>) \
-            : (dt == 1 ? kernel<8, 1 __VA_ARGS__> : dt == 2 ? kernel<8, 2 __VA_ARGS__> : kernel<8, 4 __VA_ARGS__>)
+#define SY_CROSS_DT(kernel, KS, ...)                       \
+  (dt == 1   ? kernel<KS, 1 __VA_ARGS__>                  \
+   : dt == 2 ? kernel<KS, 2 __VA_ARGS__>                  \
+   : dt == 3 ? kernel<KS, 3 __VA_ARGS__>                  \
+             : kernel<KS, 4 __VA_ARGS__>)
+#define SY_CROSS_PICK(kernel, ...)                         \
+  (ks == 2   ? SY_CROSS_DT(kernel, 2, __VA_ARGS__)        \
+   : ks == 3 ? SY_CROSS_DT(kernel, 3, __VA_ARGS__)        \
+   : ks == 4 ? SY_CROSS_DT(kernel, 4, __VA_ARGS__)        \
+   : ks == 5 ? SY_CROSS_DT(kernel, 5, __VA_ARGS__)        \
+   : ks == 6 ? SY_CROSS_DT(kernel, 6, __VA_ARGS__)        \
+             : SY_CROSS_DT(kernel, 8, __VA_ARGS__))
 #define SY_COMMA ,
 template <int NW>
 static CrossKernel pick_cross(int ks, int dt) {
@@ -892,6 +900,7 @@ static CrossKernel pick_short(int ks, int dt) { return SY_CROSS_PICK(cross_short
 static CrossKernel pick_lone(int ks, int dt) { return SY_CROSS_PICK(cross_lone_kernel); }
 #undef SY_COMMA
 #undef SY_CROSS_PICK
+#undef SY_CROSS_DT
 static CrossKernel pick_few(int kd, int hd, int rows) {
   if (std::max(kd, hd) <= 64)
     return rows == 1 ? cross_few_kernel<1, 1> : rows == 2 ? cross_few_kernel<1, 2> : cross_few_kernel<1, 4>;
@@ -910,7 +919,7 @@ static void cross_plan(CrossArgs& a, int ks, int dt, long long planes, long long
   double best = INFINITY;
   for (int w : {4, 8}) {
     // Workgroups to a CU, as their registers allow.
-    const int there = w == 8 || s == 16 ? 1 : s <= 6 && ks == 2 ? 3 : 2;
+    const int there = w == 8 || s >= 14 ? 1 : s <= 6 && ks == 2 ? 3 : 2;
     const long long whole = planes * ((row_tiles + w - 1) / w);
     for (long long x = 1; x <= std::max<long long>(1, std::min<long long>(64, key_tiles / 2)); ++x) {
       const long long rounds = (whole * x + cus * there - 1) / (cus * there);
@@ -1007,7 +1016,8 @@ int op_cross_attention(sy_ctx* ctx, const sy_cross_config* c, const sy_tensor* q
   a.c = c->scale * 1.4426950408889634f;
   a.rows = a.tq * a.group;
   const long long planes = (long long)q->n * a.kv;
-  const int ks = a.kd <= 32 ? 2 : a.kd <= 64 ? 4 : 8, dt = a.hd <= 32 ? 1 : a.hd <= 64 ? 2 : 4;
+  // Steps of 16 channels, tiles of 32.
+  const int ks = a.kd <= 32 ? 2 : a.kd <= 96 ? (a.kd + 15) / 16 : 8, dt = (a.hd + 31) / 32;
   int nw = 0;  // waves of a workgroup; 0: few rows, or few states
   bool lone = false;  // each with tiles of its own
   const long long row_tiles = (a.rows + 31) / 32;

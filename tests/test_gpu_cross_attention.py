@@ -265,3 +265,18 @@ def test_overlaps_are_refused(hip):
         for o in (vq, Tensor(vk.data, 1, 64, 1, 6, 64, 0), Tensor(vv.data + 16, 1, 64, 1, 6, 64, 0)):
             with pytest.raises(SyError, match="overlaps"):
                 hip.cross_attention(config(2, 2, 32, 32), vq, vk, vv, o)
+
+
+@pytest.mark.parametrize("kd,hd", [(36, 68), (48, 96), (52, 36), (68, 100), (80, 80), (84, 64), (96, 96), (100, 72), (32, 92), (64, 80)])
+@pytest.mark.parametrize("case", [(2, 40, 77, 2, 2), (8, 1300, 33, 8, 8), (1, 900, 1300, 6, 2), (2, 5, 2100, 2, 1), (2, 2, 700, 3, 3)],
+                         ids=str)
+def test_head_dims(hip, case, kd, hd):
+    """Every number of steps of 16 channels and tiles of 32, in each form: some of the rows of large cases are compared."""
+    n, tq, tk, heads, kv = case
+    q, k, v = tensors(n, tq, tk, heads, kv, kd, hd, 21)
+    lengths = [tk - 5 * b for b in range(n)]
+    got = run(hip, q, k, v, lengths)
+    assert np.isfinite(got).all()
+    rows = np.unique(np.r_[0:min(tq, 3), tq - min(tq, 3):tq, R.rng(22).integers(0, tq, 12)])
+    exp, bound = L.cross(q[:, rows], k, v, scaled(q, k), lengths)
+    check(got[:, rows], exp, bound)
