@@ -201,9 +201,18 @@ __device__ __forceinline__ void cross_tile(const CrossArgs& a, Key key, Value va
   bf16x8 vp[2][3];
   value(0, vp[0]);
   if (a.mask) {
+    // The top bit of every byte that is not 0, spread over a word, picks the score.
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      if (!(seen[r >> 2] >> 8 * (r & 3) & 0xff)) s[r] = -INFINITY;
+    for (int x = 0; x < 4; ++x) {
+      const unsigned t = ((seen[x] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | seen[x];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned keep = (unsigned)((int)(t << (24 - 8 * e)) >> 31);
+        const float score = s[4 * x + e];
+        const unsigned bits = (keep & __builtin_bit_cast(unsigned, score)) | (~keep & 0xff800000u);
+        s[4 * x + e] = __builtin_bit_cast(float, bits);
+      }
+    }
   }
   if (j0 + kCrossKeys > to) {
     asm volatile("");  // a branch, not 16 selects in every tile
@@ -214,7 +223,12 @@ __device__ __forceinline__ void cross_tile(const CrossArgs& a, Key key, Value va
   float mx = s[0];
 #pragma unroll
   for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-  mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.c;
+  {
+    const unsigned bits = __builtin_bit_cast(unsigned, mx);
+    const auto both = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);  // the row's other half, without LDS
+    const unsigned low = both[0], high = both[1];
+    mx = fmaxf(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high)) * a.c;
+  }
   const bool move = mx - w.top > kSlack;  // row by row, so that no row's bits hang on another's scores
   if (__any(move)) {
     const float x = move ? __builtin_amdgcn_exp2f(w.top - mx) : 1.f;
