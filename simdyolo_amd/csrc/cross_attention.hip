@@ -144,10 +144,10 @@ struct CrossRows {
 // where a score passes it by kSlack: weights reach 2^kSlack until then, which costs
 // bf16 parts nothing.
 //
-// The six products bound it where head dims are large, and the vector work beside them, which takes turns
+// The six products bound it where head dims are large, and the vector work beside them, which hardly overlaps
 // with them: 4096 queries to 8400 states of two images, 16 heads of 128 channels 2.55 ms, 221 TFLOP/s (the
 // matrix cores busy 60 per cent of the time, the vector units 27); 300 queries to 8400 masked states of eight
-// images, 8 heads of 32 channels 173 us, 119 TFLOP/s (32 and 54: 16 scores of a lane cost 340 vector instructions,
+// images, 8 heads of 32 channels 172 us, 120 TFLOP/s (32 and 54: 16 scores of a lane cost 340 vector instructions,
 // weights, their parts and the mask, against 24 matrix instructions).
 constexpr float kSlack = 8.f;
 

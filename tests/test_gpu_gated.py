@@ -234,3 +234,34 @@ def test_non_finite_of_every_form(hip, size, what):
     fine[:, [0, oc - 1]] = False
     got = run(hip, x, w, N.ACT_NONE)
     assert not np.isfinite(got[:, [0, oc - 1]]).any() and (np.abs(got - exp) <= bound)[fine].all()
+
+
+def test_graphs_that_share_the_scratch():
+    """Captured calls whose rows are split into the context's scratch, of two layers and beside another operator's."""
+    with HipContext(0) as ctx, R.Device(ctx) as d:
+        calls = []
+        for rows, ic, oc in ((3000, 320, 400), (5000, 260, 300)):
+            w = weights(oc, ic, rows)
+            layer = ctx.gated_create(*w)
+            vx, _, _ = d.view(rows_of(rows, ic, 0).reshape(1, rows, 1, ic), 1, rows)
+            vy, _, read = d.view(np.zeros((1, rows, 1, oc), np.float32), 1, rows)
+            calls.append((lambda layer=layer, vx=vx, vy=vy: ctx.gated(layer, vx, vy), vx, read, w, rows, ic))
+        big = d.view(rows_of(9000, 64, 1).reshape(1, 9000, 1, 64), 90, 100)[0]
+        norm = lambda: ctx.group_norm(big, big, 2)
+        graphs = []
+        for c in calls + [(norm,)]:
+            c[0]()
+        for c in calls + [(norm,)]:
+            ctx.graph_begin()
+            c[0]()
+            graphs.append(ctx.graph_end())
+        for turn in range(3):
+            for i, (call, vx, read, w, rows, ic) in enumerate(calls):
+                x = rows_of(rows, ic, 40 + 3 * turn + i)
+                if turn == 1:
+                    x[2, 5] = 1e-30
+                ctx.h2d(vx.data, x)
+                calls[i - 1][0]()
+                ctx.graph_launch(graphs[2])
+                ctx.graph_launch(graphs[i])
+                check(read().reshape(rows, -1), *L.gated(x, *w, N.ACT_SILU))
