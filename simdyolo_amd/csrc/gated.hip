@@ -527,7 +527,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const Gate
 // panel's steps shared out over 8 / PAN waves.  x goes through LDS in lots of kLot elements, two
 // in turn, loaded row by row in whole lines and split by the workgroup itself (a kernel of its own would
 // cost more than the products); weights come straight from memory.  Latency bounds it, and the split's vector
-// work: 748 rows of 271 to 545 channels 12.2 us, 36 TFLOP/s, 1200 of 300 to 690 16.5, 60.
+// work: 256 rows of 1024 to 688 channels 17.9 us, 40 TFLOP/s, 1200 of 600 to 690 22.6, 88.
 template <int PAN>
 __global__ __launch_bounds__(512, 2) void gated_mid_kernel(const GatedArgs a) {
   constexpr int KW = 8 / PAN, SH = kLotSteps / KW;  // waves of a panel, their steps of a lot
@@ -680,12 +680,12 @@ __global__ __launch_bounds__(512, 2) void gated_mid_kernel(const GatedArgs a) {
   }
 }
 
-// Short rows (up to 256 elements) and many: 32 PX rows by panels of output channels, one to a wave, to a
+// Short rows (up to 256 Q elements, and 128 with LANES 32) and many: 32 PX rows by panels of output channels, one to a wave, to a
 // workgroup.  It loads its rows at once, in whole lines, splits them into LDS, where they stay, and
 // goes through a column of tiles (every col_tiles-th) with the weights straight from memory and no
-// further barrier.  LANES lanes hold a row, a quad each.  The split's and the outputs' vector work bounds it, and the
+// further barrier.  LANES lanes hold a row, Q quads each.  The split's and the outputs' vector work bounds it, and the
 // launch: 1200 rows of 255 to 690 channels 10.4 us, 82 TFLOP/s, 60000 of 256 to 384 104 us, 226.
-template <int PX, int LANES>
+template <int PX, int LANES, int Q>
 __global__ __launch_bounds__(256, 2) void gated_short_kernel(const GatedArgs a) {
   constexpr int SIDE = 64 / LANES, LOADS = 8 * PX / SIDE;  // rows side by side in a wave's load; loads of a wave
   extern __shared__ u32x4 xs[];                            // [PX][steps] fragments
@@ -704,22 +704,27 @@ __global__ __launch_bounds__(256, 2) void gated_short_kernel(const GatedArgs a) 
       for (int s = 0; s < 2; ++s) wv[u][j][s] = __builtin_bit_cast(f16x8, w[j * up + 64 * s]);
   };
   {
-    const Quad q(4 * l, a.ic);
     const int mine = wave * 8 * PX + side;  // the first of a lane's rows
-    f32x4 v[LOADS];
+    f32x4 v[LOADS][Q];
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i)
-      v[i] = q.load(a.x + (unsigned long long)(unsigned)min(row0 + mine + i * SIDE, a.rows - 1) * (unsigned)a.ldx);
+    for (int i = 0; i < LOADS; ++i) {
+      const float* x = a.x + (unsigned long long)(unsigned)min(row0 + mine + i * SIDE, a.rows - 1) * (unsigned)a.ldx;
+#pragma unroll
+      for (int j = 0; j < Q; ++j) v[i][j] = Quad(4 * (l + LANES * j), a.ic).load(x);
+    }
     const int panel = min(first * 4 + wave, a.panels - 1);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) load_w(panel, u, u);
     unsigned top[LOADS], low[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      v[i] = q.mend(v[i]);
       Range range;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) range.look(v[i][e]);
+      for (int j = 0; j < Q; ++j) {
+        v[i][j] = Quad(4 * (l + LANES * j), a.ic).mend(v[i][j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) range.look(v[i][j][e]);
+      }
       low[i] = range.low;
       top[i] = lanes_max<LANES>(range.top);
     }
@@ -733,17 +738,20 @@ __global__ __launch_bounds__(256, 2) void gated_short_kernel(const GatedArgs a) 
     if (l == 0)
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) words[mine + i * SIDE] = gated_field(top[i]) | low[i];
-    const int step = l >> 2;
-    if (step < a.steps)
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int r = mine + i * SIDE;
-        u32x2 h, lo;
-        split4(v[i], exp_float(gated_field(top[i])), h, lo);
-        u32x2* at = (u32x2*)(xs + ((r >> 5) * a.steps + step) * kStep + place(step, (l >> 1) & 1, r & 31)) + (l & 1);
-        at[0] = h;
-        at[128] = lo;
-      }
+    for (int j = 0; j < Q; ++j) {
+      const int step = (l + LANES * j) >> 2;
+      if (step < a.steps)
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int r = mine + i * SIDE;
+          u32x2 h, lo;
+          split4(v[i][j], exp_float(gated_field(top[i])), h, lo);
+          u32x2* at = (u32x2*)(xs + ((r >> 5) * a.steps + step) * kStep + place(step, (l >> 1) & 1, r & 31)) + (l & 1);
+          at[0] = h;
+          at[128] = lo;
+        }
+    }
   }
   __syncthreads();
   bool plain[PX], again = false;
@@ -954,9 +962,11 @@ int op_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tenso
     hipLaunchKernelGGL(a.ic < 4 ? gated_few_kernel<true> : gated_few_kernel<false>, dim3((unsigned)grid), dim3(kFewWaves * 64), 0, ctx->stream, a);
     return check_launch("gated_few");
   }
-  if (a.ic <= 4 * 64) {
-    // Short rows: three column tiles (of 128 channels) or four at most, or a thousand tiles; else the products are so
-    // many that splitting x beforehand pays (20000 rows of 256 to 512 channels 58 us here, 53 so; to 256 33.7 and 38).
+  if (a.ic <= 512) {
+    // Short rows: three column tiles (of 128 channels) or four at most, or 900 tiles; else the products are so
+    // many that splitting x beforehand pays (20000 rows of 256 to 512 channels 58 us here, 53 so, to 256 33.7 and 38; 4000
+    // of 512 to 512 (500 tiles) 24.3 and 26.9, 2048 to 2048 (1024) 41.8 and 37.3).  Longer rows than 512: 64 KB and more of
+    // LDS, where fewer waves would hide less.
     // Where 64 rows to a workgroup make 512 of them, that, and every column tile in turn: 60000 rows of 256 to 384 channels
     // 104 us, 122 with 32 rows, 123 split beforehand; 9471 of 90 to 360 15.5 to 24, 17.9, 19.7.  With 32 rows, every
     // column tile in turn where there are 400 workgroups: 14161 of 137 to 377 26.4 us, a tile to each 30.4; 9471 of 90 to
@@ -968,18 +978,19 @@ int op_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tenso
                          ctx->stream, a);
       return check_launch("gated_short");
     };
-    if (wide >= 512 && cols <= 4) {
+    if (a.ic <= 256 && wide >= 512 && cols <= 4) {
       SY_CHECK(wide * 256LL < (1LL << 32), SY_EUNSUPPORTED, "gated grid too large");
       a.col_tiles = 1;
-      return a.steps <= 8 ? go(gated_short_kernel<2, 32>, wide, 2) : go(gated_short_kernel<2, 64>, wide, 2);
+      return a.steps <= 8 ? go(gated_short_kernel<2, 32, 1>, wide, 2) : go(gated_short_kernel<2, 64, 1>, wide, 2);
     }
-    if (cols <= 3 || (long long)a.xpanels * cols <= 1024) {
+    if ((cols <= 3 && a.ic <= 256) || (long long)a.xpanels * cols <= 900) {
       a.col_tiles = a.xpanels >= 400 ? 1 : cols;
-      return a.steps <= 8 ? go(gated_short_kernel<1, 32>, a.xpanels, 1) : go(gated_short_kernel<1, 64>, a.xpanels, 1);
+      if (a.ic > 256) return go(gated_short_kernel<1, 64, 2>, a.xpanels, 1);
+      return a.steps <= 8 ? go(gated_short_kernel<1, 32, 1>, a.xpanels, 1) : go(gated_short_kernel<1, 64, 1>, a.xpanels, 1);
     }
   }
-  // One workgroup to a CU: 1200 rows of 256 to 690 channels (228 of them) 12.2 us here, 20.4 split beforehand; to 2048
-  // channels (608) 32.8 and 25.8.
+  // One workgroup to a CU: 1200 rows of 600 to 690 channels (228 of them) 22.6 us here, 27.4 split beforehand; to 1365
+  // (418) 44.1 and 28.8.  Two panels to a workgroup where those find room, too: 400 rows of 600 to 600 14.2 us, four 20.8.
   const long long mids = a.xpanels * ((p.panels + 3LL) / 4), wide = a.xpanels * ((p.panels + 1LL) / 2);
   if (mids <= 256) {
     ProfScope prof(ctx, "gated_mid", flops, bytes);

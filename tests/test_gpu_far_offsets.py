@@ -48,7 +48,7 @@ def test_norm(hip, far, groups):
 
 
 @pytest.mark.parametrize("rows,ic,oc,pitch", [(17, 64, 96, (1 << 28) + 4), (560, 64, 256, PITCH), (560, 320, 256, PITCH),
-                                              (560, 320, 1900, PITCH)])
+                                              (560, 600, 256, PITCH), (560, 600, 1900, PITCH)])
 def test_gated(hip, far, rows, ic, oc, pitch):
     g = R.rng(2)
     x = g.standard_normal((rows, ic)).astype(np.float32)

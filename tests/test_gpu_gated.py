@@ -186,11 +186,11 @@ def test_refusals(hip):
 
 
 # rows, input channels, output channels: few rows, a middling number of tiles, many of long rows, of short ones
-FORMS = [(7, 320, 70), (200, 320, 70), (3000, 320, 400), (3000, 250, 2100), (13100, 40, 300), (33000, 64, 60), (33000, 200, 70)]
+FORMS = [(7, 320, 70), (200, 320, 70), (3000, 320, 400), (3000, 250, 2100), (300, 900, 130), (3000, 530, 400), (13100, 40, 300), (33000, 64, 60), (33000, 200, 70)]
 
 
 @pytest.mark.parametrize("size", [(33000, 250, 70), (33001, 120, 130), (13000, 250, 300), (3000, 200, 900), (3000, 256, 2100),
-                                  (200, 256, 40), (5000, 3, 40), (66000, 2, 20), (40000, 5, 9), (35000, 130, 500)], ids=str)
+                                  (200, 256, 40), (5000, 3, 40), (66000, 2, 20), (40000, 5, 9), (35000, 130, 500), (1300, 511, 200), (700, 258, 690)], ids=str)
 @pytest.mark.parametrize("pad", [0, 3])
 def test_many_short_rows(hip, size, pad):
     rows, ic, oc = size
@@ -240,7 +240,7 @@ def test_graphs_that_share_the_scratch():
     """Captured calls whose rows are split into the context's scratch, of two layers and beside another operator's."""
     with HipContext(0) as ctx, R.Device(ctx) as d:
         calls = []
-        for rows, ic, oc in ((3000, 320, 400), (5000, 260, 300)):
+        for rows, ic, oc in ((3000, 540, 400), (5000, 600, 300)):
             w = weights(oc, ic, rows)
             layer = ctx.gated_create(*w)
             vx, _, _ = d.view(rows_of(rows, ic, 0).reshape(1, rows, 1, ic), 1, rows)
