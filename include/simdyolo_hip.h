@@ -40,8 +40,9 @@
  * float32, as all are where queries are few.  With channels of one size its
  * error against float64 is 0.4 to 0.65 of plain float32's.
  * sy_cross_attention multiplies three bf16 parts as sy_attention does, and up
- * to four rows (queries times heads) of a key head, and rows that come out
- * infinite or NaN, in plain float32.  sy_gated_run multiplies pairs of f16
+ * to four rows (queries times heads) of a key head in plain float32, as it does
+ * rows that come out infinite or NaN or whose largest scaled score is 1.8e8 and
+ * more from zero.  sy_gated_run multiplies pairs of f16
  * values under a power of two of each pixel and of each output channel: an
  * operand within 2^-22 of itself (of its row's largest, 2^-50), and 2^-22 of
  * each product at most; tiles that meet a row with a nonzero element below

@@ -142,14 +142,20 @@ struct CrossRows {
 // The running maximum (Milakov and Gimelshein, 2018) is that of s c, rounded once; weights are
 // 2^(s c - m) with one rounding of the exponent.  It moves, and the sums with it, only
 // where a score passes it by kSlack: weights reach 2^kSlack until then, which costs
-// bf16 parts nothing.
+// bf16 parts nothing.  The largest score's own weight is 2^(s c - m), up to half a step of m beside 1: a factor
+// of all weights that the sum takes out again while |m| is below kFar, where it lies between 2^-8 and 2^8.  Farther out
+// it could leave no weight at all (or s c is not finite): a row whose maximum ends there is formed again in plain float32,
+// which subtracts before it multiplies.  A sum of 0 therefore means that no state was visible.
 //
 // The six products bound it where head dims are large, and the vector work beside them, which hardly overlaps
 // with them: 4096 queries to 8400 states of two images, 16 heads of 128 channels 2.55 ms, 221 TFLOP/s (the
 // matrix cores busy 60 per cent of the time, the vector units 27); 300 queries to 8400 masked states of eight
 // images, 8 heads of 32 channels 172 us, 120 TFLOP/s (32 and 54: 16 scores of a lane cost 340 vector instructions,
 // weights, their parts and the mask, against 24 matrix instructions).
-constexpr float kSlack = 8.f;
+constexpr float kSlack = 8.f, kFar = 0x1p28f;
+
+// Whether weights relative to this maximum, of a row that sees a state, say nothing.
+__device__ __forceinline__ bool cross_far(float top) { return !(__builtin_fabsf(top) < kFar); }
 
 // A row's mask bytes of the tile at j0, the lane's states four by four; 0 past `to`.
 __device__ __forceinline__ void cross_seen(const uint8_t* mask, int j0, int to, unsigned (&seen)[4]) {
@@ -295,7 +301,7 @@ __device__ __forceinline__ void cross_finish(const CrossArgs& a, const CrossRows
   const int b = plane / a.kv, g = plane - b * a.kv, row1 = min(row0 + r32, a.rows - 1);
   float l = w.sum + __shfl_xor(w.sum, 32);
   const unsigned any = w.any | (unsigned)__shfl_xor((int)w.any, 32);
-  if (any && states && w.top == -INFINITY) l = NAN;  // visible, but no finite score: again, in plain float32
+  if (any && states && cross_far(w.top)) l = NAN;  // visible, but no finite score or a far one: again, in plain float32
   // Where row 0 of the tile goes, and how far row1 is from it.
   float* out;
   long long step, mine;  // floats from row to row; to row1, where they differ
@@ -312,7 +318,7 @@ __device__ __forceinline__ void cross_finish(const CrossArgs& a, const CrossRows
     mine = qi * a.ldo + (long long)(row1 - qi * a.group) * a.hd;
     if (a.group == 1) out += row0 * a.ldo;
   }
-  const float factor = a.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;  // l is 1 and more, or there is nothing to weigh
+  const float factor = a.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;  // 0: there is nothing to weigh
   float f[16];
 #pragma unroll
   for (int r = 0; r < 16; ++r) f[r] = __shfl(factor, 8 * (r >> 2) + 4 * half + (r & 3));
@@ -810,6 +816,7 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(O[w][r][min(lane, 16 * C - 1)][e], x, y[e]);
     }
+    if (t != -INFINITY && cross_far(t)) l = NAN;  // -inf: nothing visible, or NaN already
     const bool live = lane < 16 * C && 4 * lane < a.hd;
     if (a.splits > 1) {
       const long long at = ((long long)plane * a.splits + split) * a.rows + r;
@@ -871,6 +878,7 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const CrossArgs a, long
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], off);
   }
+  if (top != -INFINITY && cross_far(top)) sum = NAN;  // a piece whose weights came to 0 may hold it
   const bool live = here && l < L && c < a.hd;
   bool again = false;
 #pragma unroll
