@@ -223,9 +223,9 @@ __device__ __forceinline__ f32x4 gated_weights(const GatedArgs& a, int which, in
   const long long panel = 2LL * (col >> 5) + which;
   const _Float16* w = (const _Float16*)(a.w + (panel * a.steps + (k >> 4)) * kStep + ((k >> 3) & 1) * 32 + (col & 31)) + (k & 7);
   const f16x4 hi = *(const f16x4*)w, lo = *(const f16x4*)(w + 512);
-  const float s = exp_float(254 - (a.w_row[panel * 32 + (col & 31)] & 0xff));
+  const int power = 127 - (a.w_row[panel * 32 + (col & 31)] & 0xff);  // -127 in channels below 2^-112
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf((float)lo[e], 1.f / 2048, (float)hi[e]) * s;
+  for (int e = 0; e < 4; ++e) v[e] = __builtin_ldexpf(__builtin_fmaf((float)lo[e], 1.f / 2048, (float)hi[e]), power);
   return v;
 }
 
