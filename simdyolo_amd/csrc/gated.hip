@@ -7,7 +7,7 @@
 // its element as long as that is not below 2^-29 of its row's largest, and within 2^-50 of the
 // largest below; what is left out, l l, is 2^-22 of the product at most.  Rows that hold a
 // nonzero element below kUneven of their largest, infinities or NaN are not multiplied so: the tiles
-// that meet them are computed in plain float32, on the float32 matrix cores.
+// that meet them are computed in plain float32, on the float32 matrix cores, from x and the weights as they were given.
 #include <algorithm>
 #include <chrono>
 #include <memory>
@@ -33,7 +33,7 @@ struct GatedPlan {
   int* w_row = nullptr;   // [panel][gate, up][32] words
   int* w_plain = nullptr; // [panel]: uneven
   float* bias = nullptr;  // [gate, up][panels * 32]
-  float* raw = nullptr;   // [gate, up][oc][ic], where a panel is uneven
+  float* raw = nullptr;   // [gate, up][oc][ic] and 4 floats that quads may reach
 };
 
 struct GatedArgs {
@@ -210,38 +210,25 @@ __global__ __launch_bounds__(512) void gated_split_kernel(const float* x, long l
   if (threadIdx.x == 0) plain[blockIdx.x] = any;
 }
 
-// Four weights of output channel `col` (gate or up) from input channel k.
+// Four weights of output channel `col` (gate or up) from input channel k: their own bits, not the pairs'.  Channels
+// past the last are the last's.
 __device__ __forceinline__ f32x4 gated_weights(const GatedArgs& a, int which, int col, int k) {
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  if (a.raw) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (col < a.oc && k + e < a.ic) v[e] = a.raw[((long long)which * a.oc + col) * a.ic + k + e];
-    return v;
-  }
-  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-  const long long panel = 2LL * (col >> 5) + which;
-  const _Float16* w = (const _Float16*)(a.w + (panel * a.steps + (k >> 4)) * kStep + ((k >> 3) & 1) * 32 + (col & 31)) + (k & 7);
-  const f16x4 hi = *(const f16x4*)w, lo = *(const f16x4*)(w + 512);
-  const int power = 127 - (a.w_row[panel * 32 + (col & 31)] & 0xff);  // -127 in channels below 2^-112
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = __builtin_ldexpf(__builtin_fmaf((float)lo[e], 1.f / 2048, (float)hi[e]), power);
-  return v;
+  const Quad q(k, a.ic);
+  return q.mend(q.load(a.raw + ((long long)which * a.oc + min(col, a.oc - 1)) * a.ic));
 }
 
-// 32 x 32 gate and up sums of a wave in plain float32, over steps [k0, k1).
+// 32 x 32 gate and up sums of a wave in plain float32, over steps [k0, k1).  Rows of four elements and more; those past the
+// last are the last's.
 __device__ __forceinline__ void gated_plain(const GatedArgs& a, long long row0, int panel, int k0, int k1, int lane,
                                             f32x16 (&acc)[2]) {
   const int half = lane >> 5, r32 = lane & 31;
-  const long long row = row0 + r32;
-  const float* x = a.x + min(row, (long long)a.rows - 1) * a.ldx;
+  const float* x = a.x + min(row0 + r32, (long long)a.rows - 1) * a.ldx;
 #pragma unroll
   for (int r = 0; r < 16; ++r) acc[0][r] = acc[1][r] = 0.f;
   for (int k = 16 * k0; k < 16 * k1; k += 8) {
     const int c = k + 4 * half;
-    f32x4 xv;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) xv[e] = row < a.rows && c + e < a.ic ? x[c + e] : 0.f;
+    const Quad q(c, a.ic);
+    const f32x4 xv = q.mend(q.load(x));
     const f32x4 g = gated_weights(a, 0, 32 * panel + r32, c), u = gated_weights(a, 1, 32 * panel + r32, c);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -862,19 +849,7 @@ static int gated_pack(sy_ctx* ctx, const float* gate, const float* up, const flo
   for (int m = 0; m < 2; ++m)
     hipLaunchKernelGGL(gated_split_kernel, dim3(p->panels), dim3(512), 0, ctx->stream, p->raw + m * values,
                        (long long)p->ic, p->oc, p->ic, p->steps, p->w, p->w_row, p->w_plain, 2, m, m == 1);
-  SY_TRY(check_launch("gated_split"));
-  std::vector<int> plain;
-  try {
-    plain.resize(p->panels);
-  } catch (const std::bad_alloc&) {
-    SY_CHECK(false, SY_ENOMEM, "no memory for a gated layer");
-  }
-  SY_TRY(sy_memcpy(ctx, plain.data(), p->w_plain, p->panels * sizeof(int), 1));
-  if (std::find(plain.begin(), plain.end(), 1) == plain.end()) {
-    SY_HIP(hipFree(p->raw));
-    p->raw = nullptr;
-  }
-  return SY_OK;
+  return check_launch("gated_split");
 }
 
 int op_gated_create(sy_ctx* ctx, const float* gate, const float* up, const float* gate_bias, const float* up_bias,
