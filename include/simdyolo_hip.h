@@ -45,8 +45,10 @@
  * more from zero.  sy_gated_run multiplies pairs of f16
  * values under a power of two of each pixel and of each output channel: an
  * operand within 2^-22 of itself (of its row's largest, 2^-50), and 2^-22 of
- * each product at most; tiles that meet a row with a nonzero element below
- * 2^-31 of its largest, an infinity or NaN are multiplied in plain float32.
+ * each product at most; pixels with a nonzero element below 2^-31 of their
+ * largest, an infinity or NaN are multiplied in plain float32 (those beside them
+ * are not: no pixel's bits depend on another's), and so are the 32 output
+ * channels from a multiple of 32 on of which one holds such weights.
  * sy_group_norm sums in 64 bits.
  *
  * Errors.  Every int-returning call returns SY_OK (0) or one of the SY_E*

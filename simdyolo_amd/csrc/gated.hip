@@ -6,8 +6,9 @@
 // output channel of G or U), and h h + (h l + l h) / 2048 is taken.  A pair is within 2^-22 of
 // its element as long as that is not below 2^-29 of its row's largest, and within 2^-50 of the
 // largest below; what is left out, l l, is 2^-22 of the product at most.  Rows that hold a
-// nonzero element below kUneven of their largest, infinities or NaN are not multiplied so: the tiles
-// that meet them are computed in plain float32, on the float32 matrix cores, from x and the weights as they were given.
+// nonzero element below kUneven of their largest, infinities or NaN are not multiplied so, but in plain float32, on the
+// float32 matrix cores, from x and the weights as they were given: such a row of x (the rows beside it keep their pairs,
+// so that no row's bits hang on another's), and all of a panel of 32 output channels that holds such weights.
 #include <algorithm>
 #include <chrono>
 #include <memory>
@@ -238,15 +239,18 @@ __device__ __forceinline__ void gated_plain(const GatedArgs& a, long long row0, 
   }
 }
 
-// A wave's 32 x 32 sums, gate and up, to the output: rows from row0, channel `col` of lane r32.
-__device__ __forceinline__ void gated_out(const GatedArgs& a, int row0, int col, int half, float (&g)[16], float (&u)[16]) {
+// A wave's 32 x 32 sums, gate and up, to the output: rows from row0, channel `col` of lane r32.  SOME: only
+// the rows whose bit is set in `rows`.
+template <bool SOME = false>
+__device__ __forceinline__ void gated_out(const GatedArgs& a, int row0, int col, int half, float (&g)[16], float (&u)[16],
+                                          unsigned rows = ~0u) {
   const float gb = a.bias[col], ub = a.bias[a.panels * 32 + col];
 #pragma unroll
   for (int r = 0; r < 16; ++r) g[r] += gb;
   activate(a.act, g);
   if (col >= a.oc) return;
   float* y = a.y + (row0 + 4 * half) * a.ldy + col;
-  if (row0 + 32 <= a.rows) {
+  if (!SOME && row0 + 32 <= a.rows) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) y[(8 * (r >> 2) + (r & 3)) * a.ldy] = g[r] * (u[r] + ub);
     return;
@@ -254,7 +258,7 @@ __device__ __forceinline__ void gated_out(const GatedArgs& a, int row0, int col,
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     const int row = 8 * (r >> 2) + (r & 3);
-    if (row0 + 4 * half + row < a.rows) y[row * a.ldy] = g[r] * (u[r] + ub);
+    if (row0 + 4 * half + row < a.rows && (!SOME || (rows >> (row + 4 * half) & 1))) y[row * a.ldy] = g[r] * (u[r] + ub);
   }
 }
 
@@ -362,21 +366,23 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_kernel(const GatedArgs a
     const int xp = (rt * WM + wm) * TM + i;
     if (xp >= a.xpanels) return;
     float g[16], u[16];
-    if (a.x_plain[xp] | a.w_plain[panel]) {
+    const int* words = a.x_row + xp * 32 + 4 * half;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int f = words[8 * (r >> 2) + (r & 3)] & 0xff;
+      g[r] = __builtin_ldexpf(__builtin_fmaf(crs[i][0][r], 1.f / 2048, acc[i][0][r]), 254 - f - gw);
+      u[r] = __builtin_ldexpf(__builtin_fmaf(crs[i][1][r], 1.f / 2048, acc[i][1][r]), 254 - f - uw);
+    }
+    const int w_plain = a.w_plain[panel];
+    if (a.x_plain[xp] | w_plain) {
       f32x16 t[2];
       gated_plain(a, (long long)xp * 32, panel, 0, a.steps, lane, t);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        g[r] = t[0][r];
-        u[r] = t[1][r];
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int f = a.x_row[xp * 32 + 8 * (r >> 2) + 4 * half + (r & 3)] & 0xff;
-        g[r] = __builtin_ldexpf(__builtin_fmaf(crs[i][0][r], 1.f / 2048, acc[i][0][r]), 254 - f - gw);
-        u[r] = __builtin_ldexpf(__builtin_fmaf(crs[i][1][r], 1.f / 2048, acc[i][1][r]), 254 - f - uw);
-      }
+      for (int r = 0; r < 16; ++r)
+        if (w_plain || (words[8 * (r >> 2) + (r & 3)] & kPlainRow)) {
+          g[r] = t[0][r];
+          u[r] = t[1][r];
+        }
     }
     gated_out(a, xp * 32, col, half, g, u);
   }
@@ -405,7 +411,8 @@ __device__ __forceinline__ void gated_plain16(const GatedArgs& a, int row0, int 
 // Few rows: 16 of them by 16 output channels to a workgroup, the steps shared out over its eight
 // waves, both operands straight from memory into the matrix instruction's registers, kAhead
 // pairs of steps at once.  A wave splits x itself while the weights are on their way, under powers of the pairs of steps
-// it has in hand, and brings each lot's sums to their true scale; a lot with an uneven row is plain by itself.
+// it has in hand, and brings each lot's sums to their true scale; a row that is uneven in a lot is
+// plain in all of the wave's, by itself.
 // The weights' bytes bound it: a row of 1024 to 2816 channels 6.6 us, 3.5 TB/s and half of it the launch, 32 rows
 // 11.0.  TINY: rows of fewer than four elements, which are not read in quads.
 constexpr int kFewWaves = 8, kAhead = 4;
@@ -424,6 +431,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const Gate
   const int w_plain = a.w_plain[panel];
   const int wf[2] = {a.w_row[panel * 64 + sub + r16] & 0xff, a.w_row[panel * 64 + 32 + sub + r16] & 0xff};
   f32x4 total[2] = {};
+  unsigned long long odd = 0;  // the lanes that met what makes their row plain
   for (int p = p0; p < p1; p += kAhead) {
     f16x8 wv[kAhead][2][2];
     f32x4 xv[kAhead][2];
@@ -463,10 +471,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const Gate
     unsigned top = range.top;
 #pragma unroll
     for (int off = 16; off < 64; off <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, off));
-    if (__any(w_plain != 0 || range.uneven(top))) {
-      for (int u = p; u < min(p + kAhead, p1); ++u) gated_plain16(a, row0, 32 * panel + sub, 32 * u, lane, total);
-      continue;
-    }
+    odd |= __ballot(range.uneven(top));
     const int field = gated_field(top);
     const float scale = exp_float(field);
     f32x4 acc[2] = {}, crs[2] = {};
@@ -490,6 +495,16 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const Gate
       for (int j = 0; j < 2; ++j)
         total[j][r] += __builtin_ldexpf(__builtin_fmaf(crs[j][r], 1.f / 2048, acc[j][r]), 254 - f - wf[j]);
     }
+  }
+  if (w_plain != 0 || odd != 0) {
+    f32x4 plain[2] = {};
+    for (int p = p0; p < p1; ++p) gated_plain16(a, row0, 32 * panel + sub, 32 * p, lane, plain);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (w_plain != 0 || (odd >> (4 * oct + r) & 0x0001000100010001ull) != 0) {  // by any of the lanes that hold the row
+        total[0][r] = plain[0][r];
+        total[1][r] = plain[1][r];
+      }
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j)
@@ -625,23 +640,28 @@ __global__ __launch_bounds__(512, 2) void gated_mid_kernel(const GatedArgs a) {
     }
     __syncthreads();
   }
-  if (__any(fields[r32] & kPlainRow) || a.w_plain[panel]) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int row = 8 * (r >> 2) + 4 * half + (r & 3), f = fields[row] & 0xff;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      sums[wave][j][row][r32] = __builtin_ldexpf(__builtin_fmaf(crs[j][r], 1.f / 2048, acc[j][r]),
+                                                 254 - f - (a.w_row[panel * 64 + 32 * j + r32] & 0xff));
+  }
+  // Plain rows' sums take the place of theirs.
+  const int w_plain = a.w_plain[panel];
+  if (__any(fields[r32] & kPlainRow) || w_plain) {
     const int share = (a.steps + KW - 1) / KW;
     gated_plain(a, row0, panel, min(part * share, a.steps), min((part + 1) * share, a.steps), lane, acc);
-  } else {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int f = fields[8 * (r >> 2) + 4 * half + (r & 3)];
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        acc[j][r] = __builtin_ldexpf(__builtin_fmaf(crs[j][r], 1.f / 2048, acc[j][r]),
-                                     254 - f - (a.w_row[panel * 64 + 32 * j + r32] & 0xff));
+      const int row = 8 * (r >> 2) + 4 * half + (r & 3);
+      if (w_plain || (fields[row] & kPlainRow)) {
+        sums[wave][0][row][r32] = acc[0][r];
+        sums[wave][1][row][r32] = acc[1][r];
+      }
     }
   }
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) sums[wave][j][8 * (r >> 2) + 4 * half + (r & 3)][r32] = acc[j][r];
   __syncthreads();
   if (first + wave / KW >= a.panels) return;
   const int col = 32 * panel + r32;
@@ -799,21 +819,22 @@ __global__ __launch_bounds__(256, 2) void gated_short_kernel(const GatedArgs a) 
       if (i == PX - 1)
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) load_w(next, u, u);
-      if (plain[i] || w_plain) {
-        again = true;
-        continue;
-      }
+      again |= plain[i] || w_plain;
+      if (w_plain) continue;
       gated_out(a, row0 + 32 * i, col, half, g, u);
     }
   }
   if (!again) return;
-  // The tiles that were left out, in plain float32 (inside the loop above they would cost it its registers).
+  // Panels that were left out and plain rows, whose outputs were not theirs yet, in plain float32 (inside the loop
+  // above they would cost it its registers).  A lane writes what it wrote there.
   for (int ct = first; 4 * ct + wave < a.panels; ct += a.col_tiles) {
     const int panel = 4 * ct + wave, col = 32 * panel + r32;
     const bool w_plain = a.w_plain[panel];
 #pragma unroll 1
     for (int i = 0; i < PX; ++i) {
-      if (!w_plain && !__any(words[32 * i + r32] & kPlainRow)) continue;
+      // (Bits of lanes past 32 repeat the others'.)
+      const unsigned rows = w_plain ? ~0u : (unsigned)__ballot(words[32 * i + r32] & kPlainRow);
+      if (rows == 0) continue;
       f32x16 t[2];
       gated_plain(a, row0 + 32 * i, panel, 0, a.steps, lane, t);
       float g[16], u[16];
@@ -822,7 +843,7 @@ __global__ __launch_bounds__(256, 2) void gated_short_kernel(const GatedArgs a) 
         g[r] = t[0][r];
         u[r] = t[1][r];
       }
-      gated_out(a, row0 + 32 * i, col, half, g, u);
+      gated_out<true>(a, row0 + 32 * i, col, half, g, u, rows);
     }
   }
 }

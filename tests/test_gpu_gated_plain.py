@@ -75,3 +75,22 @@ def test_uneven_weights_are_multiplied_plainly(hip, size, far):
         m[:, ::2] *= np.float32(2.0 ** -far)
     w += [None, g.standard_normal(oc).astype(np.float32)]
     check(run(hip, x, w, N.ACT_NONE), *plain(x, w))
+
+
+@pytest.mark.parametrize("what", [np.nan, np.inf, 1e-20, 1e12])
+@pytest.mark.parametrize("size", FORMS, ids=str)
+def test_rows_keep_their_bits_beside_any_row(hip, size, what):
+    """Rows of a tile in which others are infinite, NaN or uneven."""
+    rows, ic, oc = size
+    x, w = rows_of(rows, ic, 64), weights(oc, ic, 65)
+    layer = hip.gated_create(*w)
+    one = run(hip, x, w, layer=layer)
+    odd = np.unique(np.r_[2, 5:rows:37, rows - 1])
+    x[odd, R.rng(66).integers(0, ic, len(odd))] = what
+    two = run(hip, x, w, layer=layer)
+    keep = np.setdiff1d(np.arange(rows), odd)
+    np.testing.assert_array_equal(one[keep], two[keep])
+    if np.isfinite(what):
+        check(two[odd], *L.gated(x[odd], *w, N.ACT_SILU))
+    else:
+        assert not np.isfinite(two[odd]).any()
