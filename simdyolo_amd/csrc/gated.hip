@@ -414,7 +414,7 @@ __device__ __forceinline__ void gated_plain16(const GatedArgs& a, int row0, int 
 // it has in hand, and brings each lot's sums to their true scale; a row that is uneven in a lot is
 // plain in all of the wave's, by itself.
 // The weights' bytes bound it: a row of 1024 to 2816 channels 6.6 us, 3.5 TB/s and half of it the launch, 32 rows
-// 11.0.  TINY: rows of fewer than four elements, which are not read in quads.
+// 11.0.  TINY: rows of fewer than four elements, which are not read in quads, and plain always: pairs would save nothing.
 constexpr int kFewWaves = 8, kAhead = 4;
 template <bool TINY>
 __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const GatedArgs a) {
@@ -432,20 +432,13 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const Gate
   const int wf[2] = {a.w_row[panel * 64 + sub + r16] & 0xff, a.w_row[panel * 64 + 32 + sub + r16] & 0xff};
   f32x4 total[2] = {};
   unsigned long long odd = 0;  // the lanes that met what makes their row plain
-  for (int p = p0; p < p1; p += kAhead) {
+  for (int p = TINY ? p1 : p0; p < p1; p += kAhead) {
     f16x8 wv[kAhead][2][2];
     f32x4 xv[kAhead][2];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (TINY) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) xv[u][h][e] = xr[min(e, a.ic - 1)];
-        } else {
-          xv[u][h] = Quad(min(p + u, pairs) * 32 + 8 * oct + 4 * h, a.ic).load(xr);
-        }
-      }
+      for (int h = 0; h < 2; ++h) xv[u][h] = Quad(min(p + u, pairs) * 32 + 8 * oct + 4 * h, a.ic).load(xr);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const long long at = (long long)min(p + u, pairs - 1) * 2 * kStep;
@@ -496,12 +489,12 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const Gate
         total[j][r] += __builtin_ldexpf(__builtin_fmaf(crs[j][r], 1.f / 2048, acc[j][r]), 254 - f - wf[j]);
     }
   }
-  if (w_plain != 0 || odd != 0) {
+  if (TINY || w_plain != 0 || odd != 0) {
     f32x4 plain[2] = {};
     for (int p = p0; p < p1; ++p) gated_plain16(a, row0, 32 * panel + sub, 32 * p, lane, plain);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      if (w_plain != 0 || (odd >> (4 * oct + r) & 0x0001000100010001ull) != 0) {  // by any of the lanes that hold the row
+      if (TINY || w_plain != 0 || (odd >> (4 * oct + r) & 0x0001000100010001ull) != 0) {  // by any of the lanes that hold the row
         total[0][r] = plain[0][r];
         total[1][r] = plain[1][r];
       }

@@ -94,3 +94,10 @@ def test_rows_keep_their_bits_beside_any_row(hip, size, what):
         check(two[odd], *L.gated(x[odd], *w, N.ACT_SILU))
     else:
         assert not np.isfinite(two[odd]).any()
+
+
+@pytest.mark.parametrize("ic", [1, 2, 3])
+@pytest.mark.parametrize("rows,oc", [(1, 1), (5, 33), (40, 300), (5000, 40), (66000, 20)])
+def test_rows_of_fewer_than_four_elements(hip, rows, oc, ic):
+    x, w = rows_of(rows, ic, 67), weights(oc, ic, 68)
+    check(run(hip, x, w, N.ACT_NONE), *plain(x, w))
