@@ -53,25 +53,30 @@ struct Moments {
 
 // Mean (in two floats) and 1 / sqrt(var + eps): the hardware's estimate (2^-23 and
 // better) and one step of Newton's, where a library's division and root would
-// cost more than the rest of a token's work.
+// cost more than the rest of a token's work.  Both under a power of two, `pre`, which x is multiplied with as the mean
+// is taken off: 1 but where the spread is past 2^100, so that differences or the factor leave float32, or (without
+// eps) below 2^-100, so that the factor or the mean's second part does.
 struct Scale {
-  float hi, lo, r;
+  float hi, lo, r, pre;
 };
 __device__ __forceinline__ Scale scale_of(const NormArgs& a, const Moments& m, double p) {
-  const double d = m.s * a.share, mean = p + d;
-  double var = __builtin_fma(m.q, a.share, -d * d);
+  const double d = m.s * a.share;
+  double mean = p + d, var = __builtin_fma(m.q, a.share, -d * d);
   var = (var < 0 ? 0 : var) + a.eps;  // NaN stays
-  const double e = __builtin_amdgcn_rsq(var);
+  double e = __builtin_amdgcn_rsq(var);
+  e *= __builtin_fma(-0.5 * var * e, e, 1.5);
   Scale s;
+  s.pre = var > 0x1p200 ? 0x1p-60f : var < 0x1p-200 ? 0x1p60f : 1.f;
+  mean *= (double)s.pre;
   s.hi = (float)mean;
   s.lo = __builtin_fabsf(s.hi) < INFINITY ? (float)(mean - (double)s.hi) : 0.f;
-  s.r = (float)(e * __builtin_fma(-0.5 * var * e, e, 1.5));
+  s.r = (float)(var > 0x1p200 ? e * 0x1p60 : var < 0x1p-200 ? e * 0x1p-60 : e);
   return s;
 }
 
 // Before the activation.
 __device__ __forceinline__ float normal(float x, const Scale& s, float g, float b) {
-  return __builtin_fmaf((x - s.hi) - s.lo, s.r * g, b);
+  return __builtin_fmaf(__builtin_fmaf(x, s.pre, -s.hi) - s.lo, s.r * g, b);
 }
 
 template <int VEC>
