@@ -39,16 +39,16 @@
  * largest) and rows that come out infinite or NaN are computed in plain
  * float32, as all are where queries are few.  With channels of one size its
  * error against float64 is 0.4 to 0.65 of plain float32's.
- * sy_cross_attention multiplies three bf16 parts as sy_attention does, and up
- * to four rows (queries times heads) of a key head in plain float32, as it does
- * rows that come out infinite or NaN or whose largest scaled score is 1.8e8 and
- * more from zero.  sy_gated_run multiplies pairs of f16
- * values under a power of two of each pixel and of each output channel: an
- * operand within 2^-22 of itself (of its row's largest, 2^-50), and 2^-22 of
- * each product at most; pixels with a nonzero element below 2^-31 of their
+ * sy_cross_attention multiplies three bf16 parts as sy_attention does (all part
+ * products in one float32 sum), and in plain float32 up to four rows (queries
+ * times heads) of a key head, rows that come out infinite or NaN and rows whose
+ * largest scaled score is 1.8e8 and more from zero.  sy_gated_run multiplies
+ * pairs of f16 values under a power of two of each pixel and of each output
+ * channel: an operand within 2^-22 of itself (of its row's largest, 2^-50), and
+ * 2^-22 of each product at most; pixels with a nonzero element below 2^-31 of their
  * largest, an infinity or NaN are multiplied in plain float32 (those beside them
- * are not: no pixel's bits depend on another's), and so are the 32 output
- * channels from a multiple of 32 on of which one holds such weights.
+ * are not: no pixel's bits depend on what another holds), and so are 32 output
+ * channels of which one holds such weights, and pixels of fewer than 4 channels.
  * sy_group_norm sums in 64 bits.
  *
  * Errors.  Every int-returning call returns SY_OK (0) or one of the SY_E*
@@ -447,9 +447,8 @@ int sy_group_norm(sy_ctx* ctx, const sy_tensor* x, int groups, const float* gamm
  * NULL: all; taken between 0 and h*w of k), and of those the ones whose mask
  * byte is not 0.  A query without a visible state gets zeros; states that a
  * query does not see are not read into its result, whatever they hold.  o is a
- * view of heads * head_dim channels on q's map and overlaps no input.  Products
- * are formed as in sy_attention's fused kernel ("Precision"), sums over the
- * states in float32. */
+ * view of heads * head_dim channels on q's map and overlaps no input.  Products:
+ * see "Precision"; sums over the states in float32. */
 typedef struct sy_cross_config {
   int32_t heads, kv_heads;   /* heads % kv_heads == 0 */
   int32_t key_dim, head_dim; /* channels of a query or key head, of a value head: multiples of 4 up to 128 */

@@ -148,9 +148,9 @@ struct CrossRows {
 // which subtracts before it multiplies.  A sum of 0 therefore means that no state was visible.
 //
 // The six products bound it where head dims are large, and the vector work beside them, which hardly overlaps
-// with them: 4096 queries to 8400 states of two images, 16 heads of 128 channels 2.55 ms, 221 TFLOP/s (the
-// matrix cores busy 60 per cent of the time, the vector units 27); 300 queries to 8400 masked states of eight
-// images, 8 heads of 32 channels 172 us, 120 TFLOP/s (32 and 54: 16 scores of a lane cost 340 vector instructions,
+// with them: 4096 queries to 8400 states of two images, 16 heads of 128 channels 2.6 ms, 217 TFLOP/s (the
+// matrix cores busy 59 per cent of the time, the vector units 27); 300 queries to 8400 masked states of eight
+// images, 8 heads of 32 channels 173 us, 119 TFLOP/s (28 and 48: 16 scores of a lane cost 340 vector instructions,
 // weights, their parts and the mask, against 24 matrix instructions).
 constexpr float kSlack = 8.f, kFar = 0x1p28f;
 
@@ -492,8 +492,9 @@ __global__ __launch_bounds__(NW * 64, 2) void cross_kernel(const CrossArgs a) {
 }
 
 // Few states: a workgroup splits all of them once and goes through many rows, its
-// waves on their own, the next rows' queries under way.  Memory bounds it: 25600 queries to 77 states of four
-// images, 8 heads of 64 channels 125 us, 3.4 TB/s (outputs go past the caches, in whole lines).
+// waves on their own, the next rows' queries under way.  25600 queries to 77 states of four images, 8 heads of 64
+// channels 132 us, 3.2 TB/s (outputs go past the caches, in whole lines): without any state it is 92, memory; the products and
+// weights do not run under that (matrix cores busy 26 per cent of the time, vector units 32).
 constexpr int kShortLds = 150 * 1024, kShortWaves = 4;
 constexpr int short_bytes(int ks, int dt) { return (ks + 2 * dt) * 192 * 16; }  // of a tile
 template <int KS, int DT>

@@ -267,7 +267,7 @@ __device__ __forceinline__ void gated_out(const GatedArgs& a, int row0, int col,
 // steps at a time, two stages in turn; the weights straight into registers, a stage ahead: with both in LDS
 // its ports are busy as long as the matrix cores.  A step's fragments of x are read while the one before it
 // is multiplied, over the barrier too: it stands before a stage's last products.  The matrix cores bound it: 16384 rows of
-// 1024 to 2816 channels 518 us, 365 TFLOP/s (the cores busy 63 per cent of the time), and with the split
+// 1024 to 2816 channels 519 us, 364 TFLOP/s (the cores busy 60 per cent of the time), and with the split
 // 350 where the float32 matrix instructions could reach 150.
 template <int WM, int WN>
 __global__ __launch_bounds__(WM* WN * 64, 2) void gated_kernel(const GatedArgs a) {
@@ -413,8 +413,8 @@ __device__ __forceinline__ void gated_plain16(const GatedArgs& a, int row0, int 
 // pairs of steps at once.  A wave splits x itself while the weights are on their way, under powers of the pairs of steps
 // it has in hand, and brings each lot's sums to their true scale; a row that is uneven in a lot is
 // plain in all of the wave's, by itself.
-// The weights' bytes bound it: a row of 1024 to 2816 channels 6.6 us, 3.5 TB/s and half of it the launch, 32 rows
-// 11.0.  TINY: rows of fewer than four elements, which are not read in quads, and plain always: pairs would save nothing.
+// The weights' bytes bound it: a row of 1024 to 2816 channels 6.1 us, 3.8 TB/s and half of it the launch, 32 rows
+// 10.5.  TINY: rows of fewer than four elements, which are not read in quads, and plain always: pairs would save nothing.
 constexpr int kFewWaves = 8, kAhead = 4;
 template <bool TINY>
 __global__ __launch_bounds__(kFewWaves * 64, 2) void gated_few_kernel(const GatedArgs a) {
@@ -941,7 +941,7 @@ int op_gated_run(sy_ctx* ctx, uint64_t gated, const sy_tensor* x, const sy_tenso
   a.xpanels = (a.rows + 31) / 32;
   DeviceScope device(ctx);
   const double flops = 4.0 * rows * p.ic * p.oc, bytes = 4.0 * ((double)rows * (p.ic + p.oc) + 2.0 * p.ic * p.oc);
-  // 32 rows of 1024 to 2816 channels 11.0 us here, 17.6 as a middling number of tiles; 64 of 256 to 688 (176 workgroups)
+  // 32 rows of 1024 to 2816 channels 10.5 us here, 17.6 as a middling number of tiles; 64 of 256 to 688 (176 workgroups)
   // 6.4, 7.5 as short rows; 256 of 128 to 256 (256) 5.1 and 5.7, 400 of 128 to 256 (400) 6.3 and 6.2, 33 of 2048 to 4096 (768) 40
   // and 33 as a middling number.
   if (a.rows <= 32 || a.ic < 4 || 2LL * p.panels * ((a.rows + 15) / 16) <= 256) {
